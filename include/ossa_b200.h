@@ -266,6 +266,95 @@ OSSA_API int ossa_router_distill_grad(const void* q, const void* k, int dtype,
                                       void* workspace, size_t workspace_bytes, ossa_stream_t stream);
 
 /*
+ * ossa_topk_attention_fwd_rows under score modifiers.  No counterpart in the reference.
+ * With x = (q_i . k_j) * scale, i = q_start + row:
+ *   s = softcap * tanh(x / softcap)   (softcap 0: s = x)
+ *   s = s - slopes[h] * |i - j|       (slopes (H,) fp32, NULL: none)
+ * and key j is seen by row i of batch element b when (not causal, or j <= i, or
+ * j < prefix_len[b]) and segments[b][j] == segments[b][i] (prefix_len (B,), segments
+ * (B, Nk), int32; NULL: none; segments need q_start + Nq <= Nk).  A row that sees none of
+ * its listed keys is 0.  lse2 (NULL, or B*H*Nq floats) receives log2 of each row's sum of
+ * exp(s) (-inf for an empty row), which ossa_topk_attention_bwd reads.  Without modifiers
+ * and without lse2 the call is ossa_topk_attention_fwd_rows.
+ */
+OSSA_API int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, const void* indices,
+                                         int idx_is_64, int dtype, int B, int H, int Hkv, int Nq, int Nk, int D,
+                                         int K, float scale, int causal, int q_start, float softcap,
+                                         const float* slopes, const int32_t* segments, const int32_t* prefix_len,
+                                         void* out, float* lse2, ossa_stream_t stream);
+
+/*
+ * Gradients of ossa_topk_attention_mod_fwd (and of the plain gather: softcap 0 and NULL
+ * modifiers).  No counterpart in the reference, whose sparse forward is never trained.
+ * `out` and `lse2` are the forward's results, dout (B, H, Nq, D) the gradient of out.
+ * Writes dq (like q), dk and dv (like k and v, every key, zero where no row lists it) and,
+ * when dslopes is not NULL, the gradient of slopes ((H,) fp32).  An index that a row lists
+ * twice counts twice, as in the forward.  Repeated calls give the same bits (no float
+ * atomics).  At most 2^30 listed keys per (b, kv head): (H / Hkv) * Nq * K.
+ */
+OSSA_API size_t ossa_topk_attention_bwd_workspace_size(int B, int H, int Hkv, int Nq, int Nk, int D, int K,
+                                                       int want_dslopes);
+OSSA_API int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64,
+                                     int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale,
+                                     int causal, int q_start, float softcap, const float* slopes,
+                                     const int32_t* segments, const int32_t* prefix_len, const void* out,
+                                     const float* lse2, const void* dout, void* dq, void* dk, void* dv,
+                                     float* dslopes, void* workspace, size_t workspace_bytes, ossa_stream_t stream);
+
+/*
+ * RMS norm of every query and key head, rotation and head transpose in one pass.
+ * Additive (the patched layer's modules without head norms use ossa_rope_to_heads):
+ *   q   rows (b, n) of Hq * D values at q + b * q_sb + n * q_sn (strides in elements, each a
+ *       multiple of 16 bytes); k alike with Hk heads (Hk = 0: q alone)
+ *   y   = x * rsqrt(mean(x^2) + eps) * w per head row; w NULL: y = x
+ *   out (B, Hx, N, D) = y*cos + rotate_half(y)*sin (as ossa_rope_to_heads; without cos/sin
+ *       out = y), computed in fp32 and rounded once
+ * wq, wk: (D,) of w_dtype (fp32 or bf16).  D a multiple of 8, at most 512.
+ * The backward takes the gradients of both outputs and writes dq, dk as contiguous
+ * (B, N, Hx, D) and, where not NULL, dwq and dwk ((D,), w_dtype).  q and k may be NULL there
+ * without weights, and the workspace too.  Repeated calls give the same bits.
+ */
+OSSA_API int ossa_qk_norm_rope_fwd(const void* q, const void* k, const void* wq, const void* wk, const void* cos,
+                                   const void* sin, int cs_batched, int dtype, int w_dtype, int B, int N, int Hq,
+                                   int Hk, int D, long long q_sb, long long q_sn, long long k_sb, long long k_sn,
+                                   float eps, void* q_out, void* k_out, ossa_stream_t stream);
+OSSA_API size_t ossa_qk_norm_rope_bwd_workspace_size(int D);
+OSSA_API int ossa_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* cos,
+                                   const void* sin, int cs_batched, int dtype, int w_dtype, int B, int N, int Hq,
+                                   int Hk, int D, long long q_sb, long long q_sn, long long k_sb, long long k_sn,
+                                   float eps, const void* dq_out, const void* dk_out, void* dq, void* dk, void* dwq,
+                                   void* dwk, void* workspace, size_t workspace_bytes, ossa_stream_t stream);
+
+/*
+ * Distillation of a model's logits from a teacher's top logits.  Additive (the reference
+ * distils its router only, ossa/router.py:80-99).  Row (o, i), o < outer, i < inner, of the
+ * student's logits z (V values at logits + o * stride_outer + i * stride_inner, strides in
+ * elements) against K listed entries (ids) with the teacher's logits t (fp32, (rows, K)):
+ *   p    = softmax(t / temperature) over the entries inside [0, V) (others are ignored;
+ *          an entry listed twice counts twice)
+ *   loss = temperature^2 * sum_k p_k (log p_k - log softmax(z / temperature)_k)
+ * The total is the sum over rows of row_weight (NULL: 1) times the row's loss, divided by
+ * the weights' sum when mean = 1; a row without a listed entry weighs 0, rows of weight 0
+ * are not read, and the total is 0 when every row weighs 0.  The forward writes, where not
+ * NULL, each row's unweighted loss (0 where the row weighs 0), the total, and
+ * dlogits = d total / d z (contiguous (rows, V), the logits' dtype).  The backward writes dlogits
+ * times `grad` (one value, or one per row) from the workspace that the forward left; with
+ * skip_if_one it leaves dlogits untouched when the one value is 1.  K <= 1024.
+ */
+OSSA_API size_t ossa_top_logit_distill_workspace_size(long long rows, int K);
+OSSA_API int ossa_top_logit_distill_fwd(const void* logits, int dtype, int outer, int inner, int V,
+                                        long long stride_outer, long long stride_inner, const float* teacher,
+                                        const void* ids, int ids_are_64, int K, float temperature,
+                                        const float* row_weight, int mean, float* loss_rows, float* loss,
+                                        void* dlogits, void* workspace, size_t workspace_bytes,
+                                        ossa_stream_t stream);
+OSSA_API int ossa_top_logit_distill_bwd(const void* logits, int dtype, int outer, int inner, int V,
+                                        long long stride_outer, long long stride_inner, const void* ids,
+                                        int ids_are_64, int K, float temperature, int mean, const float* grad,
+                                        int grad_per_row, int skip_if_one, void* dlogits, const void* workspace,
+                                        size_t workspace_bytes, ossa_stream_t stream);
+
+/*
  * Rotary position embedding fused with the head transpose of the patched
  * layer (ossa/bench/sparse_forward.py:166-178: the q/k/v projections viewed as
  * (B, Hx, N, D), then Qwen2's apply_rotary_pos_emb on q and k).  Additive, for

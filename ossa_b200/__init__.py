@@ -9,6 +9,7 @@ kernels (libossa_b200.so, C ABI in include/ossa_b200.h); CPU tensors are
 rejected rather than served by a fallback.
 """
 
+from .rope import qk_norm_rope, rope_to_heads
 from .router import ContentRouter, ContentRouterConfig
 from .select import oracle_topk, router_scores, router_topk, with_diagonal
 from .sparse_attention import (
@@ -17,6 +18,7 @@ from .sparse_attention import (
     sparse_attention_forward_chunked,
 )
 from .topk_attention import HAS_TRITON, topk_attention
+from .train import top_logit_distillation_loss
 
 __all__ = [
     "ContentRouter",
@@ -30,5 +32,8 @@ __all__ = [
     "router_scores",
     "oracle_topk",
     "with_diagonal",
+    "rope_to_heads",
+    "qk_norm_rope",
+    "top_logit_distillation_loss",
 ]
 __version__ = "0.1.0"

@@ -47,6 +47,15 @@ EXPORTED = (
     "ossa_router_workspace_size_kp",
     "ossa_router_project_keys",
     "ossa_router_topk_rows_kp",
+    "ossa_topk_attention_mod_fwd",
+    "ossa_topk_attention_bwd_workspace_size",
+    "ossa_topk_attention_bwd",
+    "ossa_qk_norm_rope_fwd",
+    "ossa_qk_norm_rope_bwd_workspace_size",
+    "ossa_qk_norm_rope_bwd",
+    "ossa_top_logit_distill_workspace_size",
+    "ossa_top_logit_distill_fwd",
+    "ossa_top_logit_distill_bwd",
 )
 
 _lock = threading.Lock()
@@ -109,6 +118,27 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ossa_router_project_keys.restype = ci
     lib.ossa_router_topk_rows_kp.argtypes = [vp, ci, vp, vp, vp] + [ci] * 11 + [vp, vp, sz, vp]
     lib.ossa_router_topk_rows_kp.restype = ci
+    cl = ctypes.c_longlong
+    lib.ossa_topk_attention_mod_fwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf, vp, vp, vp, vp, vp, vp]
+    lib.ossa_topk_attention_mod_fwd.restype = ci
+    lib.ossa_topk_attention_bwd_workspace_size.argtypes = [ci] * 8
+    lib.ossa_topk_attention_bwd_workspace_size.restype = sz
+    lib.ossa_topk_attention_bwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf] + [vp] * 11 + [sz, vp]
+    lib.ossa_topk_attention_bwd.restype = ci
+    lib.ossa_qk_norm_rope_fwd.argtypes = [vp] * 6 + [ci] * 8 + [cl] * 4 + [cf, vp, vp, vp]
+    lib.ossa_qk_norm_rope_fwd.restype = ci
+    lib.ossa_qk_norm_rope_bwd_workspace_size.argtypes = [ci]
+    lib.ossa_qk_norm_rope_bwd_workspace_size.restype = sz
+    lib.ossa_qk_norm_rope_bwd.argtypes = [vp] * 6 + [ci] * 8 + [cl] * 4 + [cf] + [vp] * 7 + [sz, vp]
+    lib.ossa_qk_norm_rope_bwd.restype = ci
+    lib.ossa_top_logit_distill_workspace_size.argtypes = [cl, ci]
+    lib.ossa_top_logit_distill_workspace_size.restype = sz
+    lib.ossa_top_logit_distill_fwd.argtypes = [vp, ci, ci, ci, ci, cl, cl, vp, vp, ci, ci, cf, vp, ci, vp, vp, vp, vp,
+                                               sz, vp]
+    lib.ossa_top_logit_distill_fwd.restype = ci
+    lib.ossa_top_logit_distill_bwd.argtypes = [vp, ci, ci, ci, ci, cl, cl, vp, ci, ci, cf, ci, vp, ci, ci, vp, vp, sz,
+                                               vp]
+    lib.ossa_top_logit_distill_bwd.restype = ci
 
 
 def lib() -> ctypes.CDLL:
@@ -156,6 +186,26 @@ def dtype_code(t: torch.Tensor) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
+def on_device(device: torch.device):
+    """torch.cuda.device(device), without its cost where the device is current already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _here
+    return torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -276,6 +276,304 @@ int ossa_topk_attention_fwd(const void* q, const void* k, const void* v, const v
                                         0, out, stream);
 }
 
+// The checks that the modified gather and its backward share.
+static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, int idx_is_64, float scale,
+                          int q_start, float softcap, const int32_t* segments) {
+    int st = check_heads(B, H, Hkv, Nk);
+    if (st) return st;
+    if ((st = check_rows(Nq, Nk, q_start))) return st;
+    if (!valid_dtype(dtype)) return fail(OSSA_ERR_INVALID, "bad dtype %d", dtype);
+    if (D != 16 && D != 32 && D != 64 && D != 128 && D != 256)
+        return fail(OSSA_ERR_UNSUPPORTED, "head_dim D=%d not in {16,32,64,128,256}", D);
+    if (K < 0) return fail(OSSA_ERR_INVALID, "bad K=%d", K);
+    if (idx_is_64 != 0 && idx_is_64 != 1) return fail(OSSA_ERR_INVALID, "idx_is_64 must be 0 or 1");
+    if (!isfinite(scale)) return fail(OSSA_ERR_INVALID, "scale must be finite");
+    if (!isfinite(softcap) || softcap < 0.f) return fail(OSSA_ERR_INVALID, "softcap must be finite and >= 0");
+    if (segments && (long long)q_start + Nq > Nk)
+        return fail(OSSA_ERR_INVALID, "segments need every query position below Nk=%d (rows end at %lld)", Nk,
+                    (long long)q_start + Nq);
+    if ((long long)B * Hkv > 65535) return fail(OSSA_ERR_UNSUPPORTED, "B * Hkv = %lld > 65535", (long long)B * Hkv);
+    return OSSA_OK;
+}
+
+static ossa::ScoreMods make_mods(float scale, float softcap, const float* slopes, const int32_t* segments,
+                                 const int32_t* prefix_len, float* lse2) {
+    return ossa::ScoreMods{scale, scale * 1.4426950408889634f, softcap, softcap > 0.f ? 1.f / softcap : 0.f,
+                           softcap > 0.f || slopes ? 1 : 0, slopes, segments, prefix_len, lse2};
+}
+
+int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64,
+                                int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale, int causal,
+                                int q_start, float softcap, const float* slopes, const int32_t* segments,
+                                const int32_t* prefix_len, void* out, float* lse2, ossa_stream_t stream) {
+    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
+    if (st) return st;
+    if ((long long)B * H * Nq == 0) return OSSA_OK;
+    if (Nk == 0) return fail(OSSA_ERR_INVALID, "query rows need at least one key (Nk=0)");
+    if (!q || !k || !v || !out || (K > 0 && !indices)) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (K > 0 && !aligned16(indices)))
+        return fail(OSSA_ERR_INVALID, "q, k, v, indices and out must be 16-byte aligned");
+    ossa::GatherArgs a{q, k, v, indices, out, idx_is_64, dtype, B, H, Hkv, Nk, D, K, scale, causal ? 1 : 0};
+    a.Nq = Nq;
+    a.q0 = q_start;
+    a.mods = make_mods(scale, softcap, slopes, segments, prefix_len, lse2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (softcap == 0.f && !slopes && !segments && !prefix_len && !lse2)
+        return cuda_status(ossa::launch_gather_attn(a, s), "topk attention launch");
+    return cuda_status(ossa::launch_gather_attn_mods(a, s), "modified topk attention launch");
+}
+
+size_t ossa_topk_attention_bwd_workspace_size(int B, int H, int Hkv, int Nq, int Nk, int D, int K, int want_dslopes) {
+    if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Nq < 0 || Nk < 0 || D <= 0 || K < 0) return 0;
+    return ossa::gather_bwd_workspace_bytes(B, H, Hkv, Nq, Nk, D, K, want_dslopes != 0);
+}
+
+int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64, int dtype,
+                            int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale, int causal, int q_start,
+                            float softcap, const float* slopes, const int32_t* segments, const int32_t* prefix_len,
+                            const void* out, const float* lse2, const void* dout, void* dq, void* dk, void* dv,
+                            float* dslopes, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
+    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
+    if (st) return st;
+    if (dslopes && !slopes) return fail(OSSA_ERR_INVALID, "dslopes without slopes");
+    if ((long long)(H / Hkv) * Nq * K > (1ll << 30))
+        return fail(OSSA_ERR_UNSUPPORTED, "(H / Hkv) * Nq * K = %lld > 2^30 listed keys per kv head",
+                    (long long)(H / Hkv) * Nq * K);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const size_t es = dtype == OSSA_F32 ? 4 : 2;
+    const size_t qn = (size_t)B * H * Nq * D * es, kn = (size_t)B * Hkv * Nk * D * es;
+    if ((qn && !dq) || (kn && (!dk || !dv))) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (qn == 0 || K == 0) {  // nothing listed: every gradient is zero
+        if (qn && (st = cuda_status(cudaMemsetAsync(dq, 0, qn, s), "gradient reset"))) return st;
+        if (kn && (st = cuda_status(cudaMemsetAsync(dk, 0, kn, s), "gradient reset"))) return st;
+        if (kn && (st = cuda_status(cudaMemsetAsync(dv, 0, kn, s), "gradient reset"))) return st;
+        if (dslopes && (st = cuda_status(cudaMemsetAsync(dslopes, 0, (size_t)H * 4, s), "gradient reset"))) return st;
+        return OSSA_OK;
+    }
+    if (Nk == 0) return fail(OSSA_ERR_INVALID, "query rows need at least one key (Nk=0)");
+    if (!q || !k || !v || !out || !indices || !lse2 || !dout) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(indices) || !aligned16(dout) ||
+        !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+        return fail(OSSA_ERR_INVALID, "q, k, v, indices, out, dout, dq, dk and dv must be 16-byte aligned");
+    const size_t need = ossa::gather_bwd_workspace_bytes(B, H, Hkv, Nq, Nk, D, K, dslopes != nullptr);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+        return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    ossa::GatherBwdArgs a{};
+    a.f = ossa::GatherArgs{q, k, v, indices, const_cast<void*>(out), idx_is_64, dtype, B, H, Hkv, Nk, D, K, scale,
+                           causal ? 1 : 0};
+    a.f.Nq = Nq;
+    a.f.q0 = q_start;
+    a.f.mods = make_mods(scale, softcap, slopes, segments, prefix_len, const_cast<float*>(lse2));
+    a.dout = dout;
+    a.dq = dq;
+    a.dk = dk;
+    a.dv = dv;
+    a.dslopes = dslopes;
+    a.ws = workspace;
+    return cuda_status(ossa::launch_gather_attn_bwd(a, s), "topk attention backward launch");
+}
+
+// The checks that the head norm's forward and backward share.
+static int check_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* cos, const void* sin,
+                           int dtype, int w_dtype, int B, int N, int Hq, int Hk, int D, long long q_sb, long long q_sn,
+                           long long k_sb, long long k_sn, float eps) {
+    if (!valid_dtype(dtype)) return fail(OSSA_ERR_INVALID, "bad dtype %d", dtype);
+    if (!valid_dtype(w_dtype)) return fail(OSSA_ERR_INVALID, "bad weight dtype %d", w_dtype);
+    if (B < 0 || N < 0 || Hq <= 0 || Hk < 0 || D <= 0 || D % 8 != 0)
+        return fail(OSSA_ERR_INVALID, "bad shape B=%d N=%d heads=%d,%d D=%d (D must be a multiple of 8)", B, N, Hq, Hk, D);
+    if (D > 512) return fail(OSSA_ERR_UNSUPPORTED, "head_dim D=%d > 512", D);
+    if ((long long)B * N > (1ll << 30) || Hq > (1 << 16) || Hk > (1 << 16))
+        return fail(OSSA_ERR_UNSUPPORTED, "shape too large B=%d N=%d heads=%d,%d", B, N, Hq, Hk);
+    if (!(eps >= 0.f) || !isfinite(eps)) return fail(OSSA_ERR_INVALID, "eps must be finite and >= 0");
+    if ((!cos) != (!sin)) return fail(OSSA_ERR_INVALID, "pass both cos and sin, or neither");
+    const int unit = dtype == OSSA_F32 ? 4 : 8;  // elements of 16 bytes
+    if (q_sb % unit || q_sn % unit || (Hk && (k_sb % unit || k_sn % unit)))
+        return fail(OSSA_ERR_INVALID, "row strides must be multiples of 16 bytes");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(cos) || !aligned16(sin))
+        return fail(OSSA_ERR_INVALID, "q, k, cos and sin must be 16-byte aligned");
+    return OSSA_OK;
+}
+
+int ossa_qk_norm_rope_fwd(const void* q, const void* k, const void* wq, const void* wk, const void* cos,
+                          const void* sin, int cs_batched, int dtype, int w_dtype, int B, int N, int Hq, int Hk, int D,
+                          long long q_sb, long long q_sn, long long k_sb, long long k_sn, float eps, void* q_out,
+                          void* k_out, ossa_stream_t stream) {
+    int st = check_norm_rope(q, k, wq, wk, cos, sin, dtype, w_dtype, B, N, Hq, Hk, D, q_sb, q_sn, k_sb, k_sn, eps);
+    if (st) return st;
+    if ((long long)B * N == 0) return OSSA_OK;
+    if (!q || !q_out || (Hk && (!k || !k_out))) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned16(q_out) || !aligned16(k_out)) return fail(OSSA_ERR_INVALID, "outputs must be 16-byte aligned");
+    ossa::NormRopeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.q_sb = q_sb;
+    a.q_sn = q_sn;
+    a.k_sb = k_sb;
+    a.k_sn = k_sn;
+    a.wq = wq;
+    a.wk = wk;
+    a.w_f32 = w_dtype == OSSA_F32;
+    a.cosv = cos;
+    a.sinv = sin;
+    a.cs_batched = cs_batched ? 1 : 0;
+    a.dtype = dtype;
+    a.B = B;
+    a.N = N;
+    a.Hq = Hq;
+    a.Hk = Hk;
+    a.D = D;
+    a.eps = eps;
+    a.oq = q_out;
+    a.ok = k_out;
+    return cuda_status(ossa::launch_norm_rope_fwd(a, static_cast<cudaStream_t>(stream)), "head norm launch");
+}
+
+size_t ossa_qk_norm_rope_bwd_workspace_size(int D) { return D > 0 ? ossa::norm_rope_workspace_bytes(D) : 0; }
+
+int ossa_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const void* wk, const void* cos,
+                          const void* sin, int cs_batched, int dtype, int w_dtype, int B, int N, int Hq, int Hk, int D,
+                          long long q_sb, long long q_sn, long long k_sb, long long k_sn, float eps, const void* dq_out,
+                          const void* dk_out, void* dq, void* dk, void* dwq, void* dwk, void* workspace,
+                          size_t workspace_bytes, ossa_stream_t stream) {
+    int st = check_norm_rope(q, k, wq, wk, cos, sin, dtype, w_dtype, B, N, Hq, Hk, D, q_sb, q_sn, k_sb, k_sn, eps);
+    if (st) return st;
+    if ((dwq && !wq) || (dwk && !wk)) return fail(OSSA_ERR_INVALID, "a weight gradient without its weight");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if ((long long)B * N == 0) {
+        const size_t wn = (size_t)D * (w_dtype == OSSA_F32 ? 4 : 2);
+        if (dwq && (st = cuda_status(cudaMemsetAsync(dwq, 0, wn, s), "gradient reset"))) return st;
+        if (dwk && (st = cuda_status(cudaMemsetAsync(dwk, 0, wn, s), "gradient reset"))) return st;
+        return OSSA_OK;
+    }
+    if (!dq_out || !dq || (wq && !q) || (Hk && (!dk_out || !dk || (wk && !k))))
+        return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned16(dq_out) || !aligned16(dk_out) || !aligned16(dq) || !aligned16(dk))
+        return fail(OSSA_ERR_INVALID, "gradients must be 16-byte aligned");
+    const size_t need = ossa::norm_rope_workspace_bytes(D);
+    if ((wq || (Hk && wk)) && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    ossa::NormRopeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.q_sb = q_sb;
+    a.q_sn = q_sn;
+    a.k_sb = k_sb;
+    a.k_sn = k_sn;
+    a.wq = wq;
+    a.wk = Hk ? wk : nullptr;
+    a.w_f32 = w_dtype == OSSA_F32;
+    a.cosv = cos;
+    a.sinv = sin;
+    a.cs_batched = cs_batched ? 1 : 0;
+    a.dtype = dtype;
+    a.B = B;
+    a.N = N;
+    a.Hq = Hq;
+    a.Hk = Hk;
+    a.D = D;
+    a.eps = eps;
+    a.gq = dq_out;
+    a.gk = dk_out;
+    a.oq = dq;
+    a.ok = dk;
+    a.dwq = dwq;
+    a.dwk = Hk ? dwk : nullptr;
+    a.part = static_cast<float*>(workspace);
+    return cuda_status(ossa::launch_norm_rope_bwd(a, s), "head norm backward launch");
+}
+
+// The checks that the top-logit distillation's forward and backward share.
+static int check_logit_distill(const void* logits, int dtype, int outer, int inner, int V, const void* ids,
+                               int ids_are_64, int K, float temperature, void* workspace, size_t workspace_bytes) {
+    if (!valid_dtype(dtype)) return fail(OSSA_ERR_INVALID, "bad dtype %d", dtype);
+    if (outer < 0 || inner < 0 || V <= 0 || K <= 0)
+        return fail(OSSA_ERR_INVALID, "bad shape rows=%dx%d V=%d K=%d", outer, inner, V, K);
+    if (K > 1024) return fail(OSSA_ERR_UNSUPPORTED, "K=%d > 1024 teacher entries per row", K);
+    if (V > (1 << 30) || (long long)outer * inner > (1ll << 30))
+        return fail(OSSA_ERR_UNSUPPORTED, "shape too large rows=%dx%d V=%d", outer, inner, V);
+    if (ids_are_64 != 0 && ids_are_64 != 1) return fail(OSSA_ERR_INVALID, "ids_are_64 must be 0 or 1");
+    if (!(temperature > 0.f) || !isfinite(temperature))
+        return fail(OSSA_ERR_INVALID, "temperature must be finite and > 0");
+    if ((long long)outer * inner == 0) return fail(OSSA_ERR_INVALID, "empty input (no rows)");
+    if (!logits || !ids) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    const uintptr_t es = dtype == OSSA_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(logits) % es) return fail(OSSA_ERR_INVALID, "logits are not aligned to their type");
+    const size_t need = ossa::logit_distill_workspace_bytes((long long)outer * inner, K);
+    if (!workspace || workspace_bytes < need || !aligned16(workspace))
+        return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    return OSSA_OK;
+}
+
+size_t ossa_top_logit_distill_workspace_size(long long rows, int K) {
+    if (rows < 0 || K <= 0) return 0;
+    return ossa::logit_distill_workspace_bytes(rows, K);
+}
+
+int ossa_top_logit_distill_fwd(const void* logits, int dtype, int outer, int inner, int V, long long stride_outer,
+                               long long stride_inner, const float* teacher, const void* ids, int ids_are_64, int K,
+                               float temperature, const float* row_weight, int mean, float* loss_rows, float* loss,
+                               void* dlogits, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
+    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature, workspace,
+                                 workspace_bytes);
+    if (st) return st;
+    if (!teacher || (!loss_rows && !loss)) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    ossa::LogitDistillArgs a{};
+    a.z = logits;
+    a.sb = stride_outer;
+    a.st = stride_inner;
+    a.dtype = dtype;
+    a.outer = outer;
+    a.inner = inner;
+    a.V = V;
+    a.teacher = teacher;
+    a.ids = ids;
+    a.ids_are_64 = ids_are_64;
+    a.K = K;
+    a.tau = temperature;
+    a.row_weight = row_weight;
+    a.mean = mean ? 1 : 0;
+    a.loss_rows = loss_rows;
+    a.loss = loss;
+    a.dz = dlogits;
+    a.ws = workspace;
+    return cuda_status(ossa::launch_logit_distill_fwd(a, static_cast<cudaStream_t>(stream)),
+                       "top-logit distillation launch");
+}
+
+int ossa_top_logit_distill_bwd(const void* logits, int dtype, int outer, int inner, int V, long long stride_outer,
+                               long long stride_inner, const void* ids, int ids_are_64, int K, float temperature,
+                               int mean, const float* grad, int grad_per_row, int skip_if_one, void* dlogits,
+                               const void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
+    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature,
+                                 const_cast<void*>(workspace), workspace_bytes);
+    if (st) return st;
+    if (!grad || !dlogits) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (skip_if_one && grad_per_row) return fail(OSSA_ERR_INVALID, "skip_if_one needs a single gradient value");
+    ossa::LogitDistillArgs a{};
+    a.z = logits;
+    a.sb = stride_outer;
+    a.st = stride_inner;
+    a.dtype = dtype;
+    a.outer = outer;
+    a.inner = inner;
+    a.V = V;
+    a.ids = ids;
+    a.ids_are_64 = ids_are_64;
+    a.K = K;
+    a.tau = temperature;
+    a.mean = mean ? 1 : 0;
+    a.grad = grad;
+    a.grad_per_row = grad_per_row ? 1 : 0;
+    a.skip_if_one = skip_if_one ? 1 : 0;
+    a.dz = dlogits;
+    a.ws = const_cast<void*>(workspace);
+    return cuda_status(ossa::launch_logit_distill_bwd(a, static_cast<cudaStream_t>(stream)),
+                       "top-logit distillation backward launch");
+}
+
 int ossa_router_status(const void* workspace, int* fallback_rows, int* status) {
     if (!workspace || !aligned16(workspace)) return fail(OSSA_ERR_INVALID, "bad workspace pointer");
     int h[2] = {0, 0};

@@ -1,0 +1,16 @@
+// Gathered top-K attention forward with score modifiers (score_mods.cuh), and the row statistic
+// that its backward pass reads.
+#include "gather_attn_kernels.cuh"
+
+namespace ossa {
+
+cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream) {
+    if (a.dtype == kF32) {
+        return a.idx_is_64 ? launch_typed<float, int64_t, true>(a, stream)
+                           : launch_typed<float, int32_t, true>(a, stream);
+    }
+    return a.idx_is_64 ? launch_typed<__nv_bfloat16, int64_t, true>(a, stream)
+                       : launch_typed<__nv_bfloat16, int32_t, true>(a, stream);
+}
+
+}  // namespace ossa

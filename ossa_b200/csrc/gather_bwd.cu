@@ -1,0 +1,516 @@
+// Backward pass of the gathered top-K attention.
+//
+// Per query row i with listed keys j (score_mods.cuh), row statistic L = log2 sum 2^s2:
+//   p_j = 2^(s2_j - L),  dP_j = dO_i . v_j,  Delta_i = sum_j p_j dP_j
+//   dS_j = p_j (dP_j - Delta_i),  dX_j = dS_j * d score / d (q.k)
+//   dq_i = sum_j dX_j k_j,  dk_j = sum_i dX_ij q_i,  dv_j = sum_i p_ij dO_i
+//   dslope_h = -sum dS_ij |i - j|
+// Nothing per (row, entry) is kept by the forward: both passes here recompute s2 and dP.
+//
+//  1. The index lists are turned round: for every (b, kv head) the rows that list a key,
+//     key by key, in a fixed order (a counting sort: units of (row chunk, head) count their
+//     entries per key, the counts are scanned, every unit then writes its rows).
+//  2. Row pass, one warp per row: dq_i, Delta_i and the row's share of dslope.
+//  3. Key pass, one warp per kTile consecutive entries of a turned list, which may begin and
+//     end inside a key's run: whole runs are stored, cut ones go to per-tile partial sums.
+//  4. Join: keys whose run is cut add their partial sums in tile order; keys that nobody
+//     lists get zeros.
+// No float atomics: repeated calls give the same bits.  (Two entries of one row with the same
+// key are alike, so the order in which the counting sort places them does not show.)
+//
+// Bound: L2-to-SM traffic.  Either pass reads two rows of D values per entry.
+#include <algorithm>
+#include <cstdint>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "mma_sync.cuh"
+#include "score_mods.cuh"
+
+namespace ossa {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kKeyRange = 8192;  // keys that one CTA of the counting sort covers (32 KB of counters)
+constexpr int kTile = 256;       // entries that a warp of the key pass takes
+constexpr int kMaxChunks = 16;   // row chunks of the counting sort per head
+constexpr int kMinChunkRows = 64;
+
+struct Shape {
+    int B, H, Hkv, G, Nq, N, D, K, q0, causal;
+    int chunks, chunk_rows, units;  // units = chunks * G per (b, kv head)
+    long long cap;                  // entries per (b, kv head) at most
+    long long tiles;                // key-pass tiles per (b, kv head) at most
+};
+
+Shape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
+    Shape s{};
+    s.B = B;
+    s.H = H;
+    s.Hkv = Hkv;
+    s.G = H / Hkv;
+    s.Nq = Nq;
+    s.N = N;
+    s.D = D;
+    s.K = K;
+    s.chunks = std::max(1, std::min(kMaxChunks, Nq / kMinChunkRows));
+    s.chunk_rows = (Nq + s.chunks - 1) / s.chunks;
+    s.units = s.chunks * s.G;
+    s.cap = (long long)s.G * Nq * K;
+    s.tiles = (s.cap + kTile - 1) / kTile;
+    return s;
+}
+
+struct Layout {
+    size_t counts, base, list, delta, part, slope_rows, total;
+};
+
+Layout make_layout(const Shape& s, bool dslopes) {
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t kv = (size_t)s.B * s.Hkv, rows = (size_t)s.B * s.H * s.Nq;
+    Layout l;
+    l.counts = 0;
+    l.base = l.counts + up(kv * s.units * s.N * 4);
+    l.list = l.base + up(kv * ((size_t)s.N + 1) * 4);
+    l.delta = l.list + up(kv * s.cap * 4);
+    l.part = l.delta + up(rows * 4);
+    l.slope_rows = l.part + up(kv * s.tiles * 4 * s.D * 4);
+    l.total = l.slope_rows + (dslopes ? up(rows * 4) : 0);
+    return l;
+}
+
+// ------------------------------------------------------------------ 1. turned lists
+
+// counts[kv][unit][key]: how often the unit's rows list the key and see it.
+template <typename IdxT>
+__global__ void __launch_bounds__(kThreads)
+count_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, int* __restrict__ counts) {
+    __shared__ int hist[kKeyRange];
+    const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
+    const int nk = min(kKeyRange, s.N - k0);
+    const int b = kv / s.Hkv, h = (kv - b * s.Hkv) * s.G + unit % s.G;
+    const int r0 = unit / s.G * s.chunk_rows, r1 = min(s.Nq, r0 + s.chunk_rows);
+    for (int t = threadIdx.x; t < nk; t += kThreads) hist[t] = 0;
+    __syncthreads();
+    const int lane = threadIdx.x & 31;
+    for (int il = r0 + (threadIdx.x >> 5); il < r1; il += kWarps) {
+        const int i = s.q0 + il;
+        const RowMods<true> rm(mods, b, h, s.N, i);
+        const IdxT* irow = idx + (((size_t)b * s.H + h) * s.Nq + il) * s.K;
+        for (int e = lane; e < s.K; e += 32) {
+            const long long j = (long long)irow[e];
+            if (j >= k0 && j < k0 + nk && rm.sees(j, i, s.causal)) atomicAdd(&hist[j - k0], 1);
+        }
+    }
+    __syncthreads();
+    int* out = counts + ((size_t)kv * s.units + unit) * s.N + k0;
+    for (int t = threadIdx.x; t < nk; t += kThreads) out[t] = hist[t];
+}
+
+// counts -> exclusive prefix over the units, and the key's total in base[kv][key].
+__global__ void __launch_bounds__(kThreads)
+unit_scan_kernel(const Shape s, int* __restrict__ counts, int* __restrict__ base) {
+    const int key = blockIdx.x * kThreads + threadIdx.x, kv = blockIdx.y;
+    if (key >= s.N) return;
+    int* c = counts + (size_t)kv * s.units * s.N + key;
+    int sum = 0;
+    for (int u = 0; u < s.units; ++u) {
+        const int x = c[(size_t)u * s.N];
+        c[(size_t)u * s.N] = sum;
+        sum += x;
+    }
+    base[(size_t)kv * (s.N + 1) + key] = sum;
+}
+
+// base[kv][0..N]: exclusive prefix of the totals over the keys.
+__global__ void __launch_bounds__(1024) key_scan_kernel(const Shape s, int* __restrict__ base) {
+    __shared__ int wsum[32];
+    __shared__ int carry;
+    int* p = base + (size_t)blockIdx.x * (s.N + 1);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) carry = 0;
+    __syncthreads();
+    for (int k0 = 0; k0 < s.N; k0 += 1024) {
+        const int k = k0 + threadIdx.x;
+        const int x = k < s.N ? p[k] : 0;
+        int y = x;  // inclusive over the warp
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(kFull, y, o);
+            if (lane >= o) y += t;
+        }
+        if (lane == 31) wsum[warp] = y;
+        __syncthreads();
+        if (warp == 0) {
+            int w = wsum[lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(kFull, w, o);
+                if (lane >= o) w += t;
+            }
+            wsum[lane] = w;
+        }
+        __syncthreads();
+        const int before = carry + (warp ? wsum[warp - 1] : 0) + y - x;
+        if (k < s.N) p[k] = before;
+        __syncthreads();
+        if (threadIdx.x == 1023) carry = before + x;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) p[s.N] = carry;
+}
+
+// list[kv][position] = g * Nq + il of the rows that list a key, key by key.  One warp walks
+// the unit's rows in order; the counters of its key range live in shared memory.
+template <typename IdxT>
+__global__ void __launch_bounds__(32)
+place_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, const int* __restrict__ counts,
+             const int* __restrict__ base, int* __restrict__ list) {
+    __shared__ int next[kKeyRange];
+    const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
+    const int nk = min(kKeyRange, s.N - k0);
+    const int g = unit % s.G;
+    const int b = kv / s.Hkv, h = (kv - b * s.Hkv) * s.G + g;
+    const int r0 = unit / s.G * s.chunk_rows, r1 = min(s.Nq, r0 + s.chunk_rows);
+    const int lane = threadIdx.x;
+    const int* c = counts + ((size_t)kv * s.units + unit) * s.N + k0;
+    const int* bs = base + (size_t)kv * (s.N + 1) + k0;
+    for (int t = lane; t < nk; t += 32) next[t] = c[t] + bs[t];
+    __syncwarp();
+    int* out = list + (size_t)kv * s.cap;
+    for (int il = r0; il < r1; ++il) {
+        const int i = s.q0 + il;
+        const RowMods<true> rm(mods, b, h, s.N, i);
+        const IdxT* irow = idx + (((size_t)b * s.H + h) * s.Nq + il) * s.K;
+        for (int e = lane; e < s.K; e += 32) {
+            const long long j = (long long)irow[e];
+            if (j >= k0 && j < k0 + nk && rm.sees(j, i, s.causal)) out[atomicAdd(&next[j - k0], 1)] = g * s.Nq + il;
+        }
+        __syncwarp();  // a row's places before the next row's
+    }
+}
+
+// ------------------------------------------------------------------ 2. row pass
+
+template <typename T, int D>
+struct RowLoad {
+    static constexpr int kPer = D >= 32 ? D / 32 : 1;  // values of a row that one lane owns
+    static constexpr int kActive = D / kPer;
+    static __device__ __forceinline__ void load(const T* row, int lane, float (&v)[kPer]) {
+        if (lane < kActive) {
+            VecLoad<T, kPer>::load(row + lane * kPer, v);
+        } else {
+#pragma unroll
+            for (int t = 0; t < kPer; ++t) v[t] = 0.f;
+        }
+    }
+    static __device__ __forceinline__ void store(T* row, int lane, const float (&v)[kPer]) {
+        if (lane < kActive) {
+#pragma unroll
+            for (int t = 0; t < kPer; ++t) store_from_f32(row + lane * kPer + t, v[t]);
+        }
+    }
+};
+
+template <typename T, int D, typename IdxT>
+__global__ void __launch_bounds__(kThreads)
+row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const IdxT* __restrict__ idx,
+                const T* __restrict__ out, const T* __restrict__ dout, const Shape s, const ScoreMods mods,
+                T* __restrict__ dq, float* __restrict__ delta, float* __restrict__ slope_rows) {
+    using R = RowLoad<T, D>;
+    const int lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (row >= (long long)s.B * s.H * s.Nq) return;  // warp-uniform
+    const int bh = (int)(row / s.Nq), il = (int)(row - (long long)bh * s.Nq);
+    const int b = bh / s.H, h = bh - b * s.H, i = s.q0 + il;
+    const size_t kv = (size_t)b * s.Hkv + h / s.G;
+    const T* kb = k + kv * s.N * D;
+    const T* vb = v + kv * s.N * D;
+    const RowMods<true> rm(mods, b, h, s.N, i);
+    const float lse2 = mods.lse2[row];
+    float qv[R::kPer], dv[R::kPer], acc[R::kPer];
+    R::load(q + row * D, lane, qv);
+    R::load(dout + row * D, lane, dv);
+    float d0 = 0.f;  // Delta from the stored output, for dq
+    {
+        float o[R::kPer];
+        R::load(out + row * D, lane, o);
+#pragma unroll
+        for (int t = 0; t < R::kPer; ++t) {
+            d0 = fmaf(o[t], dv[t], d0);
+            acc[t] = 0.f;
+        }
+        d0 = warp_sum(d0);
+    }
+    float a_pd = 0.f, a_f = 0.f, a_pdf = 0.f;  // sums of p dP, p far, p dP far
+    const IdxT* irow = idx + row * s.K;
+    for (int kc = 0; kc < s.K; kc += 32) {
+        const int kk = kc + lane;
+        const long long jl = kk < s.K ? (long long)irow[kk] : -1ll;
+        const int j = jl >= 0 && jl < s.N && rm.sees(jl, i, s.causal) ? (int)jl : -1;
+        if (!__any_sync(kFull, j >= 0)) continue;
+        float x[32], y[32];
+#pragma unroll
+        for (int m = 0; m < 32; ++m) {
+            const int jm = __shfl_sync(kFull, j, m);
+            float r[R::kPer];
+            x[m] = y[m] = 0.f;
+            if (jm >= 0) {  // warp-uniform
+                R::load(kb + (size_t)jm * D, lane, r);
+#pragma unroll
+                for (int t = 0; t < R::kPer; ++t) x[m] = fmaf(qv[t], r[t], x[m]);
+                R::load(vb + (size_t)jm * D, lane, r);
+#pragma unroll
+                for (int t = 0; t < R::kPer; ++t) y[m] = fmaf(dv[t], r[t], y[m]);
+            }
+        }
+        const float dot = transpose_reduce32(x, lane);
+        const float dp = transpose_reduce32(y, lane);
+        float p = 0.f, dx = 0.f;
+        if (j >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
+            const float far = fabsf((float)(i - j));
+            p = exp2f(mods.score2_grad(dot, rm.slope, far, dx) - lse2);
+            dx *= p * (dp - d0);
+            a_pd = fmaf(p, dp, a_pd);
+            a_f = fmaf(p, far, a_f);
+            a_pdf = fmaf(p * dp, far, a_pdf);
+        }
+#pragma unroll
+        for (int m = 0; m < 32; ++m) {
+            const int jm = __shfl_sync(kFull, j, m);
+            const float w = __shfl_sync(kFull, dx, m);
+            if (jm >= 0) {
+                float r[R::kPer];
+                R::load(kb + (size_t)jm * D, lane, r);
+#pragma unroll
+                for (int t = 0; t < R::kPer; ++t) acc[t] = fmaf(w, r[t], acc[t]);
+            }
+        }
+    }
+    R::store(dq + row * D, lane, acc);
+    a_pd = warp_sum(a_pd);
+    if (lane == 0) delta[row] = a_pd;
+    if (slope_rows) {
+        a_f = warp_sum(a_f);
+        a_pdf = warp_sum(a_pdf);
+        if (lane == 0) slope_rows[row] = a_pd * a_f - a_pdf;
+    }
+}
+
+// ------------------------------------------------------------------ 3. key pass
+
+// The key whose run holds position pos (base[key] <= pos < base[key + 1]).
+__device__ __forceinline__ int key_at(const int* __restrict__ base, int N, int pos) {
+    int lo = 0, hi = N;  // base[lo] <= pos < base[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(base + mid) <= pos) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads)
+key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ dout,
+                const Shape s, const ScoreMods mods, const int* __restrict__ base, const int* __restrict__ list,
+                const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
+    using R = RowLoad<T, D>;
+    const int lane = threadIdx.x & 31, kv = blockIdx.y;
+    const long long tile = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int* bs = base + (size_t)kv * (s.N + 1);
+    const int total = bs[s.N];
+    if (tile * kTile >= total) return;  // warp-uniform
+    const int t0 = (int)(tile * kTile), t1 = min(total, t0 + kTile);
+    const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
+    const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
+    const int* ls = list + (size_t)kv * s.cap;
+    int key = key_at(bs, s.N, t0);
+    for (int pos = t0; pos < t1; ++key) {
+        const int run0 = bs[key], run1 = bs[key + 1];
+        const int end = min(run1, t1);
+        if (end <= pos) continue;  // nobody lists this key
+        float kr[R::kPer], vr[R::kPer], ak[R::kPer], av[R::kPer];
+        R::load(k + ((size_t)kv * s.N + key) * D, lane, kr);
+        R::load(v + ((size_t)kv * s.N + key) * D, lane, vr);
+#pragma unroll
+        for (int t = 0; t < R::kPer; ++t) ak[t] = av[t] = 0.f;
+        for (; pos < end; pos += 32) {
+            const int n = min(32, end - pos);
+            const int r = lane < n ? ls[pos + lane] : -1;
+            float x[32], y[32];
+#pragma unroll
+            for (int m = 0; m < 32; ++m) {
+                const int rm = __shfl_sync(kFull, r, m);
+                x[m] = y[m] = 0.f;
+                if (m < n) {  // warp-uniform
+                    float f[R::kPer];
+                    R::load(q + (rows0 + rm) * D, lane, f);
+#pragma unroll
+                    for (int t = 0; t < R::kPer; ++t) x[m] = fmaf(f[t], kr[t], x[m]);
+                    R::load(dout + (rows0 + rm) * D, lane, f);
+#pragma unroll
+                    for (int t = 0; t < R::kPer; ++t) y[m] = fmaf(f[t], vr[t], y[m]);
+                }
+            }
+            const float dot = transpose_reduce32(x, lane);
+            const float dp = transpose_reduce32(y, lane);
+            float p = 0.f, dx = 0.f;
+            const float lse2 = r >= 0 ? mods.lse2[rows0 + r] : -INFINITY;
+            if (lse2 != -INFINITY) {
+                const int g = r / s.Nq, i = s.q0 + r - g * s.Nq;
+                const float slope = mods.slopes ? mods.slopes[h0 + g] : 0.f;
+                p = exp2f(mods.score2_grad(dot, slope, fabsf((float)(i - key)), dx) - lse2);
+                dx *= p * (dp - delta[rows0 + r]);
+            }
+#pragma unroll
+            for (int m = 0; m < 32; ++m) {
+                const int rm = __shfl_sync(kFull, r, m);
+                const float pm = __shfl_sync(kFull, p, m), xm = __shfl_sync(kFull, dx, m);
+                if (m < n) {
+                    float f[R::kPer];
+                    R::load(q + (rows0 + rm) * D, lane, f);
+#pragma unroll
+                    for (int t = 0; t < R::kPer; ++t) ak[t] = fmaf(xm, f[t], ak[t]);
+                    R::load(dout + (rows0 + rm) * D, lane, f);
+#pragma unroll
+                    for (int t = 0; t < R::kPer; ++t) av[t] = fmaf(pm, f[t], av[t]);
+                }
+            }
+        }
+        pos = end;
+        if (run0 >= t0 && run1 <= t1) {
+            R::store(dk + ((size_t)kv * s.N + key) * D, lane, ak);
+            R::store(dv + ((size_t)kv * s.N + key) * D, lane, av);
+        } else {  // slot 0: the run began before this tile; slot 1: it begins here and goes on
+            float* ps = part + (((size_t)kv * s.tiles + tile) * 2 + (run0 < t0 ? 0 : 1)) * 2 * D;
+            RowLoad<float, D>::store(ps, lane, ak);
+            RowLoad<float, D>::store(ps + D, lane, av);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ 4. join
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+join_kernel(const Shape s, const int* __restrict__ base, const float* __restrict__ part, T* __restrict__ dk,
+            T* __restrict__ dv) {
+    const int lane = threadIdx.x & 31, kv = blockIdx.y;
+    const int key = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    if (key >= s.N) return;
+    const int* bs = base + (size_t)kv * (s.N + 1);
+    const int run0 = bs[key], run1 = bs[key + 1];
+    const int first = run0 / kTile, last = run1 > run0 ? (run1 - 1) / kTile : first;
+    if (run1 > run0 && first == last) return;  // stored by the key pass
+    const float* ps = part + (size_t)kv * s.tiles * 4 * s.D;
+    T* ok = dk + ((size_t)kv * s.N + key) * s.D;
+    T* ov = dv + ((size_t)kv * s.N + key) * s.D;
+    for (int d = lane; d < 2 * s.D; d += 32) {
+        float t = 0.f;
+        if (run1 > run0) {
+            t = ps[((size_t)first * 2 + 1) * 2 * s.D + d];
+#pragma unroll 4
+            for (int i = first + 1; i <= last; ++i) t += ps[(size_t)i * 2 * 2 * s.D + d];
+        }
+        if (d < s.D) store_from_f32(ok + d, t);
+        else store_from_f32(ov + d - s.D, t);
+    }
+}
+
+// dslopes[h]: the rows' shares, each thread's in row order, then a fixed tree.
+__global__ void __launch_bounds__(1024) slope_join_kernel(const Shape s, const float* __restrict__ rows, float* dslopes) {
+    __shared__ double sums[32];
+    const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double t = 0.0;
+    for (int b = 0; b < s.B; ++b)
+        for (int i = threadIdx.x; i < s.Nq; i += 1024) t += rows[((size_t)b * s.H + h) * s.Nq + i];
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
+    if (lane == 0) sums[warp] = t;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double a = 0.0;
+        for (int i = 0; i < 32; ++i) a += sums[i];
+        dslopes[h] = (float)a;
+    }
+}
+
+cudaError_t launched() {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+template <typename T, typename IdxT>
+cudaError_t bwd_typed(const GatherBwdArgs& a, const Shape& s, const Layout& l, cudaStream_t stream) {
+    char* ws = static_cast<char*>(a.ws);
+    int* counts = reinterpret_cast<int*>(ws + l.counts);
+    int* base = reinterpret_cast<int*>(ws + l.base);
+    int* list = reinterpret_cast<int*>(ws + l.list);
+    float* delta = reinterpret_cast<float*>(ws + l.delta);
+    float* part = reinterpret_cast<float*>(ws + l.part);
+    float* slope_rows = a.dslopes ? reinterpret_cast<float*>(ws + l.slope_rows) : nullptr;
+    const T *q = static_cast<const T*>(a.f.q), *k = static_cast<const T*>(a.f.k), *v = static_cast<const T*>(a.f.v);
+    const T *out = static_cast<const T*>(a.f.out), *dout = static_cast<const T*>(a.dout);
+    T *dq = static_cast<T*>(a.dq), *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
+    const IdxT* idx = static_cast<const IdxT*>(a.f.idx);
+    const ScoreMods& m = a.f.mods;
+    const unsigned kvs = (unsigned)(s.B * s.Hkv);
+    const dim3 sort_grid((unsigned)s.units, kvs, (unsigned)((s.N + kKeyRange - 1) / kKeyRange));
+    cudaError_t e;
+    count_kernel<IdxT><<<sort_grid, kThreads, 0, stream>>>(idx, s, m, counts);
+    if ((e = launched()) != cudaSuccess) return e;
+    unit_scan_kernel<<<dim3((unsigned)((s.N + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, counts, base);
+    if ((e = launched()) != cudaSuccess) return e;
+    key_scan_kernel<<<kvs, 1024, 0, stream>>>(s, base);
+    if ((e = launched()) != cudaSuccess) return e;
+    place_kernel<IdxT><<<sort_grid, 32, 0, stream>>>(idx, s, m, counts, base, list);
+    if ((e = launched()) != cudaSuccess) return e;
+    const long long rows = (long long)s.B * s.H * s.Nq;
+    const unsigned row_grid = (unsigned)((rows + kWarps - 1) / kWarps);
+    const dim3 key_grid((unsigned)((s.tiles + kWarps - 1) / kWarps), kvs);
+    switch (s.D) {
+#define OSSA_BWD_CASE(DD)                                                                                             \
+    case DD:                                                                                                          \
+        row_pass_kernel<T, DD, IdxT><<<row_grid, kThreads, 0, stream>>>(q, k, v, idx, out, dout, s, m, dq, delta,     \
+                                                                        slope_rows);                                  \
+        if ((e = launched()) != cudaSuccess) return e;                                                                \
+        key_pass_kernel<T, DD><<<key_grid, kThreads, 0, stream>>>(q, k, v, dout, s, m, base, list, delta, dk, dv,     \
+                                                                  part);                                              \
+        break;
+        OSSA_BWD_CASE(16)
+        OSSA_BWD_CASE(32)
+        OSSA_BWD_CASE(64)
+        OSSA_BWD_CASE(128)
+        OSSA_BWD_CASE(256)
+#undef OSSA_BWD_CASE
+        default: return cudaErrorInvalidValue;
+    }
+    if ((e = launched()) != cudaSuccess) return e;
+    join_kernel<T><<<dim3((unsigned)((s.N + kWarps - 1) / kWarps), kvs), kThreads, 0, stream>>>(s, base, part, dk, dv);
+    if ((e = launched()) != cudaSuccess || !a.dslopes) return e;
+    slope_join_kernel<<<s.H, 1024, 0, stream>>>(s, slope_rows, a.dslopes);
+    return launched();
+}
+
+}  // namespace
+
+size_t gather_bwd_workspace_bytes(int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes) {
+    return make_layout(make_shape(B, H, Hkv, Nq, N, D, K), dslopes).total;
+}
+
+cudaError_t launch_gather_attn_bwd(const GatherBwdArgs& a, cudaStream_t stream) {
+    Shape s = make_shape(a.f.B, a.f.H, a.f.Hkv, a.f.Nq, a.f.N, a.f.D, a.f.K);
+    s.q0 = a.f.q0;
+    s.causal = a.f.causal;
+    const Layout l = make_layout(s, a.dslopes != nullptr);
+    if (a.f.dtype == kF32)
+        return a.f.idx_is_64 ? bwd_typed<float, int64_t>(a, s, l, stream) : bwd_typed<float, int32_t>(a, s, l, stream);
+    return a.f.idx_is_64 ? bwd_typed<__nv_bfloat16, int64_t>(a, s, l, stream)
+                         : bwd_typed<__nv_bfloat16, int32_t>(a, s, l, stream);
+}
+
+}  // namespace ossa

@@ -25,6 +25,40 @@ int device_sm_count();
 bool make_row_map_16(CUtensorMap* map, const void* base, bool bf16, unsigned long long rows, int cols,
                      int box_rows);
 
+// Modifiers of the gathered attention's scores (score_mods.cuh); all zero: none.
+struct ScoreMods {
+    float scale, scale_log2;    // of q . k; times log2(e)
+    float cap, inv_cap;         // cap <= 0: no cap
+    int shaped;                 // a cap or slopes
+    const float* slopes;        // (H,) or nullptr
+    const int32_t* segments;    // (B, N) or nullptr
+    const int32_t* prefix_len;  // (B,) or nullptr
+    float* lse2;                // (B*H*Nq,) log2 of the row's sum of 2^s2, -inf for an empty row; nullptr: not wanted
+#ifdef __CUDACC__
+    // Score in base 2 of a key at distance far from dot = q . k.  Scores that only masks modify are
+    // the plain kernels' product, so that their results are too.
+    __device__ __forceinline__ float score2(float dot, float slope, float far) const {
+        if (!shaped) return dot * scale_log2;
+        const float x = dot * scale;
+        const float s = cap > 0.f ? cap * tanhf(x * inv_cap) : x;
+        return fmaf(-slope, far, s) * 1.4426950408889634f;
+    }
+    // The same, and d score / d dot in dx.
+    __device__ __forceinline__ float score2_grad(float dot, float slope, float far, float& dx) const {
+        dx = scale;
+        if (!shaped) return dot * scale_log2;
+        const float x = dot * scale;
+        float s = x;
+        if (cap > 0.f) {
+            const float t = tanhf(x * inv_cap);
+            s = cap * t;
+            dx = scale * (1.f - t * t);
+        }
+        return fmaf(-slope, far, s) * 1.4426950408889634f;
+    }
+#endif
+};
+
 struct GatherArgs {
     const void* q;
     const void* k;
@@ -38,8 +72,67 @@ struct GatherArgs {
     int causal;
     int Nq = 0;  // query rows per (b, h); 0 means N (queries are the keys' positions)
     int q0 = 0;  // position of query row 0 in the key sequence
+    ScoreMods mods = {};  // read by launch_gather_attn_mods only
 };
 cudaError_t launch_gather_attn(const GatherArgs& a, cudaStream_t stream);
+// The same attention under a.mods (a.scale is not read: a.mods.scale is).
+cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream);
+
+// Gradients of launch_gather_attn_mods (gather_bwd.cu).
+struct GatherBwdArgs {
+    GatherArgs f;        // the forward's arguments; f.out: its output, f.mods.lse2: its row statistic
+    const void* dout;    // (B, H, Nq, D)
+    void *dq, *dk, *dv;  // like q, k, v
+    float* dslopes;      // (H,) or nullptr
+    void* ws;            // gather_bwd_workspace_bytes
+};
+size_t gather_bwd_workspace_bytes(int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes);
+cudaError_t launch_gather_attn_bwd(const GatherBwdArgs& a, cudaStream_t stream);
+
+// Head norms with rotation and head transpose for queries and keys (norm_rope.cu).
+struct NormRopeArgs {
+    const void *q, *k;                 // rows (b, n): q + b * q_sb + n * q_sn, Hq * D values; k alike
+    long long q_sb, q_sn, k_sb, k_sn;  // in elements
+    const void *wq, *wk;               // (D,) or nullptr: no norm
+    int w_f32;                         // the weights (and their gradients) are fp32, else bf16
+    const void *cosv, *sinv;           // (1 or B, N, D) or nullptr: no rotation
+    int cs_batched;
+    int dtype;
+    int B, N, Hq, Hk, D;               // Hk = 0: queries alone
+    float eps;
+    const void *gq, *gk;               // backward: gradients of the outputs, (B, Hx, N, D)
+    void *oq, *ok;                     // forward: outputs (B, Hx, N, D); backward: dq, dk (B, N, Hx, D)
+    void *dwq, *dwk;                   // backward: (D,) or nullptr
+    float* part;                       // backward: norm_rope_workspace_bytes(D)
+};
+size_t norm_rope_workspace_bytes(int D);
+cudaError_t launch_norm_rope_fwd(const NormRopeArgs& a, cudaStream_t stream);
+cudaError_t launch_norm_rope_bwd(const NormRopeArgs& a, cudaStream_t stream);
+
+// Distillation from a teacher's top logits (logit_distill.cu).
+struct LogitDistillArgs {
+    const void* z;     // row (o, i): z + o * sb + i * st, V values
+    long long sb, st;  // in elements
+    int dtype;
+    int outer, inner, V;
+    const float* teacher;  // (rows, K)
+    const void* ids;       // (rows, K) int32 or int64
+    int ids_are_64;
+    int K;
+    float tau;
+    const float* row_weight;  // (rows,) or nullptr: 1
+    int mean;
+    const float* grad;  // backward: incoming gradient, one value or one per row
+    int grad_per_row;
+    int skip_if_one;    // backward: leave dz as it is when the one gradient is 1
+    float* loss_rows;   // (rows,) or nullptr
+    float* loss;        // (1,) or nullptr
+    void* dz;           // (rows, V) contiguous or nullptr
+    void* ws;           // logit_distill_workspace_bytes; the backward reads what the forward left there
+};
+size_t logit_distill_workspace_bytes(long long rows, int K);
+cudaError_t launch_logit_distill_fwd(const LogitDistillArgs& a, cudaStream_t stream);
+cudaError_t launch_logit_distill_bwd(const LogitDistillArgs& a, cudaStream_t stream);
 
 // out[row][c] = fmaf-chain over d = 0..D-1 of x[row][d] * w[c][d], for c < R.
 struct ProjectArgs {

@@ -1,0 +1,519 @@
+// Distillation from a teacher's top logits: loss and gradient over the vocabulary.
+//
+// Per row, student logits z (V values), teacher logits t at K listed entries:
+//   p = softmax(t / tau) over the listed entries inside [0, V) (repeats count each time)
+//   loss = tau^2 sum_k p_k (log p_k - (z_k / tau - lse(z / tau)))
+//   dz_v = scale * tau * (softmax(z / tau)_v - sum of p_k listed at v)
+// scale = row weight (/ the rows' weight sum for the mean) * incoming gradient.  A row
+// without a listed entry weighs nothing; a row of weight 0 is not read, its loss and
+// gradient are 0 whatever it holds.
+//
+// Bound: HBM, z read once and dz written once.  A cluster of C CTAs holds one row in
+// registers (kNV 16-byte vectors a thread), so the row's maximum and sum and then the
+// gradient come from one read: the CTAs exchange (max, sum) pairs through distributed
+// shared memory.  Clusters walk the rows with a fixed stride.  Rows too long for that are
+// read twice (kNV = 0).  Exponents are taken as exp2((z - max) * log2(e) / tau), the
+// difference first, so that entries at the type's lowest value and rows of them stay finite.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cstdint>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace ossa {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kPrepThreads = 1024;
+constexpr int kPrepBlocks = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Workspace: [counter 16 B][weight sums of the prep CTAs, double][row weight, T][row loss, T]
+// [log p, T x K][p summed over equal entries, T x K]
+struct Layout {
+    size_t wsum, weight, loss, logp, ptot, total;
+};
+
+Layout layout(long long T, int K) {
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    Layout l;
+    l.wsum = 256;
+    l.weight = l.wsum + up(kPrepBlocks * sizeof(double));
+    l.loss = l.weight + up((size_t)T * 4);
+    l.logp = l.loss + up((size_t)T * 4);
+    l.ptot = l.logp + up((size_t)T * K * 4);
+    l.total = l.ptot + up((size_t)T * K * 4);
+    return l;
+}
+
+// The teacher's rows: log p and the p of each entry summed over its repeats, the row's
+// weight, and the CTA's share of the weight sum (rows in a fixed order).  A warp per row.
+template <typename IdT>
+__global__ void __launch_bounds__(kPrepThreads)
+distill_prep_kernel(const float* __restrict__ teacher, const IdT* __restrict__ ids, const float* __restrict__ row_weight,
+                    long long T, int V, int K, float inv_tau, unsigned* counter, double* __restrict__ wsum,
+                    float* __restrict__ weight, float* __restrict__ logp, float* __restrict__ ptot) {
+    __shared__ double s_sum[kPrepThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *counter = 0u;
+    double mine = 0.0;
+    for (long long r = (long long)blockIdx.x * (kPrepThreads / 32) + warp; r < T;
+         r += (long long)gridDim.x * (kPrepThreads / 32)) {
+        const float* tr = teacher + r * K;
+        const IdT* ir = ids + r * K;
+        const float w = row_weight ? row_weight[r] : 1.f;
+        float m = -INFINITY;
+        bool any = false;
+        for (int k = lane; k < K; k += 32) {
+            const long long id = (long long)ir[k];
+            if (id >= 0 && id < V) {
+                any = true;
+                m = fmaxf(m, tr[k] * inv_tau);
+            }
+        }
+        m = warp_max(m);
+        any = __any_sync(kFull, any);
+        const float m0 = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
+        for (int k = lane; k < K; k += 32) {
+            const long long id = (long long)ir[k];
+            if (id >= 0 && id < V) sum += expf(tr[k] * inv_tau - m0);
+        }
+        const float lse = m0 + logf(warp_sum(sum));
+        for (int k = lane; k < K; k += 32) {
+            const long long id = (long long)ir[k];
+            const bool ok = id >= 0 && id < V;
+            logp[r * K + k] = ok ? tr[k] * inv_tau - lse : -INFINITY;
+        }
+        __syncwarp();
+        // p of equal entries summed in list order (every repeat gets the same sum)
+        for (int k0 = 0; k0 < K; k0 += 32) {
+            const int k = k0 + lane;
+            const long long id = k < K ? (long long)ir[k] : -1;
+            float tot = 0.f;
+            for (int j0 = 0; j0 < K; j0 += 32) {
+                const bool in = j0 + lane < K;
+                const long long jd = in ? (long long)ir[j0 + lane] : -1;
+                const float pj = in ? expf(logp[r * K + j0 + lane]) : 0.f;
+                const int n = min(32, K - j0);
+                for (int i = 0; i < n; ++i) {
+                    const long long other = __shfl_sync(kFull, jd, i);
+                    const float po = __shfl_sync(kFull, pj, i);
+                    if (other == id) tot += po;
+                }
+            }
+            if (k < K) ptot[r * K + k] = tot;
+        }
+        const float we = any ? w : 0.f;
+        if (lane == 0) weight[r] = we;
+        mine += we;
+    }
+    if (lane == 0) s_sum[warp] = mine;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < kPrepThreads / 32; ++i) t += s_sum[i];
+        wsum[blockIdx.x] = t;
+    }
+}
+
+struct Rows {
+    const void* z;
+    long long sb, st;  // row r: z + (r / inner) * sb + (r % inner) * st
+    int inner;
+    long long T;
+    int V, K;
+    const void* ids;
+    const float* grad;  // nullptr: 1
+    int grad_step;      // 0: one value, 1: one per row
+    int skip_if_one;
+    int mean;
+    int prep_blocks;
+    float tau;
+    unsigned* counter;
+    const double* wsum;
+    const float *weight, *logp, *ptot;
+    float *loss_rows, *loss;  // nullptr: not wanted
+    void* dz;                 // (T, V) contiguous, nullptr: not wanted
+};
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+    static constexpr int n = 4;
+    static constexpr uint32_t neg = 0xff800000u;  // -inf
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x);
+        x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z);
+        x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+    static constexpr int n = 8;
+    static constexpr uint32_t neg = 0xff80ff80u;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+        unpack_bf16x2(v.x, x[0], x[1]);
+        unpack_bf16x2(v.y, x[2], x[3]);
+        unpack_bf16x2(v.z, x[4], x[5]);
+        unpack_bf16x2(v.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+        uint4 o;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * t], x[2 * t + 1]);
+            w[t] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        return o;
+    }
+};
+
+__device__ __forceinline__ uint4 load_stream(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// (max, sum of exp2((z - max) c)) of two parts of a row.
+__device__ __forceinline__ void join(float& m, float& l, float m2, float l2, float c) {
+    const float mn = fmaxf(m, m2);
+    l = l * exp2f((m - mn) * c) + l2 * exp2f((m2 - mn) * c);
+    m = mn;
+}
+
+template <typename T, typename IdT, int kNV>
+__global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kernel(const Rows a) {
+    using V8 = Vec<T>;
+    constexpr int E = V8::n;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long clusters = gridDim.x / C, me = blockIdx.x / C;
+    if (a.skip_if_one && a.grad && *a.grad == 1.f) return;  // the same for every CTA
+    __shared__ float s_m[kWarps], s_l[kWarps], s_part[kWarps];
+    __shared__ float2 s_pair[2];  // this CTA's (max, sum), by row parity
+    __shared__ float s_row[2];
+    __shared__ float s_unit;
+    __shared__ bool s_last;
+    const float c = kLog2e / a.tau;
+    if (tid == 0) {  // weight of one unit of row weight
+        double w = 0.0;
+        if (a.mean)
+            for (int i = 0; i < a.prep_blocks; ++i) w += a.wsum[i];
+        s_unit = a.mean ? (w != 0.0 ? (float)(1.0 / w) : 0.f) : 1.f;
+    }
+    __syncthreads();
+    const float unit = s_unit;
+    int parity = 0;
+    for (long long r = me; r < a.T; r += clusters) {
+        const float w = a.weight[r];
+        T* out = a.dz ? static_cast<T*>(a.dz) + (size_t)r * a.V : nullptr;
+        if (w == 0.f) {  // the cluster's CTAs agree
+            if (rank == 0 && tid == 0 && a.loss_rows) a.loss_rows[r] = 0.f;
+            if (out)
+                for (int v = rank * kThreads + tid; v < a.V; v += C * kThreads) store_from_f32(out + v, 0.f);
+            continue;
+        }
+        const T* z = static_cast<const T*>(a.z) + (size_t)((r / a.inner) * a.sb + (r % a.inner) * a.st);
+        // the row: `head` single values up to a 16-byte boundary, nb vectors, single values
+        const int head = min(a.V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
+        const int nb = (a.V - head) / E;
+        const int tail0 = head + nb * E;
+        const uint4* zv = reinterpret_cast<const uint4*>(z + head);
+        const int first = rank * kThreads + tid, stride = C * kThreads;
+        // the single values lie with rank 0: threads 0.. the head, threads 32.. the tail
+        int odd = -1;
+        if (rank == 0 && tid < head) odd = tid;
+        if (rank == 0 && tid >= 32 && tail0 + tid - 32 < a.V) odd = tail0 + tid - 32;
+        const float zo = odd >= 0 ? to_f32(z[odd]) : -INFINITY;
+        uint4 d[kNV > 0 ? kNV : 1];
+        float m = fmaxf(zo, -FLT_MAX), l = 0.f;
+        if constexpr (kNV > 0) {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) {
+                const int i = first + j * stride;
+                d[j] = i < nb ? load_stream(zv + i) : make_uint4(V8::neg, V8::neg, V8::neg, V8::neg);
+            }
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) {
+                float x[E];
+                V8::unpack(d[j], x);
+#pragma unroll
+                for (int t = 0; t < E; ++t) m = fmaxf(m, x[t]);
+            }
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) {
+                float x[E];
+                V8::unpack(d[j], x);
+#pragma unroll
+                for (int t = 0; t < E; ++t) l += exp2f((x[t] - m) * c);
+            }
+        } else {
+            for (int i = first; i < nb; i += stride) {
+                float x[E];
+                V8::unpack(zv[i], x);
+                float mn = m;
+#pragma unroll
+                for (int t = 0; t < E; ++t) mn = fmaxf(mn, x[t]);
+                l *= exp2f((m - mn) * c);
+                m = mn;
+#pragma unroll
+                for (int t = 0; t < E; ++t) l += exp2f((x[t] - m) * c);
+            }
+        }
+        if (odd >= 0) l += exp2f((zo - m) * c);
+#pragma unroll
+        for (int o = 16; o >= 1; o >>= 1) {
+            const float m2 = __shfl_xor_sync(kFull, m, o), l2 = __shfl_xor_sync(kFull, l, o);
+            join(m, l, m2, l2, c);
+        }
+        if (lane == 0) {
+            s_m[warp] = m;
+            s_l[warp] = l;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 1; i < kWarps; ++i) join(m, l, s_m[i], s_l[i], c);
+            s_pair[parity] = make_float2(m, l);
+        }
+        // one barrier a row: a pair is written again two rows on, when every CTA has
+        // passed the next row's barrier and so has read it
+        cluster.sync();
+        if (tid == 0) {
+            m = -FLT_MAX;
+            l = 0.f;
+            for (int i = 0; i < C; ++i) {  // rank order in every CTA: the same bits
+                const float2 p = *cluster.map_shared_rank(&s_pair[parity], i);
+                join(m, l, p.x, p.y, c);
+            }
+            s_row[0] = m;
+            s_row[1] = l;
+        }
+        __syncthreads();
+        m = s_row[0];
+        l = s_row[1];
+        parity ^= 1;
+        const float inv = 1.f / l;
+        const IdT* ids = static_cast<const IdT*>(a.ids) + r * a.K;
+        if (out) {
+            const float g = a.grad ? a.grad[r * a.grad_step] : 1.f;
+            const float scale = g * w * unit * a.tau;
+            const float qs = inv * scale;
+            const bool same_phase = ((reinterpret_cast<uintptr_t>(out + head)) & 15) == 0;
+            auto emit = [&](int i, const uint4& raw) {
+                float x[E];
+                V8::unpack(raw, x);
+#pragma unroll
+                for (int t = 0; t < E; ++t) x[t] = exp2f((x[t] - m) * c) * qs;
+                if (same_phase) {
+                    __stcs(reinterpret_cast<uint4*>(out + head) + i, V8::pack(x));
+                } else {
+#pragma unroll
+                    for (int t = 0; t < E; ++t) store_from_f32(out + head + (size_t)i * E + t, x[t]);
+                }
+            };
+            if constexpr (kNV > 0) {
+#pragma unroll
+                for (int j = 0; j < kNV; ++j) {
+                    const int i = first + j * stride;
+                    if (i < nb) emit(i, d[j]);
+                }
+            } else {
+                for (int i = first; i < nb; i += stride) emit(i, zv[i]);
+            }
+            if (odd >= 0) store_from_f32(out + odd, exp2f((zo - m) * c) * qs);
+            __syncthreads();  // the listed entries of this CTA's part are written over
+            for (int k = tid; k < a.K; k += kThreads) {
+                const long long id = (long long)ids[k];
+                if (id < 0 || id >= a.V) continue;
+                const int v = (int)id;
+                const int owner = v < head || v >= tail0 ? 0 : ((v - head) / E / kThreads) % C;
+                if (owner != rank) continue;
+                const float q = exp2f((to_f32(z[v]) - m) * c) * inv;
+                store_from_f32(out + v, (q - a.ptot[r * a.K + k]) * scale);
+            }
+        }
+        if (a.loss_rows && rank == 0) {
+            const float log_l = logf(l), inv_tau = 1.f / a.tau;
+            float t = 0.f;
+            for (int k = tid; k < a.K; k += kThreads) {
+                const float lp = a.logp[r * a.K + k];
+                const float p = expf(lp);
+                if (p > 0.f) {  // an entry outside the vocabulary has p = 0
+                    const float lq = (to_f32(z[(long long)ids[k]]) - m) * inv_tau - log_l;
+                    t += p * (lp - lq);
+                } else if (lp != lp) {
+                    t = lp;
+                }
+            }
+            t = warp_sum(t);
+            if (lane == 0) s_part[warp] = t;
+            __syncthreads();
+            if (tid == 0) {
+                float sum = 0.f;
+                for (int i = 0; i < kWarps; ++i) sum += s_part[i];
+                a.loss_rows[r] = sum * a.tau * a.tau;
+            }
+        }
+    }
+    cluster.sync();  // no CTA leaves while another may still read its pair
+    if (!a.loss) return;
+    // the CTA that ends last adds the rows' losses, in an order that is always the same
+    if (tid == 0) {
+        __threadfence();
+        s_last = atomicAdd(a.counter, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    __shared__ double s_sum[kWarps];
+    double t = 0.0;
+    for (long long r = tid; r < a.T; r += kThreads) {
+        const float w = __ldcg(a.weight + r);
+        if (w != 0.f) t += (double)w * (double)__ldcg(a.loss_rows + r);
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
+    if (lane == 0) s_sum[warp] = t;
+    __syncthreads();
+    if (tid == 0) {
+        double sum = 0.0;
+        for (int i = 0; i < kWarps; ++i) sum += s_sum[i];
+        *a.loss = (float)(sum * (double)unit);
+    }
+}
+
+// Cluster size and vectors per thread.  A row of `vecs` vectors wants the fewest CTAs that
+// hold it in at most 6 vectors a thread (two CTAs per SM then); few rows want more CTAs a
+// row, up to 8, while they leave SMs without work.
+void pick(long long T, long long vecs, int sms, int* C, int* nv) {
+    int c = 1;
+    while (c < 8 && vecs > (long long)c * kThreads * 6) c *= 2;
+    while (c < 8 && T * c * 2 <= 2 * sms && vecs > (long long)c * kThreads) c *= 2;
+    const long long per = (vecs + (long long)c * kThreads - 1) / ((long long)c * kThreads);
+    *C = c;
+    *nv = per <= 16 ? (int)std::max<long long>(per, 1) : 0;
+}
+
+template <typename T, typename IdT, int kNV>
+cudaError_t launch_nv(const Rows& a, int C, int sms, cudaStream_t stream) {
+    auto kern = distill_rows_kernel<T, IdT, kNV>;
+    const long long resident = (long long)sms * (kNV <= 6 ? 2 : 1) / C;
+    const long long clusters = std::min<long long>(a.T, std::max<long long>(resident, 1));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(clusters * C));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)C;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+template <typename T, typename IdT>
+cudaError_t launch_rows(const Rows& a, cudaStream_t stream) {
+    const int sms = device_sm_count();
+    int C = 1, nv = 0;
+    pick(a.T, (a.V + Vec<T>::n - 1) / Vec<T>::n, sms, &C, &nv);
+    switch (nv) {
+        case 1: return launch_nv<T, IdT, 1>(a, C, sms, stream);
+        case 2: return launch_nv<T, IdT, 2>(a, C, sms, stream);
+        case 3: return launch_nv<T, IdT, 3>(a, C, sms, stream);
+        case 4: return launch_nv<T, IdT, 4>(a, C, sms, stream);
+        case 5: return launch_nv<T, IdT, 5>(a, C, sms, stream);
+        case 6: return launch_nv<T, IdT, 6>(a, C, sms, stream);
+        case 7: case 8: return launch_nv<T, IdT, 8>(a, C, sms, stream);
+        case 9: case 10: return launch_nv<T, IdT, 10>(a, C, sms, stream);
+        case 0: return launch_nv<T, IdT, 0>(a, C, sms, stream);
+        default: return launch_nv<T, IdT, 16>(a, C, sms, stream);
+    }
+}
+
+Rows make_rows(const LogitDistillArgs& a) {
+    const Layout l = layout((long long)a.outer * a.inner, a.K);
+    char* ws = static_cast<char*>(a.ws);
+    Rows r{};
+    r.z = a.z;
+    r.sb = a.sb;
+    r.st = a.st;
+    r.inner = a.inner;
+    r.T = (long long)a.outer * a.inner;
+    r.V = a.V;
+    r.K = a.K;
+    r.ids = a.ids;
+    r.mean = a.mean;
+    r.prep_blocks = (int)std::min<long long>(kPrepBlocks, (r.T + kPrepThreads / 32 - 1) / (kPrepThreads / 32));
+    r.tau = a.tau;
+    r.counter = reinterpret_cast<unsigned*>(ws);
+    r.wsum = reinterpret_cast<const double*>(ws + l.wsum);
+    r.weight = reinterpret_cast<const float*>(ws + l.weight);
+    r.logp = reinterpret_cast<const float*>(ws + l.logp);
+    r.ptot = reinterpret_cast<const float*>(ws + l.ptot);
+    r.loss_rows = a.loss_rows ? a.loss_rows : reinterpret_cast<float*>(ws + l.loss);
+    r.loss = a.loss;
+    r.dz = a.dz;
+    return r;
+}
+
+cudaError_t launch_by_type(const LogitDistillArgs& a, const Rows& r, cudaStream_t stream) {
+    if (a.dtype == kF32)
+        return a.ids_are_64 ? launch_rows<float, int64_t>(r, stream) : launch_rows<float, int32_t>(r, stream);
+    return a.ids_are_64 ? launch_rows<__nv_bfloat16, int64_t>(r, stream)
+                        : launch_rows<__nv_bfloat16, int32_t>(r, stream);
+}
+
+}  // namespace
+
+size_t logit_distill_workspace_bytes(long long T, int K) { return layout(T, K).total; }
+
+cudaError_t launch_logit_distill_fwd(const LogitDistillArgs& a, cudaStream_t stream) {
+    Rows r = make_rows(a);
+    double* wsum = const_cast<double*>(r.wsum);
+    float *weight = const_cast<float*>(r.weight), *logp = const_cast<float*>(r.logp), *ptot = const_cast<float*>(r.ptot);
+    const float inv_tau = 1.f / a.tau;
+    if (a.ids_are_64)
+        distill_prep_kernel<int64_t><<<r.prep_blocks, kPrepThreads, 0, stream>>>(
+            a.teacher, static_cast<const int64_t*>(a.ids), a.row_weight, r.T, a.V, a.K, inv_tau, r.counter, wsum, weight,
+            logp, ptot);
+    else
+        distill_prep_kernel<int32_t><<<r.prep_blocks, kPrepThreads, 0, stream>>>(
+            a.teacher, static_cast<const int32_t*>(a.ids), a.row_weight, r.T, a.V, a.K, inv_tau, r.counter, wsum, weight,
+            logp, ptot);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    note_launch();
+    return launch_by_type(a, r, stream);
+}
+
+cudaError_t launch_logit_distill_bwd(const LogitDistillArgs& a, cudaStream_t stream) {
+    Rows r = make_rows(a);
+    r.grad = a.grad;
+    r.grad_step = a.grad_per_row;
+    r.skip_if_one = a.skip_if_one;
+    r.loss_rows = nullptr;
+    r.loss = nullptr;
+    return launch_by_type(a, r, stream);
+}
+
+}  // namespace ossa

@@ -1,0 +1,45 @@
+// Modifiers of the gathered attention's scores, shared by its forward and backward kernels.
+//
+// With x = (q_i . k_j) * scale the score in base 2 is
+//   s2 = (cap tanh(x / cap) - slope_h |i - j|) * log2(e)     (no cap: x itself)
+// and key j is seen by the query at position i of batch element b when
+//   (not causal, or j <= i, or j < prefix_len[b])  and  segments[b][j] == segments[b][i].
+#pragma once
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace ossa {
+
+constexpr float kLog2E = 1.4426950408889634f;
+
+// What one query row needs of the modifiers (kMods = false: nothing but the causal rule).
+template <bool kMods>
+struct RowMods {
+    __device__ __forceinline__ RowMods(const ScoreMods&, int, int, int, int) {}
+    __device__ __forceinline__ bool sees(long long j, int i, int causal) const { return !causal || j <= i; }
+    __device__ __forceinline__ float score2(float x, int, int) const { return x; }
+};
+
+template <>
+struct RowMods<true> {
+    const int* seg;  // of batch element b, nullptr: one document
+    int seg_i, prefix;
+    float slope;
+    const ScoreMods& m;
+    __device__ __forceinline__ RowMods(const ScoreMods& mods, int b, int h, int N, int i) : m(mods) {
+        seg = mods.segments ? mods.segments + (size_t)b * N : nullptr;
+        seg_i = seg ? __ldg(seg + i) : 0;
+        prefix = mods.prefix_len ? __ldg(mods.prefix_len + b) : 0;
+        slope = mods.slopes ? __ldg(mods.slopes + h) : 0.f;
+    }
+    // j in [0, N)
+    __device__ __forceinline__ bool sees(long long j, int i, int causal) const {
+        return (!causal || j <= i || j < prefix) && (!seg || __ldg(seg + j) == seg_i);
+    }
+    __device__ __forceinline__ float score2(float dot, int i, int j) const {
+        return m.score2(dot, slope, fabsf((float)(i - j)));
+    }
+};
+
+}  // namespace ossa

@@ -6,11 +6,15 @@ projection (B, N, Hx*D) as (B, Hx, N, D), applies Qwen2's
 contiguous rows.  ``rope_to_heads`` does that in one kernel pass, with the same
 rounding as the eager expression ``x*cos + rotate_half(x)*sin``; the result is
 bit-identical to it.  Additive: the reference runs the eager ops.
+
+``qk_norm_rope`` serves layers that norm every query and key head before the rotation:
+norm, rotation and head transpose of both tensors in one kernel pass.  Both functions are
+differentiable (one backward kernel, ``ossa_qk_norm_rope_bwd``).
 """
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -21,7 +25,14 @@ def rope_to_heads(x: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = N
                   sin: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x: (B, N, n_heads * D) or (B, N, n_heads, D); cos, sin: (B or 1, N, D)
     (Qwen2's position embeddings) or both None (layout only).  Returns the
-    contiguous (B, n_heads, N, D) tensor, rotated when cos/sin are given."""
+    contiguous (B, n_heads, N, D) tensor, rotated when cos/sin are given.
+    Differentiable in x (head dims up to 512), not in cos and sin."""
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _RopeToHeads.apply(x, n_heads, cos, sin)
+    return _rope_to_heads(x, n_heads, cos, sin)
+
+
+def _rope_to_heads(x, n_heads, cos, sin):
     if (cos is None) != (sin is None):
         raise ValueError("pass both cos and sin, or neither")
     B, N = x.shape[0], x.shape[1]
@@ -51,3 +62,183 @@ def rope_to_heads(x: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = N
                                            B, N, n_heads, D, out.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(st)
     return out
+
+
+class _RopeToHeads(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, n_heads, cos, sin):
+        out = _rope_to_heads(x.detach(), n_heads, cos, sin)
+        ctx.shape = x.shape
+        if cos is not None:
+            cos, sin = _tables(cos, sin, out.shape[0], out.shape[2], out.shape[3], out.dtype)
+        ctx.save_for_backward(cos, sin)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return _norm_rope_backward(None, None, None, None, *ctx.saved_tensors, 0.0, g, None)[0].view(ctx.shape), None, \
+            None, None
+
+
+def _tables(cos, sin, B, N, D, dtype):
+    """cos, sin as the kernels read them: contiguous (B or 1, N, D) of the rows' type."""
+    cos, sin = cos.detach().to(dtype), sin.detach().to(dtype)
+    if cos.dim() == 2:
+        cos, sin = cos.unsqueeze(0), sin.unsqueeze(0)
+    if cos.shape != sin.shape or cos.dim() != 3 or cos.shape[0] not in (1, B) or tuple(cos.shape[1:]) != (N, D):
+        raise ValueError(f"cos/sin of shapes {tuple(cos.shape)}, {tuple(sin.shape)} do not match (B or 1, {N}, {D})")
+    return cos.contiguous(), sin.contiguous()
+
+
+def _rows(x, heads, name):
+    """(x, B, N, D, batch stride, row stride): x as it is where each (b, n) row of its heads lies in
+    one piece on a 16-byte boundary, else a contiguous copy."""
+    if x.dim() == 3 and heads > 0 and x.shape[2] % heads == 0:
+        D = x.shape[2] // heads
+    elif x.dim() == 4 and x.shape[2] == heads:
+        D = x.shape[3]
+    else:
+        raise ValueError(f"{name} of shape {tuple(x.shape)} is not (B, N, {heads} heads x D) or (B, N, {heads}, D)")
+    B, N = x.shape[:2]
+    sb, sn = x.stride()[:2]
+    whole = x.stride(-1) == 1 and (x.dim() == 3 or heads == 1 or x.stride(2) == D)
+    sb, sn = (sb if B > 1 else 0), (sn if N > 1 else 0)
+    if not whole or sb * x.element_size() % 16 or sn * x.element_size() % 16 or x.data_ptr() % 16:
+        x = x.contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        sn, sb = heads * D, N * heads * D
+    return x, B, N, D, sb, sn
+
+
+def _weight_code(*ws):
+    for w in ws:
+        if w is not None:
+            return _lib.OSSA_F32 if w.dtype == torch.float32 else _lib.OSSA_BF16
+    return _lib.OSSA_F32
+
+
+def _norm_rope_backward(q, k, wq, wk, cos, sin, eps, gq, gk, want=(False, False)):
+    """Gradients (dq, dk, dwq, dwk) from those of the (B, Hx, N, D) outputs; dq, dk contiguous
+    (B, N, Hx, D).  q, k are read only where there is a weight."""
+    dev, dt = gq.device, gq.dtype
+    gq = gq.contiguous()
+    B, Hq, N, D = gq.shape
+    dq = torch.empty((B, N, Hq, D), dtype=dt, device=dev)
+    dk, Hk = None, 0
+    if gk is not None:
+        gk = gk.contiguous()
+        Hk = gk.shape[1]
+        dk = torch.empty((B, N, Hk, D), dtype=dt, device=dev)
+    dwq = torch.empty_like(wq) if want[0] else None
+    dwk = torch.empty_like(wk) if want[1] else None
+    qs = ks = (0, 0)
+    if q is not None:
+        q, _, _, _, *qs = _rows(q, Hq, "q")
+    if k is not None:
+        k, _, _, _, *ks = _rows(k, Hk, "k")
+    L = _lib.lib()
+    ws, ws_bytes = None, 0
+    if wq is not None or wk is not None:
+        ws_bytes = L.ossa_qk_norm_rope_bwd_workspace_size(D)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        st = L.ossa_qk_norm_rope_bwd(
+            _lib.ptr(q), _lib.ptr(k), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
+            1 if cos is not None and cos.shape[0] == B and B > 1 else 0, _lib.dtype_code(gq), _weight_code(wq, wk),
+            B, N, Hq, Hk, D, *qs, *ks, eps, gq.data_ptr(), _lib.ptr(gk), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dwq),
+            _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    _lib.check(st)
+    return dq, dk, dwq, dwk
+
+
+def _norm_rope_forward(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps):
+    q, B, N, D, *qs = _rows(q, n_heads, "q")
+    k, _, _, _, *ks = _rows(k, n_kv_heads, "k")
+    dev = q.device
+    q_out = torch.empty((B, n_heads, N, D), dtype=q.dtype, device=dev)
+    k_out = torch.empty((B, n_kv_heads, N, D), dtype=q.dtype, device=dev)
+    if B * N > 0:
+        with _lib.on_device(dev):
+            st = _lib.lib().ossa_qk_norm_rope_fwd(
+                q.data_ptr(), k.data_ptr(), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
+                1 if cos is not None and cos.shape[0] == B and B > 1 else 0, _lib.dtype_code(q), _weight_code(wq, wk),
+                B, N, n_heads, n_kv_heads, D, *qs, *ks, eps, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_ptr(dev))
+        _lib.check(st)
+    return q_out, k_out
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, n_heads, n_kv_heads, cos, sin, eps):
+        ctx.save_for_backward(q, k, wq, wk, cos, sin)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        return _norm_rope_forward(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, cos, sin = ctx.saved_tensors
+        if gq is None and gk is None:
+            return (None,) * 9
+        need = ctx.needs_input_grad
+        if gq is None or gk is None:  # one output has no gradient: the other tensor alone
+            one = 0 if gk is None else 1
+            x, w, g = (q, wq, gq) if one == 0 else (k, wk, gk)
+            dx, _, dw, _ = _norm_rope_backward(x, None, w, None, cos, sin, ctx.eps, g, None,
+                                               want=(need[2 + one] and w is not None, False))
+            dx = dx.view(x.shape)
+            return (dx, None, dw) + (None,) * 6 if one == 0 else (None, dx, None, dw) + (None,) * 5
+        dq, dk, dwq, dwk = _norm_rope_backward(q, k, wq, wk, cos, sin, ctx.eps, gq, gk,
+                                               want=(need[2] and wq is not None, need[3] and wk is not None))
+        return dq.view(q.shape), dk.view(k.shape), dwq, dwk, None, None, None, None, None
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, *,
+                 eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head, rotation and head transpose in one pass.
+
+    q: (B, N, n_heads * D) or (B, N, n_heads, D), k alike with n_kv_heads, float32 or
+    bfloat16; views whose (b, n) rows lie in one piece (slices of a joint projection) are read
+    where they are.  q_weight, k_weight: (D,) norm weights, None for no norm of that tensor;
+    cos, sin: (B or 1, N, D) or (N, D), cast to the rows' type, or both None for no rotation.
+    Returns the contiguous (B, n_heads, N, D) and (B, n_kv_heads, N, D) tensors
+    ``rope(x * rsqrt(mean(x**2) + eps) * weight)``, computed in fp32 and rounded once.  D is a
+    multiple of 8, at most 512.
+
+    Differentiable in q, k and the weights, once; not in cos and sin.  Gradients are the same
+    bits in every call."""
+    if (cos is None) != (sin is None):
+        raise ValueError("pass both cos and sin, or neither")
+    if q.dtype != k.dtype:
+        raise TypeError(f"q and k dtypes differ: {q.dtype}, {k.dtype}")
+    _lib.dtype_code(q)
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and >= 0, got {eps}")
+    if q.dim() not in (3, 4) or k.dim() not in (3, 4) or q.shape[:2] != k.shape[:2]:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} are not (B, N, heads x D) of one B and N")
+    D = q.shape[3] if q.dim() == 4 else q.shape[2] // max(n_heads, 1)
+    Dk = k.shape[3] if k.dim() == 4 else k.shape[2] // max(n_kv_heads, 1)
+    if n_heads <= 0 or n_kv_heads <= 0 or D != Dk or q.shape[2:].numel() != n_heads * D or \
+            k.shape[2:].numel() != n_kv_heads * D:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not hold {n_heads} and {n_kv_heads} heads of one D")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (tuple(w.shape) != (D,) or not w.is_floating_point()):
+            raise ValueError(f"{name} must be ({D},) floating point; got {tuple(w.shape)} {w.dtype}")
+    kinds = {w.dtype for w in (q_weight, k_weight) if w is not None}
+    if kinds and kinds not in ({torch.float32}, {torch.bfloat16}):  # one storage type for both weights
+        q_weight = None if q_weight is None else q_weight.float()
+        k_weight = None if k_weight is None else k_weight.float()
+    q_weight = None if q_weight is None else q_weight.contiguous()
+    k_weight = None if k_weight is None else k_weight.contiguous()
+    _lib.require_cuda(*[t for t in (q, k, q_weight, k_weight, cos, sin) if t is not None])
+    if cos is not None:
+        cos, sin = _tables(cos, sin, q.shape[0], q.shape[1], D, q.dtype)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, n_heads, n_kv_heads, cos, sin, eps)
+    return _norm_rope_forward(q, k, n_heads, n_kv_heads, q_weight, k_weight, cos, sin, eps)

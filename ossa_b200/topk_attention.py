@@ -12,13 +12,17 @@ are rejected.  Differences, all additive:
   padding of ossa_b200's selectors) is treated as masked.
 * ``block_m`` and ``use_triton`` are accepted for signature compatibility and
   ignored (there is no Triton path to select).
-* forward only: the output carries no autograd history.
+* (additive) score modifiers: ``softcap`` (a tanh cap), ``slopes`` (a bias that falls
+  with distance), ``segments`` (documents packed in one row) and ``prefix_len`` (keys
+  that every query may see).
+* (additive) gradients: where q, k, v or slopes require them, the output carries
+  autograd history (``ossa_topk_attention_bwd``); the forward's values are the same.
 """
 
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -59,8 +63,12 @@ def topk_attention(
     block_m: int = 32,
     use_triton: Optional[bool] = None,
     q_start: Optional[int] = None,
+    softcap: Optional[float] = None,
+    slopes: Optional[torch.Tensor] = None,
+    segments: Optional[torch.Tensor] = None,
+    prefix_len: Union[torch.Tensor, int, None] = None,
 ) -> torch.Tensor:
-    """Top-K sparse attention forward.
+    """Top-K sparse attention, forward and (by autograd) backward.
 
     q: (B, H, N, D); k, v: (B, Hkv, N, D); topk_indices: (B, H, N, K).
     Returns (B, H, N, D) in q's dtype: per query, softmax over the K listed keys
@@ -70,8 +78,25 @@ def topk_attention(
     ``q_start`` (additive, for sequence sharding): q and topk_indices then hold
     Nq query rows at positions q_start .. q_start + Nq - 1 of a sequence whose
     Nk keys k, v hold in full; row l is masked causally against q_start + l.
+
+    Score modifiers (additive), x the scaled score of a query at position i and key j:
+    ``softcap``: x becomes softcap * tanh(x / softcap).
+    ``slopes`` (H,): slopes[h] * abs(i - j) is subtracted after the cap.
+    ``segments`` (B, Nk) or (Nk,), int32 or int64 (compared as 32-bit values): a key is
+    seen only from its own segment; every query position must be below Nk.
+    ``prefix_len`` (B,) int32 or int64, or one int: keys j < prefix_len[b] are seen by
+    every query of batch element b, whatever the causal mask says of them.
+
+    Differentiable in q, k, v and slopes, once; indices, segments and prefix_len are not.
+    An index listed twice in a row counts twice.  The gradients are the same bits in every
+    call; they need (H / Hkv) * Nq * K <= 2**30.
     """
     del block_m, use_triton
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
+                                        (slopes is not None and slopes.requires_grad))
+    if grad or softcap is not None or slopes is not None or segments is not None or prefix_len is not None:
+        return _topk_attention_modified(q, k, v, topk_indices, causal, q_start, softcap, slopes, segments, prefix_len,
+                                        grad)
     if q_start is not None:
         return _topk_attention_rows(q, k, v, topk_indices, causal, int(q_start))
     B, H, Hkv, N, D, K = _check(q, k, v, topk_indices)
@@ -110,3 +135,97 @@ def _topk_attention_rows(q, k, v, topk_indices, causal, q_start):
             float(1.0 / math.sqrt(D)), 1 if causal else 0, q_start, out.data_ptr(), _lib.stream_ptr(dev))
     _lib.check(st)
     return out
+
+
+def _int32(name, t, shapes):
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{name} must be an int32 or int64 tensor, got {getattr(t, 'dtype', type(t).__name__)}")
+    if tuple(t.shape) not in shapes:
+        raise ValueError(f"{name} of shape {tuple(t.shape)} is not {' or '.join(map(str, shapes))}")
+    return t.to(torch.int32)
+
+
+def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, segments, prefix_len, grad):
+    q0 = 0 if q_start is None else int(q_start)
+    if q0 < 0:
+        raise ValueError(f"q_start must be >= 0, got {q0}")
+    B, H, Hkv, Nq, D, K = _check(q, k, v, idx, rows=q_start is not None)
+    Nk = k.shape[2]
+    cap = 0.0
+    if softcap is not None:
+        cap = float(softcap)
+        if not (0.0 < cap < math.inf):
+            raise ValueError(f"softcap must be positive and finite, got {softcap}")
+    if slopes is not None:
+        if tuple(slopes.shape) != (H,) or not slopes.is_floating_point():
+            raise ValueError(f"slopes must be ({H},) floating point; got {tuple(slopes.shape)} {slopes.dtype}")
+        slopes = slopes.float().contiguous()
+    if segments is not None:
+        segments = _int32("segments", segments, [(B, Nk), (Nk,)])
+        if q0 + Nq > Nk:
+            raise ValueError(f"segments need every query position below {Nk}; rows end at {q0 + Nq}")
+        segments = segments.expand(B, Nk).contiguous()
+    if prefix_len is not None:
+        if isinstance(prefix_len, int):
+            if prefix_len < 0:
+                raise ValueError(f"prefix_len must be >= 0, got {prefix_len}")
+            prefix_len = torch.full((B,), min(prefix_len, Nk), dtype=torch.int32, device=q.device)
+        prefix_len = _int32("prefix_len", prefix_len, [(B,)]).contiguous()
+    _lib.dtype_code(q)
+    _lib.require_cuda(*[t for t in (q, k, v, idx, slopes, segments, prefix_len) if t is not None])
+    if grad:
+        return _TopkAttention.apply(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
+    return _mod_forward(q.contiguous(), k.contiguous(), v.contiguous(), slopes, idx.contiguous(), segments, prefix_len,
+                        causal, q0, cap, None)
+
+
+def _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
+    """The arguments that the C forward and backward begin with."""
+    B, H, Nq, D = q.shape
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(), 1 if idx.dtype == torch.int64 else 0,
+            _lib.dtype_code(q), B, H, k.shape[1], Nq, k.shape[2], D, idx.shape[-1], 1.0 / math.sqrt(D),
+            1 if causal else 0, q0, cap, _lib.ptr(slopes), _lib.ptr(segments), _lib.ptr(prefix_len))
+
+
+def _mod_forward(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap, lse2):
+    out = torch.empty_like(q)
+    if out.numel() == 0:
+        return out
+    with _lib.on_device(q.device):
+        st = _lib.lib().ossa_topk_attention_mod_fwd(
+            *_mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap), out.data_ptr(), _lib.ptr(lse2),
+            _lib.stream_ptr(q.device))
+    _lib.check(st)
+    return out
+
+
+class _TopkAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
+        q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
+        lse2 = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        out = _mod_forward(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap, lse2)
+        ctx.save_for_backward(q, k, v, slopes, idx, segments, prefix_len, out, lse2)
+        ctx.rule = (causal, q0, cap)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, slopes, idx, segments, prefix_len, out, lse2 = ctx.saved_tensors
+        dev = q.device
+        dout = dout.to(q.dtype).contiguous()
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
+        L = _lib.lib()
+        B, H, Nq, D = q.shape
+        ws_bytes = L.ossa_topk_attention_bwd_workspace_size(B, H, k.shape[1], Nq, k.shape[2], D, idx.shape[-1],
+                                                            0 if dslopes is None else 1)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with _lib.on_device(dev):
+            st = L.ossa_topk_attention_bwd(
+                *_mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), out.data_ptr(), lse2.data_ptr(),
+                dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dslopes), ws.data_ptr(),
+                ws_bytes, _lib.stream_ptr(dev))
+        _lib.check(st)
+        return dq, dk, dv, dslopes, None, None, None, None, None, None

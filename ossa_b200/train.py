@@ -22,6 +22,9 @@ Here neither exists:
   ``loss.backward()`` fills the router's ``.grad`` fields and any optimizer
   steps as in the reference loop.  q and k are inputs, not differentiated (the
   reference detaches the captured projections).
+* ``top_logit_distillation_loss`` (additive) trains the sparse model itself against its dense
+  teacher: the divergence of the model's logits from the teacher's top logits, with a gradient
+  that reads the logits once and writes it once.
 """
 
 from __future__ import annotations
@@ -33,7 +36,7 @@ import torch
 from . import _lib
 from .select import _as_kernel_input, _check_qk, _common_dtype, oracle_topk
 
-__all__ = ["dense_topk_targets", "distillation_loss"]
+__all__ = ["dense_topk_targets", "distillation_loss", "top_logit_distillation_loss"]
 
 
 def dense_topk_targets(q: torch.Tensor, k: torch.Tensor, top_k: int) -> torch.Tensor:
@@ -99,3 +102,107 @@ def distillation_loss(router, q: torch.Tensor, k: torch.Tensor, top_k: int, *,
         targets = dense_topk_targets(q, k, top_k)
     wq, wk, pb = router.q_proj[0].weight, router.k_proj[0].weight, router.pos_bias.weight
     return _DistillFn.apply(wq, wk, pb, q, k, targets, router.cfg.seq_len)
+
+
+class _TopLogitDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, teacher, ids, weight, tau, reduction, grad):
+        V, K = z.shape[-1], ids.shape[-1]
+        outer, inner = (1, z.shape[0]) if z.dim() == 2 else (z.shape[0], z.shape[1])
+        rows = outer * inner
+        so, si = (0, z.stride(0)) if z.dim() == 2 else (z.stride(0), z.stride(1))
+        dev = z.device
+        L = _lib.lib()
+        ws_bytes = L.ossa_top_logit_distill_workspace_size(rows, K)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        mean = 1 if reduction == "mean" else 0
+        each = reduction == "none"
+        loss = torch.empty(rows if each else (), dtype=torch.float32, device=dev)
+        # a single incoming gradient is 1 as a rule: the gradient is taken with the loss
+        dz = torch.empty((rows, V), dtype=z.dtype, device=dev) if grad and not each else None
+        where = (z.data_ptr(), _lib.dtype_code(z), outer, inner, V, so, si)
+        with _lib.on_device(dev):
+            st = L.ossa_top_logit_distill_fwd(
+                *where, teacher.data_ptr(), ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau,
+                _lib.ptr(weight), mean, loss.data_ptr() if each else None, None if each else loss.data_ptr(),
+                _lib.ptr(dz), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+        _lib.check(st)
+        if grad:
+            ctx.save_for_backward(z, ids)
+            ctx.kept = (ws, ws_bytes, dz)
+            ctx.rule = (where[1:], K, tau, mean, each)
+        if each and weight is not None:
+            loss.mul_(weight)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        z, ids = ctx.saved_tensors
+        ws, ws_bytes, dz = ctx.kept
+        where, K, tau, mean, each = ctx.rule
+        ctx.kept = (ws, ws_bytes, None)  # a second backward pass makes its own
+        taken = dz is not None
+        if not taken:
+            dz = torch.empty((where[1] * where[2], z.shape[-1]), dtype=z.dtype, device=z.device)
+        g = g.float().contiguous()
+        with _lib.on_device(z.device):
+            st = _lib.lib().ossa_top_logit_distill_bwd(
+                z.data_ptr(), *where, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau, mean, g.data_ptr(),
+                1 if each else 0, 1 if taken else 0, dz.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(z.device))
+        _lib.check(st)
+        return dz.view(z.shape), None, None, None, None, None, None
+
+
+def top_logit_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, *,
+                                temperature: float = 1.0, row_weight: Optional[torch.Tensor] = None,
+                                reduction: str = "mean") -> torch.Tensor:
+    """Distillation of a model from its teacher's top logits (for instance the patched sparse
+    model from the unpatched dense one), differentiable in ``logits``, once.
+
+    logits: (..., V) float32 or bfloat16 CUDA tensor; teacher_logits, teacher_indices:
+    (..., K), the teacher's logits at K listed vocabulary entries per row, int32 or int64
+    indices in any order, 1 <= K <= 1024.  Per row, over the listed entries inside [0, V) (others,
+    for instance -1, are ignored; an entry listed twice counts twice):
+
+        p = softmax(teacher / temperature)
+        loss = temperature**2 * sum(p * (log p - log_softmax(logits / temperature)[listed]))
+
+    ``row_weight`` (...): weights >= 0 of the rows; a row without a listed entry weighs 0, and a row of
+    weight 0 is not read.  ``reduction``: "mean" (the weighted sum over the sum of the weights, 0 when
+    that is 0), "sum", or "none" (each row's weighted loss).  The loss is float32.  The teacher's
+    tensors and the weights are not differentiated.
+
+    With "mean" and "sum" the gradient is computed with the loss (one read of the logits, one write),
+    for an incoming gradient of 1; another one, or a second backward pass, costs one more pass."""
+    if logits.dim() < 1 or not logits.is_floating_point():
+        raise ValueError(f"logits must be (..., V) floating point; got {tuple(logits.shape)} {logits.dtype}")
+    lead = logits.shape[:-1]
+    if teacher_indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"teacher_indices must be int32 or int64, got {teacher_indices.dtype}")
+    if teacher_indices.shape[:-1] != lead or teacher_logits.shape != teacher_indices.shape or \
+            teacher_indices.dim() != logits.dim() or teacher_indices.shape[-1] < 1:
+        raise ValueError(f"teacher tensors {tuple(teacher_logits.shape)}, {tuple(teacher_indices.shape)} do not match "
+                         f"{tuple(lead)} + (K,)")
+    if row_weight is not None and row_weight.shape != lead:
+        raise ValueError(f"row_weight {tuple(row_weight.shape)} does not match the rows {tuple(lead)}")
+    tau = float(temperature)
+    if not 0.0 < tau < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    _lib.require_cuda(*[t for t in (logits, teacher_logits, teacher_indices, row_weight) if t is not None])
+    if logits.numel() == 0:
+        if logits.shape[-1] == 0:
+            raise ValueError("logits have no vocabulary entries")
+        return logits.float().sum(-1) if reduction == "none" else logits.float().sum()
+    z = logits if logits.dtype in (torch.float32, torch.bfloat16) else logits.float()
+    if z.dim() not in (2, 3) or z.stride(-1) != 1:
+        z = z.reshape(-1, z.shape[-1]).contiguous()
+    K = teacher_indices.shape[-1]
+    teacher = teacher_logits.detach().float().reshape(-1, K).contiguous()
+    ids = teacher_indices.reshape(-1, K).contiguous()
+    weight = None if row_weight is None else row_weight.detach().float().reshape(-1).contiguous()
+    loss = _TopLogitDistill.apply(z, teacher, ids, weight, tau, reduction,
+                                  torch.is_grad_enabled() and z.requires_grad)
+    return loss.view(lead) if reduction == "none" else loss
