@@ -25,9 +25,8 @@
 //    loads of V accumulate p_m * v_m into each lane's dims.
 //  * Masked/padded slots read row 0 (always in bounds) and are zeroed, so the
 //    unrolled load loops carry no branches.
-//  * kMods compiles the same kernels with the score modifiers of score_mods.cuh (cap,
-//    distance bias, documents, prefix) and the row statistic the backward pass reads;
-//    without it the code is the unmodified gather.
+//  * kMods compiles the per-head forms with the score modifiers of score_mods.cuh (cap,
+//    distance bias, documents, prefix) and the row statistic the backward pass reads.
 #pragma once
 
 #include "bf16_dot.cuh"
@@ -293,12 +292,12 @@ static_assert(kDirectMaxN <= kStageBytes && ((size_t)8 << 9) <= (size_t)kStageBy
 static_assert(mma_warp_smem<8, true>() % 16 == 0 && mma_warp_smem<9, false>() % 16 == 0, "warp areas stay 16-byte aligned");
 static_assert(2 * (mma_smem_bytes<9, false>() + 1024) <= 233472, "two CTAs per SM");
 
-template <typename IdxT, int G, int kSlotBits, bool kDirect, bool kMods>
+template <typename IdxT, int G, int kSlotBits, bool kDirect>
 __global__ void __launch_bounds__(kMmaWarps * 32, 2)
 gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
                                  const __nv_bfloat16* __restrict__ v, const IdxT* __restrict__ idx,
                                  __nv_bfloat16* __restrict__ out, int H, int Hkv, int N, int Nq, int q0, int K,
-                                 float scale_log2, int causal, const ScoreMods mods) {
+                                 float scale_log2, int causal) {
     constexpr int D = 128;
     constexpr int kMaxU = mma_max_union<kSlotBits, kDirect>();
     constexpr int kSlots = 1 << kSlotBits;
@@ -334,7 +333,6 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
     }
 
     // ---- 2. union of the heads' keys with head bits into ukey / umask
-    const RowMods<kMods> rm(mods, b, g * G, N, i);  // what a key is seen by does not depend on the head
     int x[G][4];
 #pragma unroll
     for (int t = 0; t < G; ++t) {
@@ -343,7 +341,7 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
         for (int e = 0; e < 4; ++e) {  // K <= 128
             const int qi = lane + 32 * e;
             const long long jl = (32 * e < K && qi < K) ? (long long)irow[qi] : -1ll;
-            x[t][e] = (jl >= 0 && jl < N && rm.sees(jl, i, causal)) ? (int)jl : -1;
+            x[t][e] = (jl >= 0 && jl < N && (!causal || jl <= i)) ? (int)jl : -1;
         }
     }
     bool canon = true;
@@ -466,9 +464,9 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
         for (int t = 0; t < G; ++t) {
             const size_t row = row0 + (size_t)t * Nq;
             const uint4 qv = __ldg(reinterpret_cast<const uint4*>(q + row * D) + (lane & 15));
-            gather_row_bf16_d128<IdxT, kMods>(qv, reinterpret_cast<const uint4*>(kb) + (lane & 15),
+            gather_row_bf16_d128<IdxT, false>(qv, reinterpret_cast<const uint4*>(kb) + (lane & 15),
                                        reinterpret_cast<const uint4*>(vb) + (lane & 15), idx + row * K, K, N, i,
-                                       causal, scale_log2, out + row * D, lane, mods, b, g * G + t, row);
+                                       causal, scale_log2, out + row * D, lane, ScoreMods{}, b, g * G + t, row);
         }
         return;
     }
@@ -505,11 +503,6 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
 #pragma unroll
     for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};  // heads 2 c4, 2 c4 + 1
-    float slope[2] = {0.f, 0.f};
-    if (kMods && mods.slopes) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) slope[e] = 2 * c4 + e < G ? mods.slopes[g * G + 2 * c4 + e] : 0.f;
-    }
     const int nch = (U + kMmaChunk - 1) / kMmaChunk;
     if (nch > 0) stage_rows(st_s, kb, 0);
     for (int c = 0; c < nch; ++c) {
@@ -544,17 +537,12 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
             const unsigned hb = ul < nk ? umask[c0 + ul] : 0u;
 #pragma unroll
             for (int e = 0; e < 2; ++e) sel[h][e] = 2 * c4 + e < G && ((hb >> (2 * c4 + e)) & 1u);
-            if constexpr (kMods) {
-                const float far = ul < nk ? fabsf((float)(i - ukey[c0 + ul])) : 0.f;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) sacc[2 * h + e] = mods.score2(sacc[2 * h + e], slope[e], far);
-            }
         }
         float mx[2], alpha[2], pr[2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            const float s0 = sel[0][e] ? (kMods ? sacc[e] : sacc[e] * scale_log2) : -INFINITY;
-            const float s1 = sel[1][e] ? (kMods ? sacc[2 + e] : sacc[2 + e] * scale_log2) : -INFINITY;
+            const float s0 = sel[0][e] ? sacc[e] * scale_log2 : -INFINITY;
+            const float s1 = sel[1][e] ? sacc[2 + e] * scale_log2 : -INFINITY;
             float m = fmaxf(s0, s1);
             m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
             m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
@@ -609,12 +597,6 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
             *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
         }
     }
-    if (kMods && mods.lse2 && gq == 0) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (2 * c4 + e < G)
-                mods.lse2[row0 + (size_t)(2 * c4 + e) * Nq] = m_run[e] + log2f(l_run[e]);
-    }
 }
 
 template <typename T, typename IdxT, bool kMods>
@@ -629,15 +611,15 @@ cudaError_t launch_typed(const GatherArgs& a, cudaStream_t stream) {
     const T* v = static_cast<const T*>(a.v);
     const IdxT* ix = static_cast<const IdxT*>(a.idx);
     T* o = static_cast<T*>(a.out);
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2 && !kMods) {
         const int G = a.H / a.Hkv;
         if (a.D == 128 && a.K <= 128 && (G == 2 || G == 3 || G == 4 || G == 6 || G == 8)) {
             const bool big = a.K > 64;
             const bool direct = a.N <= kDirectMaxN && a.K <= 64;
 #define OSSA_MMA_PICK(GG)                                                                      \
-    (direct ? gather_attn_bf16_d128_mma_kernel<IdxT, GG, 8, true, kMods>                              \
-            : (big ? gather_attn_bf16_d128_mma_kernel<IdxT, GG, 9, false, kMods>                      \
-                   : gather_attn_bf16_d128_mma_kernel<IdxT, GG, 8, false, kMods>))
+    (direct ? gather_attn_bf16_d128_mma_kernel<IdxT, GG, 8, true>                              \
+            : (big ? gather_attn_bf16_d128_mma_kernel<IdxT, GG, 9, false>                      \
+                   : gather_attn_bf16_d128_mma_kernel<IdxT, GG, 8, false>))
             auto kern = G == 2 ? OSSA_MMA_PICK(2)
                       : G == 3 ? OSSA_MMA_PICK(3)
                       : G == 4 ? OSSA_MMA_PICK(4)
@@ -650,11 +632,13 @@ cudaError_t launch_typed(const GatherArgs& a, cudaStream_t stream) {
             if (e != cudaSuccess) return e;
             dim3 mgrid((Nq + kMmaWarps - 1) / kMmaWarps, a.B * a.Hkv);
             kern<<<mgrid, kMmaWarps * 32, kMmaSmem, stream>>>(q, k, v, ix, o, a.H, a.Hkv, a.N, Nq, a.q0, a.K,
-                                                              scale_log2, a.causal, a.mods);
+                                                              scale_log2, a.causal);
             e = cudaGetLastError();
             if (e == cudaSuccess) note_launch();
             return e;
         }
+    }
+    if constexpr (sizeof(T) == 2) {
         if (a.D == 128) {
             gather_attn_bf16_d128_kernel<IdxT, kMods><<<grid, block, 0, stream>>>(
                 q, k, v, ix, o, a.H, a.Hkv, a.N, Nq, a.q0, a.K, scale_log2, a.causal, qtile, a.mods);

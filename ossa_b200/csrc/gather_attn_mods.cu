@@ -1,14 +1,229 @@
 // Gathered top-K attention forward with score modifiers (score_mods.cuh), and the row statistic
-// that its backward pass reads.
+// that its backward pass reads.  Also the training form of the unmodified gather.
+//
+// bf16 rows of head_dim 128 with 2-8 query heads per kv head and at most 128 listed keys take the
+// tensor-core form below, everything else the per-head forms of gather_attn_kernels.cuh.
+//
+// One warp per query and kv head, all G heads of the group at once (query_union.cuh): every key
+// that some head lists is fetched once.  In chunks of 16 keys: S^T = K Q^T with the keys as MMA
+// rows and the heads as columns, scores and masks per (key, head), online softmax per head, then
+// O^T += V^T P^T with P^T moved into operand layout by movmatrix.  The key rows of chunk c + 1 are in
+// flight while chunk c is scored, its value rows while its softmax runs.  p is rounded to bf16 for
+// the product with the bf16 values, as in the other bf16 forms; sums and statistics are fp32.
+// A query with a key listed twice by one head, or with more than 512 different keys, takes its heads
+// one after another through the same loop.
 #include "gather_attn_kernels.cuh"
+#include "query_union.cuh"
 
 namespace ossa {
 
-cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream) {
-    if (a.dtype == kF32) {
-        return a.idx_is_64 ? launch_typed<float, int64_t, true>(a, stream)
-                           : launch_typed<float, int32_t, true>(a, stream);
+namespace {
+
+struct TanhFast {
+    __device__ __forceinline__ float operator()(float x) const { return tanh_fast(x); }
+};
+
+constexpr int kModWarps = 8;
+constexpr int kModWarpBytes = 3 * kStageChunk + kUnionCap * 4;  // key rows of two chunks, value rows of one; the list
+constexpr int kModBytes = kModWarps * kModWarpBytes;
+static_assert(kUnionArea <= 3 * kStageChunk, "the list is built in the staging area");
+static_assert(2 * (kModBytes + 1024) <= 233472, "two CTAs per SM");
+
+template <typename IdxT, int G, bool kDirect>
+__global__ void __launch_bounds__(kModWarps * 32, 2)
+mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                    const __nv_bfloat16* __restrict__ v, const IdxT* __restrict__ idx, __nv_bfloat16* __restrict__ out,
+                    int H, int Hkv, int N, int Nq, int q0, int K, int causal, const ScoreMods mods) {
+    constexpr int D = 128;
+    extern __shared__ __align__(128) uint8_t msm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int gq = lane >> 2, c4 = lane & 3;
+    const int bg = blockIdx.y;
+    const int b = bg / Hkv, g = bg - b * Hkv;
+    const int il = blockIdx.x * kModWarps + warp;
+    if (il >= Nq) return;  // warp-uniform; no CTA-wide barrier follows
+    const int i = q0 + il;
+    uint8_t* stage = msm + (size_t)warp * kModWarpBytes;
+    uint32_t* list = reinterpret_cast<uint32_t*>(stage + 3 * kStageChunk);
+    const __nv_bfloat16* kb = k + (size_t)bg * N * D;
+    const __nv_bfloat16* vb = v + (size_t)bg * N * D;
+    const size_t row0 = ((size_t)b * H + (size_t)g * G) * Nq + il;  // head t: row0 + t * Nq
+
+    uint32_t qa[16];  // q rows as the MMA's B operand: head gq
+    {
+        const uint32_t* qw = reinterpret_cast<const uint32_t*>(q + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            qa[2 * s] = gq < G ? __ldg(qw + 8 * s + c4) : 0u;
+            qa[2 * s + 1] = gq < G ? __ldg(qw + 8 * s + 4 + c4) : 0u;
+        }
     }
+    const RowMods<true> rm(mods, b, g * G, N, i);  // whether a key is seen does not depend on the head
+    auto key_of = [&](int t, int e) {
+        const long long j = (long long)idx[(row0 + (size_t)t * Nq) * K + e];
+        return j >= 0 && j < N && rm.sees(j, i, causal) ? (int)j : -1;
+    };
+    int passes = 1, U;
+    {
+        int x[G][4];
+#pragma unroll
+        for (int t = 0; t < G; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[t][e] = lane + 32 * e < K ? key_of(t, lane + 32 * e) : -1;
+        }
+        U = build_union<G, kDirect>(x, K, N, stage, list, lane);
+        if (U < 0) passes = G;
+    }
+    const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage), vst = st + 2u * kStageChunk;
+    // ldmatrix rows: keys as the A operand of S^T, values transposed as the A operand of O^T
+    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
+    const int vrow = (lane & 7) + (lane >> 4) * 8, vpc = (lane >> 3) & 1;
+    float oacc[8][4];  // O^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
+#pragma unroll
+    for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
+    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    float slope[2] = {0.f, 0.f};
+    if (mods.slopes) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) slope[e] = 2 * c4 + e < G ? mods.slopes[g * G + 2 * c4 + e] : 0.f;
+    }
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+        __syncwarp();
+        if (passes > 1) U = single_list([&](int e) { return key_of(pass, e); }, pass, K, list, lane);
+        __syncwarp();  // the list is complete, the staging area is free
+        const int nch = (U + kStageRows - 1) / kStageRows;
+        if (nch > 0) {
+            stage_listed(st, kb, list, 0, U, lane);
+            stage_commit();
+        }
+#pragma unroll 1
+        for (int c = 0; c < nch; ++c) {
+            const int c0 = c * kStageRows;
+            const bool more = c + 1 < nch;  // warp-uniform
+            __syncwarp();                   // chunk c - 1 is done with the value rows and key buffer (c + 1) & 1
+            stage_listed(vst, vb, list, c0, U, lane);
+            stage_commit();
+            if (more) {
+                stage_listed(st + (uint32_t)(((c + 1) & 1) * kStageChunk), kb, list, c0 + kStageRows, U, lane);
+                stage_commit();
+                cp_async_wait_pending<2>();
+            } else {
+                cp_async_wait_pending<1>();
+            }
+            __syncwarp();
+            const uint32_t kst = st + (uint32_t)((c & 1) * kStageChunk);
+            float sacc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                uint32_t a[4];
+                ldmatrix_x4(a, stage_piece(kst, krow, 2 * s + kpc));
+                mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], qa[2 * s], qa[2 * s + 1]);
+            }
+            // keys c0 + gq, c0 + gq + 8 x heads 2 c4, 2 c4 + 1; a head's scores sit in the lanes of equal c4
+            float sc[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = c0 + gq + 8 * h;
+                const uint32_t entry = at < U ? list[at] : 0u;
+                const float far = fabsf((float)(i - (int)(entry & 0xffffffu)));
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    sc[h][e] = (entry >> (24 + 2 * c4 + e)) & 1u
+                                   ? mods.score2(sacc[2 * h + e], slope[e], far, TanhFast()) : -INFINITY;
+            }
+            float alpha[2], pr[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float m = fmaxf(sc[0][e], sc[1][e]);
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
+                const float mx = fmaxf(m_run[e], m);
+                alpha[e] = mx == -INFINITY ? 1.f : exp2_fast(m_run[e] - mx);
+                pr[0][e] = mx == -INFINITY ? 0.f : exp2_fast(sc[0][e] - mx);
+                pr[1][e] = mx == -INFINITY ? 0.f : exp2_fast(sc[1][e] - mx);
+                float sum = pr[0][e] + pr[1][e];
+                sum += __shfl_xor_sync(kFull, sum, 4);
+                sum += __shfl_xor_sync(kFull, sum, 8);
+                sum += __shfl_xor_sync(kFull, sum, 16);
+                l_run[e] = l_run[e] * alpha[e] + sum;
+                m_run[e] = mx;
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                oacc[n][0] *= alpha[0];
+                oacc[n][1] *= alpha[1];
+                oacc[n][2] *= alpha[0];
+                oacc[n][3] *= alpha[1];
+            }
+            const uint32_t pb0 = movmatrix_trans(pack_bf16x2(pr[0][0], pr[0][1]));
+            const uint32_t pb1 = movmatrix_trans(pack_bf16x2(pr[1][0], pr[1][1]));
+            if (more) cp_async_wait_pending<1>();
+            else cp_async_wait_pending<0>();
+            __syncwarp();
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a, stage_piece(vst, vrow, 2 * mt + vpc));
+                mma_bf16_16816_a4(oacc[mt], a[0], a[1], a[2], a[3], pb0, pb1);
+            }
+        }
+    }
+    // each head's row divided by its sum and transposed back: lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
+    const float inv0 = l_run[0] == 0.f ? 0.f : 1.f / l_run[0], inv1 = l_run[1] == 0.f ? 0.f : 1.f / l_run[1];
+    __nv_bfloat16* orow = out + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D + 2 * c4;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+        const uint32_t lo = movmatrix_trans(pack_bf16x2(oacc[mt][0] * inv0, oacc[mt][1] * inv1));
+        const uint32_t hi = movmatrix_trans(pack_bf16x2(oacc[mt][2] * inv0, oacc[mt][3] * inv1));
+        if (gq < G) {
+            *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
+            *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+        }
+    }
+    if (mods.lse2 && gq == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (2 * c4 + e < G) mods.lse2[row0 + (size_t)(2 * c4 + e) * Nq] = m_run[e] + log2f(l_run[e]);
+    }
+}
+
+template <typename IdxT>
+cudaError_t launch_mma(const GatherArgs& a, cudaStream_t stream) {
+    const int G = a.H / a.Hkv;
+    const bool direct = a.N <= kUnionDirectKeys;
+#define OSSA_MOD_PICK(GG) (direct ? mod_attn_mma_kernel<IdxT, GG, true> : mod_attn_mma_kernel<IdxT, GG, false>)
+    auto kern = G == 2 ? OSSA_MOD_PICK(2)
+              : G == 3 ? OSSA_MOD_PICK(3)
+              : G == 4 ? OSSA_MOD_PICK(4)
+              : G == 6 ? OSSA_MOD_PICK(6)
+                       : OSSA_MOD_PICK(8);
+#undef OSSA_MOD_PICK
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kModBytes);
+    if (e != cudaSuccess) return e;
+    kern<<<dim3((a.Nq + kModWarps - 1) / kModWarps, a.B * a.Hkv), kModWarps * 32, kModBytes, stream>>>(
+        static_cast<const __nv_bfloat16*>(a.q), static_cast<const __nv_bfloat16*>(a.k),
+        static_cast<const __nv_bfloat16*>(a.v), static_cast<const IdxT*>(a.idx), static_cast<__nv_bfloat16*>(a.out), a.H,
+        a.Hkv, a.N, a.Nq, a.q0, a.K, a.causal, a.mods);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+}  // namespace
+
+bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K) {
+    const int G = H / Hkv;
+    return dtype == kBF16 && D == 128 && K >= 1 && K <= 128 && N <= kUnionMaxKeys &&
+           (G == 2 || G == 3 || G == 4 || G == 6 || G == 8);
+}
+
+cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream) {
+    if (gather_mma_serves(a.dtype, a.H, a.Hkv, a.N, a.D, a.K))
+        return a.idx_is_64 ? launch_mma<int64_t>(a, stream) : launch_mma<int32_t>(a, stream);
+    if (a.dtype == kF32)
+        return a.idx_is_64 ? launch_typed<float, int64_t, true>(a, stream) : launch_typed<float, int32_t, true>(a, stream);
     return a.idx_is_64 ? launch_typed<__nv_bfloat16, int64_t, true>(a, stream)
                        : launch_typed<__nv_bfloat16, int32_t, true>(a, stream);
 }

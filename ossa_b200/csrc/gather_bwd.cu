@@ -11,7 +11,7 @@
 //     key by key, in a fixed order (a counting sort: units of (row chunk, head) count their
 //     entries per key, the counts are scanned, every unit then writes its rows).
 //  2. Row pass, one warp per row: dq_i, Delta_i and the row's share of dslope.
-//  3. Key pass, one warp per kTile consecutive entries of a turned list, which may begin and
+//  3. Key pass, one warp per kBwdTile consecutive entries of a turned list, which may begin and
 //     end inside a key's run: whole runs are stored, cut ones go to per-tile partial sums.
 //  4. Join: keys whose run is cut add their partial sums in tile order; keys that nobody
 //     lists get zeros.
@@ -24,6 +24,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "gather_bwd.cuh"
 #include "mma_sync.cuh"
 #include "score_mods.cuh"
 
@@ -34,19 +35,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kKeyRange = 8192;  // keys that one CTA of the counting sort covers (32 KB of counters)
-constexpr int kTile = 256;       // entries that a warp of the key pass takes
-constexpr int kMaxChunks = 16;   // row chunks of the counting sort per head
-constexpr int kMinChunkRows = 64;
+constexpr int kMaxChunks = 32;   // row chunks of the counting sort per head
+constexpr int kMinChunkRows = 32;
+constexpr int kPlaceRows = 8;    // rows whose entries the counting sort's last step has in flight
 
-struct Shape {
-    int B, H, Hkv, G, Nq, N, D, K, q0, causal;
-    int chunks, chunk_rows, units;  // units = chunks * G per (b, kv head)
-    long long cap;                  // entries per (b, kv head) at most
-    long long tiles;                // key-pass tiles per (b, kv head) at most
-};
-
-Shape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
-    Shape s{};
+BwdShape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
+    BwdShape s{};
     s.B = B;
     s.H = H;
     s.Hkv = Hkv;
@@ -59,19 +53,20 @@ Shape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
     s.chunk_rows = (Nq + s.chunks - 1) / s.chunks;
     s.units = s.chunks * s.G;
     s.cap = (long long)s.G * Nq * K;
-    s.tiles = (s.cap + kTile - 1) / kTile;
+    s.tiles = (s.cap + kBwdTile - 1) / kBwdTile;
     return s;
 }
 
 struct Layout {
-    size_t counts, base, list, delta, part, slope_rows, total;
+    size_t keys, counts, base, list, delta, part, slope_rows, total;
 };
 
-Layout make_layout(const Shape& s, bool dslopes) {
+Layout make_layout(const BwdShape& s, bool dslopes) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     const size_t kv = (size_t)s.B * s.Hkv, rows = (size_t)s.B * s.H * s.Nq;
     Layout l;
-    l.counts = 0;
+    l.keys = 0;
+    l.counts = l.keys + up(rows * s.K * 4);
     l.base = l.counts + up(kv * s.units * s.N * 4);
     l.list = l.base + up(kv * ((size_t)s.N + 1) * 4);
     l.delta = l.list + up(kv * s.cap * 4);
@@ -83,11 +78,13 @@ Layout make_layout(const Shape& s, bool dslopes) {
 
 // ------------------------------------------------------------------ 1. turned lists
 
+// keys: the lists as int32, -1 where an entry is outside [0, N) or not seen by its row.
 // counts[kv][unit][key]: how often the unit's rows list the key and see it.
 template <typename IdxT>
 __global__ void __launch_bounds__(kThreads)
-count_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, int* __restrict__ counts) {
-    __shared__ int hist[kKeyRange];
+count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mods, int* __restrict__ keys,
+             int* __restrict__ counts) {
+    extern __shared__ int hist[];  // min(N, kKeyRange)
     const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
     const int nk = min(kKeyRange, s.N - k0);
     const int b = kv / s.Hkv, h = (kv - b * s.Hkv) * s.G + unit % s.G;
@@ -98,10 +95,12 @@ count_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, 
     for (int il = r0 + (threadIdx.x >> 5); il < r1; il += kWarps) {
         const int i = s.q0 + il;
         const RowMods<true> rm(mods, b, h, s.N, i);
-        const IdxT* irow = idx + (((size_t)b * s.H + h) * s.Nq + il) * s.K;
+        const size_t row = ((size_t)b * s.H + h) * s.Nq + il;
         for (int e = lane; e < s.K; e += 32) {
-            const long long j = (long long)irow[e];
-            if (j >= k0 && j < k0 + nk && rm.sees(j, i, s.causal)) atomicAdd(&hist[j - k0], 1);
+            const long long j = (long long)idx[row * s.K + e];
+            const bool on = j >= 0 && j < s.N && rm.sees(j, i, s.causal);
+            if (blockIdx.z == 0) keys[row * s.K + e] = on ? (int)j : -1;
+            if (on && j >= k0 && j < k0 + nk) atomicAdd(&hist[j - k0], 1);
         }
     }
     __syncthreads();
@@ -111,7 +110,7 @@ count_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, 
 
 // counts -> exclusive prefix over the units, and the key's total in base[kv][key].
 __global__ void __launch_bounds__(kThreads)
-unit_scan_kernel(const Shape s, int* __restrict__ counts, int* __restrict__ base) {
+unit_scan_kernel(const BwdShape s, int* __restrict__ counts, int* __restrict__ base) {
     const int key = blockIdx.x * kThreads + threadIdx.x, kv = blockIdx.y;
     if (key >= s.N) return;
     int* c = counts + (size_t)kv * s.units * s.N + key;
@@ -125,7 +124,7 @@ unit_scan_kernel(const Shape s, int* __restrict__ counts, int* __restrict__ base
 }
 
 // base[kv][0..N]: exclusive prefix of the totals over the keys.
-__global__ void __launch_bounds__(1024) key_scan_kernel(const Shape s, int* __restrict__ base) {
+__global__ void __launch_bounds__(1024) key_scan_kernel(const BwdShape s, int* __restrict__ base) {
     __shared__ int wsum[32];
     __shared__ int carry;
     int* p = base + (size_t)blockIdx.x * (s.N + 1);
@@ -162,13 +161,14 @@ __global__ void __launch_bounds__(1024) key_scan_kernel(const Shape s, int* __re
     if (threadIdx.x == 0) p[s.N] = carry;
 }
 
-// list[kv][position] = g * Nq + il of the rows that list a key, key by key.  One warp walks
-// the unit's rows in order; the counters of its key range live in shared memory.
-template <typename IdxT>
+// list[kv][position] = g * Nq + il of the rows that list a key, key by key.  One warp walks the
+// unit's rows in a fixed order, the counters of its key range in shared memory; the entries of
+// kPlaceRows rows are loaded together, and the next ones while these are placed, so a step costs
+// one trip to L2 and not one per row.
 __global__ void __launch_bounds__(32)
-place_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, const int* __restrict__ counts,
+place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restrict__ counts,
              const int* __restrict__ base, int* __restrict__ list) {
-    __shared__ int next[kKeyRange];
+    extern __shared__ int next[];  // min(N, kKeyRange)
     const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
     const int nk = min(kKeyRange, s.N - k0);
     const int g = unit % s.G;
@@ -180,15 +180,31 @@ place_kernel(const IdxT* __restrict__ idx, const Shape s, const ScoreMods mods, 
     for (int t = lane; t < nk; t += 32) next[t] = c[t] + bs[t];
     __syncwarp();
     int* out = list + (size_t)kv * s.cap;
-    for (int il = r0; il < r1; ++il) {
-        const int i = s.q0 + il;
-        const RowMods<true> rm(mods, b, h, s.N, i);
-        const IdxT* irow = idx + (((size_t)b * s.H + h) * s.Nq + il) * s.K;
-        for (int e = lane; e < s.K; e += 32) {
-            const long long j = (long long)irow[e];
-            if (j >= k0 && j < k0 + nk && rm.sees(j, i, s.causal)) out[atomicAdd(&next[j - k0], 1)] = g * s.Nq + il;
+    const int* rows = keys + ((size_t)b * s.H + h) * s.Nq * s.K;
+    const int parts = (s.K + 31) / 32;
+    const int steps = ((r1 - r0 + kPlaceRows - 1) / kPlaceRows) * parts;  // a step: 32 entries of kPlaceRows rows
+    auto load = [&](int step, int (&j)[kPlaceRows]) {
+        const int il = r0 + step / parts * kPlaceRows, e = (step % parts) * 32 + lane;
+#pragma unroll
+        for (int t = 0; t < kPlaceRows; ++t)
+            j[t] = step < steps && il + t < r1 && e < s.K ? rows[(size_t)(il + t) * s.K + e] - k0 : -1;
+    };
+    int j[kPlaceRows], ahead[kPlaceRows];
+    load(0, j);
+    for (int step = 0; step < steps; ++step) {
+        load(step + 1, ahead);
+        const int il = r0 + step / parts * kPlaceRows;
+        int pos[kPlaceRows];
+#pragma unroll
+        for (int t = 0; t < kPlaceRows; ++t) {
+            pos[t] = (unsigned)j[t] < (unsigned)nk ? atomicAdd(&next[j[t]], 1) : -1;
+            __syncwarp();  // a row's places before the next row's
         }
-        __syncwarp();  // a row's places before the next row's
+#pragma unroll
+        for (int t = 0; t < kPlaceRows; ++t) {
+            if (pos[t] >= 0) out[pos[t]] = g * s.Nq + il + t;
+            j[t] = ahead[t];
+        }
     }
 }
 
@@ -214,10 +230,10 @@ struct RowLoad {
     }
 };
 
-template <typename T, int D, typename IdxT>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
-row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const IdxT* __restrict__ idx,
-                const T* __restrict__ out, const T* __restrict__ dout, const Shape s, const ScoreMods mods,
+row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ keys,
+                const T* __restrict__ out, const T* __restrict__ dout, const BwdShape s, const ScoreMods mods,
                 T* __restrict__ dq, float* __restrict__ delta, float* __restrict__ slope_rows) {
     using R = RowLoad<T, D>;
     const int lane = threadIdx.x & 31;
@@ -228,7 +244,7 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     const size_t kv = (size_t)b * s.Hkv + h / s.G;
     const T* kb = k + kv * s.N * D;
     const T* vb = v + kv * s.N * D;
-    const RowMods<true> rm(mods, b, h, s.N, i);
+    const float slope = mods.slopes ? mods.slopes[h] : 0.f;
     const float lse2 = mods.lse2[row];
     float qv[R::kPer], dv[R::kPer], acc[R::kPer];
     R::load(q + row * D, lane, qv);
@@ -245,11 +261,10 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         d0 = warp_sum(d0);
     }
     float a_pd = 0.f, a_f = 0.f, a_pdf = 0.f;  // sums of p dP, p far, p dP far
-    const IdxT* irow = idx + row * s.K;
+    const int* krow = keys + row * s.K;
     for (int kc = 0; kc < s.K; kc += 32) {
         const int kk = kc + lane;
-        const long long jl = kk < s.K ? (long long)irow[kk] : -1ll;
-        const int j = jl >= 0 && jl < s.N && rm.sees(jl, i, s.causal) ? (int)jl : -1;
+        const int j = kk < s.K ? krow[kk] : -1;
         if (!__any_sync(kFull, j >= 0)) continue;
         float x[32], y[32];
 #pragma unroll
@@ -271,7 +286,7 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         float p = 0.f, dx = 0.f;
         if (j >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
             const float far = fabsf((float)(i - j));
-            p = exp2f(mods.score2_grad(dot, rm.slope, far, dx) - lse2);
+            p = exp2f(mods.score2_grad(dot, slope, far, dx, TanhExact()) - lse2);
             dx *= p * (dp - d0);
             a_pd = fmaf(p, dp, a_pd);
             a_f = fmaf(p, far, a_f);
@@ -301,29 +316,18 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 
 // ------------------------------------------------------------------ 3. key pass
 
-// The key whose run holds position pos (base[key] <= pos < base[key + 1]).
-__device__ __forceinline__ int key_at(const int* __restrict__ base, int N, int pos) {
-    int lo = 0, hi = N;  // base[lo] <= pos < base[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(base + mid) <= pos) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
 key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ dout,
-                const Shape s, const ScoreMods mods, const int* __restrict__ base, const int* __restrict__ list,
+                const BwdShape s, const ScoreMods mods, const int* __restrict__ base, const int* __restrict__ list,
                 const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
     using R = RowLoad<T, D>;
     const int lane = threadIdx.x & 31, kv = blockIdx.y;
     const long long tile = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int* bs = base + (size_t)kv * (s.N + 1);
     const int total = bs[s.N];
-    if (tile * kTile >= total) return;  // warp-uniform
-    const int t0 = (int)(tile * kTile), t1 = min(total, t0 + kTile);
+    if (tile * kBwdTile >= total) return;  // warp-uniform
+    const int t0 = (int)(tile * kBwdTile), t1 = min(total, t0 + kBwdTile);
     const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
     const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
     const int* ls = list + (size_t)kv * s.cap;
@@ -362,7 +366,7 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
             if (lse2 != -INFINITY) {
                 const int g = r / s.Nq, i = s.q0 + r - g * s.Nq;
                 const float slope = mods.slopes ? mods.slopes[h0 + g] : 0.f;
-                p = exp2f(mods.score2_grad(dot, slope, fabsf((float)(i - key)), dx) - lse2);
+                p = exp2f(mods.score2_grad(dot, slope, fabsf((float)(i - key)), dx, TanhExact()) - lse2);
                 dx *= p * (dp - delta[rows0 + r]);
             }
 #pragma unroll
@@ -396,14 +400,14 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-join_kernel(const Shape s, const int* __restrict__ base, const float* __restrict__ part, T* __restrict__ dk,
+join_kernel(const BwdShape s, const int* __restrict__ base, const float* __restrict__ part, T* __restrict__ dk,
             T* __restrict__ dv) {
     const int lane = threadIdx.x & 31, kv = blockIdx.y;
     const int key = blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (key >= s.N) return;
     const int* bs = base + (size_t)kv * (s.N + 1);
     const int run0 = bs[key], run1 = bs[key + 1];
-    const int first = run0 / kTile, last = run1 > run0 ? (run1 - 1) / kTile : first;
+    const int first = run0 / kBwdTile, last = run1 > run0 ? (run1 - 1) / kBwdTile : first;
     if (run1 > run0 && first == last) return;  // stored by the key pass
     const float* ps = part + (size_t)kv * s.tiles * 4 * s.D;
     T* ok = dk + ((size_t)kv * s.N + key) * s.D;
@@ -421,7 +425,7 @@ join_kernel(const Shape s, const int* __restrict__ base, const float* __restrict
 }
 
 // dslopes[h]: the rows' shares, each thread's in row order, then a fixed tree.
-__global__ void __launch_bounds__(1024) slope_join_kernel(const Shape s, const float* __restrict__ rows, float* dslopes) {
+__global__ void __launch_bounds__(1024) slope_join_kernel(const BwdShape s, const float* __restrict__ rows, float* dslopes) {
     __shared__ double sums[32];
     const int h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double t = 0.0;
@@ -444,55 +448,59 @@ cudaError_t launched() {
     return e;
 }
 
-template <typename T, typename IdxT>
-cudaError_t bwd_typed(const GatherBwdArgs& a, const Shape& s, const Layout& l, cudaStream_t stream) {
-    char* ws = static_cast<char*>(a.ws);
-    int* counts = reinterpret_cast<int*>(ws + l.counts);
-    int* base = reinterpret_cast<int*>(ws + l.base);
-    int* list = reinterpret_cast<int*>(ws + l.list);
-    float* delta = reinterpret_cast<float*>(ws + l.delta);
-    float* part = reinterpret_cast<float*>(ws + l.part);
-    float* slope_rows = a.dslopes ? reinterpret_cast<float*>(ws + l.slope_rows) : nullptr;
+template <typename IdxT>
+cudaError_t sort_lists(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
+    const unsigned kvs = (unsigned)(s.B * s.Hkv);
+    const dim3 grid((unsigned)s.units, kvs, (unsigned)((s.N + kKeyRange - 1) / kKeyRange));
+    const size_t smem = (size_t)std::min(s.N, kKeyRange) * sizeof(int);
+    cudaError_t e;
+    count_kernel<IdxT><<<grid, kThreads, smem, stream>>>(static_cast<const IdxT*>(a.f.idx), s, a.f.mods, w.keys, w.counts);
+    if ((e = launched()) != cudaSuccess) return e;
+    unit_scan_kernel<<<dim3((unsigned)((s.N + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, w.counts, w.base);
+    if ((e = launched()) != cudaSuccess) return e;
+    key_scan_kernel<<<kvs, 1024, 0, stream>>>(s, w.base);
+    if ((e = launched()) != cudaSuccess) return e;
+    place_kernel<<<grid, 32, smem, stream>>>(w.keys, s, w.counts, w.base, w.list);
+    return launched();
+}
+
+template <typename T>
+cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
     const T *q = static_cast<const T*>(a.f.q), *k = static_cast<const T*>(a.f.k), *v = static_cast<const T*>(a.f.v);
     const T *out = static_cast<const T*>(a.f.out), *dout = static_cast<const T*>(a.dout);
     T *dq = static_cast<T*>(a.dq), *dk = static_cast<T*>(a.dk), *dv = static_cast<T*>(a.dv);
-    const IdxT* idx = static_cast<const IdxT*>(a.f.idx);
     const ScoreMods& m = a.f.mods;
     const unsigned kvs = (unsigned)(s.B * s.Hkv);
-    const dim3 sort_grid((unsigned)s.units, kvs, (unsigned)((s.N + kKeyRange - 1) / kKeyRange));
-    cudaError_t e;
-    count_kernel<IdxT><<<sort_grid, kThreads, 0, stream>>>(idx, s, m, counts);
-    if ((e = launched()) != cudaSuccess) return e;
-    unit_scan_kernel<<<dim3((unsigned)((s.N + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, counts, base);
-    if ((e = launched()) != cudaSuccess) return e;
-    key_scan_kernel<<<kvs, 1024, 0, stream>>>(s, base);
-    if ((e = launched()) != cudaSuccess) return e;
-    place_kernel<IdxT><<<sort_grid, 32, 0, stream>>>(idx, s, m, counts, base, list);
-    if ((e = launched()) != cudaSuccess) return e;
     const long long rows = (long long)s.B * s.H * s.Nq;
     const unsigned row_grid = (unsigned)((rows + kWarps - 1) / kWarps);
     const dim3 key_grid((unsigned)((s.tiles + kWarps - 1) / kWarps), kvs);
-    switch (s.D) {
-#define OSSA_BWD_CASE(DD)                                                                                             \
-    case DD:                                                                                                          \
-        row_pass_kernel<T, DD, IdxT><<<row_grid, kThreads, 0, stream>>>(q, k, v, idx, out, dout, s, m, dq, delta,     \
-                                                                        slope_rows);                                  \
-        if ((e = launched()) != cudaSuccess) return e;                                                                \
-        key_pass_kernel<T, DD><<<key_grid, kThreads, 0, stream>>>(q, k, v, dout, s, m, base, list, delta, dk, dv,     \
-                                                                  part);                                              \
+    cudaError_t e;
+    if (gather_mma_serves(a.f.dtype, s.H, s.Hkv, s.N, s.D, s.K)) {
+        if ((e = launch_row_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
+        if ((e = launch_key_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
+    } else {
+        switch (s.D) {
+#define OSSA_BWD_CASE(DD)                                                                                               \
+    case DD:                                                                                                            \
+        row_pass_kernel<T, DD><<<row_grid, kThreads, 0, stream>>>(q, k, v, w.keys, out, dout, s, m, dq, w.delta,        \
+                                                                  w.slope_rows);                                        \
+        if ((e = launched()) != cudaSuccess) return e;                                                                  \
+        key_pass_kernel<T, DD><<<key_grid, kThreads, 0, stream>>>(q, k, v, dout, s, m, w.base, w.list, w.delta, dk, dv, \
+                                                                  w.part);                                              \
         break;
-        OSSA_BWD_CASE(16)
-        OSSA_BWD_CASE(32)
-        OSSA_BWD_CASE(64)
-        OSSA_BWD_CASE(128)
-        OSSA_BWD_CASE(256)
+            OSSA_BWD_CASE(16)
+            OSSA_BWD_CASE(32)
+            OSSA_BWD_CASE(64)
+            OSSA_BWD_CASE(128)
+            OSSA_BWD_CASE(256)
 #undef OSSA_BWD_CASE
-        default: return cudaErrorInvalidValue;
+            default: return cudaErrorInvalidValue;
+        }
+        if ((e = launched()) != cudaSuccess) return e;
     }
-    if ((e = launched()) != cudaSuccess) return e;
-    join_kernel<T><<<dim3((unsigned)((s.N + kWarps - 1) / kWarps), kvs), kThreads, 0, stream>>>(s, base, part, dk, dv);
+    join_kernel<T><<<dim3((unsigned)((s.N + kWarps - 1) / kWarps), kvs), kThreads, 0, stream>>>(s, w.base, w.part, dk, dv);
     if ((e = launched()) != cudaSuccess || !a.dslopes) return e;
-    slope_join_kernel<<<s.H, 1024, 0, stream>>>(s, slope_rows, a.dslopes);
+    slope_join_kernel<<<s.H, 1024, 0, stream>>>(s, w.slope_rows, a.dslopes);
     return launched();
 }
 
@@ -503,14 +511,22 @@ size_t gather_bwd_workspace_bytes(int B, int H, int Hkv, int Nq, int N, int D, i
 }
 
 cudaError_t launch_gather_attn_bwd(const GatherBwdArgs& a, cudaStream_t stream) {
-    Shape s = make_shape(a.f.B, a.f.H, a.f.Hkv, a.f.Nq, a.f.N, a.f.D, a.f.K);
+    BwdShape s = make_shape(a.f.B, a.f.H, a.f.Hkv, a.f.Nq, a.f.N, a.f.D, a.f.K);
     s.q0 = a.f.q0;
     s.causal = a.f.causal;
     const Layout l = make_layout(s, a.dslopes != nullptr);
-    if (a.f.dtype == kF32)
-        return a.f.idx_is_64 ? bwd_typed<float, int64_t>(a, s, l, stream) : bwd_typed<float, int32_t>(a, s, l, stream);
-    return a.f.idx_is_64 ? bwd_typed<__nv_bfloat16, int64_t>(a, s, l, stream)
-                         : bwd_typed<__nv_bfloat16, int32_t>(a, s, l, stream);
+    char* ws = static_cast<char*>(a.ws);
+    BwdBuffers w{};
+    w.keys = reinterpret_cast<int*>(ws + l.keys);
+    w.counts = reinterpret_cast<int*>(ws + l.counts);
+    w.base = reinterpret_cast<int*>(ws + l.base);
+    w.list = reinterpret_cast<int*>(ws + l.list);
+    w.delta = reinterpret_cast<float*>(ws + l.delta);
+    w.part = reinterpret_cast<float*>(ws + l.part);
+    w.slope_rows = a.dslopes ? reinterpret_cast<float*>(ws + l.slope_rows) : nullptr;
+    const cudaError_t e = a.f.idx_is_64 ? sort_lists<int64_t>(a, s, w, stream) : sort_lists<int32_t>(a, s, w, stream);
+    if (e != cudaSuccess) return e;
+    return a.f.dtype == kF32 ? passes_typed<float>(a, s, w, stream) : passes_typed<__nv_bfloat16>(a, s, w, stream);
 }
 
 }  // namespace ossa

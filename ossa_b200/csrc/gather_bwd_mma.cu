@@ -1,0 +1,424 @@
+// Tensor-core passes of the gathered attention's backward (bf16, D = 128; gather_bwd.cu has the
+// mathematics and the other shapes).  mma.sync m16n8k16: the operands are gathered rows that a warp
+// stages for itself, 16 at a time, too few and too scattered for a tcgen05 tile.
+#include <algorithm>
+#include <cstdint>
+
+#include "common.cuh"
+#include "gather_bwd.cuh"
+#include "kernels.h"
+#include "mma_sync.cuh"
+#include "query_union.cuh"
+
+namespace ossa {
+
+namespace {
+
+constexpr int D = 128;
+
+struct TanhFast {
+    __device__ __forceinline__ float operator()(float x) const { return tanh_fast(x); }
+};
+
+__device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float c) {
+    float a0, a1, b0, b1;
+    unpack_bf16x2(a, a0, a1);
+    unpack_bf16x2(b, b0, b1);
+    return fmaf(a1, b1, fmaf(a0, b0, c));
+}
+
+// ------------------------------------------------------------------ row pass
+//
+// One warp per query and kv head, all heads of the group, over the union of their keys
+// (query_union.cuh).  In chunks of 16 keys: S^T = K Q^T and dP^T = V dO^T (keys as MMA rows, heads as
+// columns), p, dS and the weights dX per (key, head), then dq^T += K^T dX^T from the same staged key
+// rows.  dX is rounded to bf16 for that product; p, dP, the sums and Delta stay fp32.  The rows of
+// chunk c + 1 are in flight while chunk c is computed.
+constexpr int kRowWarps = 6;
+constexpr int kRowWarpBytes = 4 * kStageChunk + kUnionCap * 4;  // key and value rows of two chunks; the list
+constexpr int kRowBytes = kRowWarps * kRowWarpBytes;
+static_assert(kUnionArea <= 4 * kStageChunk, "the list is built in the staging area");
+static_assert(2 * (kRowBytes + 1024) <= 233472, "two CTAs per SM");
+
+template <int G, bool kDirect>
+__global__ void __launch_bounds__(kRowWarps * 32, 2)
+row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                    const __nv_bfloat16* __restrict__ v, const int* __restrict__ keys,
+                    const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout, const BwdShape s,
+                    const ScoreMods mods, __nv_bfloat16* __restrict__ dq, float* __restrict__ delta,
+                    float* __restrict__ slope_rows) {
+    extern __shared__ __align__(128) uint8_t msm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int gq = lane >> 2, c4 = lane & 3;
+    const int kv = blockIdx.y;
+    const int b = kv / s.Hkv, g = kv - b * s.Hkv;
+    const int il = blockIdx.x * kRowWarps + warp;
+    if (il >= s.Nq) return;  // warp-uniform; no CTA-wide barrier follows
+    const int i = s.q0 + il;
+    uint8_t* stage = msm + (size_t)warp * kRowWarpBytes;
+    uint32_t* list = reinterpret_cast<uint32_t*>(stage + 4 * kStageChunk);
+    const __nv_bfloat16* kb = k + (size_t)kv * s.N * D;
+    const __nv_bfloat16* vb = v + (size_t)kv * s.N * D;
+    const size_t row0 = ((size_t)b * s.H + (size_t)g * G) * s.Nq + il;  // head t: row0 + t * Nq
+    const size_t mine = (row0 + (size_t)(gq < G ? gq : 0) * s.Nq) * D;  // head gq's row
+
+    // q and dO rows as B operands of head gq; Delta from the stored output
+    uint32_t qa[16], da[16];
+    float d0[2];
+    {
+        const uint32_t* qw = reinterpret_cast<const uint32_t*>(q + mine);
+        const uint32_t* dw = reinterpret_cast<const uint32_t*>(dout + mine);
+        const uint32_t* ow = reinterpret_cast<const uint32_t*>(out + mine);
+        float d = 0.f;
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            qa[t] = gq < G ? __ldg(qw + 4 * t + c4) : 0u;
+            da[t] = gq < G ? __ldg(dw + 4 * t + c4) : 0u;
+            d = dot_bf16x2(da[t], gq < G ? __ldg(ow + 4 * t + c4) : 0u, d);
+        }
+        d += __shfl_xor_sync(kFull, d, 1);
+        d += __shfl_xor_sync(kFull, d, 2);
+        d0[0] = __shfl_sync(kFull, d, 8 * c4);  // heads 2 c4, 2 c4 + 1
+        d0[1] = __shfl_sync(kFull, d, 8 * c4 + 4);
+    }
+    float lse2[2], slope[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int t = 2 * c4 + e;
+        lse2[e] = t < G ? mods.lse2[row0 + (size_t)t * s.Nq] : -INFINITY;
+        slope[e] = mods.slopes && t < G ? mods.slopes[g * G + t] : 0.f;
+    }
+    auto key_of = [&](int t, int e) { return keys[(row0 + (size_t)t * s.Nq) * s.K + e]; };
+    int passes = 1, U;
+    {
+        int x[G][4];
+#pragma unroll
+        for (int t = 0; t < G; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[t][e] = lane + 32 * e < s.K ? key_of(t, lane + 32 * e) : -1;
+        }
+        U = build_union<G, kDirect>(x, s.K, s.N, stage, list, lane);
+        if (U < 0) passes = G;
+    }
+    const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
+    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
+    const int trow = (lane & 7) + (lane >> 4) * 8, tpc = (lane >> 3) & 1;
+    float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
+#pragma unroll
+    for (int n = 0; n < 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+    float a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_pdf[2] = {0.f, 0.f};  // sums of p dP, p far, p dP far
+    auto stage_both = [&](int c) {
+        const uint32_t at = st + (uint32_t)((c & 1) * 2 * kStageChunk);
+        stage_listed(at, kb, list, c * kStageRows, U, lane);
+        stage_listed(at + kStageChunk, vb, list, c * kStageRows, U, lane);
+        stage_commit();
+    };
+#pragma unroll 1
+    for (int pass = 0; pass < passes; ++pass) {
+        __syncwarp();
+        if (passes > 1) U = single_list([&](int e) { return key_of(pass, e); }, pass, s.K, list, lane);
+        __syncwarp();  // the list is complete, the staging area is free
+        const int nch = (U + kStageRows - 1) / kStageRows;
+        if (nch > 0) stage_both(0);
+#pragma unroll 1
+        for (int c = 0; c < nch; ++c) {
+            const int c0 = c * kStageRows;
+            __syncwarp();  // chunk c - 1 is done with its buffers
+            if (c + 1 < nch) {
+                stage_both(c + 1);
+                cp_async_wait_pending<1>();
+            } else {
+                cp_async_wait_pending<0>();
+            }
+            __syncwarp();
+            const uint32_t kst = st + (uint32_t)((c & 1) * 2 * kStageChunk), vst = kst + kStageChunk;
+            float sacc[4] = {0.f, 0.f, 0.f, 0.f}, pacc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                uint32_t a[4];
+                ldmatrix_x4(a, stage_piece(kst, krow, 2 * t + kpc));
+                mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], qa[2 * t], qa[2 * t + 1]);
+                ldmatrix_x4(a, stage_piece(vst, krow, 2 * t + kpc));
+                mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], da[2 * t], da[2 * t + 1]);
+            }
+            // keys c0 + gq, c0 + gq + 8 x heads 2 c4, 2 c4 + 1
+            float w[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = c0 + gq + 8 * h;
+                const uint32_t entry = at < U ? list[at] : 0u;
+                const float far = fabsf((float)(i - (int)(entry & 0xffffffu)));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    w[h][e] = 0.f;
+                    if (((entry >> (24 + 2 * c4 + e)) & 1u) && lse2[e] != -INFINITY) {
+                        float dx;
+                        const float p = exp2_fast(mods.score2_grad(sacc[2 * h + e], slope[e], far, dx, TanhFast()) - lse2[e]);
+                        const float dp = pacc[2 * h + e], pd = p * dp;
+                        w[h][e] = dx * (pd - p * d0[e]);
+                        a_pd[e] += pd;
+                        a_f[e] = fmaf(p, far, a_f[e]);
+                        a_pdf[e] = fmaf(pd, far, a_pdf[e]);
+                    }
+                }
+            }
+            const uint32_t b0 = movmatrix_trans(pack_bf16x2(w[0][0], w[0][1]));
+            const uint32_t b1 = movmatrix_trans(pack_bf16x2(w[1][0], w[1][1]));
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a, stage_piece(kst, trow, 2 * mt + tpc));
+                mma_bf16_16816_a4(acc[mt], a[0], a[1], a[2], a[3], b0, b1);
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) {
+            a_pd[e] += __shfl_xor_sync(kFull, a_pd[e], o);
+            a_f[e] += __shfl_xor_sync(kFull, a_f[e], o);
+            a_pdf[e] += __shfl_xor_sync(kFull, a_pdf[e], o);
+        }
+        if (gq == 0 && 2 * c4 + e < G) {
+            const size_t row = row0 + (size_t)(2 * c4 + e) * s.Nq;
+            delta[row] = a_pd[e];
+            if (slope_rows) slope_rows[row] = a_pd[e] * a_f[e] - a_pdf[e];
+        }
+    }
+    __nv_bfloat16* orow = dq + mine + 2 * c4;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+        const uint32_t lo = movmatrix_trans(pack_bf16x2(acc[mt][0], acc[mt][1]));
+        const uint32_t hi = movmatrix_trans(pack_bf16x2(acc[mt][2], acc[mt][3]));
+        if (gq < G) {
+            *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
+            *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ key pass
+//
+// One warp per kBwdTile entries of a turned list, in groups of 16 entries whose q and dO rows are
+// staged while the group before is computed.  For the part of a group that lies in one key's run:
+// S = Q k and dP = dO v (entries as MMA rows, the key in column 0), p and dX per entry, then
+// dv^T += dO^T p and dk^T += Q^T dX with the weights in columns 0 and 1: their bf16 value and what
+// the rounding left, so the weights count with 16 bits and the sums are as good as fp32 ones.
+constexpr int kKeyWarps = 4;
+constexpr int kKeyWarpBytes = 4 * kStageChunk + 2 * D * 4;  // q and dO rows of two groups; a finished run
+constexpr int kKeyBytes = kKeyWarps * kKeyWarpBytes;
+static_assert(3 * (kKeyBytes + 1024) <= 233472, "three CTAs per SM");
+
+// A key or value row as the B operand's column 0.
+__device__ __forceinline__ void load_column(const __nv_bfloat16* row, int gq, int c4, uint32_t (&r)[16]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(row);
+#pragma unroll
+    for (int t = 0; t < 16; ++t) r[t] = gq == 0 ? __ldg(w + 4 * t + c4) : 0u;
+}
+
+// Weights of entries gq, gq + 8 (valid where c4 == 0) as B operands: column 0 rounded, column 1 the rest.
+__device__ __forceinline__ void weight_columns(float w0, float w1, int c4, uint32_t& b0, uint32_t& b1) {
+    const float h0 = __bfloat162float(__float2bfloat16_rn(w0)), h1 = __bfloat162float(__float2bfloat16_rn(w1));
+    b0 = movmatrix_trans(c4 == 0 ? pack_bf16x2(h0, w0 - h0) : 0u);
+    b1 = movmatrix_trans(c4 == 0 ? pack_bf16x2(h1, w1 - h1) : 0u);
+}
+
+__global__ void __launch_bounds__(kKeyWarps * 32, 3)
+key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                    const __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ dout, const BwdShape s,
+                    const ScoreMods mods, const int* __restrict__ base, const int* __restrict__ list,
+                    const float* __restrict__ delta, __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv,
+                    float* __restrict__ part) {
+    extern __shared__ __align__(128) uint8_t msm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int gq = lane >> 2, c4 = lane & 3, kv = blockIdx.y;
+    const long long tile = (long long)blockIdx.x * kKeyWarps + warp;
+    const int* bs = base + (size_t)kv * (s.N + 1);
+    const int total = bs[s.N];
+    if (tile * kBwdTile >= total) return;  // warp-uniform; no CTA-wide barrier follows
+    const int t0 = (int)(tile * kBwdTile), t1 = min(total, t0 + kBwdTile);
+    const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
+    const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
+    const int* ls = list + (size_t)kv * s.cap;
+    const __nv_bfloat16* qb = q + rows0 * D;
+    const __nv_bfloat16* db = dout + rows0 * D;
+    uint8_t* stage = msm + (size_t)warp * kKeyWarpBytes;
+    const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
+    float* done = reinterpret_cast<float*>(stage + 4 * kStageChunk);
+    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
+    const int trow = (lane & 7) + (lane >> 4) * 8, tpc = (lane >> 3) & 1;
+
+    // entry lane & 15 of the group at pos: its row (-1 past the tile)
+    auto entry = [&](int pos) { return pos + (lane & 15) < t1 ? ls[pos + (lane & 15)] : -1; };
+    auto stage_rows = [&](int r, int buf) {
+        const uint32_t at = st + (uint32_t)(buf * 2 * kStageChunk);
+        const int pc = lane & 15;
+#pragma unroll
+        for (int t = 0; t < kStageRows / 2; ++t) {
+            const int row = 2 * t + (lane >> 4);
+            const int rr = __shfl_sync(kFull, r, row);
+            const size_t off = (size_t)max(rr, 0) * D + pc * 8;
+            stage_copy(stage_piece(at, row, pc), qb + off, rr >= 0);
+            stage_copy(stage_piece(at + kStageChunk, row, pc), db + off, rr >= 0);
+        }
+        stage_commit();
+    };
+    float ak[8][4], av[8][4];  // dims 16 mt + gq (+8); columns 0 and 1 (lanes with c4 == 0) count
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        ak[n][0] = ak[n][1] = ak[n][2] = ak[n][3] = 0.f;
+        av[n][0] = av[n][1] = av[n][2] = av[n][3] = 0.f;
+    }
+    int key = key_at(bs, s.N, t0);
+    int run0 = bs[key], run1 = bs[key + 1];
+    uint32_t kf[16], vf[16];
+    load_column(k + ((size_t)kv * s.N + key) * D, gq, c4, kf);
+    load_column(v + ((size_t)kv * s.N + key) * D, gq, c4, vf);
+    int r = entry(t0), r_next = entry(t0 + kStageRows);
+    stage_rows(r, 0);
+#pragma unroll 1
+    for (int pos = t0, buf = 0; pos < t1; pos += kStageRows, buf ^= 1) {
+        const int r_after = entry(pos + 2 * kStageRows);
+        // this lane's entry: statistic, Delta, position and slope
+        float lse2 = -INFINITY, dl = 0.f, slope = 0.f;
+        int i = 0;
+        if (r >= 0) {
+            lse2 = mods.lse2[rows0 + r];
+            dl = delta[rows0 + r];
+            if (mods.slopes) {
+                const int g = r / s.Nq;
+                i = s.q0 + r - g * s.Nq;
+                slope = mods.slopes[h0 + g];
+            }
+        }
+        __syncwarp();  // the group before is done with its buffer
+        if (pos + kStageRows < t1) {
+            stage_rows(r_next, buf ^ 1);
+            cp_async_wait_pending<1>();
+        } else {
+            cp_async_wait_pending<0>();
+        }
+        __syncwarp();
+        const uint32_t qst = st + (uint32_t)(buf * 2 * kStageChunk), dst = qst + kStageChunk;
+        const int end = min(pos + kStageRows, t1);
+#pragma unroll 1
+        for (int p0 = pos; p0 < end;) {
+            const int p1 = min(end, run1);  // entries p0 .. p1 - 1 are of this key
+            float sacc[4] = {0.f, 0.f, 0.f, 0.f}, pacc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                uint32_t a[4];
+                ldmatrix_x4(a, stage_piece(qst, krow, 2 * t + kpc));
+                mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], kf[2 * t], kf[2 * t + 1]);
+                ldmatrix_x4(a, stage_piece(dst, krow, 2 * t + kpc));
+                mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], vf[2 * t], vf[2 * t + 1]);
+            }
+            float p[2], w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // entry gq + 8 h
+                const int e = gq + 8 * h;
+                const float l = __shfl_sync(kFull, lse2, e), d = __shfl_sync(kFull, dl, e);
+                float far = 0.f, sl = 0.f;
+                if (mods.slopes) {  // warp-uniform
+                    sl = __shfl_sync(kFull, slope, e);
+                    far = fabsf((float)(__shfl_sync(kFull, i, e) - key));
+                }
+                float dx;
+                const float s2 = mods.score2_grad(sacc[2 * h], sl, far, dx, TanhFast());
+                const bool on = pos + e >= p0 && pos + e < p1 && l != -INFINITY;
+                p[h] = on ? exp2_fast(s2 - l) : 0.f;
+                w[h] = on ? dx * p[h] * (pacc[2 * h] - d) : 0.f;
+            }
+            uint32_t pb0, pb1, wb0, wb1;
+            weight_columns(p[0], p[1], c4, pb0, pb1);
+            weight_columns(w[0], w[1], c4, wb0, wb1);
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                uint32_t a[4];
+                ldmatrix_x4_trans(a, stage_piece(dst, trow, 2 * mt + tpc));
+                mma_bf16_16816_a4(av[mt], a[0], a[1], a[2], a[3], pb0, pb1);
+                ldmatrix_x4_trans(a, stage_piece(qst, trow, 2 * mt + tpc));
+                mma_bf16_16816_a4(ak[mt], a[0], a[1], a[2], a[3], wb0, wb1);
+            }
+            p0 = p1;
+            if (p1 < run1 && p1 < t1) continue;  // the run goes on in the next group
+            // the run, or the tile, ends here
+            __syncwarp();
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                if (c4 == 0) {
+                    done[16 * mt + gq] = ak[mt][0] + ak[mt][1];
+                    done[16 * mt + gq + 8] = ak[mt][2] + ak[mt][3];
+                    done[D + 16 * mt + gq] = av[mt][0] + av[mt][1];
+                    done[D + 16 * mt + gq + 8] = av[mt][2] + av[mt][3];
+                }
+                ak[mt][0] = ak[mt][1] = ak[mt][2] = ak[mt][3] = 0.f;
+                av[mt][0] = av[mt][1] = av[mt][2] = av[mt][3] = 0.f;
+            }
+            __syncwarp();
+            const float4 dk4 = reinterpret_cast<const float4*>(done)[lane];
+            const float4 dv4 = reinterpret_cast<const float4*>(done + D)[lane];
+            if (run0 >= t0 && run1 <= t1) {
+                const size_t at = ((size_t)kv * s.N + key) * D + 4 * lane;
+                *reinterpret_cast<uint2*>(dk + at) = make_uint2(pack_bf16x2(dk4.x, dk4.y), pack_bf16x2(dk4.z, dk4.w));
+                *reinterpret_cast<uint2*>(dv + at) = make_uint2(pack_bf16x2(dv4.x, dv4.y), pack_bf16x2(dv4.z, dv4.w));
+            } else {  // slot 0: the run began before this tile; slot 1: it begins here and goes on
+                float* ps = part + (((size_t)kv * s.tiles + tile) * 2 + (run0 < t0 ? 0 : 1)) * 2 * D;
+                reinterpret_cast<float4*>(ps)[lane] = dk4;
+                reinterpret_cast<float4*>(ps + D)[lane] = dv4;
+            }
+            if (p1 < t1) {  // on to the next listed key
+                do {
+                    ++key;
+                    run0 = run1;
+                    run1 = bs[key + 1];
+                } while (run1 <= p1);
+                load_column(k + ((size_t)kv * s.N + key) * D, gq, c4, kf);
+                load_column(v + ((size_t)kv * s.N + key) * D, gq, c4, vf);
+            }
+        }
+        r = r_next;
+        r_next = r_after;
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_row_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
+    const bool direct = s.N <= kUnionDirectKeys;
+#define OSSA_ROW_PICK(GG) (direct ? row_pass_mma_kernel<GG, true> : row_pass_mma_kernel<GG, false>)
+    auto kern = s.G == 2 ? OSSA_ROW_PICK(2)
+              : s.G == 3 ? OSSA_ROW_PICK(3)
+              : s.G == 4 ? OSSA_ROW_PICK(4)
+              : s.G == 6 ? OSSA_ROW_PICK(6)
+                         : OSSA_ROW_PICK(8);
+#undef OSSA_ROW_PICK
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes);
+    if (e != cudaSuccess) return e;
+    using T = __nv_bfloat16;
+    kern<<<dim3((s.Nq + kRowWarps - 1) / kRowWarps, s.B * s.Hkv), kRowWarps * 32, kRowBytes, stream>>>(
+        static_cast<const T*>(a.f.q), static_cast<const T*>(a.f.k), static_cast<const T*>(a.f.v), w.keys,
+        static_cast<const T*>(a.f.out), static_cast<const T*>(a.dout), s, a.f.mods, static_cast<T*>(a.dq), w.delta,
+        w.slope_rows);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+cudaError_t launch_key_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
+    cudaError_t e =
+        cudaFuncSetAttribute(key_pass_mma_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyBytes);
+    if (e != cudaSuccess) return e;
+    using T = __nv_bfloat16;
+    key_pass_mma_kernel<<<dim3((unsigned)((s.tiles + kKeyWarps - 1) / kKeyWarps), (unsigned)(s.B * s.Hkv)),
+                          kKeyWarps * 32, kKeyBytes, stream>>>(
+        static_cast<const T*>(a.f.q), static_cast<const T*>(a.f.k), static_cast<const T*>(a.f.v),
+        static_cast<const T*>(a.dout), s, a.f.mods, w.base, w.list, w.delta, static_cast<T*>(a.dk),
+        static_cast<T*>(a.dv), w.part);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
+}  // namespace ossa

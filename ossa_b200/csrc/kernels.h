@@ -37,20 +37,22 @@ struct ScoreMods {
 #ifdef __CUDACC__
     // Score in base 2 of a key at distance far from dot = q . k.  Scores that only masks modify are
     // the plain kernels' product, so that their results are too.
-    __device__ __forceinline__ float score2(float dot, float slope, float far) const {
+    template <typename Tanh>
+    __device__ __forceinline__ float score2(float dot, float slope, float far, Tanh tanh_of) const {
         if (!shaped) return dot * scale_log2;
         const float x = dot * scale;
-        const float s = cap > 0.f ? cap * tanhf(x * inv_cap) : x;
+        const float s = cap > 0.f ? cap * tanh_of(x * inv_cap) : x;
         return fmaf(-slope, far, s) * 1.4426950408889634f;
     }
     // The same, and d score / d dot in dx.
-    __device__ __forceinline__ float score2_grad(float dot, float slope, float far, float& dx) const {
+    template <typename Tanh>
+    __device__ __forceinline__ float score2_grad(float dot, float slope, float far, float& dx, Tanh tanh_of) const {
         dx = scale;
         if (!shaped) return dot * scale_log2;
         const float x = dot * scale;
         float s = x;
         if (cap > 0.f) {
-            const float t = tanhf(x * inv_cap);
+            const float t = tanh_of(x * inv_cap);
             s = cap * t;
             dx = scale * (1.f - t * t);
         }
@@ -77,6 +79,8 @@ struct GatherArgs {
 cudaError_t launch_gather_attn(const GatherArgs& a, cudaStream_t stream);
 // The same attention under a.mods (a.scale is not read: a.mods.scale is).
 cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream);
+// Whether the tensor-core forms of the modified gather and its backward pass take a shape.
+bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K);
 
 // Gradients of launch_gather_attn_mods (gather_bwd.cu).
 struct GatherBwdArgs {

@@ -1,0 +1,142 @@
+// The keys that the heads of one kv head list for one query, each key once with its heads, and their
+// staging in shared memory: what the tensor-core forms of the modified gather and of its backward
+// row pass share (bf16, D = 128, G query heads per kv head, at most 128 listed keys per head).
+//
+// A warp owns a query.  Keys come as x[t][e], entry lane + 32 e of head t, -1 where the entry is
+// masked.  The list holds key | heads << 24.  It is made in the order (head, entry) of the lowest head
+// that lists a key, so it does not depend on the order in which lanes run.
+#pragma once
+
+#include "common.cuh"
+
+namespace ossa {
+
+constexpr int kUnionCap = 512;          // keys a list holds
+constexpr int kUnionDirectKeys = 4096;  // keys covered by the direct head-bit array (a byte per key)
+constexpr int kUnionSlots = 1024;       // hash slots otherwise; at least G * K, so every key finds one
+constexpr int kUnionArea = 8192;        // bytes of shared memory the build needs besides the list
+constexpr int kUnionMaxKeys = 1 << 24;  // the list's key field
+
+// Returns the list's length, or -1 when a head lists a key twice or the list would not fit: the
+// caller then takes the heads one by one (single_list).
+template <int G, bool kDirect>
+__device__ __forceinline__ int build_union(const int (&x)[G][4], int K, int N, uint8_t* area, uint32_t* list, int lane) {
+    const unsigned lt = lanemask_lt();
+    uint32_t* bits = reinterpret_cast<uint32_t*>(area);  // direct: byte j, the heads of key j
+    int* skey = reinterpret_cast<int*>(area);            // hash: keys, then head bits
+    unsigned* smask = reinterpret_cast<unsigned*>(area) + kUnionSlots;
+    if constexpr (kDirect) {
+        for (int w = lane; w < (N + 15) >> 4; w += 32) reinterpret_cast<uint4*>(bits)[w] = make_uint4(0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+        for (int u = 0; u < kUnionSlots / 128; ++u) {
+            reinterpret_cast<int4*>(skey)[lane + 32 * u] = make_int4(-1, -1, -1, -1);
+            reinterpret_cast<uint4*>(smask)[lane + 32 * u] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __syncwarp();
+    bool twice = false;
+    int slot[G][4];
+#pragma unroll
+    for (int t = 0; t < G; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            slot[t][e] = 0;
+            if (32 * e >= K) continue;  // warp-uniform
+            const int xv = x[t][e];
+            if (xv < 0) continue;
+            if constexpr (kDirect) {
+                const uint32_t sh = 8u * (uint32_t)(xv & 3) + (uint32_t)t;
+                const uint32_t old = atomicOr(&bits[xv >> 2], 1u << sh);
+                twice = twice || ((old >> sh) & 1u) != 0u;
+            } else {
+                int at = (int)(((uint32_t)xv * 2654435761u) >> 22);  // 10 bits
+                for (int probe = 0; probe < kUnionSlots; ++probe) {
+                    const int old = atomicCAS(&skey[at], -1, xv);
+                    if (old == -1 || old == xv) break;
+                    at = (at + 1) & (kUnionSlots - 1);
+                }
+                const unsigned old = atomicOr(&smask[at], 1u << t);
+                twice = twice || ((old >> t) & 1u) != 0u;
+                slot[t][e] = at;
+            }
+        }
+    }
+    if (__any_sync(kFull, twice)) return -1;
+    int U = 0;
+#pragma unroll
+    for (int t = 0; t < G; ++t) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (32 * e >= K) continue;
+            const int xv = x[t][e];
+            unsigned mk = 0u;
+            bool own = false;
+            if (xv >= 0) {
+                mk = kDirect ? (bits[xv >> 2] >> (8u * (uint32_t)(xv & 3))) & 0xffu : smask[slot[t][e]];
+                own = (mk & ((1u << t) - 1u)) == 0u;  // no lower head lists it
+            }
+            const unsigned bal = __ballot_sync(kFull, own);
+            const int pos = U + __popc(bal & lt);
+            if (own && pos < kUnionCap) list[pos] = (uint32_t)xv | mk << 24;
+            U += __popc(bal);
+        }
+    }
+    return U <= kUnionCap ? U : -1;
+}
+
+// One head's keys as a list of their own, in the order listed (key(e): entry e of the head, -1 masked).
+template <typename Key>
+__device__ __forceinline__ int single_list(Key key, int t, int K, uint32_t* list, int lane) {
+    const unsigned lt = lanemask_lt();
+    int U = 0;
+    for (int e0 = 0; e0 < K; e0 += 32) {
+        const int xv = e0 + lane < K ? key(e0 + lane) : -1;
+        const unsigned bal = __ballot_sync(kFull, xv >= 0);
+        if (xv >= 0) list[U + __popc(bal & lt)] = (uint32_t)xv | (1u << t) << 24;
+        U += __popc(bal);
+    }
+    return U;
+}
+
+// Rows of 128 bf16 values in shared memory: 16-byte pieces XOR-swizzled by the row.
+constexpr int kStageRow = 256;
+constexpr int kStageRows = 16;
+constexpr int kStageChunk = kStageRows * kStageRow;
+
+__device__ __forceinline__ uint32_t stage_piece(uint32_t base, int row, int piece) {
+    return base + (uint32_t)(row * kStageRow + ((piece ^ (row & 7)) << 4));
+}
+
+__device__ __forceinline__ void stage_copy(uint32_t dst, const void* src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Copies the rows of list entries c0 .. c0 + 15 (zeros past U) of one tensor.
+__device__ __forceinline__ void stage_listed(uint32_t dst, const __nv_bfloat16* base, const uint32_t* list, int c0, int U,
+                                             int lane) {
+    const int pc = lane & 15;
+#pragma unroll
+    for (int r = 0; r < kStageRows / 2; ++r) {
+        const int row = 2 * r + (lane >> 4);
+        const bool on = c0 + row < U;
+        const size_t key = on ? list[c0 + row] & 0xffffffu : 0u;
+        stage_copy(stage_piece(dst, row, pc), base + key * 128 + pc * 8, on);
+    }
+}
+
+// 2^x and tanh for the tensor-core forms.  ex2.approx: two units in the last place.  tanh x = 1 - 2 / (1 + e^2x)
+// is good to 2^-22 in absolute terms, which a score of size cap turns into cap * 2^-22.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float tanh_fast(float x) {
+    return 1.f - __fdividef(2.f, 1.f + exp2_fast(x * 2.885390081777927f));
+}
+
+}  // namespace ossa

@@ -13,6 +13,10 @@ namespace ossa {
 
 constexpr float kLog2E = 1.4426950408889634f;
 
+struct TanhExact {
+    __device__ __forceinline__ float operator()(float x) const { return tanhf(x); }
+};
+
 // What one query row needs of the modifiers (kMods = false: nothing but the causal rule).
 template <bool kMods>
 struct RowMods {
@@ -38,7 +42,7 @@ struct RowMods<true> {
         return (!causal || j <= i || j < prefix) && (!seg || __ldg(seg + j) == seg_i);
     }
     __device__ __forceinline__ float score2(float dot, int i, int j) const {
-        return m.score2(dot, slope, fabsf((float)(i - j)));
+        return m.score2(dot, slope, fabsf((float)(i - j)), TanhExact());
     }
 };
 

@@ -16,7 +16,8 @@ are rejected.  Differences, all additive:
   with distance), ``segments`` (documents packed in one row) and ``prefix_len`` (keys
   that every query may see).
 * (additive) gradients: where q, k, v or slopes require them, the output carries
-  autograd history (``ossa_topk_attention_bwd``); the forward's values are the same.
+  autograd history (``ossa_topk_attention_bwd``); the forward's values are then the
+  same to rounding (a bf16 output sums its keys in another order).
 """
 
 from __future__ import annotations

@@ -90,7 +90,8 @@ def _check(dtype, q, k, v, do, idx, m, *, causal=True, q0=0):
     grads = torch.autograd.grad(out, dev, do.to(DEV))
     with torch.no_grad():
         again = topk_attention(dev[0], dev[1], dev[2], topk_indices=idx.to(DEV), causal=causal, **rows, **dm)
-    assert torch.equal(out.detach(), again)  # the statistic for the backward pass changes nothing
+    if m:
+        assert torch.equal(out.detach(), again)  # the statistic for the backward pass changes nothing
     out = out.detach().cpu()
     fine = score_step(q, k) + (K + D) * 2.0 ** -24
     step = 0.0 if dtype == torch.float32 else STEP
@@ -197,9 +198,9 @@ def test_masked_places_hold_anything():
             assert (res[0][2][:, :, 50] == 0).all() and (res[0][3][:, :, :6] == 0).all()
 
 
-def test_plain_call_is_unchanged_and_differentiable():
-    """Without modifiers the values are those of the call without gradients, bit for bit (the plain
-    kernels), whatever the gradient mode; the modified kernels with neutral modifiers agree to rounding."""
+def test_plain_call_and_training_form_agree():
+    """Without modifiers and gradients the plain kernels run.  The training form and neutral modifiers
+    give the same values to rounding: both round p and the output, 2 steps each."""
     B, H, Hkv, N, D, K = 2, 12, 2, 300, 128, 64
     q, k, v, do = (t.to(DEV) for t in _inputs(torch.bfloat16, B, H, Hkv, N, N, D, seed=6))
     idx = _lists(B, H, N, N, K, 0, seed=1).to(DEV)
@@ -207,9 +208,13 @@ def test_plain_call_is_unchanged_and_differentiable():
     assert not plain.requires_grad
     leaf = q.clone().requires_grad_()
     out = topk_attention(leaf, k, v, topk_indices=idx)
-    assert out.requires_grad and torch.equal(out.detach(), plain)
+    assert out.requires_grad and rel(out.detach(), plain) < 4 * STEP
     neutral = topk_attention(q, k, v, topk_indices=idx, slopes=torch.zeros(H, device=DEV))
-    assert rel(neutral, plain) < 2 * STEP
+    assert rel(neutral, plain) < 4 * STEP
+    for dtype, d in ((torch.float32, 128), (torch.bfloat16, 64)):  # per-head forms: the same bits
+        q, k, v, do = (t.to(DEV) for t in _inputs(dtype, B, H, Hkv, N, N, d, seed=6))
+        out = topk_attention(q.requires_grad_(), k, v, topk_indices=idx)
+        assert torch.equal(out.detach(), topk_attention(q.detach(), k, v, topk_indices=idx))
 
 
 def test_same_bits_every_call():
