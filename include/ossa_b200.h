@@ -292,8 +292,8 @@ OSSA_API int ossa_topk_attention_mod_fwd(const void* q, const void* k, const voi
  * twice counts twice, as in the forward.  Repeated calls give the same bits (no float
  * atomics).  At most 2^30 listed keys per (b, kv head): (H / Hkv) * Nq * K.
  */
-OSSA_API size_t ossa_topk_attention_bwd_workspace_size(int B, int H, int Hkv, int Nq, int Nk, int D, int K,
-                                                       int want_dslopes);
+OSSA_API size_t ossa_topk_attention_bwd_workspace_size(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D,
+                                                       int K, int want_dslopes);
 OSSA_API int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64,
                                      int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale,
                                      int causal, int q_start, float softcap, const float* slopes,

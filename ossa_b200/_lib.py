@@ -121,7 +121,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     cl = ctypes.c_longlong
     lib.ossa_topk_attention_mod_fwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf, vp, vp, vp, vp, vp, vp]
     lib.ossa_topk_attention_mod_fwd.restype = ci
-    lib.ossa_topk_attention_bwd_workspace_size.argtypes = [ci] * 8
+    lib.ossa_topk_attention_bwd_workspace_size.argtypes = [ci] * 9
     lib.ossa_topk_attention_bwd_workspace_size.restype = sz
     lib.ossa_topk_attention_bwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf] + [vp] * 11 + [sz, vp]
     lib.ossa_topk_attention_bwd.restype = ci

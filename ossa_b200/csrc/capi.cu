@@ -323,9 +323,10 @@ int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, con
     return cuda_status(ossa::launch_gather_attn_mods(a, s), "modified topk attention launch");
 }
 
-size_t ossa_topk_attention_bwd_workspace_size(int B, int H, int Hkv, int Nq, int Nk, int D, int K, int want_dslopes) {
-    if (B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Nq < 0 || Nk < 0 || D <= 0 || K < 0) return 0;
-    return ossa::gather_bwd_workspace_bytes(B, H, Hkv, Nq, Nk, D, K, want_dslopes != 0);
+size_t ossa_topk_attention_bwd_workspace_size(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K,
+                                              int want_dslopes) {
+    if (!valid_dtype(dtype) || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Nq < 0 || Nk < 0 || D <= 0 || K < 0) return 0;
+    return ossa::gather_bwd_workspace_bytes(dtype, B, H, Hkv, Nq, Nk, D, K, want_dslopes != 0);
 }
 
 int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64, int dtype,
@@ -355,7 +356,7 @@ int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const v
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(indices) || !aligned16(dout) ||
         !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
         return fail(OSSA_ERR_INVALID, "q, k, v, indices, out, dout, dq, dk and dv must be 16-byte aligned");
-    const size_t need = ossa::gather_bwd_workspace_bytes(B, H, Hkv, Nq, Nk, D, K, dslopes != nullptr);
+    const size_t need = ossa::gather_bwd_workspace_bytes(dtype, B, H, Hkv, Nq, Nk, D, K, dslopes != nullptr);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
                     workspace ? workspace_bytes : (size_t)0);

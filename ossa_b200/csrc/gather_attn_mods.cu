@@ -75,9 +75,7 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         if (U < 0) passes = G;
     }
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage), vst = st + 2u * kStageChunk;
-    // ldmatrix rows: keys as the A operand of S^T, values transposed as the A operand of O^T
-    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
-    const int vrow = (lane & 7) + (lane >> 4) * 8, vpc = (lane >> 3) & 1;
+    const StageLane sl(lane);
     float oacc[8][4];  // O^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
 #pragma unroll
     for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
@@ -94,7 +92,7 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         __syncwarp();  // the list is complete, the staging area is free
         const int nch = (U + kStageRows - 1) / kStageRows;
         if (nch > 0) {
-            stage_listed(st, kb, list, 0, U, lane);
+            stage_listed(st, kb, list, 0, U, sl, lane);
             stage_commit();
         }
 #pragma unroll 1
@@ -102,10 +100,10 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             const int c0 = c * kStageRows;
             const bool more = c + 1 < nch;  // warp-uniform
             __syncwarp();                   // chunk c - 1 is done with the value rows and key buffer (c + 1) & 1
-            stage_listed(vst, vb, list, c0, U, lane);
+            stage_listed(vst, vb, list, c0, U, sl, lane);
             stage_commit();
             if (more) {
-                stage_listed(st + (uint32_t)(((c + 1) & 1) * kStageChunk), kb, list, c0 + kStageRows, U, lane);
+                stage_listed(st + (uint32_t)(((c + 1) & 1) * kStageChunk), kb, list, c0 + kStageRows, U, sl, lane);
                 stage_commit();
                 cp_async_wait_pending<2>();
             } else {
@@ -113,13 +111,17 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             }
             __syncwarp();
             const uint32_t kst = st + (uint32_t)((c & 1) * kStageChunk);
-            float sacc[4] = {0.f, 0.f, 0.f, 0.f};
+            float sacc[4] = {0.f, 0.f, 0.f, 0.f}, sacc2[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of half the length
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
+            for (int s = 0; s < 4; ++s) {  // keys as the A operand
                 uint32_t a[4];
-                ldmatrix_x4(a, stage_piece(kst, krow, 2 * s + kpc));
+                ldmatrix_x4<0>(a, kst + sl.a[s]);
                 mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], qa[2 * s], qa[2 * s + 1]);
+                ldmatrix_x4<128>(a, kst + sl.a[s]);
+                mma_bf16_16816_a4(sacc2, a[0], a[1], a[2], a[3], qa[2 * s + 8], qa[2 * s + 9]);
             }
+#pragma unroll
+            for (int s = 0; s < 4; ++s) sacc[s] += sacc2[s];
             // keys c0 + gq, c0 + gq + 8 x heads 2 c4, 2 c4 + 1; a head's scores sit in the lanes of equal c4
             float sc[2][2];
 #pragma unroll
@@ -163,10 +165,12 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             else cp_async_wait_pending<0>();
             __syncwarp();
 #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
+            for (int mt = 0; mt < 4; ++mt) {  // values transposed as the A operand
                 uint32_t a[4];
-                ldmatrix_x4_trans(a, stage_piece(vst, vrow, 2 * mt + vpc));
+                ldmatrix_x4_trans<0>(a, vst + sl.at[mt]);
                 mma_bf16_16816_a4(oacc[mt], a[0], a[1], a[2], a[3], pb0, pb1);
+                ldmatrix_x4_trans<128>(a, vst + sl.at[mt]);
+                mma_bf16_16816_a4(oacc[mt + 4], a[0], a[1], a[2], a[3], pb0, pb1);
             }
         }
     }

@@ -9,9 +9,11 @@
 //
 //  1. The index lists are turned round: for every (b, kv head) the rows that list a key,
 //     key by key, in a fixed order (a counting sort: units of (row chunk, head) count their
-//     entries per key, the counts are scanned, every unit then writes its rows).
+//     entries per key, the counts are scanned, every unit then writes its rows).  For the
+//     tensor-core key pass "key" is a block of 8 keys: neighbouring entries of an ascending list
+//     that fall into one block make one turned entry with a bit per key.
 //  2. Row pass, one warp per row: dq_i, Delta_i and the row's share of dslope.
-//  3. Key pass, one warp per kBwdTile consecutive entries of a turned list, which may begin and
+//  3. Key pass, one warp per `tile` consecutive entries of a turned list, which may begin and
 //     end inside a key's run: whole runs are stored, cut ones go to per-tile partial sums.
 //  4. Join: keys whose run is cut add their partial sums in tile order; keys that nobody
 //     lists get zeros.
@@ -34,12 +36,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kKeyRange = 8192;  // keys that one CTA of the counting sort covers (32 KB of counters)
-constexpr int kMaxChunks = 32;   // row chunks of the counting sort per head
+constexpr int kKeyRange = 8192;  // key blocks that one CTA of the counting sort covers (32 KB of counters)
+constexpr int kMaxChunks = 64;   // row chunks of the counting sort per head
 constexpr int kMinChunkRows = 32;
 constexpr int kPlaceRows = 8;    // rows whose entries the counting sort's last step has in flight
 
-BwdShape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
+BwdShape make_shape(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int K) {
     BwdShape s{};
     s.B = B;
     s.H = H;
@@ -49,11 +51,20 @@ BwdShape make_shape(int B, int H, int Hkv, int Nq, int N, int D, int K) {
     s.N = N;
     s.D = D;
     s.K = K;
-    s.chunks = std::max(1, std::min(kMaxChunks, Nq / kMinChunkRows));
+    const bool mma = gather_bwd_mma_serves(dtype, H, Hkv, Nq, N, D, K);
+    s.shift = mma ? kKeyBlockShift : 0;
+    s.NB = (N + (1 << s.shift) - 1) >> s.shift;
+    const long long kv = (long long)B * Hkv;
+    // one warp per unit in the sort's last step: enough units for 12 warps per SM, rows permitting
+    const long long want = 12ll * device_sm_count() / std::max(kv * s.G, 1ll);
+    s.chunks = (int)std::max(1ll, std::min({want, (long long)kMaxChunks, (long long)Nq / kMinChunkRows}));
     s.chunk_rows = (Nq + s.chunks - 1) / s.chunks;
     s.units = s.chunks * s.G;
     s.cap = (long long)s.G * Nq * K;
-    s.tiles = (s.cap + kBwdTile - 1) / kBwdTile;
+    // tiles: long ones store fewer cut runs, short ones fill the device (24 warps per SM)
+    const long long fair = kv * s.cap / (24ll * device_sm_count());
+    s.tile = (int)std::min(std::max((fair + 15) / 16 * 16, 64ll), mma ? 512ll : 256ll);
+    s.tiles = (s.cap + s.tile - 1) / s.tile;
     return s;
 }
 
@@ -67,26 +78,47 @@ Layout make_layout(const BwdShape& s, bool dslopes) {
     Layout l;
     l.keys = 0;
     l.counts = l.keys + up(rows * s.K * 4);
-    l.base = l.counts + up(kv * s.units * s.N * 4);
-    l.list = l.base + up(kv * ((size_t)s.N + 1) * 4);
+    l.base = l.counts + up(kv * s.units * s.NB * 4);
+    l.list = l.base + up(kv * ((size_t)s.NB + 1) * 4);
     l.delta = l.list + up(kv * s.cap * 4);
     l.part = l.delta + up(rows * 4);
-    l.slope_rows = l.part + up(kv * s.tiles * 4 * s.D * 4);
+    l.slope_rows = l.part + up(kv * s.tiles * 4 * ((size_t)s.D << s.shift) * 4);
     l.total = l.slope_rows + (dslopes ? up(rows * 4) : 0);
     return l;
 }
 
 // ------------------------------------------------------------------ 1. turned lists
 
+// A row's entries 32 e .. 32 e + 31, one per lane (key, -1: masked).  An entry follows the one before it
+// when its key is greater and in the same block; the first of such a chain stands for all, with a bit per
+// key of the block in `mask` (shift 0: every entry for itself).
+__device__ __forceinline__ bool chain_head(int key, int shift, int lane, uint32_t& mask) {
+    const int prev = __shfl_up_sync(kFull, key, 1);
+    const bool follows = shift > 0 && lane > 0 && key >= 0 && prev >= 0 && prev < key && (prev >> shift) == (key >> shift);
+    mask = 0u;
+    if (shift > 0) {  // warp-uniform
+        const unsigned tails = __ballot_sync(kFull, follows);
+        mask = key >= 0 ? 1u << (key & (kKeyBlock - 1)) : 0u;
+        // OR over the chain behind this lane: at most kKeyBlock entries, so three doublings
+#pragma unroll
+        for (int o = 1; o < kKeyBlock; o <<= 1) {
+            const uint32_t other = __shfl_down_sync(kFull, mask, o);
+            const unsigned all = (1u << o) - 1u;  // lanes lane + 1 .. lane + o
+            if ((((tails >> 1) >> lane) & all) == all) mask |= other;
+        }
+    }
+    return key >= 0 && !follows;
+}
+
 // keys: the lists as int32, -1 where an entry is outside [0, N) or not seen by its row.
-// counts[kv][unit][key]: how often the unit's rows list the key and see it.
+// counts[kv][unit][block]: the unit's entries of the key block's turned list.
 template <typename IdxT>
 __global__ void __launch_bounds__(kThreads)
 count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mods, int* __restrict__ keys,
              int* __restrict__ counts) {
-    extern __shared__ int hist[];  // min(N, kKeyRange)
+    extern __shared__ int hist[];  // min(NB, kKeyRange)
     const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
-    const int nk = min(kKeyRange, s.N - k0);
+    const int nk = min(kKeyRange, s.NB - k0);
     const int b = kv / s.Hkv, h = (kv - b * s.Hkv) * s.G + unit % s.G;
     const int r0 = unit / s.G * s.chunk_rows, r1 = min(s.Nq, r0 + s.chunk_rows);
     for (int t = threadIdx.x; t < nk; t += kThreads) hist[t] = 0;
@@ -96,44 +128,54 @@ count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mod
         const int i = s.q0 + il;
         const RowMods<true> rm(mods, b, h, s.N, i);
         const size_t row = ((size_t)b * s.H + h) * s.Nq + il;
-        for (int e = lane; e < s.K; e += 32) {
-            const long long j = (long long)idx[row * s.K + e];
-            const bool on = j >= 0 && j < s.N && rm.sees(j, i, s.causal);
-            if (blockIdx.z == 0) keys[row * s.K + e] = on ? (int)j : -1;
-            if (on && j >= k0 && j < k0 + nk) atomicAdd(&hist[j - k0], 1);
+        for (int e0 = 0; e0 < s.K; e0 += 32) {
+            const int e = e0 + lane;
+            const long long j = e < s.K ? (long long)idx[row * s.K + e] : -1ll;
+            const int key = j >= 0 && j < s.N && rm.sees(j, i, s.causal) ? (int)j : -1;
+            if (blockIdx.z == 0 && e < s.K) keys[row * s.K + e] = key;
+            uint32_t mask;
+            const bool head = chain_head(key, s.shift, lane, mask);
+            const int at = (key >> s.shift) - k0;
+            if (head && (unsigned)at < (unsigned)nk) atomicAdd(&hist[at], 1);
         }
     }
     __syncthreads();
-    int* out = counts + ((size_t)kv * s.units + unit) * s.N + k0;
+    int* out = counts + ((size_t)kv * s.units + unit) * s.NB + k0;
     for (int t = threadIdx.x; t < nk; t += kThreads) out[t] = hist[t];
 }
 
-// counts -> exclusive prefix over the units, and the key's total in base[kv][key].
+// counts -> exclusive prefix over the units, and the block's total in base[kv][block].
 __global__ void __launch_bounds__(kThreads)
 unit_scan_kernel(const BwdShape s, int* __restrict__ counts, int* __restrict__ base) {
+    constexpr int kAhead = 16;  // loads in flight
     const int key = blockIdx.x * kThreads + threadIdx.x, kv = blockIdx.y;
-    if (key >= s.N) return;
-    int* c = counts + (size_t)kv * s.units * s.N + key;
+    if (key >= s.NB) return;
+    int* c = counts + (size_t)kv * s.units * s.NB + key;
     int sum = 0;
-    for (int u = 0; u < s.units; ++u) {
-        const int x = c[(size_t)u * s.N];
-        c[(size_t)u * s.N] = sum;
-        sum += x;
+    for (int u0 = 0; u0 < s.units; u0 += kAhead) {
+        int x[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) x[u] = u0 + u < s.units ? c[(size_t)(u0 + u) * s.NB] : 0;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (u0 + u < s.units) c[(size_t)(u0 + u) * s.NB] = sum;
+            sum += x[u];
+        }
     }
-    base[(size_t)kv * (s.N + 1) + key] = sum;
+    base[(size_t)kv * (s.NB + 1) + key] = sum;
 }
 
-// base[kv][0..N]: exclusive prefix of the totals over the keys.
+// base[kv][0..NB]: exclusive prefix of the totals over the blocks.
 __global__ void __launch_bounds__(1024) key_scan_kernel(const BwdShape s, int* __restrict__ base) {
     __shared__ int wsum[32];
     __shared__ int carry;
-    int* p = base + (size_t)blockIdx.x * (s.N + 1);
+    int* p = base + (size_t)blockIdx.x * (s.NB + 1);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) carry = 0;
     __syncthreads();
-    for (int k0 = 0; k0 < s.N; k0 += 1024) {
+    for (int k0 = 0; k0 < s.NB; k0 += 1024) {
         const int k = k0 + threadIdx.x;
-        const int x = k < s.N ? p[k] : 0;
+        const int x = k < s.NB ? p[k] : 0;
         int y = x;  // inclusive over the warp
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -153,30 +195,30 @@ __global__ void __launch_bounds__(1024) key_scan_kernel(const BwdShape s, int* _
         }
         __syncthreads();
         const int before = carry + (warp ? wsum[warp - 1] : 0) + y - x;
-        if (k < s.N) p[k] = before;
+        if (k < s.NB) p[k] = before;
         __syncthreads();
         if (threadIdx.x == 1023) carry = before + x;
         __syncthreads();
     }
-    if (threadIdx.x == 0) p[s.N] = carry;
+    if (threadIdx.x == 0) p[s.NB] = carry;
 }
 
-// list[kv][position] = g * Nq + il of the rows that list a key, key by key.  One warp walks the
+// list[kv][position] = r (| mask << 24) with r = g * Nq + il of the rows that list a key block, block by block.  One warp walks the
 // unit's rows in a fixed order, the counters of its key range in shared memory; the entries of
 // kPlaceRows rows are loaded together, and the next ones while these are placed, so a step costs
 // one trip to L2 and not one per row.
 __global__ void __launch_bounds__(32)
 place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restrict__ counts,
              const int* __restrict__ base, int* __restrict__ list) {
-    extern __shared__ int next[];  // min(N, kKeyRange)
+    extern __shared__ int next[];  // min(NB, kKeyRange)
     const int unit = blockIdx.x, kv = blockIdx.y, k0 = blockIdx.z * kKeyRange;
-    const int nk = min(kKeyRange, s.N - k0);
+    const int nk = min(kKeyRange, s.NB - k0);
     const int g = unit % s.G;
     const int b = kv / s.Hkv, h = (kv - b * s.Hkv) * s.G + g;
     const int r0 = unit / s.G * s.chunk_rows, r1 = min(s.Nq, r0 + s.chunk_rows);
     const int lane = threadIdx.x;
-    const int* c = counts + ((size_t)kv * s.units + unit) * s.N + k0;
-    const int* bs = base + (size_t)kv * (s.N + 1) + k0;
+    const int* c = counts + ((size_t)kv * s.units + unit) * s.NB + k0;
+    const int* bs = base + (size_t)kv * (s.NB + 1) + k0;
     for (int t = lane; t < nk; t += 32) next[t] = c[t] + bs[t];
     __syncwarp();
     int* out = list + (size_t)kv * s.cap;
@@ -187,7 +229,7 @@ place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restri
         const int il = r0 + step / parts * kPlaceRows, e = (step % parts) * 32 + lane;
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t)
-            j[t] = step < steps && il + t < r1 && e < s.K ? rows[(size_t)(il + t) * s.K + e] - k0 : -1;
+            j[t] = step < steps && il + t < r1 && e < s.K ? rows[(size_t)(il + t) * s.K + e] : -1;
     };
     int j[kPlaceRows], ahead[kPlaceRows];
     load(0, j);
@@ -195,14 +237,17 @@ place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restri
         load(step + 1, ahead);
         const int il = r0 + step / parts * kPlaceRows;
         int pos[kPlaceRows];
+        uint32_t mask[kPlaceRows];
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t) {
-            pos[t] = (unsigned)j[t] < (unsigned)nk ? atomicAdd(&next[j[t]], 1) : -1;
+            const bool head = chain_head(j[t], s.shift, lane, mask[t]);
+            const int at = (j[t] >> s.shift) - k0;
+            pos[t] = head && (unsigned)at < (unsigned)nk ? atomicAdd(&next[at], 1) : -1;
             __syncwarp();  // a row's places before the next row's
         }
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t) {
-            if (pos[t] >= 0) out[pos[t]] = g * s.Nq + il + t;
+            if (pos[t] >= 0) out[pos[t]] = (int)((uint32_t)(g * s.Nq + il + t) | mask[t] << 24);
             j[t] = ahead[t];
         }
     }
@@ -316,6 +361,7 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
 
 // ------------------------------------------------------------------ 3. key pass
 
+// Blocks of one key (shift 0).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
 key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ dout,
@@ -326,12 +372,12 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     const long long tile = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int* bs = base + (size_t)kv * (s.N + 1);
     const int total = bs[s.N];
-    if (tile * kBwdTile >= total) return;  // warp-uniform
-    const int t0 = (int)(tile * kBwdTile), t1 = min(total, t0 + kBwdTile);
+    if (tile * s.tile >= total) return;  // warp-uniform
+    const int t0 = (int)(tile * s.tile), t1 = min(total, t0 + s.tile);
     const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
     const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
     const int* ls = list + (size_t)kv * s.cap;
-    int key = key_at(bs, s.N, t0);
+    int key = block_at(bs, s.N, t0);
     for (int pos = t0; pos < t1; ++key) {
         const int run0 = bs[key], run1 = bs[key + 1];
         const int end = min(run1, t1);
@@ -405,22 +451,25 @@ join_kernel(const BwdShape s, const int* __restrict__ base, const float* __restr
     const int lane = threadIdx.x & 31, kv = blockIdx.y;
     const int key = blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (key >= s.N) return;
-    const int* bs = base + (size_t)kv * (s.N + 1);
-    const int run0 = bs[key], run1 = bs[key + 1];
-    const int first = run0 / kBwdTile, last = run1 > run0 ? (run1 - 1) / kBwdTile : first;
+    const int* bs = base + (size_t)kv * (s.NB + 1);
+    const int blk = key >> s.shift, kk = key - (blk << s.shift);
+    const int run0 = bs[blk], run1 = bs[blk + 1];
+    const int first = run0 / s.tile, last = run1 > run0 ? (run1 - 1) / s.tile : first;
     if (run1 > run0 && first == last) return;  // stored by the key pass
-    const float* ps = part + (size_t)kv * s.tiles * 4 * s.D;
+    const size_t slot = (size_t)2 * (s.D << s.shift);  // floats of a tile's slot
+    const float* ps = part + (size_t)kv * s.tiles * 2 * slot;
     T* ok = dk + ((size_t)kv * s.N + key) * s.D;
     T* ov = dv + ((size_t)kv * s.N + key) * s.D;
     for (int d = lane; d < 2 * s.D; d += 32) {
+        const int which = d >= s.D, dd = d - which * s.D;
+        const size_t at = (size_t)which * (s.D << s.shift) + (size_t)kk * s.D + dd;
         float t = 0.f;
         if (run1 > run0) {
-            t = ps[((size_t)first * 2 + 1) * 2 * s.D + d];
+            t = ps[((size_t)first * 2 + 1) * slot + at];
 #pragma unroll 4
-            for (int i = first + 1; i <= last; ++i) t += ps[(size_t)i * 2 * 2 * s.D + d];
+            for (int i = first + 1; i <= last; ++i) t += ps[(size_t)i * 2 * slot + at];
         }
-        if (d < s.D) store_from_f32(ok + d, t);
-        else store_from_f32(ov + d - s.D, t);
+        store_from_f32((which ? ov : ok) + dd, t);
     }
 }
 
@@ -451,12 +500,12 @@ cudaError_t launched() {
 template <typename IdxT>
 cudaError_t sort_lists(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
     const unsigned kvs = (unsigned)(s.B * s.Hkv);
-    const dim3 grid((unsigned)s.units, kvs, (unsigned)((s.N + kKeyRange - 1) / kKeyRange));
-    const size_t smem = (size_t)std::min(s.N, kKeyRange) * sizeof(int);
+    const dim3 grid((unsigned)s.units, kvs, (unsigned)((s.NB + kKeyRange - 1) / kKeyRange));
+    const size_t smem = (size_t)std::min(s.NB, kKeyRange) * sizeof(int);
     cudaError_t e;
     count_kernel<IdxT><<<grid, kThreads, smem, stream>>>(static_cast<const IdxT*>(a.f.idx), s, a.f.mods, w.keys, w.counts);
     if ((e = launched()) != cudaSuccess) return e;
-    unit_scan_kernel<<<dim3((unsigned)((s.N + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, w.counts, w.base);
+    unit_scan_kernel<<<dim3((unsigned)((s.NB + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, w.counts, w.base);
     if ((e = launched()) != cudaSuccess) return e;
     key_scan_kernel<<<kvs, 1024, 0, stream>>>(s, w.base);
     if ((e = launched()) != cudaSuccess) return e;
@@ -475,7 +524,7 @@ cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuf
     const unsigned row_grid = (unsigned)((rows + kWarps - 1) / kWarps);
     const dim3 key_grid((unsigned)((s.tiles + kWarps - 1) / kWarps), kvs);
     cudaError_t e;
-    if (gather_mma_serves(a.f.dtype, s.H, s.Hkv, s.N, s.D, s.K)) {
+    if (s.shift > 0) {
         if ((e = launch_row_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
         if ((e = launch_key_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
     } else {
@@ -506,12 +555,16 @@ cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuf
 
 }  // namespace
 
-size_t gather_bwd_workspace_bytes(int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes) {
-    return make_layout(make_shape(B, H, Hkv, Nq, N, D, K), dslopes).total;
+bool gather_bwd_mma_serves(int dtype, int H, int Hkv, int Nq, int N, int D, int K) {
+    return gather_mma_serves(dtype, H, Hkv, N, D, K) && (long long)(H / Hkv) * Nq < (1ll << 24);
+}
+
+size_t gather_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes) {
+    return make_layout(make_shape(dtype, B, H, Hkv, Nq, N, D, K), dslopes).total;
 }
 
 cudaError_t launch_gather_attn_bwd(const GatherBwdArgs& a, cudaStream_t stream) {
-    BwdShape s = make_shape(a.f.B, a.f.H, a.f.Hkv, a.f.Nq, a.f.N, a.f.D, a.f.K);
+    BwdShape s = make_shape(a.f.dtype, a.f.B, a.f.H, a.f.Hkv, a.f.Nq, a.f.N, a.f.D, a.f.K);
     s.q0 = a.f.q0;
     s.causal = a.f.causal;
     const Layout l = make_layout(s, a.dslopes != nullptr);

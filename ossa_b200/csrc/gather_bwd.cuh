@@ -7,31 +7,37 @@
 
 namespace ossa {
 
-constexpr int kBwdTile = 256;  // entries that a warp of the key pass takes
+// The tensor-core key pass takes blocks of 8 neighbouring keys (one MMA's columns): a turned list then
+// holds rows with the block's keys that they list as a bit mask, r | mask << 24.  The other key pass
+// takes single keys, its list plain rows r.
+constexpr int kKeyBlockShift = 3;
+constexpr int kKeyBlock = 1 << kKeyBlockShift;
 
 struct BwdShape {
     int B, H, Hkv, G, Nq, N, D, K, q0, causal;
+    int shift, NB;                  // keys per block as a shift, key blocks
     int chunks, chunk_rows, units;  // units = chunks * G per (b, kv head)
     long long cap;                  // entries per (b, kv head) at most
+    int tile;                       // entries that a warp of the key pass takes
     long long tiles;                // key-pass tiles per (b, kv head) at most
 };
 
 struct BwdBuffers {
     int* keys;          // (B*H*Nq, K) lists, -1 where masked
-    int* counts;        // (B*Hkv, units, N)
-    int* base;          // (B*Hkv, N + 1) start of each key's run
-    int* list;          // (B*Hkv, cap) rows g * Nq + il, key by key
+    int* counts;        // (B*Hkv, units, NB)
+    int* base;          // (B*Hkv, NB + 1) start of each key block's run
+    int* list;          // (B*Hkv, cap) rows r = g * Nq + il, block by block
     float* delta;       // (B*H*Nq,) sum of p dP
-    float* part;        // (B*Hkv, tiles, 2, 2, D) sums of runs that a tile's border cuts
+    float* part;        // (B*Hkv, tiles, 2, 2, keys per block, D) sums of runs that a tile's border cuts
     float* slope_rows;  // (B*H*Nq,) or nullptr
 };
 
 cudaError_t launch_row_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream);
 cudaError_t launch_key_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream);
 
-// The key whose run holds position pos (base[key] <= pos < base[key + 1]).
-__device__ __forceinline__ int key_at(const int* __restrict__ base, int N, int pos) {
-    int lo = 0, hi = N;  // base[lo] <= pos < base[hi]
+// The block whose run holds position pos (base[block] <= pos < base[block + 1]).
+__device__ __forceinline__ int block_at(const int* __restrict__ base, int NB, int pos) {
+    int lo = 0, hi = NB;  // base[lo] <= pos < base[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (__ldg(base + mid) <= pos) lo = mid;

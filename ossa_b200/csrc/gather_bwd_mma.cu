@@ -101,16 +101,15 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         if (U < 0) passes = G;
     }
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
-    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
-    const int trow = (lane & 7) + (lane >> 4) * 8, tpc = (lane >> 3) & 1;
+    const StageLane sl(lane);
     float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
 #pragma unroll
     for (int n = 0; n < 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     float a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_pdf[2] = {0.f, 0.f};  // sums of p dP, p far, p dP far
     auto stage_both = [&](int c) {
         const uint32_t at = st + (uint32_t)((c & 1) * 2 * kStageChunk);
-        stage_listed(at, kb, list, c * kStageRows, U, lane);
-        stage_listed(at + kStageChunk, vb, list, c * kStageRows, U, lane);
+        stage_listed(at, kb, list, c * kStageRows, U, sl, lane);
+        stage_listed(at + kStageChunk, vb, list, c * kStageRows, U, sl, lane);
         stage_commit();
     };
 #pragma unroll 1
@@ -131,15 +130,19 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 cp_async_wait_pending<0>();
             }
             __syncwarp();
-            const uint32_t kst = st + (uint32_t)((c & 1) * 2 * kStageChunk), vst = kst + kStageChunk;
+            const uint32_t kst = st + (uint32_t)((c & 1) * 2 * kStageChunk);  // the value rows a chunk behind
             float sacc[4] = {0.f, 0.f, 0.f, 0.f}, pacc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
+            for (int t = 0; t < 4; ++t) {
                 uint32_t a[4];
-                ldmatrix_x4(a, stage_piece(kst, krow, 2 * t + kpc));
+                ldmatrix_x4<0>(a, kst + sl.a[t]);
                 mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], qa[2 * t], qa[2 * t + 1]);
-                ldmatrix_x4(a, stage_piece(vst, krow, 2 * t + kpc));
+                ldmatrix_x4<kStageChunk>(a, kst + sl.a[t]);
                 mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], da[2 * t], da[2 * t + 1]);
+                ldmatrix_x4<128>(a, kst + sl.a[t]);
+                mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], qa[2 * t + 8], qa[2 * t + 9]);
+                ldmatrix_x4<kStageChunk + 128>(a, kst + sl.a[t]);
+                mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], da[2 * t + 8], da[2 * t + 9]);
             }
             // keys c0 + gq, c0 + gq + 8 x heads 2 c4, 2 c4 + 1
             float w[2][2];
@@ -165,10 +168,12 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             const uint32_t b0 = movmatrix_trans(pack_bf16x2(w[0][0], w[0][1]));
             const uint32_t b1 = movmatrix_trans(pack_bf16x2(w[1][0], w[1][1]));
 #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
+            for (int mt = 0; mt < 4; ++mt) {
                 uint32_t a[4];
-                ldmatrix_x4_trans(a, stage_piece(kst, trow, 2 * mt + tpc));
+                ldmatrix_x4_trans<0>(a, kst + sl.at[mt]);
                 mma_bf16_16816_a4(acc[mt], a[0], a[1], a[2], a[3], b0, b1);
+                ldmatrix_x4_trans<128>(a, kst + sl.at[mt]);
+                mma_bf16_16816_a4(acc[mt + 4], a[0], a[1], a[2], a[3], b0, b1);
             }
         }
     }
@@ -200,28 +205,22 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 
 // ------------------------------------------------------------------ key pass
 //
-// One warp per kBwdTile entries of a turned list, in groups of 16 entries whose q and dO rows are
-// staged while the group before is computed.  For the part of a group that lies in one key's run:
-// S = Q k and dP = dO v (entries as MMA rows, the key in column 0), p and dX per entry, then
-// dv^T += dO^T p and dk^T += Q^T dX with the weights in columns 0 and 1: their bf16 value and what
-// the rounding left, so the weights count with 16 bits and the sums are as good as fp32 ones.
+// One warp per `tile` entries of a turned list (rows with the keys of one block of 8 that they list),
+// in groups of 16 entries whose q and dO rows are staged while the group before is computed.  For
+// the part of a group that lies in one block's run: S = Q K^T and dP = dO V^T (entries as MMA rows,
+// the block's keys as columns), p and dX per (entry, key) where the mask has the key's bit, then
+// dv^T += dO^T P and dk^T += Q^T dX from the same rows.  p and dX are rounded to bf16 for those
+// products, the sums are fp32.
 constexpr int kKeyWarps = 4;
-constexpr int kKeyWarpBytes = 4 * kStageChunk + 2 * D * 4;  // q and dO rows of two groups; a finished run
+constexpr int kKeyWarpBytes = 4 * kStageChunk;  // q and dO rows of two groups
 constexpr int kKeyBytes = kKeyWarps * kKeyWarpBytes;
 static_assert(3 * (kKeyBytes + 1024) <= 233472, "three CTAs per SM");
 
-// A key or value row as the B operand's column 0.
-__device__ __forceinline__ void load_column(const __nv_bfloat16* row, int gq, int c4, uint32_t (&r)[16]) {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(row);
+// A block's key or value rows as the B operand: column gq is row gq (zeros past the last key).
+__device__ __forceinline__ void load_block(const __nv_bfloat16* rows, bool in, int gq, int c4, uint32_t (&r)[16]) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(rows + (in ? gq : 0) * D);
 #pragma unroll
-    for (int t = 0; t < 16; ++t) r[t] = gq == 0 ? __ldg(w + 4 * t + c4) : 0u;
-}
-
-// Weights of entries gq, gq + 8 (valid where c4 == 0) as B operands: column 0 rounded, column 1 the rest.
-__device__ __forceinline__ void weight_columns(float w0, float w1, int c4, uint32_t& b0, uint32_t& b1) {
-    const float h0 = __bfloat162float(__float2bfloat16_rn(w0)), h1 = __bfloat162float(__float2bfloat16_rn(w1));
-    b0 = movmatrix_trans(c4 == 0 ? pack_bf16x2(h0, w0 - h0) : 0u);
-    b1 = movmatrix_trans(c4 == 0 ? pack_bf16x2(h1, w1 - h1) : 0u);
+    for (int t = 0; t < 16; ++t) r[t] = in ? __ldg(w + 4 * t + c4) : 0u;
 }
 
 __global__ void __launch_bounds__(kKeyWarps * 32, 3)
@@ -234,63 +233,66 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int gq = lane >> 2, c4 = lane & 3, kv = blockIdx.y;
     const long long tile = (long long)blockIdx.x * kKeyWarps + warp;
-    const int* bs = base + (size_t)kv * (s.N + 1);
-    const int total = bs[s.N];
-    if (tile * kBwdTile >= total) return;  // warp-uniform; no CTA-wide barrier follows
-    const int t0 = (int)(tile * kBwdTile), t1 = min(total, t0 + kBwdTile);
+    const int* bs = base + (size_t)kv * (s.NB + 1);
+    const int total = bs[s.NB];
+    if (tile * s.tile >= total) return;  // warp-uniform; no CTA-wide barrier follows
+    const int t0 = (int)(tile * s.tile), t1 = min(total, t0 + s.tile);
     const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
     const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
-    const int* ls = list + (size_t)kv * s.cap;
-    const __nv_bfloat16* qb = q + rows0 * D;
-    const __nv_bfloat16* db = dout + rows0 * D;
-    uint8_t* stage = msm + (size_t)warp * kKeyWarpBytes;
-    const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
-    float* done = reinterpret_cast<float*>(stage + 4 * kStageChunk);
-    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
-    const int trow = (lane & 7) + (lane >> 4) * 8, tpc = (lane >> 3) & 1;
+    const uint32_t* ls = reinterpret_cast<const uint32_t*>(list) + (size_t)kv * s.cap;
+    const char* qb = reinterpret_cast<const char*>(q + rows0 * D) + (lane & 15) * 16;
+    const char* db = reinterpret_cast<const char*>(dout + rows0 * D) + (lane & 15) * 16;
+    const uint32_t st = (uint32_t)__cvta_generic_to_shared(msm + (size_t)warp * kKeyWarpBytes);
+    const StageLane sl(lane);
 
-    // entry lane & 15 of the group at pos: its row (-1 past the tile)
-    auto entry = [&](int pos) { return pos + (lane & 15) < t1 ? ls[pos + (lane & 15)] : -1; };
-    auto stage_rows = [&](int r, int buf) {
+    // entry lane & 15 of the group at pos; past the tile its last entry again (and given no weight)
+    auto entry = [&](int pos) { return ls[min(pos + (lane & 15), t1 - 1)]; };
+    auto stage_rows = [&](uint32_t r, int buf) {
         const uint32_t at = st + (uint32_t)(buf * 2 * kStageChunk);
-        const int pc = lane & 15;
 #pragma unroll
         for (int t = 0; t < kStageRows / 2; ++t) {
-            const int row = 2 * t + (lane >> 4);
-            const int rr = __shfl_sync(kFull, r, row);
-            const size_t off = (size_t)max(rr, 0) * D + pc * 8;
-            stage_copy(stage_piece(at, row, pc), qb + off, rr >= 0);
-            stage_copy(stage_piece(at + kStageChunk, row, pc), db + off, rr >= 0);
+            const uint32_t row = __shfl_sync(kFull, r, 2 * t + (lane >> 4)) & 0xffffffu;
+            const void *qs = qb + (size_t)row * kStageRow, *ds = db + (size_t)row * kStageRow;
+            if (t < 4) {
+                stage_copy<0>(at + sl.w[t & 3], qs);
+                stage_copy<kStageChunk>(at + sl.w[t & 3], ds);
+            } else {
+                stage_copy<2048>(at + sl.w[t & 3], qs);
+                stage_copy<kStageChunk + 2048>(at + sl.w[t & 3], ds);
+            }
         }
         stage_commit();
     };
-    float ak[8][4], av[8][4];  // dims 16 mt + gq (+8); columns 0 and 1 (lanes with c4 == 0) count
+    float ak[8][4], av[8][4];  // dims 16 mt + gq (+8) of the block's keys 2 c4, 2 c4 + 1
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
         ak[n][0] = ak[n][1] = ak[n][2] = ak[n][3] = 0.f;
         av[n][0] = av[n][1] = av[n][2] = av[n][3] = 0.f;
     }
-    int key = key_at(bs, s.N, t0);
-    int run0 = bs[key], run1 = bs[key + 1];
+    int blk = block_at(bs, s.NB, t0);
+    int run0 = bs[blk], run1 = bs[blk + 1];
     uint32_t kf[16], vf[16];
-    load_column(k + ((size_t)kv * s.N + key) * D, gq, c4, kf);
-    load_column(v + ((size_t)kv * s.N + key) * D, gq, c4, vf);
-    int r = entry(t0), r_next = entry(t0 + kStageRows);
+    auto load_keys = [&] {
+        const size_t at = ((size_t)kv * s.N + (size_t)blk * kKeyBlock) * D;
+        const bool in = blk * kKeyBlock + gq < s.N;
+        load_block(k + at, in, gq, c4, kf);
+        load_block(v + at, in, gq, c4, vf);
+    };
+    load_keys();
+    uint32_t r = entry(t0), r_next = entry(t0 + kStageRows);
     stage_rows(r, 0);
 #pragma unroll 1
     for (int pos = t0, buf = 0; pos < t1; pos += kStageRows, buf ^= 1) {
-        const int r_after = entry(pos + 2 * kStageRows);
+        const uint32_t r_after = entry(pos + 2 * kStageRows);
         // this lane's entry: statistic, Delta, position and slope
-        float lse2 = -INFINITY, dl = 0.f, slope = 0.f;
+        const uint32_t row = r & 0xffffffu;
+        const float lse2 = mods.lse2[rows0 + row], dl = delta[rows0 + row];
+        float slope = 0.f;
         int i = 0;
-        if (r >= 0) {
-            lse2 = mods.lse2[rows0 + r];
-            dl = delta[rows0 + r];
-            if (mods.slopes) {
-                const int g = r / s.Nq;
-                i = s.q0 + r - g * s.Nq;
-                slope = mods.slopes[h0 + g];
-            }
+        if (mods.slopes) {
+            const int g = (int)row / s.Nq;
+            i = s.q0 + (int)row - g * s.Nq;
+            slope = mods.slopes[h0 + g];
         }
         __syncwarp();  // the group before is done with its buffer
         if (pos + kStageRows < t1) {
@@ -300,82 +302,106 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             cp_async_wait_pending<0>();
         }
         __syncwarp();
-        const uint32_t qst = st + (uint32_t)(buf * 2 * kStageChunk), dst = qst + kStageChunk;
+        const uint32_t qst = st + (uint32_t)(buf * 2 * kStageChunk);  // the dO rows a chunk behind
         const int end = min(pos + kStageRows, t1);
 #pragma unroll 1
         for (int p0 = pos; p0 < end;) {
-            const int p1 = min(end, run1);  // entries p0 .. p1 - 1 are of this key
+            const int p1 = min(end, run1);  // entries p0 .. p1 - 1 are of this block
             float sacc[4] = {0.f, 0.f, 0.f, 0.f}, pacc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
+            for (int t = 0; t < 4; ++t) {
                 uint32_t a[4];
-                ldmatrix_x4(a, stage_piece(qst, krow, 2 * t + kpc));
+                ldmatrix_x4<0>(a, qst + sl.a[t]);
                 mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], kf[2 * t], kf[2 * t + 1]);
-                ldmatrix_x4(a, stage_piece(dst, krow, 2 * t + kpc));
+                ldmatrix_x4<kStageChunk>(a, qst + sl.a[t]);
                 mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], vf[2 * t], vf[2 * t + 1]);
+                ldmatrix_x4<128>(a, qst + sl.a[t]);
+                mma_bf16_16816_a4(sacc, a[0], a[1], a[2], a[3], kf[2 * t + 8], kf[2 * t + 9]);
+                ldmatrix_x4<kStageChunk + 128>(a, qst + sl.a[t]);
+                mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], vf[2 * t + 8], vf[2 * t + 9]);
             }
-            float p[2], w[2];
+            float p[2][2], w[2][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {  // entry gq + 8 h
+            for (int h = 0; h < 2; ++h) {  // entry gq + 8 h x keys 2 c4, 2 c4 + 1
                 const int e = gq + 8 * h;
                 const float l = __shfl_sync(kFull, lse2, e), d = __shfl_sync(kFull, dl, e);
-                float far = 0.f, sl = 0.f;
+                uint32_t mask = __shfl_sync(kFull, r, e) >> 24;
+                if (pos + e < p0 || pos + e >= p1 || l == -INFINITY) mask = 0u;
+                float sp = 0.f;
+                int ie = 0;
                 if (mods.slopes) {  // warp-uniform
-                    sl = __shfl_sync(kFull, slope, e);
-                    far = fabsf((float)(__shfl_sync(kFull, i, e) - key));
+                    sp = __shfl_sync(kFull, slope, e);
+                    ie = __shfl_sync(kFull, i, e) - blk * kKeyBlock;
                 }
-                float dx;
-                const float s2 = mods.score2_grad(sacc[2 * h], sl, far, dx, TanhFast());
-                const bool on = pos + e >= p0 && pos + e < p1 && l != -INFINITY;
-                p[h] = on ? exp2_fast(s2 - l) : 0.f;
-                w[h] = on ? dx * p[h] * (pacc[2 * h] - d) : 0.f;
-            }
-            uint32_t pb0, pb1, wb0, wb1;
-            weight_columns(p[0], p[1], c4, pb0, pb1);
-            weight_columns(w[0], w[1], c4, wb0, wb1);
 #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
+                for (int x = 0; x < 2; ++x) {
+                    float dx;
+                    const float s2 = mods.score2_grad(sacc[2 * h + x], sp, fabsf((float)(ie - 2 * c4 - x)), dx, TanhFast());
+                    const bool on = (mask >> (2 * c4 + x)) & 1u;
+                    p[h][x] = on ? exp2_fast(s2 - l) : 0.f;
+                    w[h][x] = on ? dx * p[h][x] * (pacc[2 * h + x] - d) : 0.f;
+                }
+            }
+            const uint32_t pb0 = movmatrix_trans(pack_bf16x2(p[0][0], p[0][1]));
+            const uint32_t pb1 = movmatrix_trans(pack_bf16x2(p[1][0], p[1][1]));
+            const uint32_t wb0 = movmatrix_trans(pack_bf16x2(w[0][0], w[0][1]));
+            const uint32_t wb1 = movmatrix_trans(pack_bf16x2(w[1][0], w[1][1]));
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
                 uint32_t a[4];
-                ldmatrix_x4_trans(a, stage_piece(dst, trow, 2 * mt + tpc));
+                ldmatrix_x4_trans<kStageChunk>(a, qst + sl.at[mt]);
                 mma_bf16_16816_a4(av[mt], a[0], a[1], a[2], a[3], pb0, pb1);
-                ldmatrix_x4_trans(a, stage_piece(qst, trow, 2 * mt + tpc));
+                ldmatrix_x4_trans<0>(a, qst + sl.at[mt]);
                 mma_bf16_16816_a4(ak[mt], a[0], a[1], a[2], a[3], wb0, wb1);
+                ldmatrix_x4_trans<kStageChunk + 128>(a, qst + sl.at[mt]);
+                mma_bf16_16816_a4(av[mt + 4], a[0], a[1], a[2], a[3], pb0, pb1);
+                ldmatrix_x4_trans<128>(a, qst + sl.at[mt]);
+                mma_bf16_16816_a4(ak[mt + 4], a[0], a[1], a[2], a[3], wb0, wb1);
             }
             p0 = p1;
             if (p1 < run1 && p1 < t1) continue;  // the run goes on in the next group
             // the run, or the tile, ends here
-            __syncwarp();
-#pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-                if (c4 == 0) {
-                    done[16 * mt + gq] = ak[mt][0] + ak[mt][1];
-                    done[16 * mt + gq + 8] = ak[mt][2] + ak[mt][3];
-                    done[D + 16 * mt + gq] = av[mt][0] + av[mt][1];
-                    done[D + 16 * mt + gq + 8] = av[mt][2] + av[mt][3];
-                }
-                ak[mt][0] = ak[mt][1] = ak[mt][2] = ak[mt][3] = 0.f;
-                av[mt][0] = av[mt][1] = av[mt][2] = av[mt][3] = 0.f;
-            }
-            __syncwarp();
-            const float4 dk4 = reinterpret_cast<const float4*>(done)[lane];
-            const float4 dv4 = reinterpret_cast<const float4*>(done + D)[lane];
             if (run0 >= t0 && run1 <= t1) {
-                const size_t at = ((size_t)kv * s.N + key) * D + 4 * lane;
-                *reinterpret_cast<uint2*>(dk + at) = make_uint2(pack_bf16x2(dk4.x, dk4.y), pack_bf16x2(dk4.z, dk4.w));
-                *reinterpret_cast<uint2*>(dv + at) = make_uint2(pack_bf16x2(dv4.x, dv4.y), pack_bf16x2(dv4.z, dv4.w));
+                const bool in = blk * kKeyBlock + gq < s.N;  // after the transpose lane (gq, c4) holds key gq
+                const size_t at = ((size_t)kv * s.N + (size_t)blk * kKeyBlock + gq) * D + 2 * c4;
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt) {
+                    const uint32_t k0 = movmatrix_trans(pack_bf16x2(ak[mt][0], ak[mt][1]));
+                    const uint32_t k1 = movmatrix_trans(pack_bf16x2(ak[mt][2], ak[mt][3]));
+                    const uint32_t v0 = movmatrix_trans(pack_bf16x2(av[mt][0], av[mt][1]));
+                    const uint32_t v1 = movmatrix_trans(pack_bf16x2(av[mt][2], av[mt][3]));
+                    if (in) {
+                        *reinterpret_cast<uint32_t*>(dk + at + 16 * mt) = k0;
+                        *reinterpret_cast<uint32_t*>(dk + at + 16 * mt + 8) = k1;
+                        *reinterpret_cast<uint32_t*>(dv + at + 16 * mt) = v0;
+                        *reinterpret_cast<uint32_t*>(dv + at + 16 * mt + 8) = v1;
+                    }
+                }
             } else {  // slot 0: the run began before this tile; slot 1: it begins here and goes on
-                float* ps = part + (((size_t)kv * s.tiles + tile) * 2 + (run0 < t0 ? 0 : 1)) * 2 * D;
-                reinterpret_cast<float4*>(ps)[lane] = dk4;
-                reinterpret_cast<float4*>(ps + D)[lane] = dv4;
+                float* ps = part + (((size_t)kv * s.tiles + tile) * 2 + (run0 < t0 ? 0 : 1)) * 2 * kKeyBlock * D +
+                            2 * c4 * D + gq;
+#pragma unroll
+                for (int mt = 0; mt < 8; ++mt) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int at = (x & 1) * D + 16 * mt + (x >> 1) * 8;
+                        ps[at] = ak[mt][x];
+                        ps[kKeyBlock * D + at] = av[mt][x];
+                    }
+                }
             }
-            if (p1 < t1) {  // on to the next listed key
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                ak[n][0] = ak[n][1] = ak[n][2] = ak[n][3] = 0.f;
+                av[n][0] = av[n][1] = av[n][2] = av[n][3] = 0.f;
+            }
+            if (p1 < t1) {  // on to the next listed block
                 do {
-                    ++key;
+                    ++blk;
                     run0 = run1;
-                    run1 = bs[key + 1];
+                    run1 = bs[blk + 1];
                 } while (run1 <= p1);
-                load_column(k + ((size_t)kv * s.N + key) * D, gq, c4, kf);
-                load_column(v + ((size_t)kv * s.N + key) * D, gq, c4, vf);
+                load_keys();
             }
         }
         r = r_next;

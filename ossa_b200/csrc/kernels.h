@@ -81,6 +81,7 @@ cudaError_t launch_gather_attn(const GatherArgs& a, cudaStream_t stream);
 cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream);
 // Whether the tensor-core forms of the modified gather and its backward pass take a shape.
 bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K);
+bool gather_bwd_mma_serves(int dtype, int H, int Hkv, int Nq, int N, int D, int K);
 
 // Gradients of launch_gather_attn_mods (gather_bwd.cu).
 struct GatherBwdArgs {
@@ -90,7 +91,7 @@ struct GatherBwdArgs {
     float* dslopes;      // (H,) or nullptr
     void* ws;            // gather_bwd_workspace_bytes
 };
-size_t gather_bwd_workspace_bytes(int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes);
+size_t gather_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes);
 cudaError_t launch_gather_attn_bwd(const GatherBwdArgs& a, cudaStream_t stream);
 
 // Head norms with rotation and head transpose for queries and keys (norm_rope.cu).

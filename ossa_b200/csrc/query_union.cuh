@@ -99,31 +99,49 @@ __device__ __forceinline__ int single_list(Key key, int t, int K, uint32_t* list
     return U;
 }
 
-// Rows of 128 bf16 values in shared memory: 16-byte pieces XOR-swizzled by the row.
+// Chunks of 16 rows of 128 bf16 values in shared memory, 16-byte pieces XOR-swizzled by the row: piece c
+// of row r lies at r * 256 + ((c ^ (r & 7)) << 4).  The pieces c and c + 8 of a row are 128 bytes apart,
+// rows r and r + 8 2048, so four offsets per lane and compile-time distances reach every access.
 constexpr int kStageRow = 256;
 constexpr int kStageRows = 16;
 constexpr int kStageChunk = kStageRows * kStageRow;
 
-__device__ __forceinline__ uint32_t stage_piece(uint32_t base, int row, int piece) {
-    return base + (uint32_t)(row * kStageRow + ((piece ^ (row & 7)) << 4));
-}
+// This lane's places in a chunk.
+struct StageLane {
+    uint32_t a[4];   // ldmatrix, rows as they lie: k-step t reads a[t & 3] + 128 * (t >> 2)
+    uint32_t at[4];  // ldmatrix.trans: 16-column step t likewise
+    uint32_t w[4];   // copy of piece lane & 15 of rows 2 t + lane / 16: w[t & 3] + 2048 * (t >> 2)
+    __device__ __forceinline__ explicit StageLane(int lane) {
+        const int ar = (lane & 7) + ((lane >> 3) & 1) * 8, ac = lane >> 4;
+        const int tr = (lane & 7) + (lane >> 4) * 8, tc = (lane >> 3) & 1;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            a[t] = (uint32_t)(ar * kStageRow + (((2 * t + ac) ^ (ar & 7)) << 4));
+            at[t] = (uint32_t)(tr * kStageRow + (((2 * t + tc) ^ (tr & 7)) << 4));
+            const int wr = 2 * t + (lane >> 4);
+            w[t] = (uint32_t)(wr * kStageRow + (((lane & 15) ^ (wr & 7)) << 4));
+        }
+    }
+};
 
-__device__ __forceinline__ void stage_copy(uint32_t dst, const void* src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+template <int kOff>
+__device__ __forceinline__ void stage_copy(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1], 16;" ::"r"(dst), "l"(src), "n"(kOff) : "memory");
 }
 
 __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// Copies the rows of list entries c0 .. c0 + 15 (zeros past U) of one tensor.
+// Copies the rows of list entries c0 .. c0 + 15 of one tensor; past the list's end its last row again
+// (finite where the list's rows are, and given no weight).
 __device__ __forceinline__ void stage_listed(uint32_t dst, const __nv_bfloat16* base, const uint32_t* list, int c0, int U,
-                                             int lane) {
-    const int pc = lane & 15;
+                                             const StageLane& sl, int lane) {
+    const char* col = reinterpret_cast<const char*>(base) + (lane & 15) * 16;
 #pragma unroll
-    for (int r = 0; r < kStageRows / 2; ++r) {
-        const int row = 2 * r + (lane >> 4);
-        const bool on = c0 + row < U;
-        const size_t key = on ? list[c0 + row] & 0xffffffu : 0u;
-        stage_copy(stage_piece(dst, row, pc), base + key * 128 + pc * 8, on);
+    for (int t = 0; t < kStageRows / 2; ++t) {
+        const uint32_t key = list[min(c0 + 2 * t + (lane >> 4), U - 1)] & 0xffffffu;
+        const void* src = col + (size_t)key * kStageRow;
+        if (t < 4) stage_copy<0>(dst + sl.w[t & 3], src);
+        else stage_copy<2048>(dst + sl.w[t & 3], src);
     }
 }
 

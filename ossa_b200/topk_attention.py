@@ -220,10 +220,10 @@ class _TopkAttention(torch.autograd.Function):
         dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
         L = _lib.lib()
         B, H, Nq, D = q.shape
-        ws_bytes = L.ossa_topk_attention_bwd_workspace_size(B, H, k.shape[1], Nq, k.shape[2], D, idx.shape[-1],
-                                                            0 if dslopes is None else 1)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with _lib.on_device(dev):
+            ws_bytes = L.ossa_topk_attention_bwd_workspace_size(_lib.dtype_code(q), B, H, k.shape[1], Nq, k.shape[2], D,
+                                                                idx.shape[-1], 0 if dslopes is None else 1)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             st = L.ossa_topk_attention_bwd(
                 *_mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), out.data_ptr(), lse2.data_ptr(),
                 dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dslopes), ws.data_ptr(),

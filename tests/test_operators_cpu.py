@@ -41,11 +41,11 @@ def test_modified_attention_refusals(kw, code):
 def test_attention_backward_refusals():
     assert _mod_bwd(dslopes=16) == INV  # without slopes
     assert _mod_bwd(lse=None) == INV and _mod_bwd(dq=None) == INV and _mod_bwd(dv=24) == INV
-    need = _lib.lib().ossa_topk_attention_bwd_workspace_size(1, 4, 2, 8, 8, 128, 4, 0)
+    need = _lib.lib().ossa_topk_attention_bwd_workspace_size(BF, 1, 4, 2, 8, 8, 128, 4, 0)
     assert need > 0 and _mod_bwd(wsb=need - 1) == WS and _mod_bwd(ws=None) == WS
     assert _mod_bwd(Nq=1 << 20, Nk=1 << 20, K=1024) == UNS  # more than 2^30 listed keys per kv head
     assert _mod_fwd(B=0) == OK and _mod_fwd(Nq=0) == OK
-    assert _lib.lib().ossa_topk_attention_bwd_workspace_size(1, 4, 3, 8, 8, 128, 4, 0) == 0
+    assert _lib.lib().ossa_topk_attention_bwd_workspace_size(BF, 1, 4, 3, 8, 8, 128, 4, 0) == 0
 
 
 def _norm(fn="fwd", **kw):
