@@ -37,9 +37,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kKeyRange = 8192;  // key blocks that one CTA of the counting sort covers (32 KB of counters)
-constexpr int kMaxChunks = 64;   // row chunks of the counting sort per head
+constexpr int kMaxChunks = 128;   // row chunks of the counting sort per head
 constexpr int kMinChunkRows = 32;
-constexpr int kPlaceRows = 8;    // rows whose entries the counting sort's last step has in flight
+constexpr int kCountRows = 4;    // rows whose entries a warp of the counting sort's first step has in flight
+constexpr int kPlaceRows = 8;    // and of its last step
 
 BwdShape make_shape(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int K) {
     BwdShape s{};
@@ -55,8 +56,8 @@ BwdShape make_shape(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int 
     s.shift = mma ? kKeyBlockShift : 0;
     s.NB = (N + (1 << s.shift) - 1) >> s.shift;
     const long long kv = (long long)B * Hkv;
-    // one warp per unit in the sort's last step: enough units for 12 warps per SM, rows permitting
-    const long long want = 12ll * device_sm_count() / std::max(kv * s.G, 1ll);
+    // one warp per unit in the sort's last step: enough units for 24 warps per SM, rows permitting
+    const long long want = 24ll * device_sm_count() / std::max(kv * s.G, 1ll);
     s.chunks = (int)std::max(1ll, std::min({want, (long long)kMaxChunks, (long long)Nq / kMinChunkRows}));
     s.chunk_rows = (Nq + s.chunks - 1) / s.chunks;
     s.units = s.chunks * s.G;
@@ -89,29 +90,35 @@ Layout make_layout(const BwdShape& s, bool dslopes) {
 
 // ------------------------------------------------------------------ 1. turned lists
 
-// A row's entries 32 e .. 32 e + 31, one per lane (key, -1: masked).  An entry follows the one before it
-// when its key is greater and in the same block; the first of such a chain stands for all, with a bit per
-// key of the block in `mask` (shift 0: every entry for itself).
-__device__ __forceinline__ bool chain_head(int key, int shift, int lane, uint32_t& mask) {
+// A row's entries 32 e .. 32 e + 31, one per lane (key, -1: masked), as the words of the normalised lists.
+// Blocks of one key: the key.  Blocks of 8: an entry follows the one before it when its key is greater
+// and in the same block; the first of such a chain stands for all and carries a bit per key of the block,
+// key | bits << 24, the others have no bits.  (-1 is no such word: a chain of 8 begins at key 0 of a block.)
+__device__ __forceinline__ int list_word(int key, int shift, int lane) {
+    if (shift == 0) return key;  // warp-uniform
     const int prev = __shfl_up_sync(kFull, key, 1);
-    const bool follows = shift > 0 && lane > 0 && key >= 0 && prev >= 0 && prev < key && (prev >> shift) == (key >> shift);
-    mask = 0u;
-    if (shift > 0) {  // warp-uniform
-        const unsigned tails = __ballot_sync(kFull, follows);
-        mask = key >= 0 ? 1u << (key & (kKeyBlock - 1)) : 0u;
-        // OR over the chain behind this lane: at most kKeyBlock entries, so three doublings
+    const bool follows = lane > 0 && key >= 0 && prev >= 0 && prev < key && ((prev ^ key) >> shift) == 0;
+    const unsigned tails = __ballot_sync(kFull, follows) >> 1 >> lane;  // bit t: lane + 1 + t follows
+    uint32_t bits = key >= 0 ? 1u << (key & (kKeyBlock - 1)) : 0u;
+    // OR over the chain behind this lane: at most kKeyBlock entries, so three doublings
 #pragma unroll
-        for (int o = 1; o < kKeyBlock; o <<= 1) {
-            const uint32_t other = __shfl_down_sync(kFull, mask, o);
-            const unsigned all = (1u << o) - 1u;  // lanes lane + 1 .. lane + o
-            if ((((tails >> 1) >> lane) & all) == all) mask |= other;
-        }
+    for (int o = 1; o < kKeyBlock; o <<= 1) {
+        const uint32_t other = __shfl_down_sync(kFull, bits, o);
+        const unsigned all = (1u << o) - 1u;
+        if ((tails & all) == all) bits |= other;
     }
-    return key >= 0 && !follows;
+    return key < 0 ? -1 : (int)((uint32_t)key | (follows ? 0u : bits << 24));
 }
 
-// keys: the lists as int32, -1 where an entry is outside [0, N) or not seen by its row.
+// The block that an entry stands for, -1 where it is masked or follows another.
+__device__ __forceinline__ int word_block(int w, int shift) {
+    if (shift == 0 || w == -1) return w;
+    return (uint32_t)w >> 24 ? (w & 0xffffff) >> shift : -1;
+}
+
+// keys: the normalised lists.
 // counts[kv][unit][block]: the unit's entries of the key block's turned list.
+// A warp has the entries of kCountRows rows in flight.
 template <typename IdxT>
 __global__ void __launch_bounds__(kThreads)
 count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mods, int* __restrict__ keys,
@@ -124,19 +131,35 @@ count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mod
     for (int t = threadIdx.x; t < nk; t += kThreads) hist[t] = 0;
     __syncthreads();
     const int lane = threadIdx.x & 31;
-    for (int il = r0 + (threadIdx.x >> 5); il < r1; il += kWarps) {
-        const int i = s.q0 + il;
-        const RowMods<true> rm(mods, b, h, s.N, i);
-        const size_t row = ((size_t)b * s.H + h) * s.Nq + il;
-        for (int e0 = 0; e0 < s.K; e0 += 32) {
-            const int e = e0 + lane;
-            const long long j = e < s.K ? (long long)idx[row * s.K + e] : -1ll;
-            const int key = j >= 0 && j < s.N && rm.sees(j, i, s.causal) ? (int)j : -1;
-            if (blockIdx.z == 0 && e < s.K) keys[row * s.K + e] = key;
-            uint32_t mask;
-            const bool head = chain_head(key, s.shift, lane, mask);
-            const int at = (key >> s.shift) - k0;
-            if (head && (unsigned)at < (unsigned)nk) atomicAdd(&hist[at], 1);
+    const int* seg = mods.segments ? mods.segments + (size_t)b * s.N : nullptr;
+    const int prefix = mods.prefix_len ? mods.prefix_len[b] : 0;
+    const size_t row0 = ((size_t)b * s.H + h) * s.Nq;
+    const IdxT* ib = idx + row0 * s.K;
+    int* kb = keys + row0 * s.K;
+    for (int il0 = r0 + (threadIdx.x >> 5) * kCountRows; il0 < r1; il0 += kWarps * kCountRows) {
+        int si[kCountRows];
+#pragma unroll
+        for (int t = 0; t < kCountRows; ++t) si[t] = seg && il0 + t < r1 ? seg[s.q0 + il0 + t] : 0;
+        for (int e = lane; e - lane < s.K; e += 32) {
+            int j[kCountRows];
+#pragma unroll
+            for (int t = 0; t < kCountRows; ++t) {
+                const IdxT x = e < s.K && il0 + t < r1 ? ib[(size_t)(il0 + t) * s.K + e] : (IdxT)-1;
+                j[t] = x >= 0 && x < (IdxT)s.N ? (int)x : -1;
+                if (s.causal && j[t] > s.q0 + il0 + t && j[t] >= prefix) j[t] = -1;
+            }
+            if (seg) {
+#pragma unroll
+                for (int t = 0; t < kCountRows; ++t)
+                    if (j[t] >= 0 && seg[j[t]] != si[t]) j[t] = -1;
+            }
+#pragma unroll
+            for (int t = 0; t < kCountRows; ++t) {
+                const int w = list_word(j[t], s.shift, lane);
+                if (blockIdx.z == 0 && e < s.K && il0 + t < r1) kb[(size_t)(il0 + t) * s.K + e] = w;
+                const int at = word_block(w, s.shift) - k0;
+                if (w != -1 && (unsigned)at < (unsigned)nk) atomicAdd(&hist[at], 1);
+            }
         }
     }
     __syncthreads();
@@ -144,25 +167,38 @@ count_kernel(const IdxT* __restrict__ idx, const BwdShape s, const ScoreMods mod
     for (int t = threadIdx.x; t < nk; t += kThreads) out[t] = hist[t];
 }
 
-// counts -> exclusive prefix over the units, and the block's total in base[kv][block].
+// counts -> exclusive prefix over the units, and the block's total in base[kv][block].  A CTA takes 32
+// blocks; each of its 8 warps a contiguous part of the units, summed first and then written.
 __global__ void __launch_bounds__(kThreads)
 unit_scan_kernel(const BwdShape s, int* __restrict__ counts, int* __restrict__ base) {
-    constexpr int kAhead = 16;  // loads in flight
-    const int key = blockIdx.x * kThreads + threadIdx.x, kv = blockIdx.y;
-    if (key >= s.NB) return;
-    int* c = counts + (size_t)kv * s.units * s.NB + key;
+    constexpr int kAhead = 8;  // loads in flight
+    __shared__ int sums[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kv = blockIdx.y;
+    const int key = blockIdx.x * 32 + lane;
+    const bool on = key < s.NB;
+    int* c = counts + (size_t)kv * s.units * s.NB + (on ? key : 0);
+    const int per = (s.units + kWarps - 1) / kWarps;
+    const int u0 = min(warp * per, s.units), u1 = min(u0 + per, s.units);
     int sum = 0;
-    for (int u0 = 0; u0 < s.units; u0 += kAhead) {
+    for (int u = u0; u < u1; u += kAhead) {
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) sum += u + t < u1 ? c[(size_t)(u + t) * s.NB] : 0;
+    }
+    sums[warp][lane] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < warp; ++w) before += sums[w][lane];
+    if (on && warp == kWarps - 1) base[(size_t)kv * (s.NB + 1) + key] = before + sum;
+    for (int u = u0; u < u1; u += kAhead) {
         int x[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) x[u] = u0 + u < s.units ? c[(size_t)(u0 + u) * s.NB] : 0;
+        for (int t = 0; t < kAhead; ++t) x[t] = u + t < u1 ? c[(size_t)(u + t) * s.NB] : 0;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (u0 + u < s.units) c[(size_t)(u0 + u) * s.NB] = sum;
-            sum += x[u];
+        for (int t = 0; t < kAhead; ++t) {
+            if (on && u + t < u1) c[(size_t)(u + t) * s.NB] = before;
+            before += x[t];
         }
     }
-    base[(size_t)kv * (s.NB + 1) + key] = sum;
 }
 
 // base[kv][0..NB]: exclusive prefix of the totals over the blocks.
@@ -203,7 +239,7 @@ __global__ void __launch_bounds__(1024) key_scan_kernel(const BwdShape s, int* _
     if (threadIdx.x == 0) p[s.NB] = carry;
 }
 
-// list[kv][position] = r (| mask << 24) with r = g * Nq + il of the rows that list a key block, block by block.  One warp walks the
+// list[kv][position] = r (| bits << 24) with r = g * Nq + il of the rows that list a key block, block by block.  One warp walks the
 // unit's rows in a fixed order, the counters of its key range in shared memory; the entries of
 // kPlaceRows rows are loaded together, and the next ones while these are placed, so a step costs
 // one trip to L2 and not one per row.
@@ -223,32 +259,36 @@ place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restri
     __syncwarp();
     int* out = list + (size_t)kv * s.cap;
     const int* rows = keys + ((size_t)b * s.H + h) * s.Nq * s.K;
-    const int parts = (s.K + 31) / 32;
-    const int steps = ((r1 - r0 + kPlaceRows - 1) / kPlaceRows) * parts;  // a step: 32 entries of kPlaceRows rows
-    auto load = [&](int step, int (&j)[kPlaceRows]) {
-        const int il = r0 + step / parts * kPlaceRows, e = (step % parts) * 32 + lane;
+    // a step: 32 entries of kPlaceRows rows; il, e: where the step after the loaded one begins
+    int il = r0, e = lane;
+    int w[kPlaceRows], ahead[kPlaceRows];
+    auto load = [&](int (&x)[kPlaceRows]) {
 #pragma unroll
-        for (int t = 0; t < kPlaceRows; ++t)
-            j[t] = step < steps && il + t < r1 && e < s.K ? rows[(size_t)(il + t) * s.K + e] : -1;
+        for (int t = 0; t < kPlaceRows; ++t) x[t] = il + t < r1 && e < s.K ? rows[(size_t)(il + t) * s.K + e] : -1;
+        e += 32;
+        if (e - lane >= s.K) {
+            e = lane;
+            il += kPlaceRows;
+        }
     };
-    int j[kPlaceRows], ahead[kPlaceRows];
-    load(0, j);
-    for (int step = 0; step < steps; ++step) {
-        load(step + 1, ahead);
-        const int il = r0 + step / parts * kPlaceRows;
+    int at_row = r0;
+    load(w);
+    while (at_row < r1) {
+        const int row = at_row;
+        at_row = il;  // the row group of the next step
+        load(ahead);
         int pos[kPlaceRows];
-        uint32_t mask[kPlaceRows];
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t) {
-            const bool head = chain_head(j[t], s.shift, lane, mask[t]);
-            const int at = (j[t] >> s.shift) - k0;
-            pos[t] = head && (unsigned)at < (unsigned)nk ? atomicAdd(&next[at], 1) : -1;
+            const int at = word_block(w[t], s.shift) - k0;
+            pos[t] = w[t] != -1 && (unsigned)at < (unsigned)nk ? atomicAdd(&next[at], 1) : -1;
             __syncwarp();  // a row's places before the next row's
         }
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t) {
-            if (pos[t] >= 0) out[pos[t]] = (int)((uint32_t)(g * s.Nq + il + t) | mask[t] << 24);
-            j[t] = ahead[t];
+            const uint32_t bits = s.shift ? (uint32_t)w[t] & 0xff000000u : 0u;
+            if (pos[t] >= 0) out[pos[t]] = (int)((uint32_t)(g * s.Nq + row + t) | bits);
+            w[t] = ahead[t];
         }
     }
 }
@@ -457,19 +497,33 @@ join_kernel(const BwdShape s, const int* __restrict__ base, const float* __restr
     const int first = run0 / s.tile, last = run1 > run0 ? (run1 - 1) / s.tile : first;
     if (run1 > run0 && first == last) return;  // stored by the key pass
     const size_t slot = (size_t)2 * (s.D << s.shift);  // floats of a tile's slot
-    const float* ps = part + (size_t)kv * s.tiles * 2 * slot;
+    const float* ps = part + (size_t)kv * s.tiles * 2 * slot + (size_t)kk * s.D;
     T* ok = dk + ((size_t)kv * s.N + key) * s.D;
     T* ov = dv + ((size_t)kv * s.N + key) * s.D;
-    for (int d = lane; d < 2 * s.D; d += 32) {
-        const int which = d >= s.D, dd = d - which * s.D;
-        const size_t at = (size_t)which * (s.D << s.shift) + (size_t)kk * s.D + dd;
-        float t = 0.f;
+    for (int d = 4 * lane; d < s.D; d += 128) {
+        float k4[4] = {0.f, 0.f, 0.f, 0.f}, v4[4] = {0.f, 0.f, 0.f, 0.f};
+        auto add = [&](const float* at) {
+            const float4 x = *reinterpret_cast<const float4*>(at + d);
+            const float4 y = *reinterpret_cast<const float4*>(at + (s.D << s.shift) + d);
+            k4[0] += x.x;
+            k4[1] += x.y;
+            k4[2] += x.z;
+            k4[3] += x.w;
+            v4[0] += y.x;
+            v4[1] += y.y;
+            v4[2] += y.z;
+            v4[3] += y.w;
+        };
         if (run1 > run0) {
-            t = ps[((size_t)first * 2 + 1) * slot + at];
+            add(ps + ((size_t)first * 2 + 1) * slot);
 #pragma unroll 4
-            for (int i = first + 1; i <= last; ++i) t += ps[(size_t)i * 2 * slot + at];
+            for (int i = first + 1; i <= last; ++i) add(ps + (size_t)i * 2 * slot);
         }
-        store_from_f32((which ? ov : ok) + dd, t);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            store_from_f32(ok + d + t, k4[t]);
+            store_from_f32(ov + d + t, v4[t]);
+        }
     }
 }
 
@@ -505,7 +559,7 @@ cudaError_t sort_lists(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffe
     cudaError_t e;
     count_kernel<IdxT><<<grid, kThreads, smem, stream>>>(static_cast<const IdxT*>(a.f.idx), s, a.f.mods, w.keys, w.counts);
     if ((e = launched()) != cudaSuccess) return e;
-    unit_scan_kernel<<<dim3((unsigned)((s.NB + kThreads - 1) / kThreads), kvs), kThreads, 0, stream>>>(s, w.counts, w.base);
+    unit_scan_kernel<<<dim3((unsigned)((s.NB + 31) / 32), kvs), kThreads, 0, stream>>>(s, w.counts, w.base);
     if ((e = launched()) != cudaSuccess) return e;
     key_scan_kernel<<<kvs, 1024, 0, stream>>>(s, w.base);
     if ((e = launched()) != cudaSuccess) return e;

@@ -8,7 +8,7 @@
 namespace ossa {
 
 // The tensor-core key pass takes blocks of 8 neighbouring keys (one MMA's columns): a turned list then
-// holds rows with the block's keys that they list as a bit mask, r | mask << 24.  The other key pass
+// holds rows with the block's keys that they list as bits, r | bits << 24.  The other key pass
 // takes single keys, its list plain rows r.
 constexpr int kKeyBlockShift = 3;
 constexpr int kKeyBlock = 1 << kKeyBlockShift;
@@ -23,7 +23,7 @@ struct BwdShape {
 };
 
 struct BwdBuffers {
-    int* keys;          // (B*H*Nq, K) lists, -1 where masked
+    int* keys;          // (B*H*Nq, K) normalised lists: words as list_word makes them, -1 where masked
     int* counts;        // (B*Hkv, units, NB)
     int* base;          // (B*Hkv, NB + 1) start of each key block's run
     int* list;          // (B*Hkv, cap) rows r = g * Nq + il, block by block

@@ -88,7 +88,10 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         lse2[e] = t < G ? mods.lse2[row0 + (size_t)t * s.Nq] : -INFINITY;
         slope[e] = mods.slopes && t < G ? mods.slopes[g * G + t] : 0.f;
     }
-    auto key_of = [&](int t, int e) { return keys[(row0 + (size_t)t * s.Nq) * s.K + e]; };
+    auto key_of = [&](int t, int e) {
+        const int w = keys[(row0 + (size_t)t * s.Nq) * s.K + e];
+        return w == -1 ? -1 : w & 0xffffff;
+    };
     int passes = 1, U;
     {
         int x[G][4];

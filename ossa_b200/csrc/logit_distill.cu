@@ -31,8 +31,9 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPrepThreads = 1024;
-constexpr int kPrepBlocks = 64;
+constexpr int kMaxCluster = 8;
+constexpr int kPrepThreads = 256;
+constexpr int kPrepBlocks = 512;  // at most kThreads: the row kernel adds their weight sums, one per thread
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Workspace: [counter 16 B][weight sums of the prep CTAs, double][row weight, T][row loss, T]
@@ -190,11 +191,34 @@ __device__ __forceinline__ uint4 load_stream(const uint4* p) {
     return v;
 }
 
-// (max, sum of exp2((z - max) c)) of two parts of a row.
-__device__ __forceinline__ void join(float& m, float& l, float m2, float l2, float c) {
-    const float mn = fmaxf(m, m2);
-    l = l * exp2f((m - mn) * c) + l2 * exp2f((m2 - mn) * c);
-    m = mn;
+// 2^x, two units in the last place; below 2^-126 it is 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// (max, sum of exp2((z - max) c)) over lanes that differ in the bits below kLanes.
+template <int kLanes>
+__device__ __forceinline__ void join_lanes(float& m, float& l, float c) {
+    float top = m;
+#pragma unroll
+    for (int o = kLanes / 2; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+    l *= exp2_fast((m - top) * c);
+#pragma unroll
+    for (int o = kLanes / 2; o >= 1; o >>= 1) l += __shfl_xor_sync(kFull, l, o);
+    m = top;
+}
+
+// Sum over the CTA in a fixed order, in every thread.
+__device__ __forceinline__ double block_sum(double x, double* buf) {
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) x += __shfl_xor_sync(kFull, x, o);
+    if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = x;
+    __syncthreads();
+    double t = 0.0;
+    for (int i = 0; i < kWarps; ++i) t += buf[i];
+    return t;
 }
 
 template <typename T, typename IdT, int kNV>
@@ -206,20 +230,17 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long clusters = gridDim.x / C, me = blockIdx.x / C;
     if (a.skip_if_one && a.grad && *a.grad == 1.f) return;  // the same for every CTA
-    __shared__ float s_m[kWarps], s_l[kWarps], s_part[kWarps];
-    __shared__ float2 s_pair[2];  // this CTA's (max, sum), by row parity
-    __shared__ float s_row[2];
-    __shared__ float s_unit;
+    __shared__ float2 s_warp[kWarps];
+    __shared__ float s_part[kWarps];
+    __shared__ float2 s_pair[2][kMaxCluster];  // (max, sum) of every CTA of the cluster, by row parity
+    __shared__ double s_sum[kWarps];
     __shared__ bool s_last;
     const float c = kLog2e / a.tau;
-    if (tid == 0) {  // weight of one unit of row weight
-        double w = 0.0;
-        if (a.mean)
-            for (int i = 0; i < a.prep_blocks; ++i) w += a.wsum[i];
-        s_unit = a.mean ? (w != 0.0 ? (float)(1.0 / w) : 0.f) : 1.f;
+    float unit = 1.f;  // what a unit of row weight counts in the total
+    if (a.mean) {
+        const double w = block_sum(tid < a.prep_blocks ? a.wsum[tid] : 0.0, s_sum);
+        unit = w != 0.0 ? (float)(1.0 / w) : 0.f;
     }
-    __syncthreads();
-    const float unit = s_unit;
     int parity = 0;
     for (long long r = me; r < a.T; r += clusters) {
         const float w = a.weight[r];
@@ -262,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
                 float x[E];
                 V8::unpack(d[j], x);
 #pragma unroll
-                for (int t = 0; t < E; ++t) l += exp2f((x[t] - m) * c);
+                for (int t = 0; t < E; ++t) l += exp2_fast((x[t] - m) * c);
             }
         } else {
             for (int i = first; i < nb; i += stride) {
@@ -271,43 +292,32 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
                 float mn = m;
 #pragma unroll
                 for (int t = 0; t < E; ++t) mn = fmaxf(mn, x[t]);
-                l *= exp2f((m - mn) * c);
+                l *= exp2_fast((m - mn) * c);
                 m = mn;
 #pragma unroll
-                for (int t = 0; t < E; ++t) l += exp2f((x[t] - m) * c);
+                for (int t = 0; t < E; ++t) l += exp2_fast((x[t] - m) * c);
             }
         }
-        if (odd >= 0) l += exp2f((zo - m) * c);
-#pragma unroll
-        for (int o = 16; o >= 1; o >>= 1) {
-            const float m2 = __shfl_xor_sync(kFull, m, o), l2 = __shfl_xor_sync(kFull, l, o);
-            join(m, l, m2, l2, c);
-        }
-        if (lane == 0) {
-            s_m[warp] = m;
-            s_l[warp] = l;
-        }
+        if (odd >= 0) l += exp2_fast((zo - m) * c);
+        join_lanes<32>(m, l, c);
+        if (lane == 0) s_warp[warp] = make_float2(m, l);
         __syncthreads();
-        if (tid == 0) {
-            for (int i = 1; i < kWarps; ++i) join(m, l, s_m[i], s_l[i], c);
-            s_pair[parity] = make_float2(m, l);
+        if (warp == 0) {
+            const float2 x = s_warp[lane % kWarps];
+            m = x.x;
+            l = x.y;
+            join_lanes<kWarps>(m, l, c);
+            if (lane < C) *cluster.map_shared_rank(&s_pair[parity][rank], lane) = make_float2(m, l);
         }
         // one barrier a row: a pair is written again two rows on, when every CTA has
         // passed the next row's barrier and so has read it
         cluster.sync();
-        if (tid == 0) {
-            m = -FLT_MAX;
-            l = 0.f;
-            for (int i = 0; i < C; ++i) {  // rank order in every CTA: the same bits
-                const float2 p = *cluster.map_shared_rank(&s_pair[parity], i);
-                join(m, l, p.x, p.y, c);
-            }
-            s_row[0] = m;
-            s_row[1] = l;
+        {
+            const float2 x = lane % kMaxCluster < C ? s_pair[parity][lane % kMaxCluster] : make_float2(-FLT_MAX, 0.f);
+            m = x.x;
+            l = x.y;
+            join_lanes<kMaxCluster>(m, l, c);  // the same bits in every warp
         }
-        __syncthreads();
-        m = s_row[0];
-        l = s_row[1];
         parity ^= 1;
         const float inv = 1.f / l;
         const IdT* ids = static_cast<const IdT*>(a.ids) + r * a.K;
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
                 float x[E];
                 V8::unpack(raw, x);
 #pragma unroll
-                for (int t = 0; t < E; ++t) x[t] = exp2f((x[t] - m) * c) * qs;
+                for (int t = 0; t < E; ++t) x[t] = exp2_fast((x[t] - m) * c) * qs;
                 if (same_phase) {
                     __stcs(reinterpret_cast<uint4*>(out + head) + i, V8::pack(x));
                 } else {
@@ -337,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
             } else {
                 for (int i = first; i < nb; i += stride) emit(i, zv[i]);
             }
-            if (odd >= 0) store_from_f32(out + odd, exp2f((zo - m) * c) * qs);
+            if (odd >= 0) store_from_f32(out + odd, exp2_fast((zo - m) * c) * qs);
             __syncthreads();  // the listed entries of this CTA's part are written over
             for (int k = tid; k < a.K; k += kThreads) {
                 const long long id = (long long)ids[k];
@@ -345,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
                 const int v = (int)id;
                 const int owner = v < head || v >= tail0 ? 0 : ((v - head) / E / kThreads) % C;
                 if (owner != rank) continue;
-                const float q = exp2f((to_f32(z[v]) - m) * c) * inv;
+                const float q = exp2_fast((to_f32(z[v]) - m) * c) * inv;
                 store_from_f32(out + v, (q - a.ptot[r * a.K + k]) * scale);
             }
         }
@@ -382,21 +392,13 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    __shared__ double s_sum[kWarps];
     double t = 0.0;
     for (long long r = tid; r < a.T; r += kThreads) {
         const float w = __ldcg(a.weight + r);
         if (w != 0.f) t += (double)w * (double)__ldcg(a.loss_rows + r);
     }
-#pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) t += __shfl_xor_sync(kFull, t, o);
-    if (lane == 0) s_sum[warp] = t;
-    __syncthreads();
-    if (tid == 0) {
-        double sum = 0.0;
-        for (int i = 0; i < kWarps; ++i) sum += s_sum[i];
-        *a.loss = (float)(sum * (double)unit);
-    }
+    t = block_sum(t, s_sum);
+    if (tid == 0) *a.loss = (float)(t * (double)unit);
 }
 
 // Cluster size and vectors per thread.  A row of `vecs` vectors wants the fewest CTAs that
@@ -404,8 +406,8 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
 // row, up to 8, while they leave SMs without work.
 void pick(long long T, long long vecs, int sms, int* C, int* nv) {
     int c = 1;
-    while (c < 8 && vecs > (long long)c * kThreads * 6) c *= 2;
-    while (c < 8 && T * c * 2 <= 2 * sms && vecs > (long long)c * kThreads) c *= 2;
+    while (c < kMaxCluster && vecs > (long long)c * kThreads * 6) c *= 2;
+    while (c < kMaxCluster && T * c * 2 <= 2 * sms && vecs > (long long)c * kThreads) c *= 2;
     const long long per = (vecs + (long long)c * kThreads - 1) / ((long long)c * kThreads);
     *C = c;
     *nv = per <= 16 ? (int)std::max<long long>(per, 1) : 0;
