@@ -17,9 +17,11 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cstdint>
 
+#include "bf16_dot.cuh"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -32,6 +34,7 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxDevices = 64;
 constexpr int kPrepThreads = 256;
 constexpr int kPrepBlocks = 512;  // at most kThreads: the row kernel adds their weight sums, one per thread
 constexpr float kLog2e = 1.4426950408889634f;
@@ -128,9 +131,7 @@ distill_prep_kernel(const float* __restrict__ teacher, const IdT* __restrict__ i
 struct Rows {
     const void* z;
     long long sb, st;  // row r: z + (r / inner) * sb + (r % inner) * st
-    int inner;
-    long long T;
-    int V, K;
+    int inner, T, V, K;  // T rows
     const void* ids;
     const float* grad;  // nullptr: 1
     int grad_step;      // 0: one value, 1: one per row
@@ -157,6 +158,15 @@ struct Vec<float> {
         x[2] = __uint_as_float(v.z);
         x[3] = __uint_as_float(v.w);
     }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    // value - m
+    static __device__ __forceinline__ void minus(const uint4& v, float m, float (&x)[4]) {
+        unpack(v, x);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] -= m;
+    }
     static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
@@ -170,6 +180,21 @@ struct Vec<__nv_bfloat16> {
         unpack_bf16x2(v.y, x[2], x[3]);
         unpack_bf16x2(v.z, x[4], x[5]);
         unpack_bf16x2(v.w, x[6], x[7]);
+    }
+    static __device__ __forceinline__ float top(const uint4& v) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+        const __nv_bfloat162 t = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(t), __high2float(t));
+    }
+    // value - m as value * 1 + (-m): one mixed-precision fma each, nothing to convert
+    static __device__ __forceinline__ void minus(const uint4& v, float m, float (&x)[8]) {
+        constexpr uint32_t one = 0x3f803f80u;
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            x[2 * t] = fma_bf16<false>(w[t], one, -m);
+            x[2 * t + 1] = fma_bf16<true>(w[t], one, -m);
+        }
     }
     static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
         uint4 o;
@@ -197,6 +222,55 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+
+// x *= c, two lanes of the fp32 pipe per instruction; each product rounded as a plain one.
+template <int E>
+__device__ __forceinline__ void scale_pairs(float (&x)[E], float c) {
+    uint64_t cc;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(cc) : "f"(c));
+#pragma unroll
+    for (int t = 0; t < E; t += 2) {
+        uint64_t v;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x[t]), "f"(x[t + 1]));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(v) : "l"(cc));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(x[t]), "=f"(x[t + 1]) : "l"(v));
+    }
+}
+
+// exp2((value - m) c) of a vector.
+template <typename V, int E>
+__device__ __forceinline__ void exp_of(const uint4& v, float m, float c, float (&x)[E]) {
+    V::minus(v, m, x);
+    scale_pairs(x, c);
+#pragma unroll
+    for (int t = 0; t < E; ++t) x[t] = exp2_fast(x[t]);
+}
+
+// Pairwise sum.
+template <int E>
+__device__ __forceinline__ float sum_of(float (&x)[E]) {
+#pragma unroll
+    for (int w = E / 2; w >= 1; w /= 2) {
+#pragma unroll
+        for (int t = 0; t < w; ++t) x[t] += x[t + w];
+    }
+    return x[0];
+}
+
+// Where a row's values lie: `head` single values up to a 16-byte boundary, nb vectors, single values.
+template <typename T>
+struct RowAt {
+    const T* z;
+    int head, nb, tail0;
+    __device__ __forceinline__ RowAt(const Rows& a, int r) {
+        const int o = a.inner == a.T ? 0 : r / a.inner;
+        z = static_cast<const T*>(a.z) + (size_t)(o * a.sb + (r - o * a.inner) * a.st);
+        head = min(a.V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
+        nb = (a.V - head) / Vec<T>::n;
+        tail0 = head + nb * Vec<T>::n;
+    }
+    __device__ __forceinline__ const uint4* vec() const { return reinterpret_cast<const uint4*>(z + head); }
+};
 
 // (max, sum of exp2((z - max) c)) over lanes that differ in the bits below kLanes.
 template <int kLanes>
@@ -228,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long clusters = gridDim.x / C, me = blockIdx.x / C;
+    const int clusters = gridDim.x / C, me = blockIdx.x / C;
     if (a.skip_if_one && a.grad && *a.grad == 1.f) return;  // the same for every CTA
     __shared__ float2 s_warp[kWarps];
     __shared__ float s_part[kWarps];
@@ -241,64 +315,82 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
         const double w = block_sum(tid < a.prep_blocks ? a.wsum[tid] : 0.0, s_sum);
         unit = w != 0.0 ? (float)(1.0 / w) : 0.f;
     }
+    cluster.sync();  // every CTA has begun: its shared memory may be written from another
+    auto row_scale = [&](int r, float w) {
+        return (a.grad ? a.grad[(size_t)r * a.grad_step] : 1.f) * w * unit * a.tau;
+    };
     int parity = 0;
-    for (long long r = me; r < a.T; r += clusters) {
-        const float w = a.weight[r];
+    const int first = rank * kThreads + tid, stride = C * kThreads;
+    // this thread's vectors of the row in work; each is replaced by the next row's as soon as it is used
+    uint4 d[kNV > 0 ? kNV : 1];
+    auto load = [&](int j, const RowAt<T>& row) {
+        const int i = first + j * stride;
+        d[j] = i < row.nb ? load_stream(row.vec() + i) : make_uint4(V8::neg, V8::neg, V8::neg, V8::neg);
+    };
+    float w_next = me < a.T ? a.weight[me] : 0.f;
+    bool loaded = false;
+    for (int r = me; r < a.T; r += clusters) {
+        const float w = w_next;
+        w_next = r + clusters < a.T ? a.weight[r + clusters] : 0.f;
+        const RowAt<T> at(a, r);
+        RowAt<T> next(a, r + clusters < a.T ? r + clusters : r);
+        if (w_next == 0.f) next.nb = 0;  // no next row, or one that is not read
         T* out = a.dz ? static_cast<T*>(a.dz) + (size_t)r * a.V : nullptr;
         if (w == 0.f) {  // the cluster's CTAs agree
             if (rank == 0 && tid == 0 && a.loss_rows) a.loss_rows[r] = 0.f;
             if (out)
-                for (int v = rank * kThreads + tid; v < a.V; v += C * kThreads) store_from_f32(out + v, 0.f);
+                for (int v = first; v < a.V; v += stride) store_from_f32(out + v, 0.f);
+            loaded = false;
             continue;
         }
-        const T* z = static_cast<const T*>(a.z) + (size_t)((r / a.inner) * a.sb + (r % a.inner) * a.st);
-        // the row: `head` single values up to a 16-byte boundary, nb vectors, single values
-        const int head = min(a.V, (int)(((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / sizeof(T)));
-        const int nb = (a.V - head) / E;
-        const int tail0 = head + nb * E;
-        const uint4* zv = reinterpret_cast<const uint4*>(z + head);
-        const int first = rank * kThreads + tid, stride = C * kThreads;
+        if (kNV > 0 && !loaded) {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) load(j, at);
+        }
+        loaded = true;
+        const T* z = at.z;
+        const int head = at.head, nb = at.nb, tail0 = at.tail0;
+        const uint4* zv = at.vec();
         // the single values lie with rank 0: threads 0.. the head, threads 32.. the tail
         int odd = -1;
         if (rank == 0 && tid < head) odd = tid;
         if (rank == 0 && tid >= 32 && tail0 + tid - 32 < a.V) odd = tail0 + tid - 32;
         const float zo = odd >= 0 ? to_f32(z[odd]) : -INFINITY;
-        uint4 d[kNV > 0 ? kNV : 1];
+        // the first kThreads listed entries, one per thread: loaded with the row, used behind its sums
+        const size_t rk = (size_t)r * a.K;
+        const IdT* ids = static_cast<const IdT*>(a.ids) + rk;
+        auto listed = [&](int k) {
+            const long long id = k < a.K ? (long long)ids[k] : -1;
+            return id >= 0 && id < a.V ? (int)id : -1;
+        };
+        const int v0 = listed(tid);
+        float p0 = 0.f, lp0 = -INFINITY;
+        if (v0 >= 0) {
+            p0 = a.ptot[rk + tid];
+            lp0 = a.logp[rk + tid];
+        }
         float m = fmaxf(zo, -FLT_MAX), l = 0.f;
         if constexpr (kNV > 0) {
 #pragma unroll
-            for (int j = 0; j < kNV; ++j) {
-                const int i = first + j * stride;
-                d[j] = i < nb ? load_stream(zv + i) : make_uint4(V8::neg, V8::neg, V8::neg, V8::neg);
-            }
+            for (int j = 0; j < kNV; ++j) m = fmaxf(m, V8::top(d[j]));
 #pragma unroll
             for (int j = 0; j < kNV; ++j) {
                 float x[E];
-                V8::unpack(d[j], x);
-#pragma unroll
-                for (int t = 0; t < E; ++t) m = fmaxf(m, x[t]);
-            }
-#pragma unroll
-            for (int j = 0; j < kNV; ++j) {
-                float x[E];
-                V8::unpack(d[j], x);
-#pragma unroll
-                for (int t = 0; t < E; ++t) l += exp2_fast((x[t] - m) * c);
+                exp_of<V8>(d[j], m, c, x);
+                l += sum_of(x);
             }
         } else {
             for (int i = first; i < nb; i += stride) {
+                const uint4 v = zv[i];
+                const float mn = fmaxf(m, V8::top(v));
                 float x[E];
-                V8::unpack(zv[i], x);
-                float mn = m;
-#pragma unroll
-                for (int t = 0; t < E; ++t) mn = fmaxf(mn, x[t]);
-                l *= exp2_fast((m - mn) * c);
+                exp_of<V8>(v, mn, c, x);
+                l = l * exp2_fast((m - mn) * c) + sum_of(x);
                 m = mn;
-#pragma unroll
-                for (int t = 0; t < E; ++t) l += exp2_fast((x[t] - m) * c);
             }
         }
         if (odd >= 0) l += exp2_fast((zo - m) * c);
+        const float z0 = v0 >= 0 ? to_f32(z[v0]) : 0.f;
         join_lanes<32>(m, l, c);
         if (lane == 0) s_warp[warp] = make_float2(m, l);
         __syncthreads();
@@ -320,17 +412,27 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
         }
         parity ^= 1;
         const float inv = 1.f / l;
-        const IdT* ids = static_cast<const IdT*>(a.ids) + r * a.K;
+        if (a.loss_rows && rank == 0) {  // added up behind the barrier that follows
+            const float log_l = logf(l), inv_tau = 1.f / a.tau;
+            auto term = [&](float lp, float zk) {  // NaN teachers show, entries of p = 0 count nothing
+                const float p = expf(lp);
+                return p == 0.f ? 0.f : p * (lp - ((zk - m) * inv_tau - log_l));
+            };
+            float t = v0 >= 0 ? term(lp0, z0) : 0.f;
+            for (int k = tid + kThreads; k < a.K; k += kThreads) {
+                const int v = listed(k);
+                if (v >= 0) t += term(a.logp[rk + k], to_f32(z[v]));
+            }
+            t = warp_sum(t);
+            if (lane == 0) s_part[warp] = t;
+        }
         if (out) {
-            const float g = a.grad ? a.grad[r * a.grad_step] : 1.f;
-            const float scale = g * w * unit * a.tau;
-            const float qs = inv * scale;
+            const float qs = inv * row_scale(r, w);
             const bool same_phase = ((reinterpret_cast<uintptr_t>(out + head)) & 15) == 0;
             auto emit = [&](int i, const uint4& raw) {
                 float x[E];
-                V8::unpack(raw, x);
-#pragma unroll
-                for (int t = 0; t < E; ++t) x[t] = exp2_fast((x[t] - m) * c) * qs;
+                exp_of<V8>(raw, m, c, x);
+                scale_pairs(x, qs);
                 if (same_phase) {
                     __stcs(reinterpret_cast<uint4*>(out + head) + i, V8::pack(x));
                 } else {
@@ -343,43 +445,33 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
                 for (int j = 0; j < kNV; ++j) {
                     const int i = first + j * stride;
                     if (i < nb) emit(i, d[j]);
+                    load(j, next);
                 }
             } else {
                 for (int i = first; i < nb; i += stride) emit(i, zv[i]);
             }
             if (odd >= 0) store_from_f32(out + odd, exp2_fast((zo - m) * c) * qs);
-            __syncthreads();  // the listed entries of this CTA's part are written over
-            for (int k = tid; k < a.K; k += kThreads) {
-                const long long id = (long long)ids[k];
-                if (id < 0 || id >= a.V) continue;
-                const int v = (int)id;
-                const int owner = v < head || v >= tail0 ? 0 : ((v - head) / E / kThreads) % C;
-                if (owner != rank) continue;
-                const float q = exp2_fast((to_f32(z[v]) - m) * c) * inv;
-                store_from_f32(out + v, (q - a.ptot[r * a.K + k]) * scale);
+        } else if constexpr (kNV > 0) {
+#pragma unroll
+            for (int j = 0; j < kNV; ++j) load(j, next);
+        }
+        __syncthreads();  // the listed entries of this CTA's part are written over
+        if (out) {
+            auto owned = [&](int v) {
+                return (v < head || v >= tail0 ? 0 : ((v - head) / E / kThreads) & (C - 1)) == rank;
+            };
+            const float scale = row_scale(r, w);
+            if (v0 >= 0 && owned(v0)) store_from_f32(out + v0, (exp2_fast((z0 - m) * c) * inv - p0) * scale);
+            for (int k = tid + kThreads; k < a.K; k += kThreads) {
+                const int v = listed(k);
+                if (v < 0 || !owned(v)) continue;
+                store_from_f32(out + v, (exp2_fast((to_f32(z[v]) - m) * c) * inv - a.ptot[rk + k]) * scale);
             }
         }
-        if (a.loss_rows && rank == 0) {
-            const float log_l = logf(l), inv_tau = 1.f / a.tau;
-            float t = 0.f;
-            for (int k = tid; k < a.K; k += kThreads) {
-                const float lp = a.logp[r * a.K + k];
-                const float p = expf(lp);
-                if (p > 0.f) {  // an entry outside the vocabulary has p = 0
-                    const float lq = (to_f32(z[(long long)ids[k]]) - m) * inv_tau - log_l;
-                    t += p * (lp - lq);
-                } else if (lp != lp) {
-                    t = lp;
-                }
-            }
-            t = warp_sum(t);
-            if (lane == 0) s_part[warp] = t;
-            __syncthreads();
-            if (tid == 0) {
-                float sum = 0.f;
-                for (int i = 0; i < kWarps; ++i) sum += s_part[i];
-                a.loss_rows[r] = sum * a.tau * a.tau;
-            }
+        if (a.loss_rows && rank == 0 && tid == 0) {
+            float sum = 0.f;
+            for (int i = 0; i < kWarps; ++i) sum += s_part[i];
+            a.loss_rows[r] = sum * a.tau * a.tau;
         }
     }
     cluster.sync();  // no CTA leaves while another may still read its pair
@@ -393,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, kNV <= 6 ? 2 : 1) distill_rows_kerne
     if (!s_last) return;
     __threadfence();
     double t = 0.0;
-    for (long long r = tid; r < a.T; r += kThreads) {
+    for (int r = tid; r < a.T; r += kThreads) {
         const float w = __ldcg(a.weight + r);
         if (w != 0.f) t += (double)w * (double)__ldcg(a.loss_rows + r);
     }
@@ -414,12 +506,10 @@ void pick(long long T, long long vecs, int sms, int* C, int* nv) {
 }
 
 template <typename T, typename IdT, int kNV>
-cudaError_t launch_nv(const Rows& a, int C, int sms, cudaStream_t stream) {
+cudaError_t launch_nv(const Rows& a, int C, cudaStream_t stream) {
     auto kern = distill_rows_kernel<T, IdT, kNV>;
-    const long long resident = (long long)sms * (kNV <= 6 ? 2 : 1) / C;
-    const long long clusters = std::min<long long>(a.T, std::max<long long>(resident, 1));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(clusters * C));
+    cfg.gridDim = dim3((unsigned)C);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = stream;
     cudaLaunchAttribute at[1];
@@ -428,7 +518,20 @@ cudaError_t launch_nv(const Rows& a, int C, int sms, cudaStream_t stream) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a);
+    // as many clusters as run at once (a GPC's SMs do not divide evenly): each walks its share of the rows
+    static std::atomic<int> resident[kMaxDevices][4];  // by device and log2 C
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const int lc = C == 1 ? 0 : C == 2 ? 1 : C == 4 ? 2 : 3;
+    int n = dev < kMaxDevices ? resident[dev][lc].load(std::memory_order_relaxed) : 0;
+    if (n <= 0) {
+        if ((e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg)) != cudaSuccess) return e;
+        n = std::max(n, 1);
+        if (dev < kMaxDevices) resident[dev][lc].store(n, std::memory_order_relaxed);
+    }
+    cfg.gridDim = dim3((unsigned)(std::min(a.T, n) * C));
+    e = cudaLaunchKernelEx(&cfg, kern, a);
     if (e == cudaSuccess) note_launch();
     return e;
 }
@@ -439,16 +542,16 @@ cudaError_t launch_rows(const Rows& a, cudaStream_t stream) {
     int C = 1, nv = 0;
     pick(a.T, (a.V + Vec<T>::n - 1) / Vec<T>::n, sms, &C, &nv);
     switch (nv) {
-        case 1: return launch_nv<T, IdT, 1>(a, C, sms, stream);
-        case 2: return launch_nv<T, IdT, 2>(a, C, sms, stream);
-        case 3: return launch_nv<T, IdT, 3>(a, C, sms, stream);
-        case 4: return launch_nv<T, IdT, 4>(a, C, sms, stream);
-        case 5: return launch_nv<T, IdT, 5>(a, C, sms, stream);
-        case 6: return launch_nv<T, IdT, 6>(a, C, sms, stream);
-        case 7: case 8: return launch_nv<T, IdT, 8>(a, C, sms, stream);
-        case 9: case 10: return launch_nv<T, IdT, 10>(a, C, sms, stream);
-        case 0: return launch_nv<T, IdT, 0>(a, C, sms, stream);
-        default: return launch_nv<T, IdT, 16>(a, C, sms, stream);
+        case 1: return launch_nv<T, IdT, 1>(a, C, stream);
+        case 2: return launch_nv<T, IdT, 2>(a, C, stream);
+        case 3: return launch_nv<T, IdT, 3>(a, C, stream);
+        case 4: return launch_nv<T, IdT, 4>(a, C, stream);
+        case 5: return launch_nv<T, IdT, 5>(a, C, stream);
+        case 6: return launch_nv<T, IdT, 6>(a, C, stream);
+        case 7: case 8: return launch_nv<T, IdT, 8>(a, C, stream);
+        case 9: case 10: return launch_nv<T, IdT, 10>(a, C, stream);
+        case 0: return launch_nv<T, IdT, 0>(a, C, stream);
+        default: return launch_nv<T, IdT, 16>(a, C, stream);
     }
 }
 
@@ -460,12 +563,12 @@ Rows make_rows(const LogitDistillArgs& a) {
     r.sb = a.sb;
     r.st = a.st;
     r.inner = a.inner;
-    r.T = (long long)a.outer * a.inner;
+    r.T = a.outer * a.inner;
     r.V = a.V;
     r.K = a.K;
     r.ids = a.ids;
     r.mean = a.mean;
-    r.prep_blocks = (int)std::min<long long>(kPrepBlocks, (r.T + kPrepThreads / 32 - 1) / (kPrepThreads / 32));
+    r.prep_blocks = (int)std::min(kPrepBlocks, (r.T + kPrepThreads / 32 - 1) / (kPrepThreads / 32));
     r.tau = a.tau;
     r.counter = reinterpret_cast<unsigned*>(ws);
     r.wsum = reinterpret_cast<const double*>(ws + l.wsum);
