@@ -176,16 +176,20 @@ def version() -> str:
     return lib().ossa_version().decode()
 
 
+_DTYPE_CODES = {torch.float32: OSSA_F32, torch.bfloat16: OSSA_BF16}
+
+
 def dtype_code(t: torch.Tensor) -> int:
-    if t.dtype == torch.float32:
-        return OSSA_F32
-    if t.dtype == torch.bfloat16:
-        return OSSA_BF16
+    code = _DTYPE_CODES.get(t.dtype)
+    if code is not None:
+        return code
     raise TypeError(f"ossa_b200 kernels take float32 or bfloat16 tensors, got {t.dtype}")
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The device's current stream (the raw handle: no Stream object is made)."""
+    index = torch.cuda.current_device() if device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _Here:

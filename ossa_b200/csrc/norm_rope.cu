@@ -26,6 +26,7 @@ namespace ossa {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBwdCtas = 2;  // CTAs of the backward pass per SM
 
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
@@ -86,17 +87,62 @@ __device__ __forceinline__ Unit unit_at(const Pass& p, long long u, long long to
     return r;
 }
 
+// 8 values as loaded (bf16: 4 registers), so that rows ahead and the tables cost little to hold.
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = __ldg(reinterpret_cast<const float4*>(p));
+        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+};
+template <>
+struct Raw8<__nv_bfloat16> {
+    uint4 a;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        unpack_bf16x2(a.x, v[0], v[1]);
+        unpack_bf16x2(a.y, v[2], v[3]);
+        unpack_bf16x2(a.z, v[4], v[5]);
+        unpack_bf16x2(a.w, v[6], v[7]);
+    }
+};
+
+// The two halves of a row's piece.
+template <typename T>
+struct Pair8 {
+    Raw8<T> lo, hi;
+    __device__ __forceinline__ void load(const T* row, int l, int h, bool on) {
+        if (on) {
+            lo.load(row + l);
+            hi.load(row + h);
+        } else {
+            lo.zero();
+            hi.zero();
+        }
+    }
+    __device__ __forceinline__ void get(float (&a)[8], float (&b)[8]) const {
+        lo.get(a);
+        hi.get(b);
+    }
+};
+
+// cos and sin of a position.
 template <typename T>
 struct Tables {
-    float cl[8], ch[8], sl[8], sh[8];
+    Pair8<T> c, s;
     __device__ __forceinline__ void load(const Pass& p, int b, int n, int lo, int hi) {
         const size_t at = ((size_t)(p.cs_batched ? b : 0) * p.N + n) * p.D;
-        const T* c = static_cast<const T*>(p.cosv) + at;
-        const T* s = static_cast<const T*>(p.sinv) + at;
-        VecLoad<T, 8>::load(c + lo, cl);
-        VecLoad<T, 8>::load(c + hi, ch);
-        VecLoad<T, 8>::load(s + lo, sl);
-        VecLoad<T, 8>::load(s + hi, sh);
+        c.load(static_cast<const T*>(p.cosv) + at, lo, hi, true);
+        s.load(static_cast<const T*>(p.sinv) + at, lo, hi, true);
     }
 };
 
@@ -108,9 +154,17 @@ __device__ __forceinline__ float row_sum(float x) {
     return x;
 }
 
+// Heads whose rows a lane group loads at once: the more bytes in flight, the nearer to HBM's rate
+// (B=8, N=4096, 12 + 2 heads, bf16: one head at a time 66 us, four 48 us).
+template <typename T>
+constexpr int kHeads = sizeof(T) == 2 ? 4 : 2;
+
+// Steps of a lane group's walk over its heads, the most of the warp's groups (the row sums are warp-wide).
+__device__ __forceinline__ int warp_heads(const Unit& u) { return __reduce_max_sync(kFull, u.h1 - u.h0); }
+
 template <typename T, int L>
-__global__ void __launch_bounds__(kThreads) norm_rope_fwd_kernel(const Pass p) {
-    constexpr int D = 16 * L;
+__global__ void __launch_bounds__(kThreads, 2) norm_rope_fwd_kernel(const Pass p) {
+    constexpr int D = 16 * L, kH = kHeads<T>;
     const int l = threadIdx.x % L;
     const int lo = 8 * l, hi = D / 2 + 8 * l;
     const long long tokens = (long long)p.B * p.N, units = tokens * p.chunks;
@@ -119,53 +173,60 @@ __global__ void __launch_bounds__(kThreads) norm_rope_fwd_kernel(const Pass p) {
     const Unit u = unit_at(p, live ? u0 : units - 1, tokens);
     const Side& s = p.s[u.side];
     const bool rope = p.cosv != nullptr, norm = s.w != nullptr;
+    const T* x = static_cast<const T*>(s.x) + (size_t)(u.b * s.sb + u.n * s.sn);
+    const int heads = warp_heads(u);
+    Pair8<T> rows[kH];
+    auto load = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < kH; ++i) {
+            const int h = u.h0 + k + i;
+            rows[i].load(x + (size_t)h * D, lo, hi, live && h < u.h1);
+        }
+    };
+    load(0);
     Tables<T> cs;
     if (rope) cs.load(p, u.b, u.n, lo, hi);
     float wl[8], wh[8];
-    if (norm) {
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            wl[t] = weight_at(s.w, p.w_f32, lo + t);
-            wh[t] = weight_at(s.w, p.w_f32, hi + t);
-        }
+    for (int t = 0; t < 8; ++t) {
+        wl[t] = norm ? weight_at(s.w, p.w_f32, lo + t) : 1.f;
+        wh[t] = norm ? weight_at(s.w, p.w_f32, hi + t) : 1.f;
     }
-    const T* x = static_cast<const T*>(s.x) + (size_t)(u.b * s.sb + u.n * s.sn);
-    // every lane of a warp takes the same number of steps (the row sums are warp-wide)
-    for (int k = 0; k < p.chunk; ++k) {
-        const int h = u.h0 + k;
-        const bool on = live && h < u.h1;
-        float a[8], b[8];
-        if (on) {
-            VecLoad<T, 8>::load(x + (size_t)h * D + lo, a);
-            VecLoad<T, 8>::load(x + (size_t)h * D + hi, b);
-        } else {
+    for (int k = 0; k < heads; k += kH) {
+        if (k > 0) load(k);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) a[t] = b[t] = 0.f;
-        }
-        float ss = 0.f;
+        for (int i = 0; i < kH; ++i) {
+            const int h = u.h0 + k + i;
+            const bool on = live && h < u.h1;
+            float a[8], b[8];
+            rows[i].get(a, b);
+            if (norm) {
+                float ss = 0.f;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) ss = fmaf(a[t], a[t], fmaf(b[t], b[t], ss));
-        ss = row_sum<L>(ss);
-        if (norm) {
-            const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                for (int t = 0; t < 8; ++t) ss = fmaf(a[t], a[t], fmaf(b[t], b[t], ss));
+                const float r = rsqrtf(row_sum<L>(ss) * (1.f / D) + p.eps);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                a[t] *= r * wl[t];
-                b[t] *= r * wh[t];
+                for (int t = 0; t < 8; ++t) {
+                    a[t] *= r * wl[t];
+                    b[t] *= r * wh[t];
+                }
             }
-        }
-        if (rope) {
+            if (rope) {
+                float cl[8], ch[8], sl[8], sh[8];
+                cs.c.get(cl, ch);
+                cs.s.get(sl, sh);
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const float y = a[t];
-                a[t] = y * cs.cl[t] - b[t] * cs.sl[t];
-                b[t] = b[t] * cs.ch[t] + y * cs.sh[t];
+                for (int t = 0; t < 8; ++t) {
+                    const float y = a[t];
+                    a[t] = y * cl[t] - b[t] * sl[t];
+                    b[t] = b[t] * ch[t] + y * sh[t];
+                }
             }
-        }
-        if (on) {
-            T* o = static_cast<T*>(s.o) + (((size_t)u.b * s.H + h) * p.N + u.n) * D;
-            store8(o + lo, a);
-            store8(o + hi, b);
+            if (on) {
+                T* o = static_cast<T*>(s.o) + (((size_t)u.b * s.H + h) * p.N + u.n) * D;
+                store8(o + lo, a);
+                store8(o + hi, b);
+            }
         }
     }
 }
@@ -174,8 +235,9 @@ __global__ void __launch_bounds__(kThreads) norm_rope_fwd_kernel(const Pass p) {
 // sums for dw go to part[block][D] and are joined in block order by dw_join_kernel, so the
 // result does not depend on the order in which CTAs run.
 template <typename T, int L>
-__global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(const Pass p, int blocks0, float* __restrict__ part) {
-    constexpr int D = 16 * L, kGroups = kThreads / L;
+__global__ void __launch_bounds__(kThreads, 2)
+norm_rope_bwd_kernel(const Pass p, int blocks0, float* __restrict__ part) {
+    constexpr int D = 16 * L, kGroups = kThreads / L, kH = kHeads<T> / 2;
     __shared__ float sums[kGroups > 16 ? 16 : kGroups][D];
     const int l = threadIdx.x % L, grp = threadIdx.x / L;
     const int lo = 8 * l, hi = D / 2 + 8 * l;
@@ -195,67 +257,73 @@ __global__ void __launch_bounds__(kThreads) norm_rope_bwd_kernel(const Pass p, i
     const int chunks = side ? p.chunks - p.chunks0 : p.chunks0;
     const long long units = tokens * chunks, step = (long long)nblk * kGroups;
     const long long first = side ? tokens * p.chunks0 : 0;
-    // the CTA's groups take the same number of rounds (the row sums are warp-wide)
+    // the CTA's groups take the same number of rounds
     for (long long base = (long long)blk * kGroups; base < units; base += step) {
         const bool live = base + grp < units;
         const Unit u = unit_at(p, first + (live ? base + grp : units - 1), tokens);
+        const T* x = static_cast<const T*>(s.x) + (size_t)(u.b * s.sb + u.n * s.sn);
+        const T* g = static_cast<const T*>(s.g) + ((size_t)u.b * s.H * p.N + u.n) * D;
+        const size_t gh = (size_t)p.N * D;  // from head to head
+        const int heads = warp_heads(u);
+        Pair8<T> ax[kH], ag[kH];
+        auto load = [&](int k) {
+#pragma unroll
+            for (int i = 0; i < kH; ++i) {
+                const int h = u.h0 + k + i;
+                const bool on = live && h < u.h1;
+                ag[i].load(g + h * gh, lo, hi, on);
+                ax[i].load(x + (size_t)h * D, lo, hi, on && norm);
+            }
+        };
+        load(0);
         Tables<T> cs;
         if (rope) cs.load(p, u.b, u.n, lo, hi);
-        const T* x = static_cast<const T*>(s.x) + (size_t)(u.b * s.sb + u.n * s.sn);
-        for (int k = 0; k < p.chunk; ++k) {
-            const int h = u.h0 + k;
-            const bool on = live && h < u.h1;
-            float a[8], b[8], ga[8], gb[8];
-            if (on) {
-                const T* g = static_cast<const T*>(s.g) + (((size_t)u.b * s.H + h) * p.N + u.n) * D;
-                VecLoad<T, 8>::load(g + lo, ga);
-                VecLoad<T, 8>::load(g + hi, gb);
-                if (norm) {
-                    VecLoad<T, 8>::load(x + (size_t)h * D + lo, a);
-                    VecLoad<T, 8>::load(x + (size_t)h * D + hi, b);
-                }
-            }
-            if (!on || !norm) {
+        for (int k = 0; k < heads; k += kH) {
+            if (k > 0) load(k);
 #pragma unroll
-                for (int t = 0; t < 8; ++t) a[t] = b[t] = 0.f;
-            }
-            if (!on) {
+            for (int i = 0; i < kH; ++i) {
+                const int h = u.h0 + k + i;
+                const bool on = live && h < u.h1;
+                float a[8], b[8], ga[8], gb[8];
+                ax[i].get(a, b);
+                ag[i].get(ga, gb);
+                if (rope) {
+                    float cl[8], ch[8], sl[8], sh[8];
+                    cs.c.get(cl, ch);
+                    cs.s.get(sl, sh);
 #pragma unroll
-                for (int t = 0; t < 8; ++t) ga[t] = gb[t] = 0.f;
-            }
-            if (rope) {
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    const float y = ga[t];
-                    ga[t] = y * cs.cl[t] + gb[t] * cs.sh[t];
-                    gb[t] = gb[t] * cs.ch[t] - y * cs.sl[t];
-                }
-            }
-            if (norm) {
-                float ss = 0.f, dot = 0.f;
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    ss = fmaf(a[t], a[t], fmaf(b[t], b[t], ss));
-                    dot = fmaf(a[t], ga[t] * wl[t], fmaf(b[t], gb[t] * wh[t], dot));
-                }
-                ss = row_sum<L>(ss);
-                dot = row_sum<L>(dot);
-                const float r = rsqrtf(ss * (1.f / D) + p.eps);
-                const float c = dot * (1.f / D) * r * r;
-#pragma unroll
-                for (int t = 0; t < 8; ++t) {
-                    if (on) {  // a dead lane's zero row has r = 1/sqrt(eps), infinite at eps 0
-                        dl[t] = fmaf(ga[t], a[t] * r, dl[t]);
-                        dh[t] = fmaf(gb[t], b[t] * r, dh[t]);
+                    for (int t = 0; t < 8; ++t) {
+                        const float y = ga[t];
+                        ga[t] = y * cl[t] + gb[t] * sh[t];
+                        gb[t] = gb[t] * ch[t] - y * sl[t];
                     }
-                    ga[t] = r * (ga[t] * wl[t] - a[t] * c);
-                    gb[t] = r * (gb[t] * wh[t] - b[t] * c);
                 }
-            }
-            if (on) {
-                T* o = static_cast<T*>(s.o) + (((size_t)u.b * p.N + u.n) * s.H + h) * D;
-                store8(o + lo, ga);
-                store8(o + hi, gb);
+                if (norm) {
+                    float ss = 0.f, dot = 0.f;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        ss = fmaf(a[t], a[t], fmaf(b[t], b[t], ss));
+                        dot = fmaf(a[t], ga[t] * wl[t], fmaf(b[t], gb[t] * wh[t], dot));
+                    }
+                    ss = row_sum<L>(ss);
+                    dot = row_sum<L>(dot);
+                    const float r = rsqrtf(ss * (1.f / D) + p.eps);
+                    const float c = dot * (1.f / D) * r * r;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t) {
+                        if (on) {  // a dead lane's zero row has r = 1/sqrt(eps), infinite at eps 0
+                            dl[t] = fmaf(ga[t], a[t] * r, dl[t]);
+                            dh[t] = fmaf(gb[t], b[t] * r, dh[t]);
+                        }
+                        ga[t] = r * (ga[t] * wl[t] - a[t] * c);
+                        gb[t] = r * (gb[t] * wh[t] - b[t] * c);
+                    }
+                }
+                if (on) {
+                    T* o = static_cast<T*>(s.o) + (((size_t)u.b * p.N + u.n) * s.H + h) * D;
+                    store8(o + lo, ga);
+                    store8(o + hi, gb);
+                }
             }
         }
     }
@@ -377,23 +445,28 @@ norm_rope_any_kernel(const Pass p, int blocks0, float* __restrict__ part) {
     }
 }
 
-// dw of both sides: a warp per column adds the blocks' sums, lanes in block order, then
-// the fixed tree of a warp sum.
+// dw of both sides: a CTA takes 32 columns, each of its 8 warps every eighth block's row of sums in block
+// order; the warps' results are added in warp order.
 __global__ void __launch_bounds__(kThreads)
 dw_join_kernel(const float* __restrict__ part, int blocks0, int blocks, int D, void* dw0, void* dw1, int w_f32) {
-    const int col = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (col >= 2 * D) return;
-    const int side = col >= D, d = side ? col - D : col;
+    constexpr int kWarps = kThreads / 32;
+    __shared__ float sums[kWarps][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, side = blockIdx.y;
+    const int d = blockIdx.x * 32 + lane;
     void* out = side ? dw1 : dw0;
-    if (!out) return;
+    if (!out) return;  // CTA-uniform
     float t = 0.f;
-    for (int i = (side ? blocks0 : 0) + lane; i < (side ? blocks : blocks0); i += 32) t += part[(size_t)i * D + d];
-    t = warp_sum(t);
-    if (lane == 0) {
-        if (w_f32) static_cast<float*>(out)[d] = t;
-        else static_cast<__nv_bfloat16*>(out)[d] = __float2bfloat16_rn(t);
+    if (d < D) {
+#pragma unroll 8
+        for (int i = (side ? blocks0 : 0) + warp; i < (side ? blocks : blocks0); i += kWarps) t += part[(size_t)i * D + d];
     }
+    sums[warp][lane] = t;
+    __syncthreads();
+    if (warp != 0 || d >= D) return;
+    t = 0.f;
+    for (int w = 0; w < kWarps; ++w) t += sums[w][lane];
+    if (w_f32) static_cast<float*>(out)[d] = t;
+    else static_cast<__nv_bfloat16*>(out)[d] = __float2bfloat16_rn(t);
 }
 
 Pass make_pass(const NormRopeArgs& a, bool backward) {
@@ -431,7 +504,7 @@ bool lane_layout(int D) { return D == 16 || D == 32 || D == 64 || D == 128 || D 
 
 // CTAs of the backward pass, and how many of them are side 0's.
 void bwd_blocks(const NormRopeArgs& a, int* blocks0, int* blocks) {
-    const int most = 4 * device_sm_count();
+    const int most = kBwdCtas * device_sm_count();
     const int per = lane_layout(a.D) ? kThreads / (a.D / 16) : kThreads / 32;
     const long long rq = ((long long)a.B * a.N * a.Hq + per - 1) / per, rk = ((long long)a.B * a.N * a.Hk + per - 1) / per;
     const int H = a.Hq + a.Hk;
@@ -490,8 +563,7 @@ cudaError_t bwd_t(const NormRopeArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     note_launch();
     if (!a.dwq && !a.dwk) return cudaSuccess;
-    dw_join_kernel<<<(2 * a.D + kThreads / 32 - 1) / (kThreads / 32), kThreads, 0, stream>>>(
-        a.part, b0, blocks, a.D, a.dwq, a.dwk, a.w_f32);
+    dw_join_kernel<<<dim3((a.D + 31) / 32, 2), kThreads, 0, stream>>>(a.part, b0, blocks, a.D, a.dwq, a.dwk, a.w_f32);
     e = cudaGetLastError();
     if (e == cudaSuccess) note_launch();
     return e;
@@ -499,7 +571,7 @@ cudaError_t bwd_t(const NormRopeArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-size_t norm_rope_workspace_bytes(int D) { return (size_t)4 * device_sm_count() * D * sizeof(float); }
+size_t norm_rope_workspace_bytes(int D) { return (size_t)kBwdCtas * device_sm_count() * D * sizeof(float); }
 
 cudaError_t launch_norm_rope_fwd(const NormRopeArgs& a, cudaStream_t stream) {
     return a.dtype == kF32 ? fwd_t<float>(a, stream) : fwd_t<__nv_bfloat16>(a, stream);

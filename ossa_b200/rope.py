@@ -77,13 +77,23 @@ class _RopeToHeads(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        return _norm_rope_backward(None, None, None, None, *ctx.saved_tensors, 0.0, g, None)[0].view(ctx.shape), None, \
-            None, None
+        cos, sin = ctx.saved_tensors
+        g = g.contiguous()
+        B, H, N, D = g.shape
+        dx = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
+        args = (None, None, None, None, _lib.ptr(cos), _lib.ptr(sin),
+                1 if cos is not None and B > 1 and cos.shape[0] == B else 0, _lib.dtype_code(g), _lib.OSSA_F32, B, N, H, 0,
+                D, 0, 0, 0, 0, 0.0)
+        _norm_rope_backward(args, g, None, dx, None, None, None)
+        return dx, None, None, None
 
 
 def _tables(cos, sin, B, N, D, dtype):
     """cos, sin as the kernels read them: contiguous (B or 1, N, D) of the rows' type."""
-    cos, sin = cos.detach().to(dtype), sin.detach().to(dtype)
+    if cos.requires_grad or sin.requires_grad:
+        cos, sin = cos.detach(), sin.detach()
+    if cos.dtype != dtype or sin.dtype != dtype:
+        cos, sin = cos.to(dtype), sin.to(dtype)
     if cos.dim() == 2:
         cos, sin = cos.unsqueeze(0), sin.unsqueeze(0)
     if cos.shape != sin.shape or cos.dim() != 3 or cos.shape[0] not in (1, B) or tuple(cos.shape[1:]) != (N, D):
@@ -101,9 +111,12 @@ def _rows(x, heads, name):
     else:
         raise ValueError(f"{name} of shape {tuple(x.shape)} is not (B, N, {heads} heads x D) or (B, N, {heads}, D)")
     B, N = x.shape[:2]
-    sb, sn = x.stride()[:2]
-    whole = x.stride(-1) == 1 and (x.dim() == 3 or heads == 1 or x.stride(2) == D)
-    sb, sn = (sb if B > 1 else 0), (sn if N > 1 else 0)
+    if x.is_contiguous():
+        sn, sb, whole = heads * D, N * heads * D, True
+    else:
+        sb, sn = x.stride()[:2]
+        whole = x.stride(-1) == 1 and (x.dim() == 3 or heads == 1 or x.stride(2) == D)
+        sb, sn = (sb if B > 1 else 0), (sn if N > 1 else 0)
     if not whole or sb * x.element_size() % 16 or sn * x.element_size() % 16 or x.data_ptr() % 16:
         x = x.contiguous()
         if x.data_ptr() % 16:
@@ -112,88 +125,81 @@ def _rows(x, heads, name):
     return x, B, N, D, sb, sn
 
 
-def _weight_code(*ws):
-    for w in ws:
-        if w is not None:
-            return _lib.OSSA_F32 if w.dtype == torch.float32 else _lib.OSSA_BF16
-    return _lib.OSSA_F32
-
-
-def _norm_rope_backward(q, k, wq, wk, cos, sin, eps, gq, gk, want=(False, False)):
-    """Gradients (dq, dk, dwq, dwk) from those of the (B, Hx, N, D) outputs; dq, dk contiguous
-    (B, N, Hx, D).  q, k are read only where there is a weight."""
-    dev, dt = gq.device, gq.dtype
-    gq = gq.contiguous()
-    B, Hq, N, D = gq.shape
-    dq = torch.empty((B, N, Hq, D), dtype=dt, device=dev)
-    dk, Hk = None, 0
-    if gk is not None:
-        gk = gk.contiguous()
-        Hk = gk.shape[1]
-        dk = torch.empty((B, N, Hk, D), dtype=dt, device=dev)
-    dwq = torch.empty_like(wq) if want[0] else None
-    dwk = torch.empty_like(wk) if want[1] else None
-    qs = ks = (0, 0)
-    if q is not None:
-        q, _, _, _, *qs = _rows(q, Hq, "q")
-    if k is not None:
-        k, _, _, _, *ks = _rows(k, Hk, "k")
-    L = _lib.lib()
-    ws, ws_bytes = None, 0
-    if wq is not None or wk is not None:
-        ws_bytes = L.ossa_qk_norm_rope_bwd_workspace_size(D)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    with _lib.on_device(dev):
-        st = L.ossa_qk_norm_rope_bwd(
-            _lib.ptr(q), _lib.ptr(k), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
-            1 if cos is not None and cos.shape[0] == B and B > 1 else 0, _lib.dtype_code(gq), _weight_code(wq, wk),
-            B, N, Hq, Hk, D, *qs, *ks, eps, gq.data_ptr(), _lib.ptr(gk), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dwq),
-            _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
-    _lib.check(st)
-    return dq, dk, dwq, dwk
-
-
-def _norm_rope_forward(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps):
+def _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps):
+    """(the arguments that the C forward and backward begin with, the tensors they point into)."""
     q, B, N, D, *qs = _rows(q, n_heads, "q")
     k, _, _, _, *ks = _rows(k, n_kv_heads, "k")
-    dev = q.device
-    q_out = torch.empty((B, n_heads, N, D), dtype=q.dtype, device=dev)
-    k_out = torch.empty((B, n_kv_heads, N, D), dtype=q.dtype, device=dev)
+    w = wq if wq is not None else wk
+    args = (q.data_ptr(), k.data_ptr(), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
+            1 if cos is not None and B > 1 and cos.shape[0] == B else 0, _lib.dtype_code(q),
+            _lib.OSSA_F32 if w is None else _lib.dtype_code(w), B, N, n_heads, n_kv_heads, D, *qs, *ks, eps)
+    return args, (q, k, wq, wk, cos, sin)
+
+
+def _norm_rope_forward(args, dtype, dev):
+    B, N, Hq, Hk, D = args[9:14]
+    q_out = torch.empty((B, Hq, N, D), dtype=dtype, device=dev)
+    k_out = torch.empty((B, Hk, N, D), dtype=dtype, device=dev)
     if B * N > 0:
         with _lib.on_device(dev):
-            st = _lib.lib().ossa_qk_norm_rope_fwd(
-                q.data_ptr(), k.data_ptr(), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
-                1 if cos is not None and cos.shape[0] == B and B > 1 else 0, _lib.dtype_code(q), _weight_code(wq, wk),
-                B, N, n_heads, n_kv_heads, D, *qs, *ks, eps, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_ptr(dev))
-        _lib.check(st)
+            st = _lib.lib().ossa_qk_norm_rope_fwd(*args, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_ptr(dev))
+        if st:
+            _lib.check(st)
     return q_out, k_out
+
+
+def _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk):
+    """Writes the gradients from those of the (B, Hx, N, D) outputs."""
+    dev = gq.device
+    L = _lib.lib()
+    with _lib.on_device(dev):
+        ws, ws_bytes = None, 0
+        if args[2] is not None or args[3] is not None:
+            ws_bytes = L.ossa_qk_norm_rope_bwd_workspace_size(args[13])
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        st = L.ossa_qk_norm_rope_bwd(*args, gq.data_ptr(), _lib.ptr(gk), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dwq),
+                                     _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+    if st:
+        _lib.check(st)
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, n_heads, n_kv_heads, cos, sin, eps):
-        ctx.save_for_backward(q, k, wq, wk, cos, sin)
-        ctx.eps = eps
+        args, kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
+        ctx.save_for_backward(*kept)
+        ctx.call = (args, q.shape, k.shape)
         ctx.set_materialize_grads(False)
-        return _norm_rope_forward(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
+        return _norm_rope_forward(args, q.dtype, q.device)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin = ctx.saved_tensors
+        _, _, wq, wk, _, _ = ctx.saved_tensors  # the pointers in ctx.call lead into these
+        args, q_shape, k_shape = ctx.call
         if gq is None and gk is None:
             return (None,) * 9
+        g = gq if gq is not None else gk
+        dt, dev = g.dtype, g.device
         need = ctx.needs_input_grad
-        if gq is None or gk is None:  # one output has no gradient: the other tensor alone
-            one = 0 if gk is None else 1
-            x, w, g = (q, wq, gq) if one == 0 else (k, wk, gk)
-            dx, _, dw, _ = _norm_rope_backward(x, None, w, None, cos, sin, ctx.eps, g, None,
-                                               want=(need[2 + one] and w is not None, False))
-            dx = dx.view(x.shape)
-            return (dx, None, dw) + (None,) * 6 if one == 0 else (None, dx, None, dw) + (None,) * 5
-        dq, dk, dwq, dwk = _norm_rope_backward(q, k, wq, wk, cos, sin, ctx.eps, gq, gk,
-                                               want=(need[2] and wq is not None, need[3] and wk is not None))
-        return dq.view(q.shape), dk.view(k.shape), dwq, dwk, None, None, None, None, None
+        dq = dk = dwq = dwk = None
+        if gq is not None:
+            gq = gq.contiguous()
+            dq = torch.empty(q_shape, dtype=dt, device=dev)
+            dwq = torch.empty_like(wq) if need[2] else None
+        if gk is not None:
+            gk = gk.contiguous()
+            dk = torch.empty(k_shape, dtype=dt, device=dev)
+            dwk = torch.empty_like(wk) if need[3] else None
+        if gk is None:  # one output has no gradient: the other tensor alone, in the place of the queries
+            args = args[:1] + (None, args[2], None) + args[4:12] + (0,) + args[13:]
+            _norm_rope_backward(args, gq, None, dq, None, dwq, None)
+        elif gq is None:
+            args = (args[1], None, args[3], None) + args[4:11] + (args[12], 0, args[13], args[16], args[17]) + args[16:]
+            _norm_rope_backward(args, gk, None, dk, None, dwk, None)
+        else:
+            _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk)
+        return dq, dk, dwq, dwk, None, None, None, None, None
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int,
@@ -224,8 +230,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} are not (B, N, heads x D) of one B and N")
     D = q.shape[3] if q.dim() == 4 else q.shape[2] // max(n_heads, 1)
     Dk = k.shape[3] if k.dim() == 4 else k.shape[2] // max(n_kv_heads, 1)
-    if n_heads <= 0 or n_kv_heads <= 0 or D != Dk or q.shape[2:].numel() != n_heads * D or \
-            k.shape[2:].numel() != n_kv_heads * D:
+    if n_heads <= 0 or n_kv_heads <= 0 or D != Dk or \
+            (q.shape[2] != n_heads if q.dim() == 4 else q.shape[2] != n_heads * D) or \
+            (k.shape[2] != n_kv_heads if k.dim() == 4 else k.shape[2] != n_kv_heads * D):
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not hold {n_heads} and {n_kv_heads} heads of one D")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w is not None and (tuple(w.shape) != (D,) or not w.is_floating_point()):
@@ -241,4 +248,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int
         cos, sin = _tables(cos, sin, q.shape[0], q.shape[1], D, q.dtype)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QkNormRope.apply(q, k, q_weight, k_weight, n_heads, n_kv_heads, cos, sin, eps)
-    return _norm_rope_forward(q, k, n_heads, n_kv_heads, q_weight, k_weight, cos, sin, eps)
+    args, _kept = _call_args(q, k, n_heads, n_kv_heads, q_weight, k_weight, cos, sin, eps)
+    return _norm_rope_forward(args, q.dtype, q.device)

@@ -176,8 +176,8 @@ def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, seg
     _lib.require_cuda(*[t for t in (q, k, v, idx, slopes, segments, prefix_len) if t is not None])
     if grad:
         return _TopkAttention.apply(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
-    return _mod_forward(q.contiguous(), k.contiguous(), v.contiguous(), slopes, idx.contiguous(), segments, prefix_len,
-                        causal, q0, cap, None)
+    q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
+    return _mod_forward(_mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap), q, None)
 
 
 def _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
@@ -188,15 +188,14 @@ def _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
             1 if causal else 0, q0, cap, _lib.ptr(slopes), _lib.ptr(segments), _lib.ptr(prefix_len))
 
 
-def _mod_forward(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap, lse2):
+def _mod_forward(args, q, lse2):
     out = torch.empty_like(q)
     if out.numel() == 0:
         return out
     with _lib.on_device(q.device):
-        st = _lib.lib().ossa_topk_attention_mod_fwd(
-            *_mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap), out.data_ptr(), _lib.ptr(lse2),
-            _lib.stream_ptr(q.device))
-    _lib.check(st)
+        st = _lib.lib().ossa_topk_attention_mod_fwd(*args, out.data_ptr(), _lib.ptr(lse2), _lib.stream_ptr(q.device))
+    if st:
+        _lib.check(st)
     return out
 
 
@@ -205,28 +204,27 @@ class _TopkAttention(torch.autograd.Function):
     def forward(ctx, q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
         q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
         lse2 = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-        out = _mod_forward(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap, lse2)
+        args = _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
+        out = _mod_forward(args, q, lse2)
         ctx.save_for_backward(q, k, v, slopes, idx, segments, prefix_len, out, lse2)
-        ctx.rule = (causal, q0, cap)
+        ctx.call = args
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, slopes, idx, segments, prefix_len, out, lse2 = ctx.saved_tensors
-        dev = q.device
-        dout = dout.to(q.dtype).contiguous()
+        q, k, v, slopes, _, _, _, out, lse2 = ctx.saved_tensors  # the pointers in ctx.call lead into these
+        args, dev = ctx.call, q.device
+        dout = dout.contiguous()
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
         L = _lib.lib()
-        B, H, Nq, D = q.shape
         with _lib.on_device(dev):
-            ws_bytes = L.ossa_topk_attention_bwd_workspace_size(_lib.dtype_code(q), B, H, k.shape[1], Nq, k.shape[2], D,
-                                                                idx.shape[-1], 0 if dslopes is None else 1)
+            ws_bytes = L.ossa_topk_attention_bwd_workspace_size(*args[5:13], 0 if dslopes is None else 1)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
             st = L.ossa_topk_attention_bwd(
-                *_mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), out.data_ptr(), lse2.data_ptr(),
-                dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(dslopes), ws.data_ptr(),
-                ws_bytes, _lib.stream_ptr(dev))
-        _lib.check(st)
+                *args, out.data_ptr(), lse2.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                _lib.ptr(dslopes), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+        if st:
+            _lib.check(st)
         return dq, dk, dv, dslopes, None, None, None, None, None, None
