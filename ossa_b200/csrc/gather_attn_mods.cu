@@ -1,10 +1,11 @@
 // Gathered top-K attention forward with score modifiers (score_mods.cuh), and the row statistic
 // that its backward pass reads.  Also the training form of the unmodified gather.
 //
-// bf16 rows of head_dim 128 with 2-8 query heads per kv head and at most 128 listed keys take the
-// tensor-core form below, everything else the per-head forms of gather_attn_kernels.cuh.
+// bf16 rows of head_dim 128: few of them take a CTA per row and head (mod_attn_few_kernel); with 2-8
+// query heads per kv head and at most 128 listed keys more of them take the tensor-core form; everything
+// else takes the per-head forms of gather_attn_kernels.cuh.
 //
-// One warp per query and kv head, all G heads of the group at once (query_union.cuh): every key
+// Tensor-core form: one warp per query and kv head, all G heads of the group at once (query_union.cuh): every key
 // that some head lists is fetched once.  In chunks of 16 keys: S^T = K Q^T with the keys as MMA
 // rows and the heads as columns, scores and masks per (key, head), online softmax per head, then
 // O^T += V^T P^T with P^T moved into operand layout by movmatrix.  The key rows of chunk c + 1 are in
@@ -13,6 +14,7 @@
 // A query with a key listed twice by one head, or with more than 512 different keys, takes its heads
 // one after another through the same loop.
 #include "gather_attn_kernels.cuh"
+#include <algorithm>
 #include "query_union.cuh"
 
 namespace ossa {
@@ -193,6 +195,118 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     }
 }
 
+// Few rows (single tokens): a CTA per (query, head), a warp per 16 listed keys, so that a row is two trips
+// to memory (its list, then all its key and value rows at once) and one join through shared memory.  Half a
+// warp holds a key row, 16 bytes a lane.  Longer lists go round again with the running maximum and sum.
+constexpr int kFewKeys = 16;     // keys a warp has in flight
+constexpr int kFewMaxWarps = 8;
+// Up to this many listed keys in all (B * H * Nq * K).  12/2 heads, K = 64: single tokens against 32768 keys,
+// batch 8 3.8 us here, 18.5 us on the tensor-core form; batch 128: 11.7, 19.1; neighbouring
+// queries of one sequence, 256 of them (196,608): 21.0, 20.6.  K = 16, 1024 queries (196,608): 20.9, 12.7.
+constexpr long long kFewEntries = 1 << 17;
+
+template <typename IdxT>
+__global__ void __launch_bounds__(kFewMaxWarps * 32)
+mod_attn_few_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ k,
+                    const __nv_bfloat16* __restrict__ v, const IdxT* __restrict__ idx, __nv_bfloat16* __restrict__ out,
+                    int H, int Hkv, int N, int Nq, int q0, int K, int causal, const ScoreMods mods) {
+    constexpr int D = 128;
+    __shared__ float2 s_ml[kFewMaxWarps];
+    __shared__ float s_acc[kFewMaxWarps][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const int half = lane >> 4, hl = lane & 15, slot = lane & 7;  // this lane ends with the score of key 8 half + slot
+    const size_t row = blockIdx.x;
+    const int bh = (int)(row / Nq), i = q0 + (int)(row - (size_t)bh * Nq);
+    const int b = bh / H, h = bh - b * H;
+    const size_t kv = (size_t)b * Hkv + h / (H / Hkv);
+    const uint4* kb = reinterpret_cast<const uint4*>(k + kv * N * D) + hl;
+    const uint4* vb = reinterpret_cast<const uint4*>(v + kv * N * D) + hl;
+    const uint4 qv = __ldg(reinterpret_cast<const uint4*>(q + row * D) + hl);
+    const RowMods<true> rm(mods, b, h, N, i);
+    float m_run = -INFINITY, l_run = 0.f, acc[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[t] = 0.f;
+    for (int k0 = warp * kFewKeys; k0 < K; k0 += warps * kFewKeys) {
+        const int e = k0 + 8 * half + slot;
+        const long long jl = e < K ? (long long)idx[row * K + e] : -1;
+        const int j = jl >= 0 && jl < N && rm.sees(jl, i, causal) ? (int)jl : -1;
+        uint4 kr[8], vr[8];
+        int js[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            js[t] = __shfl_sync(kFull, j, 16 * half + t);
+            const size_t at = (size_t)max(js[t], 0) * (D / 8);
+            kr[t] = __ldg(kb + at);
+            vr[t] = __ldg(vb + at);
+        }
+        float part[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) part[t] = dot8_bf16(qv, kr[t]);
+#pragma unroll
+        for (int w = 4; w >= 1; w >>= 1) {  // sums over the half-warp; lane l keeps key l & 7
+            const bool upper = (lane & w) != 0;
+#pragma unroll
+            for (int t = 0; t < w; ++t) {
+                const float send = upper ? part[t] : part[t + w], keep = upper ? part[t + w] : part[t];
+                part[t] = keep + __shfl_xor_sync(kFull, send, w);
+            }
+        }
+        const float dot = part[0] + __shfl_xor_sync(kFull, part[0], 8);
+        const float s2 = j >= 0 ? rm.score2(dot, i, j) : -INFINITY;
+        const float m_new = fmaxf(m_run, warp_max(s2));
+        if (m_new == -INFINITY) continue;  // warp-uniform: nothing seen so far
+        const float p = j >= 0 ? exp2f(s2 - m_new) : 0.f;
+        const float alpha = exp2f(m_run - m_new);
+        l_run = l_run * alpha + 0.5f * warp_sum(p);  // every key's p sits in two lanes
+        m_run = m_new;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) acc[t] *= alpha;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const float pt = __shfl_sync(kFull, p, 16 * half + t);
+            if (js[t] < 0) continue;  // uniform over the half-warp; key 0 in its place may hold anything
+            float x[8];
+            unpack_bf16x2(vr[t].x, x[0], x[1]);
+            unpack_bf16x2(vr[t].y, x[2], x[3]);
+            unpack_bf16x2(vr[t].z, x[4], x[5]);
+            unpack_bf16x2(vr[t].w, x[6], x[7]);
+#pragma unroll
+            for (int d = 0; d < 8; ++d) acc[d] = fmaf(pt, x[d], acc[d]);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 8; ++t) acc[t] += __shfl_xor_sync(kFull, acc[t], 16);
+    if (half == 0) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t) s_acc[warp][8 * hl + t] = acc[t];
+    }
+    if (lane == 0) s_ml[warp] = make_float2(m_run, l_run);
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < warps; ++w) top = fmaxf(top, s_ml[w].x);
+    float l = 0.f;
+    for (int w = 0; w < warps; ++w) l += s_ml[w].x == -INFINITY ? s_ml[w].y : s_ml[w].y * exp2f(s_ml[w].x - top);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int d = threadIdx.x; d < D; d += blockDim.x) {
+        float t = 0.f;
+        for (int w = 0; w < warps; ++w) t += s_ml[w].x == -INFINITY ? s_acc[w][d] : s_acc[w][d] * exp2f(s_ml[w].x - top);
+        out[row * D + d] = __float2bfloat16_rn(t * inv);
+    }
+    if (mods.lse2 && threadIdx.x == 0) mods.lse2[row] = top + log2f(l);
+}
+
+template <typename IdxT>
+cudaError_t launch_few(const GatherArgs& a, cudaStream_t stream) {
+    const int warps = std::max(1, std::min(kFewMaxWarps, (a.K + kFewKeys - 1) / kFewKeys));
+    mod_attn_few_kernel<IdxT><<<(unsigned)((long long)a.B * a.H * a.Nq), warps * 32, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(a.q), static_cast<const __nv_bfloat16*>(a.k),
+        static_cast<const __nv_bfloat16*>(a.v), static_cast<const IdxT*>(a.idx), static_cast<__nv_bfloat16*>(a.out), a.H,
+        a.Hkv, a.N, a.Nq, a.q0, a.K, a.causal, a.mods);
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) note_launch();
+    return e;
+}
+
 template <typename IdxT>
 cudaError_t launch_mma(const GatherArgs& a, cudaStream_t stream) {
     const int G = a.H / a.Hkv;
@@ -224,6 +338,8 @@ bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K) {
 }
 
 cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream) {
+    if (a.dtype == kBF16 && a.D == 128 && (long long)a.B * a.H * a.Nq * a.K <= kFewEntries)
+        return a.idx_is_64 ? launch_few<int64_t>(a, stream) : launch_few<int32_t>(a, stream);
     if (gather_mma_serves(a.dtype, a.H, a.Hkv, a.N, a.D, a.K))
         return a.idx_is_64 ? launch_mma<int64_t>(a, stream) : launch_mma<int32_t>(a, stream);
     if (a.dtype == kF32)
