@@ -27,13 +27,34 @@ __device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float c) {
     return fmaf(a1, b1, fmaf(a0, b0, c));
 }
 
+// Weights as MMA operands: their bf16 value and what that rounding left (2^-17 of the weight stays), each
+// 8 x 8 half of a (rows x columns) tile transposed across the warp.
+struct Weights {
+    uint32_t hi[2], lo[2];
+    __device__ __forceinline__ explicit Weights(const float (&w)[2][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t top = pack_bf16x2(w[h][0], w[h][1]);
+            float t0, t1;
+            unpack_bf16x2(top, t0, t1);
+            hi[h] = movmatrix_trans(top);
+            lo[h] = movmatrix_trans(pack_bf16x2(w[h][0] - t0, w[h][1] - t1));
+        }
+    }
+    // acc += A W
+    __device__ __forceinline__ void mma(float (&acc)[4], const uint32_t (&a)[4]) const {
+        mma_bf16_16816_a4(acc, a[0], a[1], a[2], a[3], hi[0], hi[1]);
+        mma_bf16_16816_a4(acc, a[0], a[1], a[2], a[3], lo[0], lo[1]);
+    }
+};
+
 // ------------------------------------------------------------------ row pass
 //
 // One warp per query and kv head, all heads of the group, over the union of their keys
 // (query_union.cuh).  In chunks of 16 keys: S^T = K Q^T and dP^T = V dO^T (keys as MMA rows, heads as
 // columns), p, dS and the weights dX per (key, head), then dq^T += K^T dX^T from the same staged key
-// rows.  dX is rounded to bf16 for that product; p, dP, the sums and Delta stay fp32.  The rows of
-// chunk c + 1 are in flight while chunk c is computed.
+// rows.  dX enters that product as a bf16 value and its rest (Weights); p, dP, the sums and Delta stay
+// fp32.  The rows of chunk c + 1 are in flight while chunk c is computed.
 constexpr int kRowWarps = 6;
 constexpr int kRowWarpBytes = 4 * kStageChunk + kUnionCap * 4;  // key and value rows of two chunks; the list
 constexpr int kRowBytes = kRowWarps * kRowWarpBytes;
@@ -168,15 +189,14 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     }
                 }
             }
-            const uint32_t b0 = movmatrix_trans(pack_bf16x2(w[0][0], w[0][1]));
-            const uint32_t b1 = movmatrix_trans(pack_bf16x2(w[1][0], w[1][1]));
+            const Weights wt(w);
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
                 uint32_t a[4];
                 ldmatrix_x4_trans<0>(a, kst + sl.at[mt]);
-                mma_bf16_16816_a4(acc[mt], a[0], a[1], a[2], a[3], b0, b1);
+                wt.mma(acc[mt], a);
                 ldmatrix_x4_trans<128>(a, kst + sl.at[mt]);
-                mma_bf16_16816_a4(acc[mt + 4], a[0], a[1], a[2], a[3], b0, b1);
+                wt.mma(acc[mt + 4], a);
             }
         }
     }
@@ -212,8 +232,8 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 // in groups of 16 entries whose q and dO rows are staged while the group before is computed.  For
 // the part of a group that lies in one block's run: S = Q K^T and dP = dO V^T (entries as MMA rows,
 // the block's keys as columns), p and dX per (entry, key) where the mask has the key's bit, then
-// dv^T += dO^T P and dk^T += Q^T dX from the same rows.  p and dX are rounded to bf16 for those
-// products, the sums are fp32.
+// dv^T += dO^T P and dk^T += Q^T dX from the same rows, P and dX as bf16 values and their rests (Weights),
+// the sums fp32.
 constexpr int kKeyWarps = 4;
 constexpr int kKeyWarpBytes = 4 * kStageChunk;  // q and dO rows of two groups
 constexpr int kKeyBytes = kKeyWarps * kKeyWarpBytes;
@@ -345,21 +365,18 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     w[h][x] = on ? dx * p[h][x] * (pacc[2 * h + x] - d) : 0.f;
                 }
             }
-            const uint32_t pb0 = movmatrix_trans(pack_bf16x2(p[0][0], p[0][1]));
-            const uint32_t pb1 = movmatrix_trans(pack_bf16x2(p[1][0], p[1][1]));
-            const uint32_t wb0 = movmatrix_trans(pack_bf16x2(w[0][0], w[0][1]));
-            const uint32_t wb1 = movmatrix_trans(pack_bf16x2(w[1][0], w[1][1]));
+            const Weights pt(p), wt(w);
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
                 uint32_t a[4];
                 ldmatrix_x4_trans<kStageChunk>(a, qst + sl.at[mt]);
-                mma_bf16_16816_a4(av[mt], a[0], a[1], a[2], a[3], pb0, pb1);
+                pt.mma(av[mt], a);
                 ldmatrix_x4_trans<0>(a, qst + sl.at[mt]);
-                mma_bf16_16816_a4(ak[mt], a[0], a[1], a[2], a[3], wb0, wb1);
+                wt.mma(ak[mt], a);
                 ldmatrix_x4_trans<kStageChunk + 128>(a, qst + sl.at[mt]);
-                mma_bf16_16816_a4(av[mt + 4], a[0], a[1], a[2], a[3], pb0, pb1);
+                pt.mma(av[mt + 4], a);
                 ldmatrix_x4_trans<128>(a, qst + sl.at[mt]);
-                mma_bf16_16816_a4(ak[mt + 4], a[0], a[1], a[2], a[3], wb0, wb1);
+                wt.mma(ak[mt + 4], a);
             }
             p0 = p1;
             if (p1 < run1 && p1 < t1) continue;  // the run goes on in the next group
