@@ -26,6 +26,7 @@ struct TanhFast {
 };
 
 constexpr int kModWarps = 8;
+constexpr float kSlack = 8.f;  // p stays below 2^8 (its bf16 rounding is relative) and above what 2^-126 cuts off
 constexpr int kModWarpBytes = 3 * kStageChunk + kUnionCap * 4;  // key rows of two chunks, value rows of one; the list
 constexpr int kModBytes = kModWarps * kModWarpBytes;
 static_assert(kUnionArea <= 3 * kStageChunk, "the list is built in the staging area");
@@ -67,12 +68,19 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     };
     int passes = 1, U;
     {
+        // all heads' entries, then what hides them, in steps without branches between the loads: a wait for
+        // each entry's segment in turn took a third of the kernel's time
         int x[G][4];
 #pragma unroll
         for (int t = 0; t < G; ++t) {
+            const IdxT* irow = idx + (row0 + (size_t)t * Nq) * K + lane;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[t][e] = lane + 32 * e < K ? key_of(t, lane + 32 * e) : -1;
+            for (int e = 0; e < 4; ++e) {
+                const IdxT j = lane + 32 * e < K ? irow[32 * e] : (IdxT)-1;
+                x[t][e] = j >= 0 && j < (IdxT)N ? (int)j : -1;
+            }
         }
+        rm.hide(x, K, i, causal);
         U = build_union<G, kDirect>(x, K, N, stage, list, lane);
         if (U < 0) passes = G;
     }
@@ -136,30 +144,34 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     sc[h][e] = (entry >> (24 + 2 * c4 + e)) & 1u
                                    ? mods.score2(sacc[2 * h + e], slope[e], far, TanhFast()) : -INFINITY;
             }
-            float alpha[2], pr[2][2];
+            // p is taken against m_run, which need not be the maximum: it moves (to the maximum, with what is
+            // summed so far rescaled) only where a score exceeds it by more than 2^kSlack allows.  l_run is this
+            // lane's share of the sum; the lanes add up at the end.
+            float pr[2][2];
+            const float t0 = fmaxf(sc[0][0], sc[1][0]), t1 = fmaxf(sc[0][1], sc[1][1]);
+            if (__any_sync(kFull, t0 > m_run[0] + kSlack || t1 > m_run[1] + kSlack)) {
+                float top[2] = {t0, t1};
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float m = fmaxf(sc[0][e], sc[1][e]);
-                m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
-                m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
-                m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
-                const float mx = fmaxf(m_run[e], m);
-                alpha[e] = mx == -INFINITY ? 1.f : exp2_fast(m_run[e] - mx);
-                pr[0][e] = mx == -INFINITY ? 0.f : exp2_fast(sc[0][e] - mx);
-                pr[1][e] = mx == -INFINITY ? 0.f : exp2_fast(sc[1][e] - mx);
-                float sum = pr[0][e] + pr[1][e];
-                sum += __shfl_xor_sync(kFull, sum, 4);
-                sum += __shfl_xor_sync(kFull, sum, 8);
-                sum += __shfl_xor_sync(kFull, sum, 16);
-                l_run[e] = l_run[e] * alpha[e] + sum;
-                m_run[e] = mx;
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int o = 4; o <= 16; o <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(kFull, top[e], o));
+                    const float mx = fmaxf(m_run[e], top[e]);
+                    const float alpha = mx == -INFINITY ? 1.f : exp2_fast(m_run[e] - mx);
+                    l_run[e] *= alpha;
+                    m_run[e] = mx;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        oacc[n][e] *= alpha;
+                        oacc[n][2 + e] *= alpha;
+                    }
+                }
             }
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                oacc[n][0] *= alpha[0];
-                oacc[n][1] *= alpha[1];
-                oacc[n][2] *= alpha[0];
-                oacc[n][3] *= alpha[1];
+            for (int e = 0; e < 2; ++e) {
+                const float ref = m_run[e] == -INFINITY ? 0.f : m_run[e];  // nothing seen yet: every score is -inf
+                pr[0][e] = exp2_fast(sc[0][e] - ref);
+                pr[1][e] = exp2_fast(sc[1][e] - ref);
+                l_run[e] += pr[0][e] + pr[1][e];
             }
             const uint32_t pb0 = movmatrix_trans(pack_bf16x2(pr[0][0], pr[0][1]));
             const uint32_t pb1 = movmatrix_trans(pack_bf16x2(pr[1][0], pr[1][1]));
@@ -175,6 +187,11 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 mma_bf16_16816_a4(oacc[mt + 4], a[0], a[1], a[2], a[3], pb0, pb1);
             }
         }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o <= 16; o <<= 1) l_run[e] += __shfl_xor_sync(kFull, l_run[e], o);
     }
     // each head's row divided by its sum and transposed back: lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
     const float inv0 = l_run[0] == 0.f ? 0.f : 1.f / l_run[0], inv1 = l_run[1] == 0.f ? 0.f : 1.f / l_run[1];

@@ -11,78 +11,80 @@
 
 namespace ossa {
 
-constexpr int kUnionCap = 512;          // keys a list holds
-constexpr int kUnionDirectKeys = 4096;  // keys covered by the direct head-bit array (a byte per key)
-constexpr int kUnionSlots = 1024;       // hash slots otherwise; at least G * K, so every key finds one
-constexpr int kUnionArea = 8192;        // bytes of shared memory the build needs besides the list
-constexpr int kUnionMaxKeys = 1 << 24;  // the list's key field
+constexpr int kUnionCap = 512;           // keys a list holds
+constexpr int kUnionDirectKeys = 12288;  // keys covered by the direct form, a byte of head bits per key
+constexpr int kUnionSlots = 1024;        // hash slots otherwise; at least G * K, so every key finds one
+constexpr int kUnionArea = 12288;        // bytes of shared memory the build needs besides the list
+constexpr int kUnionMaxKeys = 1 << 24;   // the list's key field
+static_assert(kUnionDirectKeys <= kUnionArea && 5 * kUnionSlots <= kUnionArea, "the head bits fit");
 
 // Returns the list's length, or -1 when a head lists a key twice or the list would not fit: the
 // caller then takes the heads one by one (single_list).
+//
+// The heads set their bits one after another, so a plain read and write of a key's byte does: the lanes of
+// one head differ in their keys, or write the same.  A key that one head lists twice shows in its own bit, or
+// among the 32 entries taken together: these differ if they ascend without a gap, as the selectors leave
+// them, and are compared with one another otherwise.
 template <int G, bool kDirect>
 __device__ __forceinline__ int build_union(const int (&x)[G][4], int K, int N, uint8_t* area, uint32_t* list, int lane) {
     const unsigned lt = lanemask_lt();
-    uint32_t* bits = reinterpret_cast<uint32_t*>(area);  // direct: byte j, the heads of key j
-    int* skey = reinterpret_cast<int*>(area);            // hash: keys, then head bits
-    unsigned* smask = reinterpret_cast<unsigned*>(area) + kUnionSlots;
+    uint8_t* bits = area;                                  // direct: of key j; hash: of a slot
+    int* skey = reinterpret_cast<int*>(area + kUnionSlots);  // hash: the slot's key
     if constexpr (kDirect) {
         for (int w = lane; w < (N + 15) >> 4; w += 32) reinterpret_cast<uint4*>(bits)[w] = make_uint4(0u, 0u, 0u, 0u);
     } else {
 #pragma unroll
-        for (int u = 0; u < kUnionSlots / 128; ++u) {
-            reinterpret_cast<int4*>(skey)[lane + 32 * u] = make_int4(-1, -1, -1, -1);
-            reinterpret_cast<uint4*>(smask)[lane + 32 * u] = make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int u = 0; u < kUnionSlots / 512; ++u) reinterpret_cast<uint4*>(bits)[lane + 32 * u] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int u = 0; u < kUnionSlots / 128; ++u) reinterpret_cast<int4*>(skey)[lane + 32 * u] = make_int4(-1, -1, -1, -1);
     }
     __syncwarp();
+    int U = 0;
     bool twice = false;
-    int slot[G][4];
 #pragma unroll
     for (int t = 0; t < G; ++t) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            slot[t][e] = 0;
             if (32 * e >= K) continue;  // warp-uniform
             const int xv = x[t][e];
-            if (xv < 0) continue;
-            if constexpr (kDirect) {
-                const uint32_t sh = 8u * (uint32_t)(xv & 3) + (uint32_t)t;
-                const uint32_t old = atomicOr(&bits[xv >> 2], 1u << sh);
-                twice = twice || ((old >> sh) & 1u) != 0u;
-            } else {
-                int at = (int)(((uint32_t)xv * 2654435761u) >> 22);  // 10 bits
-                for (int probe = 0; probe < kUnionSlots; ++probe) {
-                    const int old = atomicCAS(&skey[at], -1, xv);
-                    if (old == -1 || old == xv) break;
-                    at = (at + 1) & (kUnionSlots - 1);
+            int at = xv;
+            if constexpr (!kDirect) {
+                if (xv >= 0) {
+                    at = (int)(((uint32_t)xv * 2654435761u) >> 22);  // 10 bits
+                    for (int probe = 0; probe < kUnionSlots; ++probe) {
+                        int cur = *reinterpret_cast<volatile int*>(skey + at);
+                        if (cur == -1) cur = atomicCAS(skey + at, -1, xv);
+                        if (cur == -1 || cur == xv) break;
+                        at = (at + 1) & (kUnionSlots - 1);
+                    }
                 }
-                const unsigned old = atomicOr(&smask[at], 1u << t);
-                twice = twice || ((old >> t) & 1u) != 0u;
-                slot[t][e] = at;
+                __syncwarp();
             }
+            const int before = __shfl_up_sync(kFull, xv, 1);
+            const unsigned valid = __ballot_sync(kFull, xv >= 0);
+            const unsigned after = __ballot_sync(kFull, xv >= 0 && lane > 0 && before >= 0 && before < xv);
+            if (__popc(valid & ~after) > 1) {  // warp-uniform
+                const unsigned same = __match_any_sync(kFull, xv >= 0 ? xv : -1 - lane);
+                twice = twice || same != 1u << lane;
+            }
+            const unsigned old = xv >= 0 ? bits[at] : 1u;
+            twice = twice || (xv >= 0 && ((old >> t) & 1u) != 0u);
+            __syncwarp();
+            if (xv >= 0) bits[at] = (uint8_t)(old | 1u << t);
+            const unsigned own = __ballot_sync(kFull, old == 0u);  // no head before lists it
+            const int pos = U + __popc(own & lt);
+            // the list holds the place of the head bits until they are complete
+            if (old == 0u && pos < kUnionCap) list[pos] = (uint32_t)at;
+            U += __popc(own);
+            __syncwarp();
         }
     }
-    if (__any_sync(kFull, twice)) return -1;
-    int U = 0;
-#pragma unroll
-    for (int t = 0; t < G; ++t) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (32 * e >= K) continue;
-            const int xv = x[t][e];
-            unsigned mk = 0u;
-            bool own = false;
-            if (xv >= 0) {
-                mk = kDirect ? (bits[xv >> 2] >> (8u * (uint32_t)(xv & 3))) & 0xffu : smask[slot[t][e]];
-                own = (mk & ((1u << t) - 1u)) == 0u;  // no lower head lists it
-            }
-            const unsigned bal = __ballot_sync(kFull, own);
-            const int pos = U + __popc(bal & lt);
-            if (own && pos < kUnionCap) list[pos] = (uint32_t)xv | mk << 24;
-            U += __popc(bal);
-        }
+    if (__any_sync(kFull, twice) || U > kUnionCap) return -1;
+    for (int u = lane; u < U; u += 32) {
+        const uint32_t at = list[u];
+        list[u] = (kDirect ? at : (uint32_t)skey[at]) | (uint32_t)bits[at] << 24;
     }
-    return U <= kUnionCap ? U : -1;
+    return U;
 }
 
 // One head's keys as a list of their own, in the order listed (key(e): entry e of the head, -1 masked).

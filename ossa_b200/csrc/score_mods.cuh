@@ -41,6 +41,26 @@ struct RowMods<true> {
     __device__ __forceinline__ bool sees(long long j, int i, int causal) const {
         return (!causal || j <= i || j < prefix) && (!seg || __ldg(seg + j) == seg_i);
     }
+    // x[t][e] = -1 for the keys in [0, N) that the row does not see; entries with 32 e >= K are -1.
+    template <int G>
+    __device__ __forceinline__ void hide(int (&x)[G][4], int K, int i, int causal) const {
+        const int last = causal ? max(i, prefix - 1) : 0x7fffffff;  // j <= i or j < prefix
+#pragma unroll
+        for (int t = 0; t < G; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[t][e] = x[t][e] > last ? -1 : x[t][e];
+        }
+        if (!seg) return;  // the same for the whole grid
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (32 * e >= K) continue;  // warp-uniform
+            int of[G];
+#pragma unroll
+            for (int t = 0; t < G; ++t) of[t] = __ldg(seg + max(x[t][e], 0));
+#pragma unroll
+            for (int t = 0; t < G; ++t) x[t][e] = of[t] == seg_i ? x[t][e] : -1;
+        }
+    }
     __device__ __forceinline__ float score2(float dot, int i, int j) const {
         return m.score2(dot, slope, fabsf((float)(i - j)), TanhExact());
     }
