@@ -177,16 +177,16 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 const float far = fabsf((float)(i - (int)(entry & 0xffffffu)));
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    w[h][e] = 0.f;
-                    if (((entry >> (24 + 2 * c4 + e)) & 1u) && lse2[e] != -INFINITY) {
-                        float dx;
-                        const float p = exp2_fast(mods.score2_grad(sacc[2 * h + e], slope[e], far, dx, TanhFast()) - lse2[e]);
-                        const float dp = pacc[2 * h + e], pd = p * dp;
-                        w[h][e] = dx * (pd - p * d0[e]);
-                        a_pd[e] += pd;
-                        a_f[e] = fmaf(p, far, a_f[e]);
-                        a_pdf[e] = fmaf(pd, far, a_pdf[e]);
-                    }
+                    // selects, no branch: what a masked place computes may not be finite and is dropped
+                    const bool on = ((entry >> (24 + 2 * c4 + e)) & 1u) && lse2[e] != -INFINITY;
+                    float dx;
+                    const float s2 = mods.score2_grad(sacc[2 * h + e], slope[e], far, dx, TanhFast());
+                    const float p = on ? exp2_fast(s2 - lse2[e]) : 0.f;
+                    const float pd = on ? p * pacc[2 * h + e] : 0.f;
+                    w[h][e] = on ? dx * (pd - p * d0[e]) : 0.f;
+                    a_pd[e] += pd;
+                    a_f[e] = fmaf(p, far, a_f[e]);
+                    a_pdf[e] = fmaf(pd, far, a_pdf[e]);
                 }
             }
             const Weights wt(w);
