@@ -16,7 +16,11 @@ modules, then:
 * o_proj and the ``(out, None)`` return as the reference;
 * (additive) RoPE and the head transpose of q/k/v run as one kernel pass per
   tensor (``rope_to_heads``), bit-identical to ``apply_rotary_pos_emb`` plus the
-  layout copies.
+  layout copies; a layer that norms its query and key heads (``q_norm``, ``k_norm``
+  RMS modules) has norm, RoPE and transpose of both in one pass (``qk_norm_rope``);
+* (additive) the layer trains: every step but the selection is differentiable
+  (gradients flow through the selected keys' attention, the selection is a
+  constant), and ``PatchPlan`` carries the score modifiers of ``topk_attention``.
 
 Deliberate difference: the reference casts router logits to the model dtype
 before ``torch.topk`` (:193), which ties ~15% of rows at the K-th boundary in
@@ -29,12 +33,12 @@ from __future__ import annotations
 
 from dataclasses import dataclass
 from pathlib import Path
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
 from .. import select
-from ..rope import rope_to_heads
+from ..rope import qk_norm_rope, rope_to_heads
 from ..router import ContentRouter, ContentRouterConfig
 from ..topk_attention import topk_attention
 
@@ -46,6 +50,31 @@ class PatchPlan:
     layers: tuple[int, ...] = ()       # which layers to patch; empty = none
     routers: dict[int, ContentRouter] | None = None  # layer_idx -> router
     impl: str = "mask"                 # "mask" (top-K + forced diagonal) | "gather"
+    # Score modifiers of every patched layer, as topk_attention takes them (additive).  They act on the
+    # attention, not on the selection: a row's K keys may lie in other documents, which hides them.
+    softcap: Optional[float] = None
+    slopes: Optional[torch.Tensor] = None                    # (H,)
+    segments: Optional[torch.Tensor] = None                  # (B, N) or (N,)
+    prefix_len: Union[torch.Tensor, int, None] = None        # (B,) or one int
+
+
+def _head_norms(layer_module):
+    """(q weight, k weight, eps) of the layer's query and key head norms, None if it has none."""
+    norms = [getattr(layer_module, name, None) for name in ("q_norm", "k_norm")]
+    if norms == [None, None]:
+        return None
+    eps = []
+    for norm in norms:
+        weight = getattr(norm, "weight", None)
+        e = getattr(norm, "variance_epsilon", getattr(norm, "eps", None))
+        if weight is None or weight.shape != (layer_module.head_dim,) or e is None or \
+                getattr(norm, "bias", None) is not None or isinstance(norm, torch.nn.LayerNorm):
+            raise TypeError("q_norm and k_norm must both be RMS norms over head_dim (weight and eps, no bias); "
+                            f"got {type(norm).__name__}")
+        eps.append(float(e))
+    if eps[0] != eps[1]:
+        raise TypeError(f"q_norm and k_norm must have one eps, got {eps[0]} and {eps[1]}")
+    return norms[0].weight, norms[1].weight, eps[0]
 
 
 def _router_params(router):
@@ -90,8 +119,9 @@ def _patch_layer(model, plan: PatchPlan):
     for layer_idx in plan.layers:
         layer_module = model.model.layers[layer_idx].self_attn
         original_forward = layer_module.forward
+        head_norms = _head_norms(layer_module)
 
-        def make_forward(layer_module=layer_module, captured_idx=layer_idx):
+        def make_forward(layer_module=layer_module, captured_idx=layer_idx, normed=head_norms is not None):
             def new_forward(hidden_states, attention_mask=None, position_ids=None,
                             past_key_values=None, output_attentions=False,
                             use_cache=False, cache_position=None,
@@ -104,13 +134,19 @@ def _patch_layer(model, plan: PatchPlan):
                 # projections, then RoPE and the (B, heads, N, D) layout in one kernel
                 # pass per tensor (bit-identical to apply_rotary_pos_emb + contiguous)
                 cos, sin = position_embeddings if position_embeddings is not None else (None, None)
-                q = rope_to_heads(layer_module.q_proj(hidden_states), n_heads, cos, sin)
-                k = rope_to_heads(layer_module.k_proj(hidden_states), n_kv_heads, cos, sin)
+                q, k = layer_module.q_proj(hidden_states), layer_module.k_proj(hidden_states)
+                if normed:
+                    wq, wk, eps = _head_norms(layer_module)
+                    q, k = qk_norm_rope(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps=eps)
+                else:
+                    q = rope_to_heads(q, n_heads, cos, sin)
+                    k = rope_to_heads(k, n_kv_heads, cos, sin)
                 v = rope_to_heads(layer_module.v_proj(hidden_states), n_kv_heads)
 
                 with torch.no_grad():
                     idx = select_indices(plan, captured_idx, q, k)
-                out = topk_attention(q, k, v, topk_indices=idx, causal=True)
+                out = topk_attention(q, k, v, topk_indices=idx, causal=True, softcap=plan.softcap,
+                                     slopes=plan.slopes, segments=plan.segments, prefix_len=plan.prefix_len)
 
                 out = out.transpose(1, 2).reshape(B, N, n_heads * head_dim)
                 out = layer_module.o_proj(out)
