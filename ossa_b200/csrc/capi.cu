@@ -311,8 +311,10 @@ int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, con
     if ((long long)B * H * Nq == 0) return OSSA_OK;
     if (Nk == 0) return fail(OSSA_ERR_INVALID, "query rows need at least one key (Nk=0)");
     if (!q || !k || !v || !out || (K > 0 && !indices)) return fail(OSSA_ERR_INVALID, "null pointer argument");
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || (K > 0 && !aligned16(indices)))
-        return fail(OSSA_ERR_INVALID, "q, k, v, indices and out must be 16-byte aligned");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out))
+        return fail(OSSA_ERR_INVALID, "q, k, v and out must be 16-byte aligned");
+    if (K > 0 && reinterpret_cast<uintptr_t>(indices) % (idx_is_64 ? 8 : 4))
+        return fail(OSSA_ERR_INVALID, "indices are not aligned to their type");
     ossa::GatherArgs a{q, k, v, indices, out, idx_is_64, dtype, B, H, Hkv, Nk, D, K, scale, causal ? 1 : 0};
     a.Nq = Nq;
     a.q0 = q_start;
@@ -353,9 +355,11 @@ int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const v
     }
     if (Nk == 0) return fail(OSSA_ERR_INVALID, "query rows need at least one key (Nk=0)");
     if (!q || !k || !v || !out || !indices || !lse2 || !dout) return fail(OSSA_ERR_INVALID, "null pointer argument");
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(indices) || !aligned16(dout) ||
-        !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
-        return fail(OSSA_ERR_INVALID, "q, k, v, indices, out, dout, dq, dk and dv must be 16-byte aligned");
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) || !aligned16(dq) ||
+        !aligned16(dk) || !aligned16(dv))
+        return fail(OSSA_ERR_INVALID, "q, k, v, out, dout, dq, dk and dv must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(indices) % (idx_is_64 ? 8 : 4))
+        return fail(OSSA_ERR_INVALID, "indices are not aligned to their type");
     const size_t need = ossa::gather_bwd_workspace_bytes(dtype, B, H, Hkv, Nq, Nk, D, K, dslopes != nullptr);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,

@@ -44,7 +44,7 @@ struct RowMods<true> {
     // x[t][e] = -1 for the keys in [0, N) that the row does not see; entries with 32 e >= K are -1.
     template <int G>
     __device__ __forceinline__ void hide(int (&x)[G][4], int K, int i, int causal) const {
-        const int last = causal ? max(i, prefix - 1) : 0x7fffffff;  // j <= i or j < prefix
+        const int last = causal ? max(i, max(prefix, 0) - 1) : 0x7fffffff;  // j <= i or j < prefix
 #pragma unroll
         for (int t = 0; t < G; ++t) {
 #pragma unroll

@@ -166,30 +166,33 @@ def _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk):
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, n_heads, n_kv_heads, cos, sin, eps):
-        args, kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
-        ctx.save_for_backward(*kept)
-        ctx.call = (args, q.shape, k.shape)
+        ctx.save_for_backward(q, k, wq, wk, cos, sin)
+        ctx.rule = (n_heads, n_kv_heads, eps)
         ctx.set_materialize_grads(False)
+        args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
         return _norm_rope_forward(args, q.dtype, q.device)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
-        _, _, wq, wk, _, _ = ctx.saved_tensors  # the pointers in ctx.call lead into these
-        args, q_shape, k_shape = ctx.call
         if gq is None and gk is None:
             return (None,) * 9
+        # saved tensors may come back as others than were saved (checkpointing, offloading): their
+        # places and strides are taken anew
+        q, k, wq, wk, cos, sin = ctx.saved_tensors
+        n_heads, n_kv_heads, eps = ctx.rule
+        args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
         g = gq if gq is not None else gk
         dt, dev = g.dtype, g.device
         need = ctx.needs_input_grad
         dq = dk = dwq = dwk = None
         if gq is not None:
             gq = gq.contiguous()
-            dq = torch.empty(q_shape, dtype=dt, device=dev)
+            dq = torch.empty(q.shape, dtype=dt, device=dev)
             dwq = torch.empty_like(wq) if need[2] else None
         if gk is not None:
             gk = gk.contiguous()
-            dk = torch.empty(k_shape, dtype=dt, device=dev)
+            dk = torch.empty(k.shape, dtype=dt, device=dev)
             dwk = torch.empty_like(wk) if need[3] else None
         if gk is None:  # one output has no gradient: the other tensor alone, in the place of the queries
             args = args[:1] + (None, args[2], None) + args[4:12] + (0,) + args[13:]

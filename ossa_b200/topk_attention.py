@@ -207,14 +207,15 @@ class _TopkAttention(torch.autograd.Function):
         args = _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
         out = _mod_forward(args, q, lse2)
         ctx.save_for_backward(q, k, v, slopes, idx, segments, prefix_len, out, lse2)
-        ctx.call = args
+        ctx.rule = (causal, q0, cap)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, slopes, _, _, _, out, lse2 = ctx.saved_tensors  # the pointers in ctx.call lead into these
-        args, dev = ctx.call, q.device
+        # saved tensors may come back as others than were saved (checkpointing, offloading)
+        q, k, v, slopes, idx, segments, prefix_len, out, lse2 = ctx.saved_tensors
+        args, dev = _mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), q.device
         dout = dout.contiguous()
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None

@@ -29,7 +29,7 @@ def _mod_bwd(**kw):
 BAD_MOD = [(dict(H=5), INV), (dict(D=96), UNS), (dict(dtype=3), INV), (dict(K=-1), INV), (dict(i64=2), INV),
            (dict(scale=NAN), INV), (dict(cap=-1.0), INV), (dict(cap=INF), INV), (dict(cap=NAN), INV),
            (dict(q0=-1), INV), (dict(seg=16, q0=1), INV), (dict(B=40000, H=2, Hkv=2), UNS), (dict(q=None), INV),
-           (dict(k=8), INV), (dict(idx=None), INV), (dict(Nk=0), INV)]
+           (dict(k=8), INV), (dict(idx=18), INV), (dict(idx=None), INV), (dict(Nk=0), INV)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_MOD)

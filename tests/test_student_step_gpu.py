@@ -177,3 +177,80 @@ def test_prefill_then_single_tokens():
         kc[:, :, t:t + 1], vc[:, :, t:t + 1] = k1, v[:, :, t:t + 1]
         out.append(topk_attention(q1, kc, vc, topk_indices=idx[:, :, t:t + 1].contiguous(), q_start=t, **opts))
     assert rel(torch.cat(out, dim=2), full) < 4 * 2.0 ** -8
+
+
+def _step_of_all(q, k, v, w, table, idx, segments, teacher, teacher_ids, out_w):
+    """The operators one after another, from projections to a loss."""
+    from ossa_b200 import qk_norm_rope, rope_to_heads, topk_attention
+
+    qr, kr = qk_norm_rope(q, k, 4, 2, w, w, table[0], table[1])
+    vr = rope_to_heads(v, 2)
+    out = topk_attention(qr, kr, vr, topk_indices=idx, softcap=5.0, segments=segments)
+    return top_logit_distillation_loss(out.transpose(1, 2).flatten(2) @ out_w, teacher, teacher_ids)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_checkpointed_offloaded_and_two_at_once(dtype):
+    """Saved tensors that come back as other tensors (non-reentrant checkpointing, offloading to the
+    host), joint projections whose slices are read in place, two steps on two streams at once: the same
+    bits as the plain step."""
+    from torch.utils.checkpoint import checkpoint
+
+    B, N, D = 2, 90, 128
+    g = torch.Generator().manual_seed(11)
+
+    def make(seed):
+        g.manual_seed(seed)
+        joint = torch.randn(B, N, 8 * D, generator=g).to(dtype).to(DEV).requires_grad_()
+        w = torch.randn(D, generator=g).to(dtype).to(DEV).requires_grad_()
+        table = torch.randn(2, 1, N, D, generator=g).to(dtype).to(DEV)
+        idx = torch.randint(-1, N, (B, 4, N, 20), generator=g).int().to(DEV)
+        seg = torch.sort(torch.randint(0, 2, (B, N), generator=g), dim=1).values.to(DEV)
+        teacher = torch.randn(B, N, 12, generator=g).to(DEV)
+        ids = torch.randint(0, 77, (B, N, 12), generator=g).to(DEV)
+        out_w = torch.randn(4 * D, 77, generator=g).to(dtype).to(DEV).requires_grad_()
+        return joint, w, out_w, (table, idx, seg, teacher, ids)
+
+    def loss_of(joint, w, out_w, rest):
+        table, idx, seg, teacher, ids = rest
+        return _step_of_all(joint[..., :4 * D], joint[..., 4 * D:6 * D], joint[..., 6 * D:], w, table, idx, seg, teacher, ids,
+                            out_w)
+
+    def grads(run, args):
+        loss = run(args)
+        return [loss.detach()] + list(torch.autograd.grad(loss, args[:3]))
+
+    args, other = make(1), make(2)
+    want = grads(lambda a: loss_of(*a), args)
+    want_other = grads(lambda a: loss_of(*a), other)
+    got = grads(lambda a: checkpoint(loss_of, *a, use_reentrant=False), args)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+    def offloaded(a):
+        with torch.autograd.graph.save_on_cpu():
+            return loss_of(*a)
+
+    assert all(torch.equal(a, b) for a, b in zip(want, grads(offloaded, args)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    both = []
+    for s, a in zip(streams, (args, other)):
+        with torch.cuda.stream(s):
+            both.append(grads(lambda x: loss_of(*x), a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, both[0]))
+    assert all(torch.equal(a, b) for a, b in zip(want_other, both[1]))
+
+
+def test_an_unaligned_index_slice():
+    """Index rows that begin off any 16-byte boundary (K = 5, a slice of the batch)."""
+    from ossa_b200 import topk_attention
+
+    g = torch.Generator().manual_seed(1)
+    q = torch.randn(3, 2, 7, 64, generator=g).to(DEV)
+    idx = torch.randint(0, 7, (3, 2, 7, 5), generator=g).int().to(DEV)
+    whole = topk_attention(q, q, q, topk_indices=idx, softcap=3.0)
+    x = q[1:].clone().requires_grad_()
+    part = topk_attention(x, x, x, topk_indices=idx[1:], softcap=3.0)
+    assert torch.equal(part.detach(), whole[1:])
+    assert torch.isfinite(torch.autograd.grad(part.sum(), x)[0]).all()
