@@ -80,7 +80,7 @@ class _RopeToHeads(torch.autograd.Function):
         cos, sin = ctx.saved_tensors
         g = g.contiguous()
         B, H, N, D = g.shape
-        dx = torch.empty(ctx.shape, dtype=g.dtype, device=g.device)
+        dx = g.new_empty(ctx.shape)
         args = (None, None, None, None, _lib.ptr(cos), _lib.ptr(sin),
                 1 if cos is not None and B > 1 and cos.shape[0] == B else 0, _lib.dtype_code(g), _lib.OSSA_F32, B, N, H, 0,
                 D, 0, 0, 0, 0, 0.0)
@@ -136,10 +136,11 @@ def _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps):
     return args, (q, k, wq, wk, cos, sin)
 
 
-def _norm_rope_forward(args, dtype, dev):
+def _norm_rope_forward(args, like):
+    dev = like.device
     B, N, Hq, Hk, D = args[9:14]
-    q_out = torch.empty((B, Hq, N, D), dtype=dtype, device=dev)
-    k_out = torch.empty((B, Hk, N, D), dtype=dtype, device=dev)
+    q_out = like.new_empty((B, Hq, N, D))
+    k_out = like.new_empty((B, Hk, N, D))
     if B * N > 0:
         with _lib.on_device(dev):
             st = _lib.lib().ossa_qk_norm_rope_fwd(*args, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_ptr(dev))
@@ -156,7 +157,7 @@ def _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk):
         ws, ws_bytes = None, 0
         if args[2] is not None or args[3] is not None:
             ws_bytes = L.ossa_qk_norm_rope_bwd_workspace_size(args[13])
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws = gq.new_empty(ws_bytes, dtype=torch.uint8)
         st = L.ossa_qk_norm_rope_bwd(*args, gq.data_ptr(), _lib.ptr(gk), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dwq),
                                      _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
     if st:
@@ -170,7 +171,7 @@ class _QkNormRope(torch.autograd.Function):
         ctx.rule = (n_heads, n_kv_heads, eps)
         ctx.set_materialize_grads(False)
         args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
-        return _norm_rope_forward(args, q.dtype, q.device)
+        return _norm_rope_forward(args, q)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -182,17 +183,15 @@ class _QkNormRope(torch.autograd.Function):
         q, k, wq, wk, cos, sin = ctx.saved_tensors
         n_heads, n_kv_heads, eps = ctx.rule
         args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
-        g = gq if gq is not None else gk
-        dt, dev = g.dtype, g.device
         need = ctx.needs_input_grad
         dq = dk = dwq = dwk = None
         if gq is not None:
             gq = gq.contiguous()
-            dq = torch.empty(q.shape, dtype=dt, device=dev)
+            dq = gq.new_empty(q.shape)
             dwq = torch.empty_like(wq) if need[2] else None
         if gk is not None:
             gk = gk.contiguous()
-            dk = torch.empty(k.shape, dtype=dt, device=dev)
+            dk = gk.new_empty(k.shape)
             dwk = torch.empty_like(wk) if need[3] else None
         if gk is None:  # one output has no gradient: the other tensor alone, in the place of the queries
             args = args[:1] + (None, args[2], None) + args[4:12] + (0,) + args[13:]
@@ -252,4 +251,4 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
         return _QkNormRope.apply(q, k, q_weight, k_weight, n_heads, n_kv_heads, cos, sin, eps)
     args, _kept = _call_args(q, k, n_heads, n_kv_heads, q_weight, k_weight, cos, sin, eps)
-    return _norm_rope_forward(args, q.dtype, q.device)
+    return _norm_rope_forward(args, q)

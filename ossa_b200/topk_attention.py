@@ -203,7 +203,7 @@ class _TopkAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
         q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
-        lse2 = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+        lse2 = q.new_empty(q.shape[:3], dtype=torch.float32)
         args = _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
         out = _mod_forward(args, q, lse2)
         ctx.save_for_backward(q, k, v, slopes, idx, segments, prefix_len, out, lse2)
@@ -222,7 +222,7 @@ class _TopkAttention(torch.autograd.Function):
         L = _lib.lib()
         with _lib.on_device(dev):
             ws_bytes = L.ossa_topk_attention_bwd_workspace_size(*args[5:13], 0 if dslopes is None else 1)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws = q.new_empty(ws_bytes, dtype=torch.uint8)
             st = L.ossa_topk_attention_bwd(
                 *args, out.data_ptr(), lse2.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                 _lib.ptr(dslopes), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))

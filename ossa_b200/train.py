@@ -114,12 +114,12 @@ class _TopLogitDistill(torch.autograd.Function):
         dev = z.device
         L = _lib.lib()
         ws_bytes = L.ossa_top_logit_distill_workspace_size(rows, K)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws = z.new_empty(ws_bytes, dtype=torch.uint8)
         mean = 1 if reduction == "mean" else 0
         each = reduction == "none"
-        loss = torch.empty(rows if each else (), dtype=torch.float32, device=dev)
+        loss = z.new_empty(rows if each else (), dtype=torch.float32)
         # a single incoming gradient is 1 as a rule: the gradient is taken with the loss
-        dz = torch.empty((rows, V), dtype=z.dtype, device=dev) if grad and not each else None
+        dz = z.new_empty((rows, V)) if grad and not each else None
         where = (z.data_ptr(), _lib.dtype_code(z), outer, inner, V, so, si)
         with _lib.on_device(dev):
             st = L.ossa_top_logit_distill_fwd(
@@ -144,8 +144,8 @@ class _TopLogitDistill(torch.autograd.Function):
         ctx.kept = (ws, ws_bytes, None)  # a second backward pass makes its own
         taken = dz is not None
         if not taken:
-            dz = torch.empty((where[1] * where[2], z.shape[-1]), dtype=z.dtype, device=z.device)
-        g = g.float().contiguous()
+            dz = z.new_empty((where[1] * where[2], z.shape[-1]))
+        g = g.contiguous()  # fp32, as the loss
         with _lib.on_device(z.device):
             st = _lib.lib().ossa_top_logit_distill_bwd(
                 z.data_ptr(), *where, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau, mean, g.data_ptr(),
