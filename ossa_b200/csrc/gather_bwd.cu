@@ -20,7 +20,9 @@
 // No float atomics: repeated calls give the same bits.  (Two entries of one row with the same
 // key are alike, so the order in which the counting sort places them does not show.)
 //
-// Bound: L2-to-SM traffic.  Either pass reads two rows of D values per entry.
+// Bound: L2-to-SM traffic.  Either pass reads two rows of D values per entry (the row pass's tensor-core form
+// per key of the heads' union, the key pass's per row and key block), which no tile keeps: the rows that list
+// a key are scattered.
 #include <algorithm>
 #include <cstdint>
 
@@ -56,15 +58,19 @@ BwdShape make_shape(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int 
     s.shift = mma ? kKeyBlockShift : 0;
     s.NB = (N + (1 << s.shift) - 1) >> s.shift;
     const long long kv = (long long)B * Hkv;
-    // one warp per unit in the sort's last step: enough units for 24 warps per SM, rows permitting
+    // One warp per unit in the sort's last step: enough units for 24 warps per SM, rows permitting.  Fewer
+    // leave it waiting, more cost in the scan over units (count + place + scan, us, at 16, 32, 64, 128, 256
+    // chunks: B=2, 12/2 heads, N=4096, K=64: 92, 68, 56, 59, 82; B=1, N=8192, K=128: 305, 174, 133, 126, 137).
     const long long want = 24ll * device_sm_count() / std::max(kv * s.G, 1ll);
     s.chunks = (int)std::max(1ll, std::min({want, (long long)kMaxChunks, (long long)Nq / kMinChunkRows}));
     s.chunk_rows = (Nq + s.chunks - 1) / s.chunks;
     s.units = s.chunks * s.G;
     s.cap = (long long)s.G * Nq * K;
-    // tiles: long ones store fewer cut runs, short ones fill the device (24 warps per SM)
-    const long long fair = kv * s.cap / (24ll * device_sm_count());
-    s.tile = (int)std::min(std::max((fair + 15) / 16 * 16, 64ll), mma ? 512ll : 256ll);
+    // Tiles: long ones store fewer cut runs, short ones fill the device (key pass + join, us, at tiles of 128,
+    // 256, 512, 1024: the two shapes above 241, 198, 186, 219 and 617, 488, 432, 404; fp32 B=2, 6/3 heads, N=517,
+    // K=33, at 64, 128, 256, 512: 59, 58, 84, 151).  84 tiles per SM fit all three.
+    const long long fair = kv * s.cap / (84ll * device_sm_count());
+    s.tile = (int)std::min(std::max((fair + 15) / 16 * 16, 64ll), mma ? 1024ll : 256ll);
     s.tiles = (s.cap + s.tile - 1) / s.tile;
     return s;
 }
