@@ -9,8 +9,8 @@
 // that some head lists is fetched once.  In chunks of 16 keys: S^T = K Q^T with the keys as MMA
 // rows and the heads as columns, scores and masks per (key, head), online softmax per head, then
 // O^T += V^T P^T with P^T moved into operand layout by movmatrix.  The key rows of chunk c + 1 are in
-// flight while chunk c is scored, its value rows while its softmax runs.  p is rounded to bf16 for
-// the product with the bf16 values, as in the other bf16 forms; sums and statistics are fp32.
+// flight while chunk c is scored, its value rows while its softmax runs.  p enters the product with the
+// bf16 values as a bf16 value and its rest (Weights); sums and statistics are fp32.
 // A query with a key listed twice by one head, or with more than 512 different keys, takes its heads
 // one after another through the same loop.
 //
@@ -30,7 +30,7 @@ struct TanhFast {
 };
 
 constexpr int kModWarps = 8;
-constexpr float kSlack = 8.f;  // p stays below 2^8 (its bf16 rounding is relative) and above what 2^-126 cuts off
+constexpr float kSlack = 8.f;  // p stays below 2^8 (its rounding is relative) and above what 2^-126 cuts off
 constexpr int kModWarpBytes = 3 * kStageChunk + kUnionCap * 4;  // key rows of two chunks, value rows of one; the list
 constexpr int kModBytes = kModWarps * kModWarpBytes;
 static_assert(kUnionArea <= 3 * kStageChunk, "the list is built in the staging area");
@@ -177,8 +177,7 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 pr[1][e] = exp2_fast(sc[1][e] - ref);
                 l_run[e] += pr[0][e] + pr[1][e];
             }
-            const uint32_t pb0 = movmatrix_trans(pack_bf16x2(pr[0][0], pr[0][1]));
-            const uint32_t pb1 = movmatrix_trans(pack_bf16x2(pr[1][0], pr[1][1]));
+            const Weights pw(pr);
             if (more) cp_async_wait_pending<1>();
             else cp_async_wait_pending<0>();
             __syncwarp();
@@ -186,9 +185,9 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             for (int mt = 0; mt < 4; ++mt) {  // values transposed as the A operand
                 uint32_t a[4];
                 ldmatrix_x4_trans<0>(a, vst + sl.at[mt]);
-                mma_bf16_16816_a4(oacc[mt], a[0], a[1], a[2], a[3], pb0, pb1);
+                pw.mma(oacc[mt], a);
                 ldmatrix_x4_trans<128>(a, vst + sl.at[mt]);
-                mma_bf16_16816_a4(oacc[mt + 4], a[0], a[1], a[2], a[3], pb0, pb1);
+                pw.mma(oacc[mt + 4], a);
             }
         }
     }

@@ -64,4 +64,25 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                  : "r"(addr), "n"(kOff));
 }
 
+// Weights as MMA operands: their bf16 value and what that rounding left (2^-17 of the weight stays), each
+// 8 x 8 half of a (rows x columns) tile transposed across the warp.
+struct Weights {
+    uint32_t hi[2], lo[2];
+    __device__ __forceinline__ explicit Weights(const float (&w)[2][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t top = pack_bf16x2(w[h][0], w[h][1]);
+            float t0, t1;
+            unpack_bf16x2(top, t0, t1);
+            hi[h] = movmatrix_trans(top);
+            lo[h] = movmatrix_trans(pack_bf16x2(w[h][0] - t0, w[h][1] - t1));
+        }
+    }
+    // acc += A W
+    __device__ __forceinline__ void mma(float (&acc)[4], const uint32_t (&a)[4]) const {
+        mma_bf16_16816_a4(acc, a[0], a[1], a[2], a[3], hi[0], hi[1]);
+        mma_bf16_16816_a4(acc, a[0], a[1], a[2], a[3], lo[0], lo[1]);
+    }
+};
+
 }  // namespace ossa
