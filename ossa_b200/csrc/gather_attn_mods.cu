@@ -70,7 +70,7 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         const long long j = (long long)idx[(row0 + (size_t)t * Nq) * K + e];
         return j >= 0 && j < N && rm.sees(j, i, causal) ? (int)j : -1;
     };
-    int passes = 1, U;
+    int U;
     {
         // all heads' entries, then what hides them, in steps without branches between the loads: a wait for
         // each entry's segment in turn took a third of the kernel's time
@@ -86,8 +86,9 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         }
         rm.hide(x, K, i, causal);
         U = build_union<G, kDirect>(x, K, N, stage, list, lane);
-        if (U < 0) passes = G;
     }
+    const bool single = U < 0;  // the heads one by one
+    const int passes = single ? G : 1;
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage), vst = st + 2u * kStageChunk;
     const StageLane sl(lane);
     float oacc[8][4];  // O^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
@@ -102,7 +103,7 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
         __syncwarp();
-        if (passes > 1) U = single_list([&](int e) { return key_of(pass, e); }, pass, K, list, lane);
+        if (single) U = single_list([&](int e) { return key_of(pass, e); }, pass, K, list, lane);
         __syncwarp();  // the list is complete, the staging area is free
         const int nch = (U + kStageRows - 1) / kStageRows;
         if (nch > 0) {
@@ -335,7 +336,9 @@ cudaError_t launch_mma(const GatherArgs& a, cudaStream_t stream) {
     auto kern = G == 2 ? OSSA_MOD_PICK(2)
               : G == 3 ? OSSA_MOD_PICK(3)
               : G == 4 ? OSSA_MOD_PICK(4)
+              : G == 5 ? OSSA_MOD_PICK(5)
               : G == 6 ? OSSA_MOD_PICK(6)
+              : G == 7 ? OSSA_MOD_PICK(7)
                        : OSSA_MOD_PICK(8);
 #undef OSSA_MOD_PICK
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kModBytes);
@@ -351,16 +354,14 @@ cudaError_t launch_mma(const GatherArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K) {
-    const int G = H / Hkv;
-    return dtype == kBF16 && D == 128 && K >= 1 && K <= 128 && N <= kUnionMaxKeys &&
-           (G == 2 || G == 3 || G == 4 || G == 6 || G == 8);
+bool gather_union_serves(int dtype, int H, int Hkv, int N, int D, int K) {
+    return dtype == kBF16 && D == 128 && K >= 1 && K <= 128 && N <= kUnionMaxKeys && H / Hkv <= 8;
 }
 
 cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream) {
     if (a.dtype == kBF16 && a.D == 128 && (long long)a.B * a.H * a.Nq * a.K <= kFewEntries)
         return a.idx_is_64 ? launch_few<int64_t>(a, stream) : launch_few<int32_t>(a, stream);
-    if (gather_mma_serves(a.dtype, a.H, a.Hkv, a.N, a.D, a.K))
+    if (a.H > a.Hkv && gather_union_serves(a.dtype, a.H, a.Hkv, a.N, a.D, a.K))
         return a.idx_is_64 ? launch_mma<int64_t>(a, stream) : launch_mma<int32_t>(a, stream);
     if (a.dtype == kF32)
         return a.idx_is_64 ? launch_typed<float, int64_t, true>(a, stream) : launch_typed<float, int32_t, true>(a, stream);

@@ -54,7 +54,8 @@ BwdShape make_shape(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int 
     s.N = N;
     s.D = D;
     s.K = K;
-    const bool mma = gather_bwd_mma_serves(dtype, H, Hkv, Nq, N, D, K);
+    // the tensor-core key pass: bf16 rows of 128, rows and keys in 24 bits each
+    const bool mma = dtype == kBF16 && D == 128 && N <= (1 << 24) && (long long)s.G * Nq < (1ll << 24);
     s.shift = mma ? kKeyBlockShift : 0;
     s.NB = (N + (1 << s.shift) - 1) >> s.shift;
     const long long kv = (long long)B * Hkv;
@@ -355,7 +356,8 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     const int* krow = keys + row * s.K;
     for (int kc = 0; kc < s.K; kc += 32) {
         const int kk = kc + lane;
-        const int j = kk < s.K ? krow[kk] : -1;
+        int j = kk < s.K ? krow[kk] : -1;
+        if (s.shift && j != -1) j &= 0xffffff;  // the key of a word (list_word)
         if (!__any_sync(kFull, j >= 0)) continue;
         float x[32], y[32];
 #pragma unroll
@@ -584,16 +586,32 @@ cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuf
     const unsigned row_grid = (unsigned)((rows + kWarps - 1) / kWarps);
     const dim3 key_grid((unsigned)((s.tiles + kWarps - 1) / kWarps), kvs);
     cudaError_t e;
+    if (s.shift > 0 && gather_union_serves(a.f.dtype, s.H, s.Hkv, s.N, s.D, s.K)) {
+        e = launch_row_pass_mma(a, s, w, stream);
+    } else {
+        switch (s.D) {
+#define OSSA_BWD_CASE(DD)                                                                                        \
+    case DD:                                                                                                     \
+        row_pass_kernel<T, DD><<<row_grid, kThreads, 0, stream>>>(q, k, v, w.keys, out, dout, s, m, dq, w.delta, \
+                                                                  w.slope_rows);                                 \
+        break;
+            OSSA_BWD_CASE(16)
+            OSSA_BWD_CASE(32)
+            OSSA_BWD_CASE(64)
+            OSSA_BWD_CASE(128)
+            OSSA_BWD_CASE(256)
+#undef OSSA_BWD_CASE
+            default: return cudaErrorInvalidValue;
+        }
+        e = launched();
+    }
+    if (e != cudaSuccess) return e;
     if (s.shift > 0) {
-        if ((e = launch_row_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
-        if ((e = launch_key_pass_mma(a, s, w, stream)) != cudaSuccess) return e;
+        e = launch_key_pass_mma(a, s, w, stream);
     } else {
         switch (s.D) {
 #define OSSA_BWD_CASE(DD)                                                                                               \
     case DD:                                                                                                            \
-        row_pass_kernel<T, DD><<<row_grid, kThreads, 0, stream>>>(q, k, v, w.keys, out, dout, s, m, dq, w.delta,        \
-                                                                  w.slope_rows);                                        \
-        if ((e = launched()) != cudaSuccess) return e;                                                                  \
         key_pass_kernel<T, DD><<<key_grid, kThreads, 0, stream>>>(q, k, v, dout, s, m, w.base, w.list, w.delta, dk, dv, \
                                                                   w.part);                                              \
         break;
@@ -605,8 +623,9 @@ cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuf
 #undef OSSA_BWD_CASE
             default: return cudaErrorInvalidValue;
         }
-        if ((e = launched()) != cudaSuccess) return e;
+        e = launched();
     }
+    if (e != cudaSuccess) return e;
     join_kernel<T><<<dim3((unsigned)((s.N + kWarps - 1) / kWarps), kvs), kThreads, 0, stream>>>(s, w.base, w.part, dk, dv);
     if ((e = launched()) != cudaSuccess || !a.dslopes) return e;
     slope_join_kernel<<<s.H, 1024, 0, stream>>>(s, w.slope_rows, a.dslopes);
@@ -614,10 +633,6 @@ cudaError_t passes_typed(const GatherBwdArgs& a, const BwdShape& s, const BwdBuf
 }
 
 }  // namespace
-
-bool gather_bwd_mma_serves(int dtype, int H, int Hkv, int Nq, int N, int D, int K) {
-    return gather_mma_serves(dtype, H, Hkv, N, D, K) && (long long)(H / Hkv) * Nq < (1ll << 24);
-}
 
 size_t gather_bwd_workspace_bytes(int dtype, int B, int H, int Hkv, int Nq, int N, int D, int K, bool dslopes) {
     return make_layout(make_shape(dtype, B, H, Hkv, Nq, N, D, K), dslopes).total;

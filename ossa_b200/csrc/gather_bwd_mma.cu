@@ -98,7 +98,7 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         const int w = keys[(row0 + (size_t)t * s.Nq) * s.K + e];
         return w == -1 ? -1 : w & 0xffffff;
     };
-    int passes = 1, U;
+    int U;
     {
         int x[G][4];
 #pragma unroll
@@ -107,8 +107,9 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             for (int e = 0; e < 4; ++e) x[t][e] = lane + 32 * e < s.K ? key_of(t, lane + 32 * e) : -1;
         }
         U = build_union<G, kDirect>(x, s.K, s.N, stage, list, lane);
-        if (U < 0) passes = G;
     }
+    const bool single = U < 0;  // the heads one by one
+    const int passes = single ? G : 1;
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
     const StageLane sl(lane);
     float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
@@ -124,7 +125,7 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 #pragma unroll 1
     for (int pass = 0; pass < passes; ++pass) {
         __syncwarp();
-        if (passes > 1) U = single_list([&](int e) { return key_of(pass, e); }, pass, s.K, list, lane);
+        if (single) U = single_list([&](int e) { return key_of(pass, e); }, pass, s.K, list, lane);
         __syncwarp();  // the list is complete, the staging area is free
         const int nch = (U + kStageRows - 1) / kStageRows;
         if (nch > 0) stage_both(0);
@@ -419,10 +420,13 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 cudaError_t launch_row_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream) {
     const bool direct = s.N <= kUnionDirectKeys;
 #define OSSA_ROW_PICK(GG) (direct ? row_pass_mma_kernel<GG, true> : row_pass_mma_kernel<GG, false>)
-    auto kern = s.G == 2 ? OSSA_ROW_PICK(2)
+    auto kern = s.G == 1 ? OSSA_ROW_PICK(1)
+              : s.G == 2 ? OSSA_ROW_PICK(2)
               : s.G == 3 ? OSSA_ROW_PICK(3)
               : s.G == 4 ? OSSA_ROW_PICK(4)
+              : s.G == 5 ? OSSA_ROW_PICK(5)
               : s.G == 6 ? OSSA_ROW_PICK(6)
+              : s.G == 7 ? OSSA_ROW_PICK(7)
                          : OSSA_ROW_PICK(8);
 #undef OSSA_ROW_PICK
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes);

@@ -79,9 +79,9 @@ struct GatherArgs {
 cudaError_t launch_gather_attn(const GatherArgs& a, cudaStream_t stream);
 // The same attention under a.mods (a.scale is not read: a.mods.scale is).
 cudaError_t launch_gather_attn_mods(const GatherArgs& a, cudaStream_t stream);
-// Whether the tensor-core forms of the modified gather and its backward pass take a shape.
-bool gather_mma_serves(int dtype, int H, int Hkv, int N, int D, int K);
-bool gather_bwd_mma_serves(int dtype, int H, int Hkv, int Nq, int N, int D, int K);
+// Whether the tensor-core forms that take a query's heads at once (the modified gather's, its backward's row
+// pass) serve a shape.
+bool gather_union_serves(int dtype, int H, int Hkv, int N, int D, int K);
 
 // Gradients of launch_gather_attn_mods (gather_bwd.cu).
 struct GatherBwdArgs {

@@ -134,7 +134,24 @@ CASES = [
     (1, 4, 1, 33, 33, 256, 9, "cap prefix"),
     (1, 6, 2, 60, 60, 128, 150, "slopes docs"),
     (1, 8, 4, 200, 200, 128, 24, "cap"),
+    (1, 7, 1, 150, 150, 128, 100, "cap slopes"),
+    (2, 14, 2, 90, 90, 128, 64, "docs"),
+    (1, 10, 2, 140, 140, 128, 128, ""),
+    (1, 3, 3, 600, 600, 128, 90, "cap docs"),
+    (1, 9, 1, 70, 70, 128, 40, "slopes"),
+    (1, 16, 2, 260, 260, 128, 128, "prefix"),
 ]
+
+
+@pytest.mark.parametrize("Nk", [12288, 12289, 20000])
+def test_many_keys(Nk):
+    """On either side of what the heads' union covers with a byte per key; lists with and without repeats."""
+    B, H, Hkv, Nq, D, K = 1, 6, 2, 100, 128, 64
+    q, k, v, do = _inputs(torch.bfloat16, B, H, Hkv, Nq, Nk, D, seed=Nk)
+    idx = _lists(B, H, Nq, Nk, K, Nk - Nq, seed=4)
+    idx[:, :, ::3, 5] = idx[:, :, ::3, 4]
+    idx[:, :, 1::7] = idx[:, :, 1::7].flip(-1)
+    _check(torch.bfloat16, q, k, v, do, idx, _mods(["cap", "docs"], B, H, Nk, seed=1), q0=Nk - Nq)
 
 
 @pytest.mark.parametrize("kind", ["causal", "any"])
