@@ -322,18 +322,42 @@ struct RowLoad {
     }
 };
 
+// Rows that a warp holds in registers at once in the passes below: each is fetched once for its dot product
+// and its weighted sum (fp32, 12/2 heads, N=4096, K=64: fetched again for the sum, 32 at a time, the key
+// pass took 1199 us, the row pass 328; held 8 at a time 259 and 208).
+template <int D>
+constexpr int kHeld = RowLoad<float, D>::kPer <= 4 ? 8 : 4;
+
+// Sums x[0..n-1] over the warp; lane l ends with the total of x[l % n].
+template <int n>
+__device__ __forceinline__ float reduce_held(float (&x)[n], int lane) {
+#pragma unroll
+    for (int w = n / 2; w >= 1; w >>= 1) {
+        const bool upper = (lane & w) != 0;
+#pragma unroll
+        for (int t = 0; t < w; ++t) {
+            const float send = upper ? x[t] : x[t + w], keep = upper ? x[t + w] : x[t];
+            x[t] = keep + __shfl_xor_sync(kFull, send, w);
+        }
+    }
+#pragma unroll
+    for (int o = n; o < 32; o <<= 1) x[0] += __shfl_xor_sync(kFull, x[0], o);
+    return x[0];
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
 row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const int* __restrict__ keys,
                 const T* __restrict__ out, const T* __restrict__ dout, const BwdShape s, const ScoreMods mods,
                 T* __restrict__ dq, float* __restrict__ delta, float* __restrict__ slope_rows) {
     using R = RowLoad<T, D>;
+    constexpr int B = kHeld<D>;
     const int lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (row >= (long long)s.B * s.H * s.Nq) return;  // warp-uniform
     const int bh = (int)(row / s.Nq), il = (int)(row - (long long)bh * s.Nq);
-    const int b = bh / s.H, h = bh - b * s.H, i = s.q0 + il;
-    const size_t kv = (size_t)b * s.Hkv + h / s.G;
+    const int batch = bh / s.H, h = bh - batch * s.H, i = s.q0 + il;
+    const size_t kv = (size_t)batch * s.Hkv + h / s.G;
     const T* kb = k + kv * s.N * D;
     const T* vb = v + kv * s.N * D;
     const float slope = mods.slopes ? mods.slopes[h] : 0.f;
@@ -358,42 +382,46 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         const int kk = kc + lane;
         int j = kk < s.K ? krow[kk] : -1;
         if (s.shift && j != -1) j &= 0xffffff;  // the key of a word (list_word)
-        if (!__any_sync(kFull, j >= 0)) continue;
-        float x[32], y[32];
+        const unsigned some = __ballot_sync(kFull, j >= 0);
+        for (int m0 = 0; m0 < 32; m0 += B) {
+            if (((some >> m0) & ((1u << B) - 1u)) == 0u) continue;  // warp-uniform
+            float kr[B][R::kPer], x[B], y[B];
 #pragma unroll
-        for (int m = 0; m < 32; ++m) {
-            const int jm = __shfl_sync(kFull, j, m);
-            float r[R::kPer];
-            x[m] = y[m] = 0.f;
-            if (jm >= 0) {  // warp-uniform
-                R::load(kb + (size_t)jm * D, lane, r);
-#pragma unroll
-                for (int t = 0; t < R::kPer; ++t) x[m] = fmaf(qv[t], r[t], x[m]);
-                R::load(vb + (size_t)jm * D, lane, r);
-#pragma unroll
-                for (int t = 0; t < R::kPer; ++t) y[m] = fmaf(dv[t], r[t], y[m]);
+            for (int t = 0; t < B; ++t) {
+                const int jt = max(__shfl_sync(kFull, j, m0 + t), 0);
+                R::load(kb + (size_t)jt * D, lane, kr[t]);
             }
-        }
-        const float dot = transpose_reduce32(x, lane);
-        const float dp = transpose_reduce32(y, lane);
-        float p = 0.f, dx = 0.f;
-        if (j >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
-            const float far = fabsf((float)(i - j));
-            p = exp2f(mods.score2_grad(dot, slope, far, dx, TanhExact()) - lse2);
-            dx *= p * (dp - d0);
-            a_pd = fmaf(p, dp, a_pd);
-            a_f = fmaf(p, far, a_f);
-            a_pdf = fmaf(p * dp, far, a_pdf);
-        }
 #pragma unroll
-        for (int m = 0; m < 32; ++m) {
-            const int jm = __shfl_sync(kFull, j, m);
-            const float w = __shfl_sync(kFull, dx, m);
-            if (jm >= 0) {
+            for (int t = 0; t < B; ++t) {
+                const int jt = max(__shfl_sync(kFull, j, m0 + t), 0);
                 float r[R::kPer];
-                R::load(kb + (size_t)jm * D, lane, r);
+                R::load(vb + (size_t)jt * D, lane, r);
+                x[t] = y[t] = 0.f;
 #pragma unroll
-                for (int t = 0; t < R::kPer; ++t) acc[t] = fmaf(w, r[t], acc[t]);
+                for (int d = 0; d < R::kPer; ++d) {
+                    x[t] = fmaf(qv[d], kr[t][d], x[t]);
+                    y[t] = fmaf(dv[d], r[d], y[t]);
+                }
+            }
+            const float dot = reduce_held<B>(x, lane), dp = reduce_held<B>(y, lane);
+            const int je = __shfl_sync(kFull, j, m0 + lane % B);  // this lane's entry
+            float p = 0.f, dx = 0.f;
+            if (je >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
+                const float far = fabsf((float)(i - je));
+                p = exp2f(mods.score2_grad(dot, slope, far, dx, TanhExact()) - lse2);
+                dx *= p * (dp - d0);
+                if (lane < B) {
+                    a_pd = fmaf(p, dp, a_pd);
+                    a_f = fmaf(p, far, a_f);
+                    a_pdf = fmaf(p * dp, far, a_pdf);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < B; ++t) {
+                const float w = __shfl_sync(kFull, dx, t);
+                if (__shfl_sync(kFull, j, m0 + t) < 0) continue;  // warp-uniform; key 0 in its place may hold anything
+#pragma unroll
+                for (int d = 0; d < R::kPer; ++d) acc[d] = fmaf(w, kr[t][d], acc[d]);
             }
         }
     }
@@ -416,14 +444,15 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
                 const BwdShape s, const ScoreMods mods, const int* __restrict__ base, const int* __restrict__ list,
                 const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ part) {
     using R = RowLoad<T, D>;
+    constexpr int B = kHeld<D>;
     const int lane = threadIdx.x & 31, kv = blockIdx.y;
     const long long tile = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int* bs = base + (size_t)kv * (s.N + 1);
     const int total = bs[s.N];
     if (tile * s.tile >= total) return;  // warp-uniform
     const int t0 = (int)(tile * s.tile), t1 = min(total, t0 + s.tile);
-    const int b = kv / s.Hkv, h0 = (kv - b * s.Hkv) * s.G;
-    const size_t rows0 = ((size_t)b * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
+    const int batch = kv / s.Hkv, h0 = (kv - batch * s.Hkv) * s.G;
+    const size_t rows0 = ((size_t)batch * s.H + h0) * s.Nq;  // row of list entry r: rows0 + r
     const int* ls = list + (size_t)kv * s.cap;
     int key = block_at(bs, s.N, t0);
     for (int pos = t0; pos < t1; ++key) {
@@ -437,44 +466,44 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         for (int t = 0; t < R::kPer; ++t) ak[t] = av[t] = 0.f;
         for (; pos < end; pos += 32) {
             const int n = min(32, end - pos);
-            const int r = lane < n ? ls[pos + lane] : -1;
-            float x[32], y[32];
+            const int r = ls[pos + min(lane, n - 1)];  // past the run its last row again, without weight
+            const int g = r / s.Nq, i = s.q0 + r - g * s.Nq;
+            const float lse2 = lane < n ? mods.lse2[rows0 + r] : -INFINITY, dl = delta[rows0 + r];
+            const float slope = mods.slopes ? mods.slopes[h0 + g] : 0.f;
+            for (int m0 = 0; m0 < n; m0 += B) {
+                float qr[B][R::kPer], dr[B][R::kPer], x[B], y[B];
 #pragma unroll
-            for (int m = 0; m < 32; ++m) {
-                const int rm = __shfl_sync(kFull, r, m);
-                x[m] = y[m] = 0.f;
-                if (m < n) {  // warp-uniform
-                    float f[R::kPer];
-                    R::load(q + (rows0 + rm) * D, lane, f);
-#pragma unroll
-                    for (int t = 0; t < R::kPer; ++t) x[m] = fmaf(f[t], kr[t], x[m]);
-                    R::load(dout + (rows0 + rm) * D, lane, f);
-#pragma unroll
-                    for (int t = 0; t < R::kPer; ++t) y[m] = fmaf(f[t], vr[t], y[m]);
+                for (int t = 0; t < B; ++t) {
+                    const size_t row = rows0 + __shfl_sync(kFull, r, m0 + t);
+                    R::load(q + row * D, lane, qr[t]);
+                    R::load(dout + row * D, lane, dr[t]);
                 }
-            }
-            const float dot = transpose_reduce32(x, lane);
-            const float dp = transpose_reduce32(y, lane);
-            float p = 0.f, dx = 0.f;
-            const float lse2 = r >= 0 ? mods.lse2[rows0 + r] : -INFINITY;
-            if (lse2 != -INFINITY) {
-                const int g = r / s.Nq, i = s.q0 + r - g * s.Nq;
-                const float slope = mods.slopes ? mods.slopes[h0 + g] : 0.f;
-                p = exp2f(mods.score2_grad(dot, slope, fabsf((float)(i - key)), dx, TanhExact()) - lse2);
-                dx *= p * (dp - delta[rows0 + r]);
-            }
 #pragma unroll
-            for (int m = 0; m < 32; ++m) {
-                const int rm = __shfl_sync(kFull, r, m);
-                const float pm = __shfl_sync(kFull, p, m), xm = __shfl_sync(kFull, dx, m);
-                if (m < n) {
-                    float f[R::kPer];
-                    R::load(q + (rows0 + rm) * D, lane, f);
+                for (int t = 0; t < B; ++t) {
+                    x[t] = y[t] = 0.f;
 #pragma unroll
-                    for (int t = 0; t < R::kPer; ++t) ak[t] = fmaf(xm, f[t], ak[t]);
-                    R::load(dout + (rows0 + rm) * D, lane, f);
+                    for (int d = 0; d < R::kPer; ++d) {
+                        x[t] = fmaf(qr[t][d], kr[d], x[t]);
+                        y[t] = fmaf(dr[t][d], vr[d], y[t]);
+                    }
+                }
+                const float dot = reduce_held<B>(x, lane), dp = reduce_held<B>(y, lane);
+                const int e = m0 + lane % B;  // this lane's entry
+                const float le = __shfl_sync(kFull, lse2, e), de = __shfl_sync(kFull, dl, e);
+                const float se = __shfl_sync(kFull, slope, e), far = fabsf((float)(__shfl_sync(kFull, i, e) - key));
+                float p = 0.f, dx = 0.f;
+                if (le != -INFINITY) {
+                    p = exp2f(mods.score2_grad(dot, se, far, dx, TanhExact()) - le);
+                    dx *= p * (dp - de);
+                }
 #pragma unroll
-                    for (int t = 0; t < R::kPer; ++t) av[t] = fmaf(pm, f[t], av[t]);
+                for (int t = 0; t < B; ++t) {
+                    const float pt = __shfl_sync(kFull, p, t), xt = __shfl_sync(kFull, dx, t);
+#pragma unroll
+                    for (int d = 0; d < R::kPer; ++d) {
+                        ak[d] = fmaf(xt, qr[t][d], ak[d]);
+                        av[d] = fmaf(pt, dr[t][d], av[d]);
+                    }
                 }
             }
         }
