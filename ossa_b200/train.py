@@ -104,14 +104,23 @@ def distillation_loss(router, q: torch.Tensor, k: torch.Tensor, top_k: int, *,
     return _DistillFn.apply(wq, wk, pb, q, k, targets, router.cfg.seq_len)
 
 
+def _logit_rows(z):
+    """(what the C calls take of the logits first, z): rows where they lie; z is 2-D or 3-D."""
+    if z.stride(-1) != 1:
+        z = z.contiguous()
+    if z.dim() == 2:
+        outer, inner, so, si = 1, z.shape[0], 0, z.stride(0)
+    else:
+        outer, inner, so, si = z.shape[0], z.shape[1], z.stride(0), z.stride(1)
+    return (z.data_ptr(), _lib.dtype_code(z), outer, inner, z.shape[-1], so, si), z
+
+
 class _TopLogitDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, teacher, ids, weight, tau, reduction, grad):
-        V, K = z.shape[-1], ids.shape[-1]
-        outer, inner = (1, z.shape[0]) if z.dim() == 2 else (z.shape[0], z.shape[1])
-        rows = outer * inner
-        so, si = (0, z.stride(0)) if z.dim() == 2 else (z.stride(0), z.stride(1))
-        dev = z.device
+        K, dev = ids.shape[-1], z.device
+        where, z = _logit_rows(z)
+        rows = where[2] * where[3]
         L = _lib.lib()
         ws_bytes = L.ossa_top_logit_distill_workspace_size(rows, K)
         ws = z.new_empty(ws_bytes, dtype=torch.uint8)
@@ -119,8 +128,7 @@ class _TopLogitDistill(torch.autograd.Function):
         each = reduction == "none"
         loss = z.new_empty(rows if each else (), dtype=torch.float32)
         # a single incoming gradient is 1 as a rule: the gradient is taken with the loss
-        dz = z.new_empty((rows, V)) if grad and not each else None
-        where = (z.data_ptr(), _lib.dtype_code(z), outer, inner, V, so, si)
+        dz = z.new_empty((rows, z.shape[-1])) if grad and not each else None
         with _lib.on_device(dev):
             st = L.ossa_top_logit_distill_fwd(
                 *where, teacher.data_ptr(), ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau,
@@ -130,7 +138,7 @@ class _TopLogitDistill(torch.autograd.Function):
         if grad:
             ctx.save_for_backward(z, ids)
             ctx.kept = (ws, ws_bytes, dz)
-            ctx.rule = (where[1:], K, tau, mean, each)
+            ctx.rule = (tau, mean, each)
         if each and weight is not None:
             loss.mul_(weight)
         return loss
@@ -140,15 +148,17 @@ class _TopLogitDistill(torch.autograd.Function):
     def backward(ctx, g):
         z, ids = ctx.saved_tensors
         ws, ws_bytes, dz = ctx.kept
-        where, K, tau, mean, each = ctx.rule
+        tau, mean, each = ctx.rule
+        # the saved logits may come back in another place and layout (offloading): rows are taken anew
+        where, z = _logit_rows(z)
         ctx.kept = (ws, ws_bytes, None)  # a second backward pass makes its own
         taken = dz is not None
         if not taken:
-            dz = z.new_empty((where[1] * where[2], z.shape[-1]))
+            dz = z.new_empty((where[2] * where[3], z.shape[-1]))
         g = g.contiguous()  # fp32, as the loss
         with _lib.on_device(z.device):
             st = _lib.lib().ossa_top_logit_distill_bwd(
-                z.data_ptr(), *where, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau, mean, g.data_ptr(),
+                *where, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, ids.shape[-1], tau, mean, g.data_ptr(),
                 1 if each else 0, 1 if taken else 0, dz.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(z.device))
         _lib.check(st)
         return dz.view(z.shape), None, None, None, None, None, None
