@@ -212,6 +212,12 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def packed(t: torch.Tensor) -> torch.Tensor:
+    """t contiguous and on a 16-byte boundary: itself, or a copy (a gradient may be a piece of a larger one)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

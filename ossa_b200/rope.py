@@ -78,7 +78,7 @@ class _RopeToHeads(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         cos, sin = ctx.saved_tensors
-        g = g.contiguous()
+        g = _lib.packed(g)
         B, H, N, D = g.shape
         dx = g.new_empty(ctx.shape)
         args = (None, None, None, None, _lib.ptr(cos), _lib.ptr(sin),
@@ -98,7 +98,7 @@ def _tables(cos, sin, B, N, D, dtype):
         cos, sin = cos.unsqueeze(0), sin.unsqueeze(0)
     if cos.shape != sin.shape or cos.dim() != 3 or cos.shape[0] not in (1, B) or tuple(cos.shape[1:]) != (N, D):
         raise ValueError(f"cos/sin of shapes {tuple(cos.shape)}, {tuple(sin.shape)} do not match (B or 1, {N}, {D})")
-    return cos.contiguous(), sin.contiguous()
+    return _lib.packed(cos), _lib.packed(sin)
 
 
 def _rows(x, heads, name):
@@ -118,9 +118,7 @@ def _rows(x, heads, name):
         whole = x.stride(-1) == 1 and (x.dim() == 3 or heads == 1 or x.stride(2) == D)
         sb, sn = (sb if B > 1 else 0), (sn if N > 1 else 0)
     if not whole or sb * x.element_size() % 16 or sn * x.element_size() % 16 or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
+        x = _lib.packed(x)
         sn, sb = heads * D, N * heads * D
     return x, B, N, D, sb, sn
 
@@ -186,11 +184,11 @@ class _QkNormRope(torch.autograd.Function):
         need = ctx.needs_input_grad
         dq = dk = dwq = dwk = None
         if gq is not None:
-            gq = gq.contiguous()
+            gq = _lib.packed(gq)
             dq = gq.new_empty(q.shape)
             dwq = torch.empty_like(wq) if need[2] else None
         if gk is not None:
-            gk = gk.contiguous()
+            gk = _lib.packed(gk)
             dk = gk.new_empty(k.shape)
             dwk = torch.empty_like(wk) if need[3] else None
         if gk is None:  # one output has no gradient: the other tensor alone, in the place of the queries

@@ -176,7 +176,7 @@ def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, seg
     _lib.require_cuda(*[t for t in (q, k, v, idx, slopes, segments, prefix_len) if t is not None])
     if grad:
         return _TopkAttention.apply(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
-    q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
+    q, k, v, idx = _lib.packed(q), _lib.packed(k), _lib.packed(v), idx.contiguous()
     return _mod_forward(_mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap), q, None)
 
 
@@ -202,7 +202,7 @@ def _mod_forward(args, q, lse2):
 class _TopkAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
-        q, k, v, idx = q.contiguous(), k.contiguous(), v.contiguous(), idx.contiguous()
+        q, k, v, idx = _lib.packed(q), _lib.packed(k), _lib.packed(v), idx.contiguous()
         lse2 = q.new_empty(q.shape[:3], dtype=torch.float32)
         args = _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
         out = _mod_forward(args, q, lse2)
@@ -216,7 +216,7 @@ class _TopkAttention(torch.autograd.Function):
         # saved tensors may come back as others than were saved (checkpointing, offloading)
         q, k, v, slopes, idx, segments, prefix_len, out, lse2 = ctx.saved_tensors
         args, dev = _mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), q.device
-        dout = dout.contiguous()
+        dout = _lib.packed(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
         L = _lib.lib()
