@@ -12,7 +12,8 @@
 // flight while chunk c is scored, its value rows while its softmax runs.  p enters the product with the
 // bf16 values as a bf16 value and its rest (Weights); sums and statistics are fp32.
 // A query with a key listed twice by one head, or with more than 512 different keys, takes its heads
-// one after another through the same loop.
+// one after another through the same loop.  So does one whose result is not finite: a key that only some of
+// the heads list has no weight for the others, and 0 times its value row must be 0 there.
 //
 // Bound: shared-memory traffic and issue (16 KB a chunk of 16 keys, 12 KB of it operands).  Measured: packed
 // prefill B=2, 12/2 heads, N=4096, K=64, slopes: 108 us, 39 us of it for the lists, documents and the union of
@@ -87,21 +88,20 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         rm.hide(x, K, i, causal);
         U = build_union<G, kDirect>(x, K, N, stage, list, lane);
     }
-    const bool single = U < 0;  // the heads one by one
-    const int passes = single ? G : 1;
+    bool single = U < 0;  // the heads one by one
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage), vst = st + 2u * kStageChunk;
     const StageLane sl(lane);
-    float oacc[8][4];  // O^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
-#pragma unroll
-    for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
     float slope[2] = {0.f, 0.f};
     if (mods.slopes) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) slope[e] = 2 * c4 + e < G ? mods.slopes[g * G + 2 * c4 + e] : 0.f;
     }
 #pragma unroll 1
-    for (int pass = 0; pass < passes; ++pass) {
+    for (int pass = 0;;) {
+        float oacc[8][4];  // O^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
+#pragma unroll
+        for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
+        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
         __syncwarp();
         if (single) U = single_list([&](int e) { return key_of(pass, e); }, pass, K, list, lane);
         __syncwarp();  // the list is complete, the staging area is free
@@ -191,28 +191,44 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 pw.mma(oacc[mt + 4], a);
             }
         }
-    }
+        if (!single) {
+            float bad = 0.f;  // 0 while every sum is finite
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+            for (int n = 0; n < 8; ++n) {
 #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) l_run[e] += __shfl_xor_sync(kFull, l_run[e], o);
-    }
-    // each head's row divided by its sum and transposed back: lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
-    const float inv0 = l_run[0] == 0.f ? 0.f : 1.f / l_run[0], inv1 = l_run[1] == 0.f ? 0.f : 1.f / l_run[1];
-    __nv_bfloat16* orow = out + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D + 2 * c4;
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-        const uint32_t lo = movmatrix_trans(pack_bf16x2(oacc[mt][0] * inv0, oacc[mt][1] * inv1));
-        const uint32_t hi = movmatrix_trans(pack_bf16x2(oacc[mt][2] * inv0, oacc[mt][3] * inv1));
-        if (gq < G) {
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+                for (int x = 0; x < 4; ++x) bad = fmaf(oacc[n][x], 0.f, bad);
+            }
+            if (__any_sync(kFull, bad != 0.f)) {
+                single = true;
+                continue;
+            }
         }
-    }
-    if (mods.lse2 && gq == 0) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (2 * c4 + e < G) mods.lse2[row0 + (size_t)(2 * c4 + e) * Nq] = m_run[e] + log2f(l_run[e]);
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) l_run[e] += __shfl_xor_sync(kFull, l_run[e], o);
+        }
+        // each head's row divided by its sum and transposed back: lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
+        const float inv0 = l_run[0] == 0.f ? 0.f : 1.f / l_run[0], inv1 = l_run[1] == 0.f ? 0.f : 1.f / l_run[1];
+        __nv_bfloat16* orow = out + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D + 2 * c4;
+        const bool mine = single ? gq == pass : gq < G;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+            const uint32_t lo = movmatrix_trans(pack_bf16x2(oacc[mt][0] * inv0, oacc[mt][1] * inv1));
+            const uint32_t hi = movmatrix_trans(pack_bf16x2(oacc[mt][2] * inv0, oacc[mt][3] * inv1));
+            if (mine) {
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+            }
+        }
+        if (mods.lse2 && gq == 0) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int t = 2 * c4 + e;
+                if (single ? t == pass : t < G) mods.lse2[row0 + (size_t)t * Nq] = m_run[e] + log2f(l_run[e]);
+            }
+        }
+        if (!single || ++pass == G) break;
     }
 }
 

@@ -17,8 +17,8 @@
 //     end inside a key's run: whole runs are stored, cut ones go to per-tile partial sums.
 //  4. Join: keys whose run is cut add their partial sums in tile order; keys that nobody
 //     lists get zeros.
-// No float atomics: repeated calls give the same bits.  (Two entries of one row with the same
-// key are alike, so the order in which the counting sort places them does not show.)
+// No float atomics, and the sort's places do not depend on the order in which atomics run (entry_place):
+// repeated calls give the same bits.
 //
 // Bound: L2-to-SM traffic.  Either pass reads two rows of D values per entry (the row pass's tensor-core form
 // per key of the heads' union, the key pass's per row and key block), which no tile keeps: the rows that list
@@ -246,8 +246,20 @@ __global__ void __launch_bounds__(1024) key_scan_kernel(const BwdShape s, int* _
     if (threadIdx.x == 0) p[s.NB] = carry;
 }
 
-// list[kv][position] = r (| bits << 24) with r = g * Nq + il of the rows that list a key block, block by block.  One warp walks the
-// unit's rows in a fixed order, the counters of its key range in shared memory; the entries of
+// The place of this lane's entry (block at, on: it has one) behind the counter of its block.  Entries of one
+// row that share a block take theirs in lane order: ascending lists have none (`some`, `follow`: lanes that
+// hold a key, those whose key exceeds the lane's before), others are matched.
+__device__ __forceinline__ int entry_place(int* next, int at, bool on, unsigned some, unsigned follow, int lane) {
+    if (__popc(some & ~follow) <= 1) return on ? atomicAdd(&next[at], 1) : -1;  // warp-uniform; no block twice
+    const unsigned same = __match_any_sync(kFull, on ? at : -1 - lane);
+    const int rank = __popc(same & lanemask_lt()), first = on ? next[at] : 0;
+    __syncwarp();
+    if (on && rank == 0) next[at] = first + __popc(same);
+    return on ? first + rank : -1;
+}
+
+// list[kv][position] = r (| bits << 24) with r = g * Nq + il of the rows that list a key block, block by
+// block.  One warp walks the unit's rows in a fixed order, the counters of its key range in shared memory; the entries of
 // kPlaceRows rows are loaded together, and the next ones while these are placed, so a step costs
 // one trip to L2 and not one per row.
 __global__ void __launch_bounds__(32)
@@ -288,7 +300,10 @@ place_kernel(const int* __restrict__ keys, const BwdShape s, const int* __restri
 #pragma unroll
         for (int t = 0; t < kPlaceRows; ++t) {
             const int at = word_block(w[t], s.shift) - k0;
-            pos[t] = w[t] != -1 && (unsigned)at < (unsigned)nk ? atomicAdd(&next[at], 1) : -1;
+            const int key = w[t] == -1 || s.shift == 0 ? w[t] : w[t] & 0xffffff, before = __shfl_up_sync(kFull, key, 1);
+            const unsigned some = __ballot_sync(kFull, key >= 0);
+            const unsigned follow = __ballot_sync(kFull, key >= 0 && lane > 0 && before >= 0 && before < key);
+            pos[t] = entry_place(next, at, w[t] != -1 && (unsigned)at < (unsigned)nk, some, follow, lane);
             __syncwarp();  // a row's places before the next row's
         }
 #pragma unroll

@@ -39,7 +39,8 @@ __device__ __forceinline__ float dot_bf16x2(uint32_t a, uint32_t b, float c) {
 // (query_union.cuh).  In chunks of 16 keys: S^T = K Q^T and dP^T = V dO^T (keys as MMA rows, heads as
 // columns), p, dS and the weights dX per (key, head), then dq^T += K^T dX^T from the same staged key
 // rows.  dX enters that product as a bf16 value and its rest (Weights); p, dP, the sums and Delta stay
-// fp32.  The rows of chunk c + 1 are in flight while chunk c is computed.
+// fp32.  The rows of chunk c + 1 are in flight while chunk c is computed.  Where the list has no room, or
+// the result is not finite (0 times the key row of another head), the heads go one by one, as in the forward.
 constexpr int kRowWarps = 6;
 constexpr int kRowWarpBytes = 4 * kStageChunk + kUnionCap * 4;  // key and value rows of two chunks; the list
 constexpr int kRowBytes = kRowWarps * kRowWarpBytes;
@@ -108,14 +109,9 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         }
         U = build_union<G, kDirect>(x, s.K, s.N, stage, list, lane);
     }
-    const bool single = U < 0;  // the heads one by one
-    const int passes = single ? G : 1;
+    bool single = U < 0;  // the heads one by one
     const uint32_t st = (uint32_t)__cvta_generic_to_shared(stage);
     const StageLane sl(lane);
-    float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
-#pragma unroll
-    for (int n = 0; n < 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    float a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_pdf[2] = {0.f, 0.f};  // sums of p dP, p far, p dP far
     auto stage_both = [&](int c) {
         const uint32_t at = st + (uint32_t)((c & 1) * 2 * kStageChunk);
         stage_listed(at, kb, list, c * kStageRows, U, sl, lane);
@@ -123,7 +119,11 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         stage_commit();
     };
 #pragma unroll 1
-    for (int pass = 0; pass < passes; ++pass) {
+    for (int pass = 0;;) {
+        float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
+#pragma unroll
+        for (int n = 0; n < 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        float a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_pdf[2] = {0.f, 0.f};  // sums of p dP, p far, p dP far
         __syncwarp();
         if (single) U = single_list([&](int e) { return key_of(pass, e); }, pass, s.K, list, lane);
         __syncwarp();  // the list is complete, the staging area is free
@@ -185,30 +185,45 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 wt.mma(acc[mt + 4], a);
             }
         }
-    }
+        if (G > 1 && !single) {
+            float bad = 0.f;  // 0 while every sum is finite
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+            for (int n = 0; n < 8; ++n) {
 #pragma unroll
-        for (int o = 4; o <= 16; o <<= 1) {
-            a_pd[e] += __shfl_xor_sync(kFull, a_pd[e], o);
-            a_f[e] += __shfl_xor_sync(kFull, a_f[e], o);
-            a_pdf[e] += __shfl_xor_sync(kFull, a_pdf[e], o);
+                for (int x = 0; x < 4; ++x) bad = fmaf(acc[n][x], 0.f, bad);
+            }
+            if (__any_sync(kFull, bad != 0.f)) {
+                single = true;
+                continue;
+            }
         }
-        if (gq == 0 && 2 * c4 + e < G) {
-            const size_t row = row0 + (size_t)(2 * c4 + e) * s.Nq;
-            delta[row] = a_pd[e];
-            if (slope_rows) slope_rows[row] = a_pd[e] * a_f[e] - a_pdf[e];
-        }
-    }
-    __nv_bfloat16* orow = dq + mine + 2 * c4;
 #pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-        const uint32_t lo = movmatrix_trans(pack_bf16x2(acc[mt][0], acc[mt][1]));
-        const uint32_t hi = movmatrix_trans(pack_bf16x2(acc[mt][2], acc[mt][3]));
-        if (gq < G) {
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) {
+                a_pd[e] += __shfl_xor_sync(kFull, a_pd[e], o);
+                a_f[e] += __shfl_xor_sync(kFull, a_f[e], o);
+                a_pdf[e] += __shfl_xor_sync(kFull, a_pdf[e], o);
+            }
+            const int t = 2 * c4 + e;
+            if (gq == 0 && (single ? t == pass : t < G)) {
+                const size_t row = row0 + (size_t)t * s.Nq;
+                delta[row] = a_pd[e];
+                if (slope_rows) slope_rows[row] = a_pd[e] * a_f[e] - a_pdf[e];
+            }
         }
+        __nv_bfloat16* orow = dq + mine + 2 * c4;
+        const bool own = single ? gq == pass : gq < G;
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) {
+            const uint32_t lo = movmatrix_trans(pack_bf16x2(acc[mt][0], acc[mt][1]));
+            const uint32_t hi = movmatrix_trans(pack_bf16x2(acc[mt][2], acc[mt][3]));
+            if (own) {
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+            }
+        }
+        if (!single || ++pass == G) break;
     }
 }
 
@@ -219,7 +234,8 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 // the part of a group that lies in one block's run: S = Q K^T and dP = dO V^T (entries as MMA rows,
 // the block's keys as columns), p and dX per (entry, key) where the mask has the key's bit, then
 // dv^T += dO^T P and dk^T += Q^T dX from the same rows, P and dX as bf16 values and their rests (Weights),
-// the sums fp32.
+// the sums fp32.  A group with a row that is not finite (its products with every key of the block are not)
+// is summed entry by entry instead: 0 times such a row must be 0 for the keys that it does not list.
 constexpr int kKeyWarps = 4;
 constexpr int kKeyWarpBytes = 4 * kStageChunk;  // q and dO rows of two groups
 constexpr int kKeyBytes = kKeyWarps * kKeyWarpBytes;
@@ -330,6 +346,7 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 mma_bf16_16816_a4(pacc, a[0], a[1], a[2], a[3], vf[2 * t + 8], vf[2 * t + 9]);
             }
             float p[2][2], w[2][2];
+            unsigned stray = 0u;  // entries (bit 4 e) whose products with every key of the block are not finite
 #pragma unroll
             for (int h = 0; h < 2; ++h) {  // entry gq + 8 h x keys 2 c4, 2 c4 + 1
                 const int e = gq + 8 * h;
@@ -350,19 +367,48 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     p[h][x] = on ? exp2_fast(s2 - l) : 0.f;
                     w[h][x] = on ? dx * p[h][x] * (pacc[2 * h + x] - d) : 0.f;
                 }
+                const float both = fminf(fabsf(sacc[2 * h] + pacc[2 * h]), fabsf(sacc[2 * h + 1] + pacc[2 * h + 1]));
+                const unsigned b4 = __ballot_sync(kFull, !(both < INFINITY));
+                stray |= b4 & b4 >> 1 & b4 >> 2 & b4 >> 3 & 0x11111111u;
             }
-            const Weights pt(p), wt(w);
+            if (stray == 0u) {  // warp-uniform
+                const Weights pt(p), wt(w);
 #pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                uint32_t a[4];
-                ldmatrix_x4_trans<kStageChunk>(a, qst + sl.at[mt]);
-                pt.mma(av[mt], a);
-                ldmatrix_x4_trans<0>(a, qst + sl.at[mt]);
-                wt.mma(ak[mt], a);
-                ldmatrix_x4_trans<kStageChunk + 128>(a, qst + sl.at[mt]);
-                pt.mma(av[mt + 4], a);
-                ldmatrix_x4_trans<128>(a, qst + sl.at[mt]);
-                wt.mma(ak[mt + 4], a);
+                for (int mt = 0; mt < 4; ++mt) {
+                    uint32_t a[4];
+                    ldmatrix_x4_trans<kStageChunk>(a, qst + sl.at[mt]);
+                    pt.mma(av[mt], a);
+                    ldmatrix_x4_trans<0>(a, qst + sl.at[mt]);
+                    wt.mma(ak[mt], a);
+                    ldmatrix_x4_trans<kStageChunk + 128>(a, qst + sl.at[mt]);
+                    pt.mma(av[mt + 4], a);
+                    ldmatrix_x4_trans<128>(a, qst + sl.at[mt]);
+                    wt.mma(ak[mt + 4], a);
+                }
+            } else {
+                const uint8_t* rows = msm + (size_t)warp * kKeyWarpBytes + buf * 2 * kStageChunk;
+#pragma unroll 1
+                for (int e = 0; e < kStageRows; ++e) {
+                    const float l = __shfl_sync(kFull, lse2, e);
+                    uint32_t mask = __shfl_sync(kFull, r, e) >> 24;
+                    if (pos + e < p0 || pos + e >= p1 || l == -INFINITY) mask = 0u;
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int from = (e & 7) * 4 + c4;  // the lane with this entry's weights
+                        const float pe = __shfl_sync(kFull, e < 8 ? p[0][x] : p[1][x], from);
+                        const float we = __shfl_sync(kFull, e < 8 ? w[0][x] : w[1][x], from);
+                        if (!((mask >> (2 * c4 + x)) & 1u)) continue;
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) {  // dim 8 n + gq
+                            const __nv_bfloat16* at = reinterpret_cast<const __nv_bfloat16*>(
+                                rows + e * kStageRow + ((n ^ (e & 7)) << 4)) + gq;
+                            float& k_sum = ak[n >> 1][2 * (n & 1) + x];
+                            float& v_sum = av[n >> 1][2 * (n & 1) + x];
+                            k_sum = fmaf(we, to_f32(at[0]), k_sum);
+                            v_sum = fmaf(pe, to_f32(at[kStageChunk / 2]), v_sum);
+                        }
+                    }
+                }
             }
             p0 = p1;
             if (p1 < run1 && p1 < t1) continue;  // the run goes on in the next group

@@ -91,3 +91,89 @@ def test_norms_off_boundaries(dtype, D):
         return (*[t.detach() for t in out], *grads, *torch.autograd.grad(rope, x, place(gq)))
 
     assert all(torch.equal(a, b) for a, b in zip(run(lambda t: t), run(_shifted)))
+
+
+def _bounds(q, k, D, K, dtype):
+    """(of the output, of a gradient) in the norm of a tensor: two and three roundings of the type."""
+    fine = score_step(q, k) + (K + D) * 2.0 ** -24
+    step = STEP if dtype == torch.bfloat16 else 0.0
+    return 2 * step + 8 * fine, 3 * step + 8 * fine
+
+
+@pytest.mark.parametrize("dtype,H,Hkv", [(torch.bfloat16, 6, 2), (torch.bfloat16, 8, 1), (torch.bfloat16, 2, 2),
+                                         (torch.bfloat16, 9, 1), (torch.float32, 4, 2)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("repeats", [False, True])
+def test_padding_that_is_not_finite(dtype, H, Hkv, bad, repeats):
+    """Behind the sequence lies padding, a segment of its own, whose rows hold anything; its first keys share a
+    block of 8 with the last real ones.  Real rows and keys get what they get without it."""
+    B, N, real, D, K = 1, 700, 687, 128, 32
+    g = _gen(11)
+    q, do = (torch.randn(B, H, N, D, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(B, Hkv, N, D, generator=g).to(dtype) for _ in range(2))
+    idx = torch.rand(B, H, N, N, generator=g).topk(K, dim=-1).indices
+    idx[:, :, real:, :3] = torch.tensor([real, real + 1, 5])  # padding lists padding (and what it does not see)
+    idx = idx.sort(dim=-1).values
+    if repeats:
+        idx[..., 1] = idx[..., 0]
+    seg = (torch.arange(N) >= real).int()
+    clean = [t[:, :, :real].double().requires_grad_() for t in (q, k, v)]
+    lists = torch.where(idx[:, :, :real] < real, idx[:, :, :real], -1)
+    ref = attention(*clean, lists, causal=False)[0]
+    want = torch.autograd.grad(ref, clean, do[:, :, :real].double())
+    for t in (q, k, v, do):
+        t[:, :, real:] = bad
+    dev = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = topk_attention(*dev, topk_indices=idx.to(DEV), causal=False, segments=seg.to(DEV))
+    got = torch.autograd.grad(out, dev, do.to(DEV))
+    of_out, of_grad = _bounds(q[:, :, :real], k[:, :, :real], D, K, dtype)
+    assert rel(out.detach().cpu()[:, :, :real], ref.detach()) <= of_out
+    for name, x, w in zip(("dq", "dk", "dv"), got, want):
+        assert rel(x.cpu()[:, :, :real], w) <= of_grad, name
+
+
+@pytest.mark.parametrize("H,N,K", [(3, 1400, 32), (8, 520, 32), (4, 13000, 8)])
+def test_a_key_that_one_head_lists_is_not_finite(H, N, K):
+    """The other heads of the group get what they get without it."""
+    B, D, key = 1, 128, 5
+    dtype = torch.bfloat16
+    g = _gen(13)
+    q, do = (torch.randn(B, H, N, D, generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(B, 1, N, D, generator=g).to(dtype) for _ in range(2))
+    idx = torch.randint(0, N, (B, H, N, K), generator=g).sort(dim=-1).values
+    idx[idx == key] = -1
+    ref_in = [t.double() for t in (q, k, v)]
+    ref_in[0].requires_grad_()
+    ref = attention(*ref_in, idx, causal=False)[0]
+    (want,) = torch.autograd.grad(ref, ref_in[:1], do.double())
+    of_out, of_grad = _bounds(q, k, D, K, dtype)
+    idx[:, 0, :, 3] = key
+    k[0, 0, key] = float("inf")
+    v[0, 0, key] = float("nan")
+    dev = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = topk_attention(*dev, topk_indices=idx.to(DEV), causal=False)
+    dq = torch.autograd.grad(out, dev, do.to(DEV))[0]
+    assert rel(out.detach().cpu()[:, 1:], ref.detach()[:, 1:]) <= of_out
+    assert rel(dq.cpu()[:, 1:], want[:, 1:]) <= of_grad
+
+
+@pytest.mark.parametrize("dtype,H,Hkv,D", [(torch.bfloat16, 6, 2, 128), (torch.float32, 2, 2, 64)])
+def test_lists_in_any_order(dtype, H, Hkv, D):
+    """Many entries of a row in one block of keys, in any order, repeats among them: the same gradients for
+    the same lists, to rounding for another order."""
+    B, N, K = 2, 300, 40
+    g = _gen(17)
+    q, do = (torch.randn(B, H, N, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    k, v = (torch.randn(B, Hkv, N, D, generator=g).to(dtype).to(DEV) for _ in range(2))
+    idx = torch.randint(-1, 48, (B, H, N, K), generator=g)
+
+    def run(i):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = topk_attention(*leaves, topk_indices=i.to(DEV), causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    first = run(idx)
+    assert all(torch.equal(a, b) for _ in range(3) for a, b in zip(first, run(idx)))
+    _, of_grad = _bounds(q.cpu(), k.cpu(), D, K, dtype)
+    for a, b in zip(first, run(idx.sort(dim=-1).values)):
+        assert rel(a, b) <= 2 * of_grad
