@@ -58,6 +58,16 @@ class PatchPlan:
     prefix_len: Union[torch.Tensor, int, None] = None        # (B,) or one int
 
 
+def _norms_as(norm, weight, eps):
+    """Whether the module is the norm that qk_norm_rope computes (others store their weight as an offset from 1)."""
+    with torch.no_grad():
+        x = torch.linspace(-1.0, 1.5, weight.numel(), device=weight.device, dtype=weight.dtype)
+        want = x.float() * torch.rsqrt(x.float().pow(2).mean() + eps) * weight.float()
+        got = norm(x.unsqueeze(0)).squeeze(0).float()
+        # as many roundings of its type as a norm may make; an offset shows far above them
+        return bool(((got - want).abs() <= 16 * torch.finfo(weight.dtype).eps * want.abs() + 1e-30).all())
+
+
 def _head_norms(layer_module):
     """(q weight, k weight, eps) of the layer's query and key head norms, None if it has none."""
     norms = [getattr(layer_module, name, None) for name in ("q_norm", "k_norm")]
@@ -72,6 +82,8 @@ def _head_norms(layer_module):
             raise TypeError("q_norm and k_norm must both be RMS norms over head_dim (weight and eps, no bias); "
                             f"got {type(norm).__name__}")
         eps.append(float(e))
+        if not _norms_as(norm, weight, float(e)):
+            raise TypeError(f"{type(norm).__name__} does not compute x * rsqrt(mean(x**2) + eps) * weight")
     if eps[0] != eps[1]:
         raise TypeError(f"q_norm and k_norm must have one eps, got {eps[0]} and {eps[1]}")
     return norms[0].weight, norms[1].weight, eps[0]
@@ -121,7 +133,7 @@ def _patch_layer(model, plan: PatchPlan):
         original_forward = layer_module.forward
         head_norms = _head_norms(layer_module)
 
-        def make_forward(layer_module=layer_module, captured_idx=layer_idx, normed=head_norms is not None):
+        def make_forward(layer_module=layer_module, captured_idx=layer_idx, eps=head_norms and head_norms[2]):
             def new_forward(hidden_states, attention_mask=None, position_ids=None,
                             past_key_values=None, output_attentions=False,
                             use_cache=False, cache_position=None,
@@ -135,8 +147,8 @@ def _patch_layer(model, plan: PatchPlan):
                 # pass per tensor (bit-identical to apply_rotary_pos_emb + contiguous)
                 cos, sin = position_embeddings if position_embeddings is not None else (None, None)
                 q, k = layer_module.q_proj(hidden_states), layer_module.k_proj(hidden_states)
-                if normed:
-                    wq, wk, eps = _head_norms(layer_module)
+                if eps is not None:
+                    wq, wk = layer_module.q_norm.weight, layer_module.k_norm.weight
                     q, k = qk_norm_rope(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps=eps)
                 else:
                     q = rope_to_heads(q, n_heads, cos, sin)

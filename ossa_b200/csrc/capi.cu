@@ -276,6 +276,9 @@ int ossa_topk_attention_fwd(const void* q, const void* k, const void* v, const v
                                         0, out, stream);
 }
 
+// Listed keys of one kv head that the backward's turned lists hold (32-bit places).
+static constexpr long long kMaxTurned = 1ll << 30;
+
 // The checks that the modified gather and its backward share.
 static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, int idx_is_64, float scale,
                           int q_start, float softcap, const int32_t* segments) {
@@ -328,6 +331,7 @@ int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, con
 size_t ossa_topk_attention_bwd_workspace_size(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K,
                                               int want_dslopes) {
     if (!valid_dtype(dtype) || B < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || Nq < 0 || Nk < 0 || D <= 0 || K < 0) return 0;
+    if ((long long)(H / Hkv) * Nq * K > kMaxTurned) return 0;  // refused by the backward call
     return ossa::gather_bwd_workspace_bytes(dtype, B, H, Hkv, Nq, Nk, D, K, want_dslopes != 0);
 }
 
@@ -339,7 +343,7 @@ int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const v
     int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
     if (st) return st;
     if (dslopes && !slopes) return fail(OSSA_ERR_INVALID, "dslopes without slopes");
-    if ((long long)(H / Hkv) * Nq * K > (1ll << 30))
+    if ((long long)(H / Hkv) * Nq * K > kMaxTurned)
         return fail(OSSA_ERR_UNSUPPORTED, "(H / Hkv) * Nq * K = %lld > 2^30 listed keys per kv head",
                     (long long)(H / Hkv) * Nq * K);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -167,3 +167,30 @@ def test_distillation_loss_refusals(kw, err):
     a.update(kw)
     with pytest.raises(err):
         top_logit_distillation_loss(**a)
+
+
+def test_patching_refuses_other_norms():
+    """A norm that stores its weight as an offset from 1 is not the one that the patched layer computes."""
+    from types import SimpleNamespace
+
+    from ossa_b200.bench.sparse_forward import _head_norms
+
+    class Norm(torch.nn.Module):
+        def __init__(self, offset, dtype):
+            super().__init__()
+            self.offset, self.eps = offset, 1e-6
+            self.weight = torch.nn.Parameter((0.9 + 0.2 * torch.rand(64, generator=torch.Generator().manual_seed(1))).to(dtype))
+
+        def forward(self, x):
+            return x * torch.rsqrt(x.square().mean(-1, keepdim=True) + self.eps) * (self.offset + self.weight)
+
+    for dtype in (torch.float32, torch.bfloat16):
+        good, other = Norm(0.0, dtype), Norm(1.0, dtype)
+        wq, wk, eps = _head_norms(SimpleNamespace(q_norm=good, k_norm=good, head_dim=64))
+        assert wq is good.weight and wk is good.weight and eps == 1e-6
+        with pytest.raises(TypeError):
+            _head_norms(SimpleNamespace(q_norm=good, k_norm=other, head_dim=64))
+
+
+def test_the_backward_workspace_of_refused_sizes():
+    assert _lib.lib().ossa_topk_attention_bwd_workspace_size(BF, 1, 4, 2, 1 << 20, 1 << 20, 128, 1024, 0) == 0
