@@ -177,3 +177,78 @@ def test_lists_in_any_order(dtype, H, Hkv, D):
     _, of_grad = _bounds(q.cpu(), k.cpu(), D, K, dtype)
     for a, b in zip(first, run(idx.sort(dim=-1).values)):
         assert rel(a, b) <= 2 * of_grad
+
+
+def test_attention_far_into_a_long_cache():
+    """Key rows more than 2^31 elements behind the first: the last 64 keys of every head, against a cache of
+    those alone.  Nothing else is written before or listed."""
+    B, H, Hkv, N, D, K, near = 2, 4, 2, 4_200_003, 128, 24, 64
+    assert B * Hkv * N * D > 2 ** 31
+    g = _gen(19)
+    for Nq in (1, 300):
+        q, do = (torch.randn(B, H, Nq, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+        small = [torch.randn(B, Hkv, near, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2)]
+        k, v = (torch.empty(B, Hkv, N, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        for far, t in zip((k, v), small):
+            far[:, :, N - near:] = t
+        idx = torch.randint(0, near, (B, H, Nq, K), generator=g).to(DEV)
+        res = []
+        for (kk, vv), off in ((small, 0), ((k, v), N - near)):
+            leaves = [t.detach().requires_grad_() for t in (q, kk, vv)]
+            out = topk_attention(*leaves, topk_indices=idx + off, causal=False, q_start=off, softcap=5.0)
+            dq, dk, dv = torch.autograd.grad(out, leaves, do)
+            if off:
+                assert not dk[:, :, :off].any() and not dv[:, :, :off].any()
+                dk, dv = dk[:, :, off:].clone(), dv[:, :, off:].clone()
+            res.append((out.detach(), dq, dk, dv))
+            del leaves, out
+        del k, v
+        _, of_grad = _bounds(q.cpu(), small[0].cpu(), D, K, torch.bfloat16)
+        for a, b in zip(*res):  # other blocks of keys, other tiles: equal to rounding
+            assert rel(a, b) <= 2 * of_grad
+
+
+def test_distillation_of_many_rows():
+    """Rows more than 2^31 logits behind the first; those before weigh nothing and are not read."""
+    T, V, K, near = 16_500, 131_072, 9, 5
+    assert (T - near) * V > 2 ** 31
+    g = _gen(23)
+    z = torch.empty(T, V, dtype=torch.bfloat16, device=DEV)
+    z[T - near:] = (torch.randn(near, V, generator=g) * 2).to(DEV)
+    ids = torch.randint(0, V, (T, K), generator=g).to(DEV)
+    teacher = torch.randn(T, K, generator=g).to(DEV)
+    weight = torch.zeros(T, device=DEV)
+    weight[T - near:] = 1.0
+    z.requires_grad_()
+    loss = top_logit_distillation_loss(z, teacher, ids, row_weight=weight)
+    (dz,) = torch.autograd.grad(loss, z)
+    part = z.detach()[T - near:].clone().requires_grad_()
+    small = top_logit_distillation_loss(part, teacher[T - near:], ids[T - near:])
+    (want,) = torch.autograd.grad(small, part)
+    # few rows are split over more thread blocks: the sums in another order
+    assert abs(loss.item() - small.item()) <= 2.0 ** -16 * abs(small.item())
+    assert rel(dz[T - near:], want) <= 2.0 ** -8 + 2.0 ** -16
+    assert not dz[:T - near].any()
+
+
+def test_norms_of_many_rows():
+    """Tokens more than 2^31 elements behind the first, bit for bit as in a call of their own."""
+    N, Hq, Hk, D, near = 1_400_000, 12, 2, 128, 37
+    assert (N - near) * Hq * D > 2 ** 31
+    g = _gen(29)
+    q, k = (torch.empty(1, N, h, D, dtype=torch.bfloat16, device=DEV) for h in (Hq, Hk))
+    cos, sin = (torch.empty(1, N, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for t in (q, k, cos, sin):
+        t[:, N - near:] = torch.randn(t[:, N - near:].shape, generator=g).to(DEV)
+    wq, wk = (torch.rand(D, generator=g).to(DEV) + 0.5 for _ in range(2))
+    gq, gk = (torch.empty(1, h, N, D, dtype=torch.bfloat16, device=DEV) for h in (Hq, Hk))
+    for t in (gq, gk):
+        t[:, :, N - near:] = torch.randn(t[:, :, N - near:].shape, generator=g).to(DEV)
+    res = []
+    for n0 in (N - near, 0):
+        leaves = [t[:, n0:].clone().requires_grad_() for t in (q, k)]
+        out = qk_norm_rope(*leaves, Hq, Hk, wq, wk, cos[:, n0:], sin[:, n0:])
+        grads = torch.autograd.grad(out, leaves, (gq[:, :, n0:], gk[:, :, n0:]))
+        res.append([t.detach()[:, :, -near:].clone() for t in out] + [t[:, -near:].clone() for t in grads])
+        del leaves, out, grads
+    assert all(torch.equal(a, b) for a, b in zip(*res))
