@@ -8,6 +8,7 @@ point raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 
 import torch
@@ -161,6 +162,25 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The trainable operators' autograd nodes (csrc/autograd.cpp), built on first use when missing or out of date."""
+    global _native
+    if _native is not None:
+        return _native
+    lib()
+    with _lock:
+        if _native is None:
+            path = _build.build_autograd()
+            spec = importlib.util.spec_from_file_location("ossa_b200._autograd", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            _native = module
+    return _native
+
+
 def check(status: int) -> None:
     if status != OSSA_OK:
         msg = lib().ossa_last_error_string().decode(errors="replace")
@@ -190,32 +210,6 @@ def stream_ptr(device: torch.device) -> int:
     """The device's current stream (the raw handle: no Stream object is made)."""
     index = torch.cuda.current_device() if device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)
-
-
-class _Here:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
-
-
-_here = _Here()
-
-
-def on_device(device: torch.device):
-    """torch.cuda.device(device), without its cost where the device is current already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _here
-    return torch.cuda.device(device)
-
-
-def packed(t: torch.Tensor) -> torch.Tensor:
-    """t contiguous and on a 16-byte boundary: itself, or a copy (a gradient may be a piece of a larger one)."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -1,16 +1,18 @@
-"""Builds libossa_b200.so (the sm_100a kernels behind the C ABI) in-tree.
+"""Builds libossa_b200.so (the sm_100a kernels behind the C ABI) and _autograd.so (the trainable
+operators' autograd nodes, over that library and torch's) in-tree.
 
-Run ``python -m ossa_b200.build`` or call :func:`build`.  The library is
-written next to this file so that it travels with the source tree; nothing is
-installed into site-packages and no JIT cache is used.
+Run ``python -m ossa_b200.build`` or call :func:`build`.  Both are written next to this file so
+that they travel with the source tree; nothing is installed into site-packages and no JIT cache is used.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,6 +21,8 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libossa_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
+AUTOGRAD_SRC = CSRC / "autograd.cpp"
+AUTOGRAD_PATH = PKG_DIR / "_autograd.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -46,6 +50,13 @@ def _inputs() -> list[Path]:
     return sources() + sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
 
 
+def autograd_is_stale() -> bool:
+    if not AUTOGRAD_PATH.exists():
+        return True
+    built = AUTOGRAD_PATH.stat().st_mtime
+    return any(p.stat().st_mtime > built for p in (AUTOGRAD_SRC, INCLUDE / "ossa_b200.h"))
+
+
 def is_stale() -> bool:
     if not LIB_PATH.exists():
         return True
@@ -53,8 +64,35 @@ def is_stale() -> bool:
     return any(p.stat().st_mtime > built for p in _inputs())
 
 
+def build_autograd(force: bool = False, verbose: bool = False) -> Path:
+    """Compiles ``csrc/autograd.cpp`` against torch's headers and links ``_autograd.so`` to the library."""
+    if not force and not autograd_is_stale():
+        return AUTOGRAD_PATH
+    torch_dir = Path(importlib.util.find_spec("torch").origin).parent
+    inc, nvcc = torch_dir / "include", Path(_nvcc()).resolve()
+    tmp = AUTOGRAD_PATH.with_suffix(f".{os.getpid()}.tmp")
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{INCLUDE}",
+           "-isystem", str(inc), "-isystem", str(inc / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(nvcc.parent.parent / "include"),
+           str(AUTOGRAD_SRC), "-o", str(tmp), f"-L{PKG_DIR}", "-lossa_b200", "-Wl,-rpath,$ORIGIN",
+           f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
+    if res.returncode != 0:
+        raise RuntimeError("autograd.cpp failed:\n" + res.stdout.decode(errors="replace"))
+    os.replace(tmp, AUTOGRAD_PATH)
+    return AUTOGRAD_PATH
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compiles every ``csrc/*.cu`` for sm_100a and links ``libossa_b200.so``."""
+    """Compiles every ``csrc/*.cu`` for sm_100a, links ``libossa_b200.so`` and builds ``_autograd.so`` on it."""
+    _build_library(force, verbose)
+    build_autograd(force, verbose)
+    return LIB_PATH
+
+
+def _build_library(force: bool, verbose: bool) -> Path:
     if not force and not is_stale():
         return LIB_PATH
     nvcc = _nvcc()

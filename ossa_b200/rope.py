@@ -9,7 +9,7 @@ bit-identical to it.  Additive: the reference runs the eager ops.
 
 ``qk_norm_rope`` serves layers that norm every query and key head before the rotation:
 norm, rotation and head transpose of both tensors in one kernel pass.  Both functions are
-differentiable (one backward kernel, ``ossa_qk_norm_rope_bwd``).
+differentiable (csrc/autograd.cpp; one backward kernel, ``ossa_qk_norm_rope_bwd``).
 """
 
 from __future__ import annotations
@@ -26,13 +26,7 @@ def rope_to_heads(x: torch.Tensor, n_heads: int, cos: Optional[torch.Tensor] = N
     """x: (B, N, n_heads * D) or (B, N, n_heads, D); cos, sin: (B or 1, N, D)
     (Qwen2's position embeddings) or both None (layout only).  Returns the
     contiguous (B, n_heads, N, D) tensor, rotated when cos/sin are given.
-    Differentiable in x (head dims up to 512), not in cos and sin."""
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _RopeToHeads.apply(x, n_heads, cos, sin)
-    return _rope_to_heads(x, n_heads, cos, sin)
-
-
-def _rope_to_heads(x, n_heads, cos, sin):
+    Differentiable in x (head dims up to 512), once, not in cos and sin."""
     if (cos is None) != (sin is None):
         raise ValueError("pass both cos and sin, or neither")
     B, N = x.shape[0], x.shape[1]
@@ -52,6 +46,8 @@ def _rope_to_heads(x, n_heads, cos, sin):
         if cos.shape != sin.shape or cos.shape[0] not in (1, B) or tuple(cos.shape[1:]) != (N, D):
             raise ValueError(f"cos/sin of shape {tuple(cos.shape)} do not match (B or 1, {N}, {D})")
         cs = (cos.contiguous(), sin.contiguous())
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _lib.native().rope_to_heads(x, *([t.detach() for t in cs] if cs else (None, None)), n_heads)
     out = torch.empty((B, n_heads, N, D), dtype=xc.dtype, device=dev)
     if out.numel() == 0:
         return out
@@ -64,32 +60,8 @@ def _rope_to_heads(x, n_heads, cos, sin):
     return out
 
 
-class _RopeToHeads(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, n_heads, cos, sin):
-        out = _rope_to_heads(x.detach(), n_heads, cos, sin)
-        ctx.shape = x.shape
-        if cos is not None:
-            cos, sin = _tables(cos, sin, out.shape[0], out.shape[2], out.shape[3], out.dtype)
-        ctx.save_for_backward(cos, sin)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        cos, sin = ctx.saved_tensors
-        g = _lib.packed(g)
-        B, H, N, D = g.shape
-        dx = g.new_empty(ctx.shape)
-        args = (None, None, None, None, _lib.ptr(cos), _lib.ptr(sin),
-                1 if cos is not None and B > 1 and cos.shape[0] == B else 0, _lib.dtype_code(g), _lib.OSSA_F32, B, N, H, 0,
-                D, 0, 0, 0, 0, 0.0)
-        _norm_rope_backward(args, g, None, dx, None, None, None)
-        return dx, None, None, None
-
-
 def _tables(cos, sin, B, N, D, dtype):
-    """cos, sin as the kernels read them: contiguous (B or 1, N, D) of the rows' type."""
+    """cos, sin as (B or 1, N, D) of the rows' type."""
     if cos.requires_grad or sin.requires_grad:
         cos, sin = cos.detach(), sin.detach()
     if cos.dtype != dtype or sin.dtype != dtype:
@@ -98,108 +70,7 @@ def _tables(cos, sin, B, N, D, dtype):
         cos, sin = cos.unsqueeze(0), sin.unsqueeze(0)
     if cos.shape != sin.shape or cos.dim() != 3 or cos.shape[0] not in (1, B) or tuple(cos.shape[1:]) != (N, D):
         raise ValueError(f"cos/sin of shapes {tuple(cos.shape)}, {tuple(sin.shape)} do not match (B or 1, {N}, {D})")
-    return _lib.packed(cos), _lib.packed(sin)
-
-
-def _rows(x, heads, name):
-    """(x, B, N, D, batch stride, row stride): x as it is where each (b, n) row of its heads lies in
-    one piece on a 16-byte boundary, else a contiguous copy."""
-    if x.dim() == 3 and heads > 0 and x.shape[2] % heads == 0:
-        D = x.shape[2] // heads
-    elif x.dim() == 4 and x.shape[2] == heads:
-        D = x.shape[3]
-    else:
-        raise ValueError(f"{name} of shape {tuple(x.shape)} is not (B, N, {heads} heads x D) or (B, N, {heads}, D)")
-    B, N = x.shape[:2]
-    if x.is_contiguous():
-        sn, sb, whole = heads * D, N * heads * D, True
-    else:
-        sb, sn = x.stride()[:2]
-        whole = x.stride(-1) == 1 and (x.dim() == 3 or heads == 1 or x.stride(2) == D)
-        sb, sn = (sb if B > 1 else 0), (sn if N > 1 else 0)
-    if not whole or sb * x.element_size() % 16 or sn * x.element_size() % 16 or x.data_ptr() % 16:
-        x = _lib.packed(x)
-        sn, sb = heads * D, N * heads * D
-    return x, B, N, D, sb, sn
-
-
-def _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps):
-    """(the arguments that the C forward and backward begin with, the tensors they point into)."""
-    q, B, N, D, *qs = _rows(q, n_heads, "q")
-    k, _, _, _, *ks = _rows(k, n_kv_heads, "k")
-    w = wq if wq is not None else wk
-    args = (q.data_ptr(), k.data_ptr(), _lib.ptr(wq), _lib.ptr(wk), _lib.ptr(cos), _lib.ptr(sin),
-            1 if cos is not None and B > 1 and cos.shape[0] == B else 0, _lib.dtype_code(q),
-            _lib.OSSA_F32 if w is None else _lib.dtype_code(w), B, N, n_heads, n_kv_heads, D, *qs, *ks, eps)
-    return args, (q, k, wq, wk, cos, sin)
-
-
-def _norm_rope_forward(args, like):
-    dev = like.device
-    B, N, Hq, Hk, D = args[9:14]
-    q_out = like.new_empty((B, Hq, N, D))
-    k_out = like.new_empty((B, Hk, N, D))
-    if B * N > 0:
-        with _lib.on_device(dev):
-            st = _lib.lib().ossa_qk_norm_rope_fwd(*args, q_out.data_ptr(), k_out.data_ptr(), _lib.stream_ptr(dev))
-        if st:
-            _lib.check(st)
-    return q_out, k_out
-
-
-def _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk):
-    """Writes the gradients from those of the (B, Hx, N, D) outputs."""
-    dev = gq.device
-    L = _lib.lib()
-    with _lib.on_device(dev):
-        ws, ws_bytes = None, 0
-        if args[2] is not None or args[3] is not None:
-            ws_bytes = L.ossa_qk_norm_rope_bwd_workspace_size(args[13])
-            ws = gq.new_empty(ws_bytes, dtype=torch.uint8)
-        st = L.ossa_qk_norm_rope_bwd(*args, gq.data_ptr(), _lib.ptr(gk), dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dwq),
-                                     _lib.ptr(dwk), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
-    if st:
-        _lib.check(st)
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, n_heads, n_kv_heads, cos, sin, eps):
-        ctx.save_for_backward(q, k, wq, wk, cos, sin)
-        ctx.rule = (n_heads, n_kv_heads, eps)
-        ctx.set_materialize_grads(False)
-        args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
-        return _norm_rope_forward(args, q)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        if gq is None and gk is None:
-            return (None,) * 9
-        # saved tensors may come back as others than were saved (checkpointing, offloading): their
-        # places and strides are taken anew
-        q, k, wq, wk, cos, sin = ctx.saved_tensors
-        n_heads, n_kv_heads, eps = ctx.rule
-        args, _kept = _call_args(q, k, n_heads, n_kv_heads, wq, wk, cos, sin, eps)
-        need = ctx.needs_input_grad
-        dq = dk = dwq = dwk = None
-        if gq is not None:
-            gq = _lib.packed(gq)
-            dq = gq.new_empty(q.shape)
-            dwq = torch.empty_like(wq) if need[2] else None
-        if gk is not None:
-            gk = _lib.packed(gk)
-            dk = gk.new_empty(k.shape)
-            dwk = torch.empty_like(wk) if need[3] else None
-        if gk is None:  # one output has no gradient: the other tensor alone, in the place of the queries
-            args = args[:1] + (None, args[2], None) + args[4:12] + (0,) + args[13:]
-            _norm_rope_backward(args, gq, None, dq, None, dwq, None)
-        elif gq is None:
-            args = (args[1], None, args[3], None) + args[4:11] + (args[12], 0, args[13], args[16], args[17]) + args[16:]
-            _norm_rope_backward(args, gk, None, dk, None, dwk, None)
-        else:
-            _norm_rope_backward(args, gq, gk, dq, dk, dwq, dwk)
-        return dq, dk, dwq, dwk, None, None, None, None, None
+    return cos, sin
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int,
@@ -246,7 +117,5 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, n_heads: int, n_kv_heads: int
     _lib.require_cuda(*[t for t in (q, k, q_weight, k_weight, cos, sin) if t is not None])
     if cos is not None:
         cos, sin = _tables(cos, sin, q.shape[0], q.shape[1], D, q.dtype)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, n_heads, n_kv_heads, cos, sin, eps)
-    args, _kept = _call_args(q, k, n_heads, n_kv_heads, q_weight, k_weight, cos, sin, eps)
-    return _norm_rope_forward(args, q)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    return _lib.native().qk_norm_rope(q, k, q_weight, k_weight, cos, sin, n_heads, n_kv_heads, eps, grad)

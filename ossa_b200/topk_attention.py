@@ -16,7 +16,7 @@ are rejected.  Differences, all additive:
   with distance), ``segments`` (documents packed in one row) and ``prefix_len`` (keys
   that every query may see).
 * (additive) gradients: where q, k, v or slopes require them, the output carries
-  autograd history (``ossa_topk_attention_bwd``); the forward's values are then the
+  autograd history (csrc/autograd.cpp, ``ossa_topk_attention_bwd``); the forward's values are then the
   same to rounding (a bf16 output sums its keys in another order).
 """
 
@@ -174,58 +174,4 @@ def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, seg
         prefix_len = _int32("prefix_len", prefix_len, [(B,)]).contiguous()
     _lib.dtype_code(q)
     _lib.require_cuda(*[t for t in (q, k, v, idx, slopes, segments, prefix_len) if t is not None])
-    if grad:
-        return _TopkAttention.apply(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
-    q, k, v, idx = _lib.packed(q), _lib.packed(k), _lib.packed(v), idx.contiguous()
-    return _mod_forward(_mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap), q, None)
-
-
-def _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
-    """The arguments that the C forward and backward begin with."""
-    B, H, Nq, D = q.shape
-    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), idx.data_ptr(), 1 if idx.dtype == torch.int64 else 0,
-            _lib.dtype_code(q), B, H, k.shape[1], Nq, k.shape[2], D, idx.shape[-1], 1.0 / math.sqrt(D),
-            1 if causal else 0, q0, cap, _lib.ptr(slopes), _lib.ptr(segments), _lib.ptr(prefix_len))
-
-
-def _mod_forward(args, q, lse2):
-    out = torch.empty_like(q)
-    if out.numel() == 0:
-        return out
-    with _lib.on_device(q.device):
-        st = _lib.lib().ossa_topk_attention_mod_fwd(*args, out.data_ptr(), _lib.ptr(lse2), _lib.stream_ptr(q.device))
-    if st:
-        _lib.check(st)
-    return out
-
-
-class _TopkAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap):
-        q, k, v, idx = _lib.packed(q), _lib.packed(k), _lib.packed(v), idx.contiguous()
-        lse2 = q.new_empty(q.shape[:3], dtype=torch.float32)
-        args = _mod_args(q, k, v, slopes, idx, segments, prefix_len, causal, q0, cap)
-        out = _mod_forward(args, q, lse2)
-        ctx.save_for_backward(q, k, v, slopes, idx, segments, prefix_len, out, lse2)
-        ctx.rule = (causal, q0, cap)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        # saved tensors may come back as others than were saved (checkpointing, offloading)
-        q, k, v, slopes, idx, segments, prefix_len, out, lse2 = ctx.saved_tensors
-        args, dev = _mod_args(q, k, v, slopes, idx, segments, prefix_len, *ctx.rule), q.device
-        dout = _lib.packed(dout)
-        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        dslopes = torch.empty_like(slopes) if ctx.needs_input_grad[3] else None
-        L = _lib.lib()
-        with _lib.on_device(dev):
-            ws_bytes = L.ossa_topk_attention_bwd_workspace_size(*args[5:13], 0 if dslopes is None else 1)
-            ws = q.new_empty(ws_bytes, dtype=torch.uint8)
-            st = L.ossa_topk_attention_bwd(
-                *args, out.data_ptr(), lse2.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                _lib.ptr(dslopes), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
-        if st:
-            _lib.check(st)
-        return dq, dk, dv, dslopes, None, None, None, None, None, None
+    return _lib.native().topk_attention(q, k, v, slopes, idx, segments, prefix_len, bool(causal), q0, cap, grad)

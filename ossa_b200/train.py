@@ -104,66 +104,6 @@ def distillation_loss(router, q: torch.Tensor, k: torch.Tensor, top_k: int, *,
     return _DistillFn.apply(wq, wk, pb, q, k, targets, router.cfg.seq_len)
 
 
-def _logit_rows(z):
-    """(what the C calls take of the logits first, z): rows where they lie; z is 2-D or 3-D."""
-    if z.stride(-1) != 1:
-        z = z.contiguous()
-    if z.dim() == 2:
-        outer, inner, so, si = 1, z.shape[0], 0, z.stride(0)
-    else:
-        outer, inner, so, si = z.shape[0], z.shape[1], z.stride(0), z.stride(1)
-    return (z.data_ptr(), _lib.dtype_code(z), outer, inner, z.shape[-1], so, si), z
-
-
-class _TopLogitDistill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, z, teacher, ids, weight, tau, reduction, grad):
-        K, dev = ids.shape[-1], z.device
-        where, z = _logit_rows(z)
-        rows = where[2] * where[3]
-        L = _lib.lib()
-        ws_bytes = L.ossa_top_logit_distill_workspace_size(rows, K)
-        ws = z.new_empty(ws_bytes, dtype=torch.uint8)
-        mean = 1 if reduction == "mean" else 0
-        each = reduction == "none"
-        loss = z.new_empty(rows if each else (), dtype=torch.float32)
-        # a single incoming gradient is 1 as a rule: the gradient is taken with the loss
-        dz = z.new_empty((rows, z.shape[-1])) if grad and not each else None
-        with _lib.on_device(dev):
-            st = L.ossa_top_logit_distill_fwd(
-                *where, teacher.data_ptr(), ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, K, tau,
-                _lib.ptr(weight), mean, loss.data_ptr() if each else None, None if each else loss.data_ptr(),
-                _lib.ptr(dz), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
-        _lib.check(st)
-        if grad:
-            ctx.save_for_backward(z, ids)
-            ctx.kept = (ws, ws_bytes, dz)
-            ctx.rule = (tau, mean, each)
-        if each and weight is not None:
-            loss.mul_(weight)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        z, ids = ctx.saved_tensors
-        ws, ws_bytes, dz = ctx.kept
-        tau, mean, each = ctx.rule
-        # the saved logits may come back in another place and layout (offloading): rows are taken anew
-        where, z = _logit_rows(z)
-        ctx.kept = (ws, ws_bytes, None)  # a second backward pass makes its own
-        taken = dz is not None
-        if not taken:
-            dz = z.new_empty((where[2] * where[3], z.shape[-1]))
-        g = g.contiguous()  # fp32, as the loss
-        with _lib.on_device(z.device):
-            st = _lib.lib().ossa_top_logit_distill_bwd(
-                *where, ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, ids.shape[-1], tau, mean, g.data_ptr(),
-                1 if each else 0, 1 if taken else 0, dz.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(z.device))
-        _lib.check(st)
-        return dz.view(z.shape), None, None, None, None, None, None
-
-
 def top_logit_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_indices: torch.Tensor, *,
                                 temperature: float = 1.0, row_weight: Optional[torch.Tensor] = None,
                                 reduction: str = "mean") -> torch.Tensor:
@@ -213,6 +153,6 @@ def top_logit_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tens
     teacher = teacher_logits.detach().float().reshape(-1, K).contiguous()
     ids = teacher_indices.reshape(-1, K).contiguous()
     weight = None if row_weight is None else row_weight.detach().float().reshape(-1).contiguous()
-    loss = _TopLogitDistill.apply(z, teacher, ids, weight, tau, reduction,
-                                  torch.is_grad_enabled() and z.requires_grad)
+    loss = _lib.native().top_logit_distill(z, teacher, ids, weight, tau, ("none", "sum", "mean").index(reduction),
+                                           torch.is_grad_enabled() and z.requires_grad)
     return loss.view(lead) if reduction == "none" else loss
