@@ -4,7 +4,7 @@
 //
 // Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 146 us, of
 // which 57 us for the rows' q, dO, output and lists and the union of keys (144 of 384 on average), key pass
-// 174 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
+// 181 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
 // (8 KB in, 16 KB out as operands): 5.4 GB, 155 us at 128 bytes a cycle and SM, which is what bounds it; the
 // per-head forms of gather_bwd.cu took 752 and 1147 us here.
 #include <algorithm>

@@ -252,3 +252,56 @@ def test_norms_of_many_rows():
         res.append([t.detach()[:, :, -near:].clone() for t in out] + [t[:, -near:].clone() for t in grads])
         del leaves, out, grads
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+def test_differentiable_once():
+    """A second derivative is refused, not taken for zero."""
+    g = _gen(31)
+    q = torch.randn(1, 2, 20, 64, generator=g).to(DEV).requires_grad_()
+    idx = torch.randint(0, 20, (1, 2, 20, 4), generator=g).to(DEV)
+    x = torch.randn(1, 5, 2 * 64, generator=g).to(DEV).requires_grad_()
+    z = torch.randn(6, 50, generator=g).to(DEV).requires_grad_()
+    ids = torch.rand(6, 50, generator=g).topk(3, dim=-1).indices.to(DEV)
+    t = torch.randn(6, 3, generator=g).to(DEV)
+    w = torch.rand(64, generator=g).to(DEV)
+    calls = [(q, lambda: topk_attention(q, q, q, topk_indices=idx)),
+             (x, lambda: qk_norm_rope(x, x, 2, 2, w, w)[0]),
+             (x, lambda: rope_to_heads(x, 2)),
+             (z, lambda: top_logit_distillation_loss(z, t, ids))]
+    for leaf, call in calls:
+        out = call()
+        up = torch.ones_like(out).requires_grad_()
+        (first,) = torch.autograd.grad(out, leaf, up, create_graph=True)
+        (plain,) = torch.autograd.grad(call(), leaf, torch.ones_like(out))
+        assert torch.equal(first.detach(), plain)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            first.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_of_the_norm_weights(dtype):
+    """Each weight without the other, each wanted or not: its gradient is the one that both have together."""
+    B, N, Hq, Hk, D = 2, 9, 3, 2, 64
+    g = _gen(37)
+    q, k = (torch.randn(B, N, h * D, generator=g).to(dtype).to(DEV) for h in (Hq, Hk))
+    gq, gk = (torch.randn(B, h, N, D, generator=g).to(dtype).to(DEV) for h in (Hq, Hk))
+    wq, wk = (torch.rand(D, generator=g).to(DEV) + 0.5 for _ in range(2))
+
+    def grads(uq, uk, want):
+        out = qk_norm_rope(q, k, Hq, Hk, uq, uk)
+        return torch.autograd.grad(out, want, (gq, gk))
+
+    a, b = wq.clone().requires_grad_(), wk.clone().requires_grad_()
+    dq, dk = grads(a, b, [a, b])
+    for got, want in ((grads(a, None, [a]), dq), (grads(None, b, [b]), dk), (grads(a, wk, [a]), dq), (grads(wq, b, [b]), dk)):
+        assert rel(got[0], want) <= 2.0 ** -18  # the rows of one tensor may go to more thread blocks
+
+
+def test_errors_keep_their_type():
+    from ossa_b200._lib import OSSA_ERR_UNSUPPORTED, OssaError
+
+    q = torch.zeros(1, 1, 4, 96, device=DEV, requires_grad=True)
+    idx = torch.zeros(1, 1, 4, 2, dtype=torch.int32, device=DEV)
+    with pytest.raises(OssaError, match="head_dim") as e:
+        topk_attention(q, q, q, topk_indices=idx)
+    assert e.value.status == OSSA_ERR_UNSUPPORTED
