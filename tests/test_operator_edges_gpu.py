@@ -305,3 +305,86 @@ def test_errors_keep_their_type():
     with pytest.raises(OssaError, match="head_dim") as e:
         topk_attention(q, q, q, topk_indices=idx)
     assert e.value.status == OSSA_ERR_UNSUPPORTED
+
+
+def _all_calls(dtype=torch.bfloat16):
+    g = _gen(41)
+    x = torch.randn(2, 30, 4 * 128, generator=g).to(dtype).to(DEV)
+    y = torch.randn(2, 30, 2 * 128, generator=g).to(dtype).to(DEV)
+    w = (torch.rand(128, generator=g) + 0.5).to(DEV)
+    cs = [torch.randn(1, 30, 128, generator=g).to(dtype).to(DEV) for _ in range(2)]
+    idx = torch.randint(-1, 30, (2, 4, 30, 7), generator=g).to(DEV)
+    seg = (torch.arange(30) // 9).int().to(DEV)
+    z = torch.randn(2, 30, 77, generator=g).to(dtype).to(DEV)
+    ids = torch.rand(2, 30, 77, generator=g).topk(5, dim=-1).indices.to(DEV)
+    t = torch.randn(2, 30, 5, generator=g).to(DEV)
+
+    def attend(a, b, c):
+        q, k = qk_norm_rope(a, b, 4, 2, w, w, *cs)
+        return topk_attention(q, k, rope_to_heads(b, 2), topk_indices=idx, segments=seg, softcap=5.0), c
+
+    return (x, y, z), lambda a, b, c: (attend(a, b, c)[0], top_logit_distillation_loss(c, t, ids, temperature=2.0))
+
+
+def test_inference_mode():
+    """In inference mode, and without gradients on tensors made there, the calls give what they give without it."""
+    leaves, call = _all_calls()
+    with torch.no_grad():
+        want = call(*leaves)
+    with torch.inference_mode():
+        inner = [t.clone() for t in leaves]
+        assert all(torch.equal(a, b) for a, b in zip(want, call(*inner)))
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(want, call(*inner)))
+    assert not any(t.requires_grad for t in call(*leaves))
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_nothing_stays_behind(backward):
+    """Calls whose results are dropped, with or without their backward pass, leave no memory held."""
+    leaves, call = _all_calls()
+    leaves = [t.requires_grad_() for t in leaves]
+
+    def step():
+        out, loss = call(*leaves)
+        if backward:
+            torch.autograd.grad(out.float().sum() + loss, leaves)
+
+    for _ in range(3):
+        step()
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    for _ in range(20):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == held
+
+
+def test_from_several_threads():
+    """Two threads on streams of their own, each with its leaves: what each gets alone."""
+    import threading
+
+    leaves, call = _all_calls()
+
+    def grads():
+        own = [t.detach().clone().requires_grad_() for t in leaves]
+        out, loss = call(*own)
+        return torch.autograd.grad(out.float().sum() + loss, own)
+
+    want = grads()
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(n):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                got[n] = grads()
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for n in range(2) for a, b in zip(want, got[n]))
