@@ -46,6 +46,12 @@ struct On {
     explicit On(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
 };
 
+// A size as the C ABI takes it.
+int i32(int64_t n) {
+    TORCH_CHECK_VALUE(n <= INT32_MAX, "a size of ", n, " exceeds 32 bits");
+    return (int)n;
+}
+
 const void* in(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* to(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 template <typename T>
@@ -116,7 +122,7 @@ int batched(const Tensor& cos, int64_t B) { return cos.defined() && B > 1 && cos
 void norm_rope_backward(const Rows& q, const Rows& k, const Tensor& wq, const Tensor& wk, const Tensor& cos,
                         const Tensor& sin, double eps, const Tensor& gq, const Tensor& gk, const Tensor& dq,
                         const Tensor& dk, const Tensor& dwq, const Tensor& dwk) {
-    const int B = (int)gq.size(0), N = (int)gq.size(2), D = (int)gq.size(3);
+    const int B = i32(gq.size(0)), N = i32(gq.size(2)), D = i32(gq.size(3));
     const Tensor& w = wq.defined() ? wq : wk;
     On on(gq);
     Tensor ws;
@@ -124,7 +130,7 @@ void norm_rope_backward(const Rows& q, const Rows& k, const Tensor& wq, const Te
     if (w.defined()) ws = bytes(n = ossa_qk_norm_rope_bwd_workspace_size(D), gq);
     check(ossa_qk_norm_rope_bwd(
         in(q.x), in(k.x), in(wq), in(wk), in(cos), in(sin), batched(cos, B), dtype_code(gq),
-        w.defined() ? dtype_code(w) : OSSA_F32, B, N, (int)q.H, (int)k.H, D, q.sb, q.sn, k.sb, k.sn, (float)eps, in(gq),
+        w.defined() ? dtype_code(w) : OSSA_F32, B, N, i32(q.H), i32(k.H), D, q.sb, q.sn, k.sb, k.sn, (float)eps, in(gq),
         in(gk), to(dq), to(dk), to(dwq), to(dwk), to(ws), n, on.stream));
 }
 
@@ -140,7 +146,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
             const Tensor& w = wq.defined() ? wq : wk;
             On on(q);
             check(ossa_qk_norm_rope_fwd(in(a.x), in(b.x), in(wq), in(wk), in(cos), in(sin), batched(cos, B), dtype_code(q),
-                                        w.defined() ? dtype_code(w) : OSSA_F32, (int)B, (int)N, (int)Hq, (int)Hk, (int)a.D,
+                                        w.defined() ? dtype_code(w) : OSSA_F32, i32(B), i32(N), i32(Hq), i32(Hk), i32(a.D),
                                         a.sb, a.sn, b.sb, b.sn, (float)eps, to(oq), to(ok), on.stream));
         }
         if (grad) {
@@ -192,7 +198,7 @@ struct RopeToHeads : torch::autograd::Function<RopeToHeads> {
         Tensor out = at::empty({B, H, N, D}, x.options());
         if (out.numel() > 0) {
             On on(x);
-            check(ossa_rope_to_heads(in(xc), in(cos), in(sin), batched(cos, B), dtype_code(x), (int)B, (int)N, (int)H, (int)D,
+            check(ossa_rope_to_heads(in(xc), in(cos), in(sin), batched(cos, B), dtype_code(x), i32(B), i32(N), i32(H), i32(D),
                                      to(out), on.stream));
         }
         ctx->save_for_backward({cos, sin});
@@ -216,9 +222,9 @@ struct RopeToHeads : torch::autograd::Function<RopeToHeads> {
 // ------------------------------------------------------------------ modified attention
 
 #define OSSA_ATTENTION_ARGS(q, k, v, slopes, idx, segments, prefix, causal, q0, cap)                                       \
-    in(q), in(k), in(v), in(idx), is_64(idx), dtype_code(q), (int)q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), \
-        (int)k.size(2), (int)q.size(3), (int)idx.size(3), (float)(1.0 / std::sqrt((double)q.size(3))), causal ? 1 : 0,       \
-        (int)q0, (float)cap, in_as<float>(slopes), in_as<int32_t>(segments), in_as<int32_t>(prefix)
+    in(q), in(k), in(v), in(idx), is_64(idx), dtype_code(q), i32(q.size(0)), i32(q.size(1)), i32(k.size(1)), i32(q.size(2)), \
+        i32(k.size(2)), i32(q.size(3)), i32(idx.size(3)), (float)(1.0 / std::sqrt((double)q.size(3))), causal ? 1 : 0,       \
+        i32(q0), (float)cap, in_as<float>(slopes), in_as<int32_t>(segments), in_as<int32_t>(prefix)
 
 struct TopkAttention : torch::autograd::Function<TopkAttention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Maybe& slopes_,
@@ -255,8 +261,8 @@ struct TopkAttention : torch::autograd::Function<TopkAttention> {
         if (slopes.defined() && ctx->needs_input_grad(3)) dslopes = at::empty_like(slopes);
         On on(q);
         const size_t n = ossa_topk_attention_bwd_workspace_size(
-            dtype_code(q), (int)q.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), (int)k.size(2), (int)q.size(3),
-            (int)idx.size(3), dslopes.defined() ? 1 : 0);
+            dtype_code(q), i32(q.size(0)), i32(q.size(1)), i32(k.size(1)), i32(q.size(2)), i32(k.size(2)), i32(q.size(3)),
+            i32(idx.size(3)), dslopes.defined() ? 1 : 0);
         const Tensor ws = bytes(n, q);
         check(ossa_topk_attention_bwd(OSSA_ATTENTION_ARGS(q, k, v, slopes, idx, segments, prefix, causal, q0, cap), in(s[7]),
                                       in_as<float>(s[8]), in(dout), to(dq), to(dk), to(dv), to_f32(dslopes), to(ws), n,
@@ -280,12 +286,12 @@ struct Logits {
     explicit Logits(const Tensor& t) : z(t.stride(-1) == 1 ? t : t.contiguous()) {
         const int64_t d = z.dim();
         if (d == 3) {
-            outer = (int)z.size(0);
+            outer = i32(z.size(0));
             so = z.stride(0);
         }
-        inner = (int)z.size(d - 2);
+        inner = i32(z.size(d - 2));
         si = z.stride(d - 2);
-        V = (int)z.size(d - 1);
+        V = i32(z.size(d - 1));
     }
     int64_t rows() const { return (int64_t)outer * inner; }
 };
@@ -296,7 +302,7 @@ struct TopLogitDistill : torch::autograd::Function<TopLogitDistill> {
                           const Maybe& weight_, double tau, int64_t reduction, bool grad) {
         const Logits l(z);
         const Tensor weight = opt(weight_);
-        const int K = (int)ids.size(1);
+        const int K = i32(ids.size(1));
         const bool each = reduction == 0;
         const size_t n = ossa_top_logit_distill_workspace_size(l.rows(), K);
         Tensor ws = bytes(n, z), dz;
@@ -336,7 +342,7 @@ struct TopLogitDistill : torch::autograd::Function<TopLogitDistill> {
         if (!taken) dz = at::empty({l.rows(), l.V}, l.z.options());
         On on(l.z);
         check(ossa_top_logit_distill_bwd(in(l.z), dtype_code(l.z), l.outer, l.inner, l.V, l.so, l.si, in(ids), is_64(ids),
-                                         (int)ids.size(1), (float)ctx->saved_data["tau"].toDouble(), reduction == 2 ? 1 : 0,
+                                         i32(ids.size(1)), (float)ctx->saved_data["tau"].toDouble(), reduction == 2 ? 1 : 0,
                                          in_as<float>(up), reduction == 0 ? 1 : 0, taken ? 1 : 0, to(dz), in(ws),
                                          (size_t)ws.numel(), on.stream));
         variable_list out(7);

@@ -388,3 +388,11 @@ def test_from_several_threads():
     for t in threads:
         t.join()
     assert all(torch.equal(a, b) for n in range(2) for a, b in zip(want, got[n]))
+
+
+def test_positions_past_32_bits_are_refused():
+    q = torch.zeros(1, 1, 4, 64, device=DEV)
+    idx = torch.zeros(1, 1, 4, 2, dtype=torch.int32, device=DEV)
+    for q_start in (2 ** 31, 2 ** 32, 2 ** 31 - 2):
+        with pytest.raises((ValueError, RuntimeError)):
+            topk_attention(q, q, q, topk_indices=idx, q_start=q_start, softcap=2.0)
