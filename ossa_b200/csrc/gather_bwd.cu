@@ -391,7 +391,7 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         }
         d0 = warp_sum(d0);
     }
-    float a_pd = 0.f, a_f = 0.f, a_pdf = 0.f;  // sums of p dP, p far, p dP far
+    float a_p = 0.f, a_pd = 0.f, a_f = 0.f, a_xf = 0.f;  // sums of p, p dP, p far, p (dP - d0) far
     const int* krow = keys + row * s.K;
     for (int kc = 0; kc < s.K; kc += 32) {
         const int kk = kc + lane;
@@ -424,11 +424,13 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
             if (je >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
                 const float far = fabsf((float)(i - je));
                 p = exp2f(mods.score2_grad(dot, slope, far, dx, TanhExact()) - lse2);
-                dx *= p * (dp - d0);
+                const float ds = p * (dp - d0);
+                dx *= ds;
                 if (lane < B) {
+                    a_p += p;
                     a_pd = fmaf(p, dp, a_pd);
                     a_f = fmaf(p, far, a_f);
-                    a_pdf = fmaf(p * dp, far, a_pdf);
+                    a_xf = fmaf(ds, far, a_xf);
                 }
             }
 #pragma unroll
@@ -441,12 +443,10 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
         }
     }
     R::store(dq + row * D, lane, acc);
-    a_pd = warp_sum(a_pd);
-    if (lane == 0) delta[row] = a_pd;
-    if (slope_rows) {
-        a_f = warp_sum(a_f);
-        a_pdf = warp_sum(a_pdf);
-        if (lane == 0) slope_rows[row] = a_pd * a_f - a_pdf;
+    const RowSums sums(warp_sum(a_p), warp_sum(a_pd), warp_sum(a_f), warp_sum(a_xf), d0);
+    if (lane == 0) {
+        delta[row] = sums.delta;
+        if (slope_rows) slope_rows[row] = sums.slope;
     }
 }
 

@@ -35,6 +35,18 @@ struct BwdBuffers {
 cudaError_t launch_row_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream);
 cudaError_t launch_key_pass_mma(const GatherBwdArgs& a, const BwdShape& s, const BwdBuffers& w, cudaStream_t stream);
 
+// What a row's sums give: Delta, and its share of -dslope, sum p (dP - Delta) far.  The rounding of the row's
+// statistic and of p keeps the sum of p from being 1, so both are divided by it.  xf is sum p (dP - d0) far with d0
+// near Delta: as the difference of sum p dP far and Delta sum p far the share lost three quarters of its accuracy.
+struct RowSums {
+    float delta, slope;
+    __device__ __forceinline__ RowSums(float p, float pd, float f, float xf, float d0) {
+        const float inv = p == 0.f ? 0.f : 1.f / p;
+        delta = pd * inv;
+        slope = ((delta - d0) * f - xf) * inv;
+    }
+};
+
 // The block whose run holds position pos (base[block] <= pos < base[block + 1]).
 __device__ __forceinline__ int block_at(const int* __restrict__ base, int NB, int pos) {
     int lo = 0, hi = NB;  // base[lo] <= pos < base[hi]

@@ -2,7 +2,7 @@
 // mathematics and the other shapes).  mma.sync m16n8k16: the operands are gathered rows that a warp
 // stages for itself, 16 at a time, too few and too scattered for a tcgen05 tile.
 //
-// Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 146 us, of
+// Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 148 us, of
 // which 57 us for the rows' q, dO, output and lists and the union of keys (144 of 384 on average), key pass
 // 181 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
 // (8 KB in, 16 KB out as operands): 5.4 GB, 155 us at 128 bytes a cycle and SM, which is what bounds it; the
@@ -123,7 +123,8 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         float acc[8][4];  // dq^T: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
 #pragma unroll
         for (int n = 0; n < 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        float a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_pdf[2] = {0.f, 0.f};  // sums of p dP, p far, p dP far
+        // sums of p, p dP, p far, p (dP - d0) far
+        float a_p[2] = {0.f, 0.f}, a_pd[2] = {0.f, 0.f}, a_f[2] = {0.f, 0.f}, a_xf[2] = {0.f, 0.f};
         __syncwarp();
         if (single) U = single_list([&](int e) { return key_of(pass, e); }, pass, s.K, list, lane);
         __syncwarp();  // the list is complete, the staging area is free
@@ -169,10 +170,12 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     const float s2 = mods.score2_grad(sacc[2 * h + e], slope[e], far, dx, TanhFast());
                     const float p = on ? exp2_fast(s2 - lse2[e]) : 0.f;
                     const float pd = on ? p * pacc[2 * h + e] : 0.f;
-                    w[h][e] = on ? dx * (pd - p * d0[e]) : 0.f;
+                    const float ds = on ? pd - p * d0[e] : 0.f;
+                    w[h][e] = on ? dx * ds : 0.f;
+                    a_p[e] += p;
                     a_pd[e] += pd;
                     a_f[e] = fmaf(p, far, a_f[e]);
-                    a_pdf[e] = fmaf(pd, far, a_pdf[e]);
+                    a_xf[e] = fmaf(ds, far, a_xf[e]);
                 }
             }
             const Weights wt(w);
@@ -201,15 +204,17 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
             for (int o = 4; o <= 16; o <<= 1) {
+                a_p[e] += __shfl_xor_sync(kFull, a_p[e], o);
                 a_pd[e] += __shfl_xor_sync(kFull, a_pd[e], o);
                 a_f[e] += __shfl_xor_sync(kFull, a_f[e], o);
-                a_pdf[e] += __shfl_xor_sync(kFull, a_pdf[e], o);
+                a_xf[e] += __shfl_xor_sync(kFull, a_xf[e], o);
             }
             const int t = 2 * c4 + e;
             if (gq == 0 && (single ? t == pass : t < G)) {
                 const size_t row = row0 + (size_t)t * s.Nq;
-                delta[row] = a_pd[e];
-                if (slope_rows) slope_rows[row] = a_pd[e] * a_f[e] - a_pdf[e];
+                const RowSums sums(a_p[e], a_pd[e], a_f[e], a_xf[e], d0[e]);
+                delta[row] = sums.delta;
+                if (slope_rows) slope_rows[row] = sums.slope;
             }
         }
         __nv_bfloat16* orow = dq + mine + 2 * c4;
