@@ -423,7 +423,7 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
             float p = 0.f, dx = 0.f;
             if (je >= 0 && lse2 != -INFINITY) {  // -inf: every score of the row is, its output was 0
                 const float far = fabsf((float)(i - je));
-                p = exp2f(mods.score2_grad(dot, slope, far, dx, TanhExact()) - lse2);
+                p = exp2f(mods.log2_p(dot, slope, far, lse2, dx, TanhExact()));
                 const float ds = p * (dp - d0);
                 dx *= ds;
                 if (lane < B) {
@@ -508,7 +508,7 @@ key_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
                 const float se = __shfl_sync(kFull, slope, e), far = fabsf((float)(__shfl_sync(kFull, i, e) - key));
                 float p = 0.f, dx = 0.f;
                 if (le != -INFINITY) {
-                    p = exp2f(mods.score2_grad(dot, se, far, dx, TanhExact()) - le);
+                    p = exp2f(mods.log2_p(dot, se, far, le, dx, TanhExact()));
                     dx *= p * (dp - de);
                 }
 #pragma unroll

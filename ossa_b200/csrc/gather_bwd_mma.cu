@@ -167,8 +167,8 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                     // selects, no branch: what a masked place computes may not be finite and is dropped
                     const bool on = ((entry >> (24 + 2 * c4 + e)) & 1u) && lse2[e] != -INFINITY;
                     float dx;
-                    const float s2 = mods.score2_grad(sacc[2 * h + e], slope[e], far, dx, TanhFast());
-                    const float p = on ? exp2_fast(s2 - lse2[e]) : 0.f;
+                    const float x = mods.log2_p(sacc[2 * h + e], slope[e], far, lse2[e], dx, TanhFast());
+                    const float p = on ? exp2_fast(x) : 0.f;
                     const float pd = on ? p * pacc[2 * h + e] : 0.f;
                     const float ds = on ? pd - p * d0[e] : 0.f;
                     w[h][e] = on ? dx * ds : 0.f;
@@ -367,9 +367,9 @@ key_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     float dx;
-                    const float s2 = mods.score2_grad(sacc[2 * h + x], sp, fabsf((float)(ie - 2 * c4 - x)), dx, TanhFast());
+                    const float y = mods.log2_p(sacc[2 * h + x], sp, fabsf((float)(ie - 2 * c4 - x)), l, dx, TanhFast());
                     const bool on = (mask >> (2 * c4 + x)) & 1u;
-                    p[h][x] = on ? exp2_fast(s2 - l) : 0.f;
+                    p[h][x] = on ? exp2_fast(y) : 0.f;
                     w[h][x] = on ? dx * p[h][x] * (pacc[2 * h + x] - d) : 0.f;
                 }
                 const float both = fminf(fabsf(sacc[2 * h] + pacc[2 * h]), fabsf(sacc[2 * h + 1] + pacc[2 * h + 1]));

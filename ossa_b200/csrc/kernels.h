@@ -44,11 +44,11 @@ struct ScoreMods {
         const float s = cap > 0.f ? cap * tanh_of(x * inv_cap) : x;
         return fmaf(-slope, far, s) * 1.4426950408889634f;
     }
-    // The same, and d score / d dot in dx.
+    // The same less lse2 (one rounding for both), and d score / d dot in dx.
     template <typename Tanh>
-    __device__ __forceinline__ float score2_grad(float dot, float slope, float far, float& dx, Tanh tanh_of) const {
+    __device__ __forceinline__ float log2_p(float dot, float slope, float far, float lse, float& dx, Tanh tanh_of) const {
         dx = scale;
-        if (!shaped) return dot * scale_log2;
+        if (!shaped) return fmaf(dot, scale_log2, -lse);
         const float x = dot * scale;
         float s = x;
         if (cap > 0.f) {
@@ -56,7 +56,7 @@ struct ScoreMods {
             s = cap * t;
             dx = scale * (1.f - t * t);
         }
-        return fmaf(-slope, far, s) * 1.4426950408889634f;
+        return fmaf(fmaf(-slope, far, s), 1.4426950408889634f, -lse);
     }
 #endif
 };
