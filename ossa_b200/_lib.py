@@ -120,11 +120,11 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ossa_router_topk_rows_kp.argtypes = [vp, ci, vp, vp, vp] + [ci] * 11 + [vp, vp, sz, vp]
     lib.ossa_router_topk_rows_kp.restype = ci
     cl = ctypes.c_longlong
-    lib.ossa_topk_attention_mod_fwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf, vp, vp, vp, vp, vp, vp]
+    lib.ossa_topk_attention_mod_fwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf] + [vp] * 7
     lib.ossa_topk_attention_mod_fwd.restype = ci
     lib.ossa_topk_attention_bwd_workspace_size.argtypes = [ci] * 9
     lib.ossa_topk_attention_bwd_workspace_size.restype = sz
-    lib.ossa_topk_attention_bwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf] + [vp] * 11 + [sz, vp]
+    lib.ossa_topk_attention_bwd.argtypes = [vp] * 4 + [ci] * 9 + [cf, ci, ci, cf] + [vp] * 12 + [sz, vp]
     lib.ossa_topk_attention_bwd.restype = ci
     lib.ossa_qk_norm_rope_fwd.argtypes = [vp] * 6 + [ci] * 8 + [cl] * 4 + [cf, vp, vp, vp]
     lib.ossa_qk_norm_rope_fwd.restype = ci

@@ -232,15 +232,18 @@ struct TopkAttention : torch::autograd::Function<TopkAttention> {
                           double cap, bool grad) {
         const Tensor q = packed(q_), k = packed(k_), v = packed(v_), idx = idx_.contiguous();
         const Tensor slopes = opt(slopes_), segments = opt(segments_), prefix = opt(prefix_);
-        Tensor out = at::empty(q.sizes(), q.options()), lse2;
-        if (grad) lse2 = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+        Tensor out = at::empty(q.sizes(), q.options()), lse2, rest;
+        if (grad) {
+            lse2 = at::empty(q.sizes().slice(0, 3), q.options().dtype(at::kFloat));
+            if (q.scalar_type() == at::kBFloat16) rest = at::empty(q.sizes(), q.options());
+        }
         if (out.numel() > 0) {
             On on(q);
             check(ossa_topk_attention_mod_fwd(OSSA_ATTENTION_ARGS(q, k, v, slopes, idx, segments, prefix, causal, q0, cap),
-                                              to(out), to_f32(lse2), on.stream));
+                                              to(out), to_f32(lse2), to(rest), on.stream));
         }
         if (grad) {
-            ctx->save_for_backward({q, k, v, slopes, idx, segments, prefix, out, lse2});
+            ctx->save_for_backward({q, k, v, slopes, idx, segments, prefix, out, lse2, rest});
             ctx->saved_data["causal"] = causal;
             ctx->saved_data["q0"] = q0;
             ctx->saved_data["cap"] = cap;
@@ -265,7 +268,7 @@ struct TopkAttention : torch::autograd::Function<TopkAttention> {
             i32(idx.size(3)), dslopes.defined() ? 1 : 0);
         const Tensor ws = bytes(n, q);
         check(ossa_topk_attention_bwd(OSSA_ATTENTION_ARGS(q, k, v, slopes, idx, segments, prefix, causal, q0, cap), in(s[7]),
-                                      in_as<float>(s[8]), in(dout), to(dq), to(dk), to(dv), to_f32(dslopes), to(ws), n,
+                                      in_as<float>(s[8]), in(s[9]), in(dout), to(dq), to(dk), to(dv), to_f32(dslopes), to(ws), n,
                                       on.stream));
         variable_list out(11);
         out[0] = dq;

@@ -300,15 +300,16 @@ static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int 
 }
 
 static ossa::ScoreMods make_mods(float scale, float softcap, const float* slopes, const int32_t* segments,
-                                 const int32_t* prefix_len, float* lse2) {
+                                 const int32_t* prefix_len, float* lse2, void* out_rest) {
     return ossa::ScoreMods{scale, scale * 1.4426950408889634f, softcap, softcap > 0.f ? 1.f / softcap : 0.f,
-                           softcap > 0.f || slopes ? 1 : 0, slopes, segments, prefix_len, lse2};
+                           softcap > 0.f || slopes ? 1 : 0, slopes, segments, prefix_len, lse2, out_rest};
 }
 
 int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64,
                                 int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale, int causal,
                                 int q_start, float softcap, const float* slopes, const int32_t* segments,
-                                const int32_t* prefix_len, void* out, float* lse2, ossa_stream_t stream) {
+                                const int32_t* prefix_len, void* out, float* lse2, void* out_rest,
+                                ossa_stream_t stream) {
     int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
     if (st) return st;
     if ((long long)B * H * Nq == 0) return OSSA_OK;
@@ -321,9 +322,11 @@ int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, con
     ossa::GatherArgs a{q, k, v, indices, out, idx_is_64, dtype, B, H, Hkv, Nk, D, K, scale, causal ? 1 : 0};
     a.Nq = Nq;
     a.q0 = q_start;
-    a.mods = make_mods(scale, softcap, slopes, segments, prefix_len, lse2);
+    if (out_rest && (dtype != OSSA_BF16 || !aligned16(out_rest)))
+        return fail(OSSA_ERR_INVALID, "out_rest goes with bf16 outputs and must be 16-byte aligned");
+    a.mods = make_mods(scale, softcap, slopes, segments, prefix_len, lse2, out_rest);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (softcap == 0.f && !slopes && !segments && !prefix_len && !lse2)
+    if (softcap == 0.f && !slopes && !segments && !prefix_len && !lse2 && !out_rest)
         return cuda_status(ossa::launch_gather_attn(a, s), "topk attention launch");
     return cuda_status(ossa::launch_gather_attn_mods(a, s), "modified topk attention launch");
 }
@@ -338,8 +341,8 @@ size_t ossa_topk_attention_bwd_workspace_size(int dtype, int B, int H, int Hkv, 
 int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const void* indices, int idx_is_64, int dtype,
                             int B, int H, int Hkv, int Nq, int Nk, int D, int K, float scale, int causal, int q_start,
                             float softcap, const float* slopes, const int32_t* segments, const int32_t* prefix_len,
-                            const void* out, const float* lse2, const void* dout, void* dq, void* dk, void* dv,
-                            float* dslopes, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
+                            const void* out, const float* lse2, const void* out_rest, const void* dout, void* dq,
+                            void* dk, void* dv, float* dslopes, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
     int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
     if (st) return st;
     if (dslopes && !slopes) return fail(OSSA_ERR_INVALID, "dslopes without slopes");
@@ -373,7 +376,10 @@ int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const v
                            causal ? 1 : 0};
     a.f.Nq = Nq;
     a.f.q0 = q_start;
-    a.f.mods = make_mods(scale, softcap, slopes, segments, prefix_len, const_cast<float*>(lse2));
+    if (out_rest && (dtype != OSSA_BF16 || !aligned16(out_rest)))
+        return fail(OSSA_ERR_INVALID, "out_rest goes with bf16 outputs and must be 16-byte aligned");
+    a.f.mods = make_mods(scale, softcap, slopes, segments, prefix_len, const_cast<float*>(lse2),
+                         const_cast<void*>(out_rest));
     a.dout = dout;
     a.dq = dq;
     a.dk = dk;

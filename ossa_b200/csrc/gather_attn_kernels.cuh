@@ -151,6 +151,13 @@ gather_attn_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
             T* orow = out + row * D + lane * DPL;
 #pragma unroll
             for (int t = 0; t < DPL; ++t) store_from_f32(orow + t, acc[t] * inv);
+            if constexpr (kMods && sizeof(T) == 2) {
+                if (mods.rest) {
+                    __nv_bfloat16* rrow = static_cast<__nv_bfloat16*>(mods.rest) + row * D + lane * DPL;
+#pragma unroll
+                    for (int t = 0; t < DPL; ++t) rrow[t] = __float2bfloat16_rn(bf16_rest(acc[t] * inv));
+                }
+            }
         }
         if (kMods && mods.lse2 && lane == 0) mods.lse2[row] = m_run + log2f(l_run);
     }
@@ -205,17 +212,25 @@ __device__ __forceinline__ void gather_row_bf16_d128(uint4 qv, const uint4* __re
         l_run = l_run * alpha + warp_sum(p);
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] *= alpha;
-        const uint32_t pbits = bf16_pair_bits(p);
+        const uint32_t pbits = bf16_pair_bits(p), prest = kMods ? bf16_pair_bits(bf16_rest(p)) : 0u;
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
             const uint32_t pm = __shfl_sync(kFull, pbits, 16 * half + m);
             uint4 vr = __ldg(vb + (size_t)max(js[m], 0) * (D / 8));
             if (kMods && js[m] < 0) vr = make_uint4(0u, 0u, 0u, 0u);  // key 0 may be masked and not finite
             axpy8_bf16(pm, vr, acc);
+            // the training form takes p as a bf16 value and its rest, as the tensor-core form does
+            if (kMods) axpy8_bf16(__shfl_sync(kFull, prest, 16 * half + m), vr, acc);
         }
         m_run = m_new;
     }
-    store_row_bf16(acc, l_run, orow, lane);
+    store_row_bf16(acc, l_run, orow, lane);  // acc: the sums over both half-warps from here on
+    if (kMods && mods.rest && lane < 16) {
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        __nv_bfloat16* rrow = static_cast<__nv_bfloat16*>(mods.rest) + row * D + 8 * lane;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) rrow[t] = __float2bfloat16_rn(bf16_rest(acc[t] * inv));
+    }
     if (kMods && mods.lse2 && lane == 0) mods.lse2[row] = m_run + log2f(l_run);
 }
 

@@ -221,6 +221,18 @@ mod_attn_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
                 *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
             }
         }
+        if (mods.rest) {
+            __nv_bfloat16* rrow = static_cast<__nv_bfloat16*>(mods.rest) + (orow - out);
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                const uint32_t lo = movmatrix_trans(pack_bf16x2(bf16_rest(oacc[mt][0] * inv0), bf16_rest(oacc[mt][1] * inv1)));
+                const uint32_t hi = movmatrix_trans(pack_bf16x2(bf16_rest(oacc[mt][2] * inv0), bf16_rest(oacc[mt][3] * inv1)));
+                if (mine) {
+                    *reinterpret_cast<uint32_t*>(rrow + 16 * mt) = lo;
+                    *reinterpret_cast<uint32_t*>(rrow + 16 * mt + 8) = hi;
+                }
+            }
+        }
         if (mods.lse2 && gq == 0) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -328,6 +340,7 @@ mod_attn_few_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         float t = 0.f;
         for (int w = 0; w < warps; ++w) t += s_ml[w].x == -INFINITY ? s_acc[w][d] : s_acc[w][d] * exp2f(s_ml[w].x - top);
         out[row * D + d] = __float2bfloat16_rn(t * inv);
+        if (mods.rest) static_cast<__nv_bfloat16*>(mods.rest)[row * D + d] = __float2bfloat16_rn(bf16_rest(t * inv));
     }
     if (mods.lse2 && threadIdx.x == 0) mods.lse2[row] = top + log2f(l);
 }

@@ -380,10 +380,18 @@ row_pass_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __res
     float qv[R::kPer], dv[R::kPer], acc[R::kPer];
     R::load(q + row * D, lane, qv);
     R::load(dout + row * D, lane, dv);
-    float d0 = 0.f;  // Delta from the stored output, for dq
+    float d0 = 0.f;  // Delta from the stored output (and its rest), for dq
     {
         float o[R::kPer];
         R::load(out + row * D, lane, o);
+        if constexpr (sizeof(T) == 2) {
+            if (mods.rest) {
+                float rest[R::kPer];
+                R::load(static_cast<const T*>(mods.rest) + row * D, lane, rest);
+#pragma unroll
+                for (int t = 0; t < R::kPer; ++t) o[t] += rest[t];
+            }
+        }
 #pragma unroll
         for (int t = 0; t < R::kPer; ++t) {
             d0 = fmaf(o[t], dv[t], d0);

@@ -2,9 +2,9 @@
 // mathematics and the other shapes).  mma.sync m16n8k16: the operands are gathered rows that a warp
 // stages for itself, 16 at a time, too few and too scattered for a tcgen05 tile.
 //
-// Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 148 us, of
+// Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 156 us, of
 // which 57 us for the rows' q, dO, output and lists and the union of keys (144 of 384 on average), key pass
-// 181 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
+// 183 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
 // (8 KB in, 16 KB out as operands): 5.4 GB, 155 us at 128 bytes a cycle and SM, which is what bounds it; the
 // per-head forms of gather_bwd.cu took 752 and 1147 us here.
 #include <algorithm>
@@ -69,7 +69,7 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
     const size_t row0 = ((size_t)b * s.H + (size_t)g * G) * s.Nq + il;  // head t: row0 + t * Nq
     const size_t mine = (row0 + (size_t)(gq < G ? gq : 0) * s.Nq) * D;  // head gq's row
 
-    // q and dO rows as B operands of head gq; Delta from the stored output
+    // q and dO rows as B operands of head gq; Delta from the stored output (and its rest)
     uint32_t qa[16], da[16];
     float d0[2];
     {
@@ -82,6 +82,11 @@ row_pass_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
             qa[t] = gq < G ? __ldg(qw + 4 * t + c4) : 0u;
             da[t] = gq < G ? __ldg(dw + 4 * t + c4) : 0u;
             d = dot_bf16x2(da[t], gq < G ? __ldg(ow + 4 * t + c4) : 0u, d);
+        }
+        if (mods.rest) {
+            const uint32_t* rw = reinterpret_cast<const uint32_t*>(static_cast<const __nv_bfloat16*>(mods.rest) + mine);
+#pragma unroll
+            for (int t = 0; t < 16; ++t) d = dot_bf16x2(da[t], gq < G ? __ldg(rw + 4 * t + c4) : 0u, d);
         }
         d += __shfl_xor_sync(kFull, d, 1);
         d += __shfl_xor_sync(kFull, d, 2);

@@ -34,6 +34,7 @@ struct ScoreMods {
     const int32_t* segments;    // (B, N) or nullptr
     const int32_t* prefix_len;  // (B,) or nullptr
     float* lse2;                // (B*H*Nq,) log2 of the row's sum of 2^s2, -inf for an empty row; nullptr: not wanted
+    void* rest;                 // like a bf16 output: what rounding it left; nullptr: not wanted
 #ifdef __CUDACC__
     // Score in base 2 of a key at distance far from dot = q . k.  Scores that only masks modify are
     // the plain kernels' product, so that their results are too.

@@ -148,8 +148,8 @@ __device__ __forceinline__ void stage_listed(uint32_t dst, const __nv_bfloat16* 
 }
 
 // 2^x and tanh for the tensor-core forms.  ex2.approx: two units in the last place.  tanh x = 1 - 2 / (1 + e^2x)
-// is good to 2^-22 in absolute terms, which a score of size cap turns into cap * 2^-22; below 0.4, where most
-// scores of a cap lie, x times a polynomial in x^2 (least maximal relative error there, 2^-29) takes its place.
+// is good to 2^-22 in absolute terms, which a score of size cap turns into cap * 2^-22; below 1, where most
+// scores of a cap lie, x times a polynomial in x^2 (least maximal relative error there, 2^-23) takes its place.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -158,11 +158,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 __device__ __forceinline__ float tanh_fast(float x) {
     const float u = x * x;
-    float p = fmaf(0.01866922713816166f, u, -0.05353522673249245f);
-    p = fmaf(p, u, 0.13330897688865662f);
-    p = fmaf(p, u, -0.3333328366279602f);
-    p = fmaf(p, u, 1.f);
-    return u < 0.16f ? p * x : 1.f - __fdividef(2.f, 1.f + exp2_fast(x * 2.885390081777927f));
+    float p = fmaf(0.0010410227114334702f, u, -0.0062033794820308685f);
+    p = fmaf(p, u, 0.020289981737732887f);
+    p = fmaf(p, u, -0.05345702916383743f);
+    p = fmaf(p, u, 0.13325203955173492f);
+    p = fmaf(p, u, -0.33332839608192444f);
+    p = fmaf(p, u, 0.9999999403953552f);
+    return u < 1.f ? p * x : 1.f - __fdividef(2.f, 1.f + exp2_fast(x * 2.885390081777927f));
 }
 
 }  // namespace ossa

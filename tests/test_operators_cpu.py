@@ -13,14 +13,14 @@ INF, NAN = float("inf"), float("nan")
 
 def _mod_fwd(**kw):
     a = dict(q=16, k=16, v=16, idx=16, i64=0, dtype=BF, B=1, H=4, Hkv=2, Nq=8, Nk=8, D=128, K=4, scale=0.1, causal=1,
-             q0=0, cap=0.0, slopes=None, seg=None, prefix=None, out=16, lse=16, stream=None)
+             q0=0, cap=0.0, slopes=None, seg=None, prefix=None, out=16, lse=16, rest=None, stream=None)
     a.update(kw)
     return _lib.lib().ossa_topk_attention_mod_fwd(*a.values())
 
 
 def _mod_bwd(**kw):
     a = dict(q=16, k=16, v=16, idx=16, i64=0, dtype=BF, B=1, H=4, Hkv=2, Nq=8, Nk=8, D=128, K=4, scale=0.1, causal=1,
-             q0=0, cap=0.0, slopes=None, seg=None, prefix=None, out=16, lse=16, dout=16, dq=16, dk=16, dv=16,
+             q0=0, cap=0.0, slopes=None, seg=None, prefix=None, out=16, lse=16, rest=None, dout=16, dq=16, dk=16, dv=16,
              dslopes=None, ws=256, wsb=1 << 30, stream=None)
     a.update(kw)
     return _lib.lib().ossa_topk_attention_bwd(*a.values())
@@ -29,7 +29,8 @@ def _mod_bwd(**kw):
 BAD_MOD = [(dict(H=5), INV), (dict(D=96), UNS), (dict(dtype=3), INV), (dict(K=-1), INV), (dict(i64=2), INV),
            (dict(scale=NAN), INV), (dict(cap=-1.0), INV), (dict(cap=INF), INV), (dict(cap=NAN), INV),
            (dict(q0=-1), INV), (dict(seg=16, q0=1), INV), (dict(B=40000, H=2, Hkv=2), UNS), (dict(q=None), INV),
-           (dict(k=8), INV), (dict(idx=18), INV), (dict(idx=None), INV), (dict(Nk=0), INV)]
+           (dict(k=8), INV), (dict(idx=18), INV), (dict(idx=None), INV), (dict(Nk=0), INV),
+           (dict(rest=24), INV), (dict(rest=16, dtype=F32), INV)]
 
 
 @pytest.mark.parametrize("kw,code", BAD_MOD)
