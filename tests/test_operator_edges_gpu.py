@@ -1,6 +1,8 @@
 """Training calls at their edges: gradients and inputs off 16-byte boundaries, saved tensors that come back in
 another layout, rows that are not finite beside rows that are, lists in any order."""
 
+import gc
+
 import pytest
 import torch
 
@@ -353,6 +355,7 @@ def test_nothing_stays_behind(backward):
     for _ in range(3):
         step()
     torch.cuda.synchronize()
+    gc.collect()  # what earlier tests left in reference cycles would go during the loop below
     held = torch.cuda.memory_allocated()
     for _ in range(20):
         step()
