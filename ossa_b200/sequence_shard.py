@@ -13,6 +13,12 @@ rank's query blocks against all keys with the query-row-range entry points
 rank's output rows equal the matching rows of the unsharded computation.
 Outputs stay sharded.  Every rank takes the same collective steps in the same
 order; nothing waits on another rank inside a kernel.
+
+Gradients flow back through the gather of k and v: each rank's gradient of the whole
+sequence is cut into the ranks' blocks, one all-to-all brings every rank the parts of its
+own, and they are summed in fp32 in rank order.  A backward pass is a collective step
+like the forward: k and v require gradients on every rank or on none, and every rank
+runs it.
 """
 
 from __future__ import annotations
@@ -46,11 +52,45 @@ def local_rows(x: torch.Tensor, world: int, rank: int) -> torch.Tensor:
     return torch.cat([x[:, :, s:e] for s, e in blocks], dim=2).contiguous()
 
 
+class _GatherSequence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x_local, world, group):
+        ctx.world, ctx.group = world, group
+        return _gather_blocks(x_local, world, group)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return _sum_blocks(grad, ctx.world, ctx.group), None, None
+
+
 def gather_sequence(x_local: torch.Tensor, world: int, group=None) -> torch.Tensor:
     """Inverse of ``local_rows`` across ranks: every rank gets the full
-    (B, heads, N, D) tensor from each rank's (B, heads, 2 * blk, D) blocks."""
+    (B, heads, N, D) tensor from each rank's (B, heads, 2 * blk, D) blocks.
+    Differentiable, once: the gradient of a rank's blocks is the sum of every rank's."""
     if world == 1:
         return x_local.contiguous()
+    if torch.is_grad_enabled() and x_local.requires_grad:
+        return _GatherSequence.apply(x_local, world, group)
+    return _gather_blocks(x_local, world, group)
+
+
+def _sum_blocks(grad: torch.Tensor, world: int, group) -> torch.Tensor:
+    """The adjoint of ``_gather_blocks``: grad (B, heads, N, D) of every rank -> the sum over ranks
+    of this rank's (B, heads, 2 * blk, D) blocks, in fp32 (fp64 for fp64) and rounded once."""
+    B, Hx, n, D = grad.shape
+    blk = n // (2 * world)
+    g = grad.reshape(B, Hx, 2 * world, blk, D)
+    # block r and block 2P-1-r go to rank r
+    parts = torch.stack([g[:, :, :world], g[:, :, world:].flip(2)], dim=3)  # (B, Hx, rank, half, blk, D)
+    parts = parts.permute(2, 0, 1, 3, 4, 5).reshape(world, B, Hx, 2 * blk, D).contiguous()
+    mine = torch.empty_like(parts)
+    dist.all_to_all_single(mine, parts, group=group)
+    acc = torch.float64 if grad.dtype == torch.float64 else torch.float32
+    return mine.to(acc).sum(dim=0).to(grad.dtype)
+
+
+def _gather_blocks(x_local: torch.Tensor, world: int, group) -> torch.Tensor:
     x_local = x_local.contiguous()
     B, Hx, two_blk, D = x_local.shape
     blk = two_blk // 2
@@ -79,6 +119,9 @@ def sharded_routed_attention(q_local: torch.Tensor, k_local: torch.Tensor, v_loc
     query rows, (B, H, 2*blk, D).  ``select_fn`` / ``attend_fn`` default to this
     package's CUDA kernels (``router_topk``, ``topk_attention``) and take the
     same arguments.
+
+    Differentiable in q_local, k_local and v_local (the selection is a constant): each
+    rank's gradients are the matching rows of the unsharded ones, for the sum of all ranks' losses.
     """
     own_select = select_fn is None
     select_fn = select_fn or router_topk
