@@ -118,12 +118,13 @@ gather_attn_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
             const float dot = transpose_reduce32(part, lane);
             const float s = !valid ? -INFINITY : kMods && mods.shaped ? rm.score2(dot, i, (int)j) : dot;
             const float m_new = fmaxf(m_run, warp_max(s));
-            if (m_new == -INFINITY) {  // warp-uniform: nothing valid so far
+            if (m_new == -INFINITY && !(kMods && shows_nan(s))) {  // warp-uniform: nothing valid so far
                 __syncwarp();
                 continue;
             }
-            const float p = valid ? exp2f(s - m_new) : 0.f;
-            const float alpha = exp2f(m_run - m_new);
+            const float ref = kMods && m_new == -INFINITY ? 0.f : m_new;
+            const float p = valid ? exp2f(s - ref) : 0.f;
+            const float alpha = exp2f(m_run - ref);
             l_run = l_run * alpha + warp_sum(p);
 #pragma unroll
             for (int t = 0; t < DPL; ++t) acc[t] *= alpha;
@@ -206,9 +207,10 @@ __device__ __forceinline__ void gather_row_bf16_d128(uint4 qv, const uint4* __re
         const float dot = transpose_reduce16(part, lane);
         const float sc = !valid ? -INFINITY : kMods ? rm.score2(dot, i, jv) : dot * scale_log2;
         const float m_new = fmaxf(m_run, warp_max(sc));
-        if (m_new == -INFINITY) continue;  // warp-uniform: nothing valid so far
-        const float p = valid ? exp2f(sc - m_new) : 0.f;
-        const float alpha = exp2f(m_run - m_new);
+        if (m_new == -INFINITY && !(kMods && shows_nan(sc))) continue;  // warp-uniform: nothing valid so far
+        const float ref = kMods && m_new == -INFINITY ? 0.f : m_new;
+        const float p = valid ? exp2f(sc - ref) : 0.f;
+        const float alpha = exp2f(m_run - ref);
         l_run = l_run * alpha + warp_sum(p);
 #pragma unroll
         for (int t = 0; t < 8; ++t) acc[t] *= alpha;

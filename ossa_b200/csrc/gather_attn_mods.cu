@@ -303,9 +303,10 @@ mod_attn_few_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __
         const float dot = part[0] + __shfl_xor_sync(kFull, part[0], 8);
         const float s2 = j >= 0 ? rm.score2(dot, i, j) : -INFINITY;
         const float m_new = fmaxf(m_run, warp_max(s2));
-        if (m_new == -INFINITY) continue;  // warp-uniform: nothing seen so far
-        const float p = j >= 0 ? exp2f(s2 - m_new) : 0.f;
-        const float alpha = exp2f(m_run - m_new);
+        if (m_new == -INFINITY && !shows_nan(s2)) continue;  // warp-uniform: nothing seen so far
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float p = j >= 0 ? exp2f(s2 - ref) : 0.f;
+        const float alpha = exp2f(m_run - ref);
         l_run = l_run * alpha + 0.5f * warp_sum(p);  // every key's p sits in two lanes
         m_run = m_new;
 #pragma unroll

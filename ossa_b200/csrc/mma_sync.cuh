@@ -21,6 +21,10 @@ __device__ __forceinline__ float transpose_reduce32(float (&part)[32], int lane)
     return part[0];
 }
 
+// Whether some lane's score is NaN.  A maximum passes over NaN, so scores whose maximum is -inf may hold it beside
+// masked ones: taken against 0 then, they make the row's sum and output NaN.
+__device__ __forceinline__ bool shows_nan(float s) { return __any_sync(kFull, s != s); }
+
 // mma.sync m16n8k16 with all four A registers (rows 0..15).
 __device__ __forceinline__ void mma_bf16_16816_a4(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                   uint32_t b0, uint32_t b1) {
