@@ -118,11 +118,11 @@ gather_attn_fwd_kernel(const T* __restrict__ q, const T* __restrict__ k,
             const float dot = transpose_reduce32(part, lane);
             const float s = !valid ? -INFINITY : kMods && mods.shaped ? rm.score2(dot, i, (int)j) : dot;
             const float m_new = fmaxf(m_run, warp_max(s));
-            if (m_new == -INFINITY && !(kMods && shows_nan(s))) {  // warp-uniform: nothing valid so far
+            if (m_new == -INFINITY && !shows_nan(s)) {  // warp-uniform: nothing valid so far
                 __syncwarp();
                 continue;
             }
-            const float ref = kMods && m_new == -INFINITY ? 0.f : m_new;
+            const float ref = m_new == -INFINITY ? 0.f : m_new;
             const float p = valid ? exp2f(s - ref) : 0.f;
             const float alpha = exp2f(m_run - ref);
             l_run = l_run * alpha + warp_sum(p);
@@ -207,8 +207,8 @@ __device__ __forceinline__ void gather_row_bf16_d128(uint4 qv, const uint4* __re
         const float dot = transpose_reduce16(part, lane);
         const float sc = !valid ? -INFINITY : kMods ? rm.score2(dot, i, jv) : dot * scale_log2;
         const float m_new = fmaxf(m_run, warp_max(sc));
-        if (m_new == -INFINITY && !(kMods && shows_nan(sc))) continue;  // warp-uniform: nothing valid so far
-        const float ref = kMods && m_new == -INFINITY ? 0.f : m_new;
+        if (m_new == -INFINITY && !shows_nan(sc)) continue;  // warp-uniform: nothing valid so far
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
         const float p = valid ? exp2f(sc - ref) : 0.f;
         const float alpha = exp2f(m_run - ref);
         l_run = l_run * alpha + warp_sum(p);
@@ -565,9 +565,10 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
             m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
             m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
             mx[e] = fmaxf(m_run[e], m);
-            alpha[e] = mx[e] == -INFINITY ? 1.f : exp2f(m_run[e] - mx[e]);
-            pr[0][e] = mx[e] == -INFINITY ? 0.f : exp2f(s0 - mx[e]);
-            pr[1][e] = mx[e] == -INFINITY ? 0.f : exp2f(s1 - mx[e]);
+            const float ref = mx[e] == -INFINITY ? 0.f : mx[e];  // nothing selected so far, or NaN alone
+            alpha[e] = exp2f(m_run[e] - ref);
+            pr[0][e] = exp2f(s0 - ref);
+            pr[1][e] = exp2f(s1 - ref);
             float sum = pr[0][e] + pr[1][e];
             sum += __shfl_xor_sync(kFull, sum, 4);
             sum += __shfl_xor_sync(kFull, sum, 8);
