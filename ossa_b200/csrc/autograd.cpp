@@ -7,7 +7,8 @@
 // and backward 162 us, 97 (of which torch's own part of any such call is about 50); forward alone 25, 17.
 // The distillation loss and its gradient 126, 78.
 //
-// Every gradient is that of the C entry points in ossa_b200.h; each node is differentiable once.
+// Every gradient is that of the C entry points in ossa_b200.h; each node is differentiable once, and refuses to be
+// differentiated twice where the second derivative is not zero.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -75,9 +76,10 @@ Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like
 using Maybe = std::optional<Tensor>;
 Tensor opt(const Maybe& t) { return t.has_value() ? *t : Tensor(); }
 
-// What a backward pass returns when a graph of it is wanted: the gradients, which refuse to be differentiated.
-variable_list once(variable_list grads, const variable_list& incoming, bool graph) {
-    bool any = false;
+// What a backward pass returns when a graph of it is wanted: the gradients, which refuse to be differentiated
+// where they depend on something that has a gradient: an incoming one, or (bent) the operator's own inputs.
+variable_list once(variable_list grads, const variable_list& incoming, bool graph, bool bent) {
+    bool any = bent;
     for (const Tensor& g : incoming) any = any || (g.defined() && g.requires_grad());
     if (!graph || !any) return grads;
     variable_list leaves;
@@ -154,6 +156,8 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
             ctx->saved_data["Hq"] = Hq;
             ctx->saved_data["Hk"] = Hk;
             ctx->saved_data["eps"] = eps;
+            // without its weight a tensor is only rotated, and the output is linear in a weight alone
+            ctx->saved_data["bent"] = (wq.defined() && q.requires_grad()) || (wk.defined() && k.requires_grad());
             ctx->set_materialize_grads(false);
         }
         return {oq, ok};
@@ -187,7 +191,7 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
             norm_rope_backward(b, Rows(), wk, none, cos, sin, eps, gk, none, out[1], none, out[3], none);
         else
             norm_rope_backward(a, b, wq, wk, cos, sin, eps, gq, gk, out[0], out[1], out[2], out[3]);
-        return once(std::move(out), g, graph);
+        return once(std::move(out), g, graph, ctx->saved_data["bent"].toBool());
     }
 };
 
@@ -215,7 +219,7 @@ struct RopeToHeads : torch::autograd::Function<RopeToHeads> {
         Rows a;
         a.H = gq.size(1);
         norm_rope_backward(a, Rows(), none, none, s[0], s[1], 0.0, gq, none, dx, none, none, none);
-        return once({dx, Tensor(), Tensor(), Tensor()}, g, graph);
+        return once({dx, Tensor(), Tensor(), Tensor()}, g, graph, false);
     }
 };
 
@@ -275,7 +279,7 @@ struct TopkAttention : torch::autograd::Function<TopkAttention> {
         out[1] = dk;
         out[2] = dv;
         out[3] = dslopes;
-        return once(std::move(out), g, graph);
+        return once(std::move(out), g, graph, true);
     }
 };
 
@@ -350,7 +354,7 @@ struct TopLogitDistill : torch::autograd::Function<TopLogitDistill> {
                                          (size_t)ws.numel(), on.stream));
         variable_list out(7);
         out[0] = dz.view(l.z.sizes());
-        return once(std::move(out), g, graph);
+        return once(std::move(out), g, graph, true);
     }
 };
 
