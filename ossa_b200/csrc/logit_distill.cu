@@ -70,10 +70,12 @@ Layout layout(long long T, int K) {
 
 // The teacher's rows: p, p log p and the p of each entry summed over its repeats, the row's
 // weight, and the CTA's share of the weight sum (rows in a fixed order).  A warp per row.
+// log p = (t - max) / tau - log sum, the difference first and divided: neither a common offset of the row's logits nor
+// their size costs p any of its digits, and rows of the type's lowest value stay finite.
 template <typename IdT>
 __global__ void __launch_bounds__(kPrepThreads)
 distill_prep_kernel(const float* __restrict__ teacher, const IdT* __restrict__ ids, const float* __restrict__ row_weight,
-                    int T, int V, int K, float inv_tau, unsigned* counter, double* __restrict__ wsum,
+                    int T, int V, int K, float tau, unsigned* counter, double* __restrict__ wsum,
                     float* __restrict__ weight, float2* __restrict__ plogp, float* __restrict__ ptot,
                     int* __restrict__ ids32) {
     constexpr int kPrepWarps = kPrepThreads / 32;
@@ -90,20 +92,21 @@ distill_prep_kernel(const float* __restrict__ teacher, const IdT* __restrict__ i
             const IdT id = ids[rk + k];
             const bool ok = id >= 0 && id < (IdT)V;
             ids32[rk + k] = ok ? (int)id : -1;
-            if (ok) m = fmaxf(m, teacher[rk + k] * inv_tau);
+            if (ok) m = fmaxf(m, teacher[rk + k]);
             any = any || ok;
         }
         m = warp_max(m);
         any = __any_sync(kFull, any);
         __syncwarp();  // this row's ids32 are read by other lanes below
-        const float m0 = m == -INFINITY ? 0.f : m;
         float sum = 0.f;
         for (int k = lane; k < K; k += 32)
-            if (ids32[rk + k] >= 0) sum += expf(teacher[rk + k] * inv_tau - m0);
-        const float lse = m0 + logf(warp_sum(sum));
+            if (ids32[rk + k] >= 0) sum += expf((teacher[rk + k] - m) / tau);
+        sum = warp_sum(sum);
+        const float log_sum = logf(sum);
         for (int k = lane; k < K; k += 32) {
-            const float lp = ids32[rk + k] >= 0 ? teacher[rk + k] * inv_tau - lse : -INFINITY, p = expf(lp);
-            plogp[rk + k] = make_float2(p, p == 0.f ? 0.f : p * lp);
+            const bool ok = ids32[rk + k] >= 0;
+            const float d = ok ? (teacher[rk + k] - m) / tau : 0.f, p = ok ? expf(d) / sum : 0.f;
+            plogp[rk + k] = make_float2(p, p == 0.f ? 0.f : p * (d - log_sum));
         }
         __syncwarp();
         // p of equal entries summed in list order (every repeat gets the same sum)
@@ -458,9 +461,11 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
             ++n;
             const float inv = 1.f / l, scale = row_scale(r, w);
             if (a.loss_rows && rank == 0) {
-                const float log_l = logf(l), inv_tau = 1.f / a.tau;
-                auto term = [&](float2 x, float zk) {  // a teacher's NaN shows, an entry of p = 0 counts nothing
-                    return x.x == 0.f ? 0.f : x.y - x.x * ((zk - m) * inv_tau - log_l);
+                const float log_l = logf(l);
+                // tau times an entry's share, which no small tau takes out of range; a teacher's NaN shows, an entry
+                // of p = 0 counts nothing
+                auto term = [&](float2 x, float zk) {
+                    return x.x == 0.f ? 0.f : a.tau * x.y - x.x * ((zk - m) - a.tau * log_l);
                 };
                 float sum = 0.f;
 #pragma unroll
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
                     if (vk >= 0) sum += term(a.plogp[e], to_f32(row.z[vk]));
                 }
                 sum = warp_sum(sum);
-                if (lane == 0) a.loss_rows[r] = sum * a.tau * a.tau;
+                if (lane == 0) a.loss_rows[r] = sum * a.tau;
             }
             if (a.dz) {
 #pragma unroll
@@ -755,14 +760,13 @@ cudaError_t launch_logit_distill_fwd(const LogitDistillArgs& a, cudaStream_t str
     double* wsum = const_cast<double*>(r.wsum);
     float *weight = const_cast<float*>(r.weight), *ptot = const_cast<float*>(r.ptot);
     float2* plogp = const_cast<float2*>(r.plogp);
-    const float inv_tau = 1.f / a.tau;
     if (a.ids_are_64)
         distill_prep_kernel<int64_t><<<r.prep_blocks, kPrepThreads, 0, stream>>>(
-            a.teacher, static_cast<const int64_t*>(a.ids), a.row_weight, r.T, a.V, a.K, inv_tau, r.counter, wsum, weight,
+            a.teacher, static_cast<const int64_t*>(a.ids), a.row_weight, r.T, a.V, a.K, a.tau, r.counter, wsum, weight,
             plogp, ptot, const_cast<int*>(r.ids));
     else
         distill_prep_kernel<int32_t><<<r.prep_blocks, kPrepThreads, 0, stream>>>(
-            a.teacher, static_cast<const int32_t*>(a.ids), a.row_weight, r.T, a.V, a.K, inv_tau, r.counter, wsum, weight,
+            a.teacher, static_cast<const int32_t*>(a.ids), a.row_weight, r.T, a.V, a.K, a.tau, r.counter, wsum, weight,
             plogp, ptot, const_cast<int*>(r.ids));
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
