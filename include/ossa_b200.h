@@ -268,7 +268,7 @@ OSSA_API int ossa_router_distill_grad(const void* q, const void* k, int dtype,
 /*
  * ossa_topk_attention_fwd_rows under score modifiers.  No counterpart in the reference.
  * With x = (q_i . k_j) * scale, i = q_start + row:
- *   s = softcap * tanh(x / softcap)   (softcap 0: s = x)
+ *   s = softcap * tanh(x / softcap)   (softcap 0: s = x; else at least 2^-126)
  *   s = s - slopes[h] * |i - j|       (slopes (H,) fp32, NULL: none)
  * and key j is seen by row i of batch element b when (not causal, or j <= i, or
  * j < prefix_len[b]) and segments[b][j] == segments[b][i] (prefix_len (B,), segments
@@ -340,7 +340,7 @@ OSSA_API int ossa_qk_norm_rope_bwd(const void* q, const void* k, const void* wq,
  * NULL, each row's unweighted loss (0 where the row weighs 0), the total, and
  * dlogits = d total / d z (contiguous (rows, V), the logits' dtype).  The backward writes dlogits
  * times `grad` (one value, or one per row) from the workspace that the forward left; with
- * skip_if_one it leaves dlogits untouched when the one value is 1.  K <= 1024.
+ * skip_if_one it leaves dlogits untouched when the one value is 1.  K <= 1024, temperature >= 2^-126.
  */
 OSSA_API size_t ossa_top_logit_distill_workspace_size(long long rows, int K);
 OSSA_API int ossa_top_logit_distill_fwd(const void* logits, int dtype, int outer, int inner, int V,

@@ -5,6 +5,7 @@
 #include "kernels.h"
 
 #include <atomic>
+#include <float.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -291,7 +292,8 @@ static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int 
     if (K < 0) return fail(OSSA_ERR_INVALID, "bad K=%d", K);
     if (idx_is_64 != 0 && idx_is_64 != 1) return fail(OSSA_ERR_INVALID, "idx_is_64 must be 0 or 1");
     if (!isfinite(scale)) return fail(OSSA_ERR_INVALID, "scale must be finite");
-    if (!isfinite(softcap) || softcap < 0.f) return fail(OSSA_ERR_INVALID, "softcap must be finite and >= 0");
+    if (!isfinite(softcap) || softcap < 0.f || (softcap > 0.f && softcap < FLT_MIN))  // below, 1 / softcap overflows
+        return fail(OSSA_ERR_INVALID, "softcap must be 0, or finite and at least 2^-126");
     if (segments && (long long)q_start + Nq > Nk)
         return fail(OSSA_ERR_INVALID, "segments need every query position below Nk=%d (rows end at %lld)", Nk,
                     (long long)q_start + Nq);
@@ -509,8 +511,8 @@ static int check_logit_distill(const void* logits, int dtype, int outer, int inn
     if (V > (1 << 30) || (long long)outer * inner > (1ll << 30))
         return fail(OSSA_ERR_UNSUPPORTED, "shape too large rows=%dx%d V=%d", outer, inner, V);
     if (ids_are_64 != 0 && ids_are_64 != 1) return fail(OSSA_ERR_INVALID, "ids_are_64 must be 0 or 1");
-    if (!(temperature > 0.f) || !isfinite(temperature))
-        return fail(OSSA_ERR_INVALID, "temperature must be finite and > 0");
+    if (!(temperature >= FLT_MIN) || !isfinite(temperature))  // below, log2(e) / temperature overflows
+        return fail(OSSA_ERR_INVALID, "temperature must be finite and at least 2^-126");
     if ((long long)outer * inner == 0) return fail(OSSA_ERR_INVALID, "empty input (no rows)");
     if (!logits || !ids) return fail(OSSA_ERR_INVALID, "null pointer argument");
     const uintptr_t es = dtype == OSSA_F32 ? 4 : 2;

@@ -33,6 +33,8 @@ from . import _lib
 # is usable.  Here the fused sm_100a kernel is the only implementation.
 HAS_TRITON = True
 
+_F32 = torch.finfo(torch.float32)
+
 
 def _check(q, k, v, idx, rows=False):
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -81,7 +83,7 @@ def topk_attention(
     Nk keys k, v hold in full; row l is masked causally against q_start + l.
 
     Score modifiers (additive), x the scaled score of a query at position i and key j:
-    ``softcap``: x becomes softcap * tanh(x / softcap).
+    ``softcap``: x becomes softcap * tanh(x / softcap); at least 2^-126 and finite in float32.
     ``slopes`` (H,): slopes[h] * abs(i - j) is subtracted after the cap.
     ``segments`` (B, Nk) or (Nk,), int32 or int64 (compared as 32-bit values): a key is
     seen only from its own segment; every query position must be below Nk.
@@ -155,8 +157,8 @@ def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, seg
     cap = 0.0
     if softcap is not None:
         cap = float(softcap)
-        if not (0.0 < cap < math.inf):
-            raise ValueError(f"softcap must be positive and finite, got {softcap}")
+        if not (_F32.tiny <= cap <= _F32.max):  # as the kernels hold it
+            raise ValueError(f"softcap must lie in the normal range of float32, got {softcap}")
     if slopes is not None:
         if tuple(slopes.shape) != (H,) or not slopes.is_floating_point():
             raise ValueError(f"slopes must be ({H},) floating point; got {tuple(slopes.shape)} {slopes.dtype}")

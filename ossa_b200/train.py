@@ -38,6 +38,8 @@ from .select import _as_kernel_input, _check_qk, _common_dtype, oracle_topk
 
 __all__ = ["dense_topk_targets", "distillation_loss", "top_logit_distillation_loss"]
 
+_F32 = torch.finfo(torch.float32)
+
 
 def dense_topk_targets(q: torch.Tensor, k: torch.Tensor, top_k: int) -> torch.Tensor:
     """Top-k keys of the causal dense attention softmax(q k^T / sqrt(D)) per
@@ -137,8 +139,8 @@ def top_logit_distillation_loss(logits: torch.Tensor, teacher_logits: torch.Tens
     if row_weight is not None and row_weight.shape != lead:
         raise ValueError(f"row_weight {tuple(row_weight.shape)} does not match the rows {tuple(lead)}")
     tau = float(temperature)
-    if not 0.0 < tau < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not _F32.tiny <= tau <= _F32.max:  # as the kernels hold it
+        raise ValueError(f"temperature must be positive, in the normal range of float32; got {temperature}")
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
     _lib.require_cuda(*[t for t in (logits, teacher_logits, teacher_indices, row_weight) if t is not None])
