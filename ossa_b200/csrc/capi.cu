@@ -525,7 +525,7 @@ static int check_logit_distill(const void* logits, int dtype, int outer, int inn
 }
 
 size_t ossa_top_logit_distill_workspace_size(long long rows, int K) {
-    if (rows < 0 || K <= 0) return 0;
+    if (rows < 0 || rows > (1ll << 30) || K <= 0 || K > 1024) return 0;  // refused by the calls
     return ossa::logit_distill_workspace_bytes(rows, K);
 }
 

@@ -1,9 +1,9 @@
-"""Arguments that fp32 cannot hold are refused, not rounded to another meaning."""
+"""Arguments that fp32 cannot hold are refused, not rounded to another meaning; sizes that are refused get no workspace."""
 
 import pytest
 import torch
 
-from ossa_b200 import top_logit_distillation_loss, topk_attention
+from ossa_b200 import _lib, top_logit_distillation_loss, topk_attention
 from test_operators_cpu import BF, INF, INV, _distill, _mod_bwd, _mod_fwd, _qkv
 
 
@@ -28,3 +28,8 @@ def test_temperatures_outside_fp32(tau):
         small = float(torch.tensor(tau, dtype=torch.float32))
         for fn in ("fwd", "bwd"):
             assert _distill(fn, tau=small) == INV
+
+
+def test_the_distillation_workspace_of_refused_sizes():
+    size = _lib.lib().ossa_top_logit_distill_workspace_size
+    assert size(10, 1024) > 0 and size(10, 1025) == 0 and size((1 << 30) + 1, 4) == 0
