@@ -363,12 +363,17 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
     __shared__ double s_sum[kBlock / 32];
     __shared__ bool s_last;
     const float c = kLog2e / a.tau;
-    float unit = 1.f;  // what a unit of row weight counts in the total
+    // What a unit of row weight counts in the total, times 2^-up: where fp32 does not hold the inverse of the weights' sum,
+    // a power of two goes over to the incoming gradient.
+    float unit = 1.f;
+    int up = 0;
     if (a.mean) {
         double w = 0.0;
         for (int i = tid; i < a.prep_blocks; i += kBlock) w += a.wsum[i];
         w = block_sum(w, s_sum);
-        unit = w != 0.0 ? (float)(1.0 / w) : 0.f;
+        if (w < 0x1p-100) up = 100;
+        else if (w > 0x1p+100) up = -100;
+        unit = w != 0.0 ? (float)(1.0 / scalbn(w, up)) : 0.f;
     }
     if (C > 1) {
         if (tid == 0) {
@@ -378,8 +383,8 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
         }
         cluster.sync();  // every CTA has begun: its shared memory may be written from another
     }
-    const float g_all = a.grad && a.grad_step == 0 ? *a.grad : 1.f;
-    auto row_scale = [&](int r, float w) { return (a.grad && a.grad_step ? a.grad[r] : g_all) * w * unit * a.tau; };
+    const float g_all = scalbnf(a.grad && a.grad_step == 0 ? *a.grad : 1.f, up);
+    auto row_scale = [&](int r, float w) { return (a.grad && a.grad_step ? scalbnf(a.grad[r], up) : g_all) * w * unit * a.tau; };
     auto weight_at = [&](int r) { return r < a.T ? a.weight[r] : 0.f; };
     // The barrier behind a row's sums: the list warp and the others reach it from different places.
     auto row_barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kBlock) : "memory"); };
@@ -641,7 +646,7 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
         if (w != 0.f) t += (double)w * (double)__ldcg(a.loss_rows + r);
     }
     t = block_sum(t, s_sum);
-    if (tid == 0) *a.loss = (float)(t * (double)unit);
+    if (tid == 0) *a.loss = (float)(scalbn(t, up) * (double)unit);
 }
 
 // Cluster size and vectors per thread.  A row of `vecs` vectors wants the fewest CTAs that hold it in at
