@@ -15,13 +15,17 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
+#include <mutex>
 #include <optional>
 #include <stdexcept>
 #include <string>
 #include <tuple>
+#include <utility>
 
 #include "ossa_b200.h"
 
@@ -303,60 +307,85 @@ struct Logits {
     int64_t rows() const { return (int64_t)outer * inner; }
 };
 
-struct TopLogitDistill : torch::autograd::Function<TopLogitDistill> {
-    // reduction: 0 none, 1 sum, 2 mean
-    static Tensor forward(AutogradContext* ctx, const Tensor& z, const Tensor& teacher, const Tensor& ids,
-                          const Maybe& weight_, double tau, int64_t reduction, bool grad) {
+// Its own node: the gradient taken with the loss is held as a saved variable, so that hooks (checkpointing, offloading)
+// and the graph's release reach it, and is given away by the first backward pass, which a list of saved variables cannot do.
+struct TopLogitDistillBackward : torch::autograd::Node {
+    torch::autograd::SavedVariable z, ids, ws, dz;
+    bool taken = false;  // dz waits for its first backward pass
+    double tau = 1.0;
+    int64_t reduction = 0;  // 0 none, 1 sum, 2 mean
+
+    std::string name() const override { return "TopLogitDistillBackward"; }
+
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (auto* v : {&z, &ids, &ws, &dz}) v->reset_data();
+    }
+
+    variable_list apply(variable_list&& g) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        const bool graph = at::GradMode::is_enabled();
+        at::AutoGradMode off(false);
+        if (!g[0].defined()) return {Tensor()};
+        // the saved logits may come back in another place and layout (offloading): rows are taken anew
+        const Logits l(z.unpack());
+        const Tensor list = ids.unpack(), work = ws.unpack(), up = g[0].contiguous();  // fp32, as the loss
+        const bool first = std::exchange(taken, false);
+        Tensor out;
+        if (first) {
+            out = dz.unpack();
+            dz.reset_data();
+        } else {
+            out = at::empty({l.rows(), l.V}, l.z.options());
+        }
+        {
+            On on(l.z);
+            check(ossa_top_logit_distill_bwd(in(l.z), dtype_code(l.z), l.outer, l.inner, l.V, l.so, l.si, in(list), is_64(list),
+                                             i32(list.size(1)), (float)tau, reduction == 2 ? 1 : 0, in_as<float>(up),
+                                             reduction == 0 ? 1 : 0, first ? 1 : 0, to(out), in(work), (size_t)work.numel(),
+                                             on.stream));
+        }
+        return once({out.view(l.z.sizes())}, g, graph, true);
+    }
+};
+
+Tensor top_logit_distill(const Tensor& z, const Tensor& teacher, const Tensor& ids, const Maybe& weight_, double tau,
+                         int64_t reduction, bool grad) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!z._fw_grad(0).defined(), "top_logit_distillation_loss has no forward-mode derivative");
+    const bool each = reduction == 0;
+    Tensor loss, ws, dz;
+    {
+        at::AutoGradMode off(false);
         const Logits l(z);
         const Tensor weight = opt(weight_);
         const int K = i32(ids.size(1));
-        const bool each = reduction == 0;
         const size_t n = ossa_top_logit_distill_workspace_size(l.rows(), K);
-        Tensor ws = bytes(n, z), dz;
+        ws = bytes(n, z);
         const auto f32 = z.options().dtype(at::kFloat);
-        Tensor loss = each ? at::empty({l.rows()}, f32) : at::empty({}, f32);
+        loss = each ? at::empty({l.rows()}, f32) : at::empty({}, f32);
         // a single incoming gradient is 1 as a rule: the gradient is taken with the loss
         if (grad && !each) dz = at::empty({l.rows(), l.V}, z.options());
-        {
-            On on(z);
-            check(ossa_top_logit_distill_fwd(in(l.z), dtype_code(z), l.outer, l.inner, l.V, l.so, l.si, in_as<float>(teacher),
-                                             in(ids), is_64(ids), K, (float)tau, in_as<float>(weight), reduction == 2 ? 1 : 0,
-                                             each ? to_f32(loss) : nullptr, each ? nullptr : to_f32(loss), to(dz), to(ws), n,
-                                             on.stream));
-        }
-        if (grad) {
-            ctx->save_for_backward({z, ids});
-            ctx->saved_data["ws"] = ws;
-            ctx->saved_data["dz"] = dz;
-            ctx->saved_data["tau"] = tau;
-            ctx->saved_data["reduction"] = reduction;
-        }
+        On on(z);
+        check(ossa_top_logit_distill_fwd(in(l.z), dtype_code(z), l.outer, l.inner, l.V, l.so, l.si, in_as<float>(teacher),
+                                         in(ids), is_64(ids), K, (float)tau, in_as<float>(weight), reduction == 2 ? 1 : 0,
+                                         each ? to_f32(loss) : nullptr, each ? nullptr : to_f32(loss), to(dz), to(ws), n,
+                                         on.stream));
         if (each && weight.defined()) loss.mul_(weight);
-        return loss;
     }
-
-    static variable_list backward(AutogradContext* ctx, variable_list g) {
-        const bool graph = at::GradMode::is_enabled();
-        at::AutoGradMode off(false);
-        const variable_list s = ctx->get_saved_variables();
-        // the saved logits may come back in another place and layout (offloading): rows are taken anew
-        const Logits l(s[0]);
-        const Tensor &ids = s[1], ws = ctx->saved_data["ws"].toTensor(), up = g[0].contiguous();  // fp32, as the loss
-        const int64_t reduction = ctx->saved_data["reduction"].toInt();
-        Tensor dz = ctx->saved_data["dz"].toTensor();
-        ctx->saved_data["dz"] = Tensor();  // a second backward pass makes its own
-        const bool taken = dz.defined();
-        if (!taken) dz = at::empty({l.rows(), l.V}, l.z.options());
-        On on(l.z);
-        check(ossa_top_logit_distill_bwd(in(l.z), dtype_code(l.z), l.outer, l.inner, l.V, l.so, l.si, in(ids), is_64(ids),
-                                         i32(ids.size(1)), (float)ctx->saved_data["tau"].toDouble(), reduction == 2 ? 1 : 0,
-                                         in_as<float>(up), reduction == 0 ? 1 : 0, taken ? 1 : 0, to(dz), in(ws),
-                                         (size_t)ws.numel(), on.stream));
-        variable_list out(7);
-        out[0] = dz.view(l.z.sizes());
-        return once(std::move(out), g, graph, true);
+    if (grad) {
+        std::shared_ptr<TopLogitDistillBackward> node(new TopLogitDistillBackward, torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(z));
+        node->z = torch::autograd::SavedVariable(z, false);
+        node->ids = torch::autograd::SavedVariable(ids, false);
+        node->ws = torch::autograd::SavedVariable(ws, false);
+        node->taken = dz.defined();
+        if (dz.defined()) node->dz = torch::autograd::SavedVariable(dz, false);
+        node->tau = tau;
+        node->reduction = reduction;
+        torch::autograd::set_history(loss, node);
     }
-};
+    return loss;
+}
 
 }  // namespace
 
@@ -383,7 +412,5 @@ PYBIND11_MODULE(_autograd, m) {
                                bool grad) {
         return TopkAttention::apply(q, k, v, slopes, idx, segments, prefix, causal, q0, cap, grad);
     }, NoGil());
-    m.def("top_logit_distill", [](T z, T teacher, T ids, O weight, double tau, int64_t reduction, bool grad) {
-        return TopLogitDistill::apply(z, teacher, ids, weight, tau, reduction, grad);
-    }, NoGil());
+    m.def("top_logit_distill", &top_logit_distill, NoGil());
 }
