@@ -1,4 +1,4 @@
-"""Builds libossa_b200.so (the sm_100a kernels behind the C ABI) and _autograd.so (the trainable
+"""Builds libossa_b200.so (the sm_100a kernels behind the C ABI) and _autograd.<abi>.so (the trainable
 operators' autograd nodes, over that library and torch's) in-tree.
 
 Run ``python -m ossa_b200.build`` or call :func:`build`.  Both are written next to this file so
@@ -7,13 +7,14 @@ that they travel with the source tree; nothing is installed into site-packages a
 
 from __future__ import annotations
 
-import importlib.util
 import os
 import shutil
 import subprocess
 import sys
 import sysconfig
 from pathlib import Path
+
+import torch
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
@@ -22,7 +23,15 @@ INCLUDE = REPO_DIR / "include"
 LIB_NAME = "libossa_b200.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 AUTOGRAD_SRC = CSRC / "autograd.cpp"
-AUTOGRAD_PATH = PKG_DIR / "_autograd.so"
+
+
+def _autograd_name() -> str:
+    """The interpreter's and torch's versions are in the module's name: it is bound to the C++ ABI of both, and one
+    built for others is not taken."""
+    return f"_autograd.{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}.so"
+
+
+AUTOGRAD_PATH = PKG_DIR / _autograd_name()
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -65,10 +74,10 @@ def is_stale() -> bool:
 
 
 def build_autograd(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles ``csrc/autograd.cpp`` against torch's headers and links ``_autograd.so`` to the library."""
+    """Compiles ``csrc/autograd.cpp`` against torch's headers and links the module to the library."""
     if not force and not autograd_is_stale():
         return AUTOGRAD_PATH
-    torch_dir = Path(importlib.util.find_spec("torch").origin).parent
+    torch_dir = Path(torch.__file__).resolve().parent
     inc, nvcc = torch_dir / "include", Path(_nvcc()).resolve()
     tmp = AUTOGRAD_PATH.with_suffix(f".{os.getpid()}.tmp")
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-I{INCLUDE}",
@@ -86,7 +95,7 @@ def build_autograd(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compiles every ``csrc/*.cu`` for sm_100a, links ``libossa_b200.so`` and builds ``_autograd.so`` on it."""
+    """Compiles every ``csrc/*.cu`` for sm_100a, links ``libossa_b200.so`` and builds the autograd module on it."""
     _build_library(force, verbose)
     build_autograd(force, verbose)
     return LIB_PATH
