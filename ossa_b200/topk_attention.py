@@ -173,6 +173,8 @@ def _topk_attention_modified(q, k, v, idx, causal, q_start, softcap, slopes, seg
             if prefix_len < 0:
                 raise ValueError(f"prefix_len must be >= 0, got {prefix_len}")
             prefix_len = torch.full((B,), min(prefix_len, Nk), dtype=torch.int32, device=q.device)
+        elif isinstance(prefix_len, torch.Tensor) and prefix_len.dtype == torch.int64:
+            prefix_len = prefix_len.clamp(0, Nk)  # a length past 32 bits is still one
         prefix_len = _int32("prefix_len", prefix_len, [(B,)]).contiguous()
     _lib.dtype_code(q)
     _lib.require_cuda(*[t for t in (q, k, v, idx, slopes, segments, prefix_len) if t is not None])

@@ -1,9 +1,9 @@
-"""Arguments at the ends of their ranges: weights whose sum leaves the range of fp32."""
+"""Arguments at the ends of their ranges: prefix lengths past 32 bits, weights whose sum leaves the range of fp32."""
 
 import pytest
 import torch
 
-from ossa_b200 import top_logit_distillation_loss
+from ossa_b200 import top_logit_distillation_loss, topk_attention
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -11,6 +11,18 @@ DEV = "cuda:0"
 
 def _gen(seed):
     return torch.Generator().manual_seed(seed)
+
+
+def test_prefix_lengths_past_32_bits():
+    """An int64 length is compared as the number it is: past the last key it opens every key."""
+    B, H, N, D, K = 4, 2, 30, 64, 9
+    g = _gen(1)
+    q, k, v = (torch.randn(B, H, N, D, generator=g).to(DEV) for _ in range(3))
+    idx = torch.randint(0, N, (B, H, N, K), generator=g).to(DEV)
+    lengths = torch.tensor([2 ** 31, 2 ** 40 + 3, -2 ** 40 + 5, 7])
+    want = topk_attention(q, k, v, topk_indices=idx, prefix_len=torch.tensor([N, N, 0, 7], device=DEV))
+    assert torch.equal(topk_attention(q, k, v, topk_indices=idx, prefix_len=lengths.to(DEV)), want)
+    assert torch.equal(want[0], topk_attention(q[:1], k[:1], v[:1], topk_indices=idx[:1], causal=False)[0])
 
 
 @pytest.mark.parametrize("scale", [2.0 ** -138, 2.0 ** 125])
