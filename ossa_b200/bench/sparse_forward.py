@@ -71,7 +71,7 @@ def _norms_as(norm, weight, eps):
 def _head_norms(layer_module):
     """(q weight, k weight, eps) of the layer's query and key head norms, None if it has none."""
     norms = [getattr(layer_module, name, None) for name in ("q_norm", "k_norm")]
-    if norms == [None, None]:
+    if all(norm is None or isinstance(norm, torch.nn.Identity) for norm in norms):
         return None
     eps = []
     for norm in norms:
