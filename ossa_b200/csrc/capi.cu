@@ -63,6 +63,10 @@ int cuda_status(cudaError_t e, const char* what) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether every pointer (NULL too) lies on a boundary of n bytes.
+template <typename... P>
+bool aligned_to(uintptr_t n, const P*... p) { return (... && (reinterpret_cast<uintptr_t>(p) % n == 0)); }
+
 constexpr size_t kAlign = 256;
 size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
 
@@ -282,7 +286,8 @@ static constexpr long long kMaxTurned = 1ll << 30;
 
 // The checks that the modified gather and its backward share.
 static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int D, int K, int idx_is_64, float scale,
-                          int q_start, float softcap, const int32_t* segments) {
+                          int q_start, float softcap, const float* slopes, const int32_t* segments,
+                          const int32_t* prefix_len, const float* lse2) {
     int st = check_heads(B, H, Hkv, Nk);
     if (st) return st;
     if ((st = check_rows(Nq, Nk, q_start))) return st;
@@ -298,6 +303,8 @@ static int check_modified(int dtype, int B, int H, int Hkv, int Nq, int Nk, int 
         return fail(OSSA_ERR_INVALID, "segments need every query position below Nk=%d (rows end at %lld)", Nk,
                     (long long)q_start + Nq);
     if ((long long)B * Hkv > 65535) return fail(OSSA_ERR_UNSUPPORTED, "B * Hkv = %lld > 65535", (long long)B * Hkv);
+    if (!aligned_to(4, slopes, segments, prefix_len, lse2))
+        return fail(OSSA_ERR_INVALID, "slopes, segments, prefix_len and lse2 must be aligned to their types");
     return OSSA_OK;
 }
 
@@ -312,7 +319,8 @@ int ossa_topk_attention_mod_fwd(const void* q, const void* k, const void* v, con
                                 int q_start, float softcap, const float* slopes, const int32_t* segments,
                                 const int32_t* prefix_len, void* out, float* lse2, void* out_rest,
                                 ossa_stream_t stream) {
-    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
+    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, slopes, segments,
+                            prefix_len, lse2);
     if (st) return st;
     if ((long long)B * H * Nq == 0) return OSSA_OK;
     if (Nk == 0) return fail(OSSA_ERR_INVALID, "query rows need at least one key (Nk=0)");
@@ -345,9 +353,11 @@ int ossa_topk_attention_bwd(const void* q, const void* k, const void* v, const v
                             float softcap, const float* slopes, const int32_t* segments, const int32_t* prefix_len,
                             const void* out, const float* lse2, const void* out_rest, const void* dout, void* dq,
                             void* dk, void* dv, float* dslopes, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
-    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, segments);
+    int st = check_modified(dtype, B, H, Hkv, Nq, Nk, D, K, idx_is_64, scale, q_start, softcap, slopes, segments,
+                            prefix_len, lse2);
     if (st) return st;
     if (dslopes && !slopes) return fail(OSSA_ERR_INVALID, "dslopes without slopes");
+    if (!aligned_to(4, dslopes)) return fail(OSSA_ERR_INVALID, "dslopes is not aligned to its type");
     if ((long long)(H / Hkv) * Nq * K > kMaxTurned)
         return fail(OSSA_ERR_UNSUPPORTED, "(H / Hkv) * Nq * K = %lld > 2^30 listed keys per kv head",
                     (long long)(H / Hkv) * Nq * K);
@@ -409,6 +419,7 @@ static int check_norm_rope(const void* q, const void* k, const void* wq, const v
         return fail(OSSA_ERR_INVALID, "row strides must be multiples of 16 bytes");
     if (!aligned16(q) || !aligned16(k) || !aligned16(cos) || !aligned16(sin))
         return fail(OSSA_ERR_INVALID, "q, k, cos and sin must be 16-byte aligned");
+    if (!aligned_to(w_dtype == OSSA_F32 ? 4 : 2, wq, wk)) return fail(OSSA_ERR_INVALID, "weights are not aligned to their type");
     return OSSA_OK;
 }
 
@@ -456,6 +467,8 @@ int ossa_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const vo
     int st = check_norm_rope(q, k, wq, wk, cos, sin, dtype, w_dtype, B, N, Hq, Hk, D, q_sb, q_sn, k_sb, k_sn, eps);
     if (st) return st;
     if ((dwq && !wq) || (dwk && !wk)) return fail(OSSA_ERR_INVALID, "a weight gradient without its weight");
+    if (!aligned_to(w_dtype == OSSA_F32 ? 4 : 2, dwq, dwk))
+        return fail(OSSA_ERR_INVALID, "weight gradients are not aligned to their type");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if ((long long)B * N == 0) {
         const size_t wn = (size_t)D * (w_dtype == OSSA_F32 ? 4 : 2);
@@ -503,7 +516,8 @@ int ossa_qk_norm_rope_bwd(const void* q, const void* k, const void* wq, const vo
 
 // The checks that the top-logit distillation's forward and backward share.
 static int check_logit_distill(const void* logits, int dtype, int outer, int inner, int V, const void* ids,
-                               int ids_are_64, int K, float temperature, void* workspace, size_t workspace_bytes) {
+                               int ids_are_64, int K, float temperature, const void* dlogits, void* workspace,
+                               size_t workspace_bytes) {
     if (!valid_dtype(dtype)) return fail(OSSA_ERR_INVALID, "bad dtype %d", dtype);
     if (outer < 0 || inner < 0 || V <= 0 || K <= 0)
         return fail(OSSA_ERR_INVALID, "bad shape rows=%dx%d V=%d K=%d", outer, inner, V, K);
@@ -516,7 +530,8 @@ static int check_logit_distill(const void* logits, int dtype, int outer, int inn
     if ((long long)outer * inner == 0) return fail(OSSA_ERR_INVALID, "empty input (no rows)");
     if (!logits || !ids) return fail(OSSA_ERR_INVALID, "null pointer argument");
     const uintptr_t es = dtype == OSSA_F32 ? 4 : 2;
-    if (reinterpret_cast<uintptr_t>(logits) % es) return fail(OSSA_ERR_INVALID, "logits are not aligned to their type");
+    if (!aligned_to(es, logits, dlogits)) return fail(OSSA_ERR_INVALID, "logits are not aligned to their type");
+    if (!aligned_to(ids_are_64 ? 8 : 4, ids)) return fail(OSSA_ERR_INVALID, "ids are not aligned to their type");
     const size_t need = ossa::logit_distill_workspace_bytes((long long)outer * inner, K);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return fail(OSSA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) required, got %zu", need,
@@ -533,10 +548,12 @@ int ossa_top_logit_distill_fwd(const void* logits, int dtype, int outer, int inn
                                long long stride_inner, const float* teacher, const void* ids, int ids_are_64, int K,
                                float temperature, const float* row_weight, int mean, float* loss_rows, float* loss,
                                void* dlogits, void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
-    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature, workspace,
+    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature, dlogits, workspace,
                                  workspace_bytes);
     if (st) return st;
     if (!teacher || (!loss_rows && !loss)) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned_to(4, teacher, row_weight, loss_rows, loss))
+        return fail(OSSA_ERR_INVALID, "teacher, row_weight and losses must be aligned to their type");
     ossa::LogitDistillArgs a{};
     a.z = logits;
     a.sb = stride_outer;
@@ -564,10 +581,11 @@ int ossa_top_logit_distill_bwd(const void* logits, int dtype, int outer, int inn
                                long long stride_inner, const void* ids, int ids_are_64, int K, float temperature,
                                int mean, const float* grad, int grad_per_row, int skip_if_one, void* dlogits,
                                const void* workspace, size_t workspace_bytes, ossa_stream_t stream) {
-    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature,
+    int st = check_logit_distill(logits, dtype, outer, inner, V, ids, ids_are_64, K, temperature, dlogits,
                                  const_cast<void*>(workspace), workspace_bytes);
     if (st) return st;
     if (!grad || !dlogits) return fail(OSSA_ERR_INVALID, "null pointer argument");
+    if (!aligned_to(4, grad)) return fail(OSSA_ERR_INVALID, "grad is not aligned to its type");
     if (skip_if_one && grad_per_row) return fail(OSSA_ERR_INVALID, "skip_if_one needs a single gradient value");
     ossa::LogitDistillArgs a{};
     a.z = logits;
