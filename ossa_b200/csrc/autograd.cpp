@@ -74,6 +74,14 @@ Tensor packed(const Tensor& t) {
     return on_16(c) ? c : c.clone();
 }
 
+// The saved tensors of a backward pass: hooks (checkpointing, offloading, compression) may bring them back in another
+// place and layout, and the C ABI takes addresses.
+variable_list saved(AutogradContext* ctx) {
+    variable_list s = ctx->get_saved_variables();
+    for (Tensor& t : s) t = packed(t);
+    return s;
+}
+
 Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
 
 // Operands that may be absent: an undefined tensor is no argument of a node's forward.
@@ -172,10 +180,8 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
         at::AutoGradMode off(false);
         variable_list out(10);
         if (!g[0].defined() && !g[1].defined()) return out;
-        // saved tensors may come back as others than were saved (checkpointing, offloading): their
-        // places and strides are taken anew
-        const variable_list s = ctx->get_saved_variables();
-        const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3], &cos = s[4], &sin = s[5], none;
+        const variable_list s = ctx->get_saved_variables();  // q and k as rows, wherever they lie now
+        const Tensor &q = s[0], &k = s[1], wq = packed(s[2]), wk = packed(s[3]), cos = packed(s[4]), sin = packed(s[5]), none;
         const Rows a(q, ctx->saved_data["Hq"].toInt()), b(k, ctx->saved_data["Hk"].toInt());
         const double eps = ctx->saved_data["eps"].toDouble();
         Tensor gq, gk;
@@ -217,7 +223,7 @@ struct RopeToHeads : torch::autograd::Function<RopeToHeads> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const bool graph = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
-        const variable_list s = ctx->get_saved_variables();
+        const variable_list s = saved(ctx);
         const Tensor gq = packed(g[0]), none;
         Tensor dx = at::empty(ctx->saved_data["shape"].toIntVector(), gq.options());
         Rows a;
@@ -262,7 +268,7 @@ struct TopkAttention : torch::autograd::Function<TopkAttention> {
     static variable_list backward(AutogradContext* ctx, variable_list g) {
         const bool graph = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
-        const variable_list s = ctx->get_saved_variables();
+        const variable_list s = saved(ctx);
         const Tensor &q = s[0], &k = s[1], &v = s[2], &slopes = s[3], &idx = s[4], &segments = s[5], &prefix = s[6];
         const bool causal = ctx->saved_data["causal"].toBool();
         const int64_t q0 = ctx->saved_data["q0"].toInt();
@@ -327,13 +333,12 @@ struct TopLogitDistillBackward : torch::autograd::Node {
         const bool graph = at::GradMode::is_enabled();
         at::AutoGradMode off(false);
         if (!g[0].defined()) return {Tensor()};
-        // the saved logits may come back in another place and layout (offloading): rows are taken anew
-        const Logits l(z.unpack());
-        const Tensor list = ids.unpack(), work = ws.unpack(), up = g[0].contiguous();  // fp32, as the loss
+        const Logits l(z.unpack());  // rows, wherever they lie now
+        const Tensor list = packed(ids.unpack()), work = packed(ws.unpack()), up = g[0].contiguous();  // fp32, as the loss
         const bool first = std::exchange(taken, false);
         Tensor out;
         if (first) {
-            out = dz.unpack();
+            out = packed(dz.unpack());
             dz.reset_data();
         } else {
             out = at::empty({l.rows(), l.V}, l.z.options());
