@@ -51,7 +51,8 @@ class PatchPlan:
     routers: dict[int, ContentRouter] | None = None  # layer_idx -> router
     impl: str = "mask"                 # "mask" (top-K + forced diagonal) | "gather"
     # Score modifiers of every patched layer, as topk_attention takes them (additive).  They act on the
-    # attention, not on the selection: a row's K keys may lie in other documents, which hides them.
+    # attention, not on the selection: a row's K keys may lie in other documents, which hides them (a row of
+    # impl "gather" whose keys all do gives 0).
     softcap: Optional[float] = None
     slopes: Optional[torch.Tensor] = None                    # (H,)
     segments: Optional[torch.Tensor] = None                  # (B, N) or (N,)

@@ -317,7 +317,7 @@ struct Logits {
 // and the graph's release reach it, and is given away by the first backward pass, which a list of saved variables cannot do.
 struct TopLogitDistillBackward : torch::autograd::Node {
     torch::autograd::SavedVariable z, ids, ws, dz;
-    bool taken = false;  // dz waits for its first backward pass
+    bool waiting = false;  // dz is there for the first backward pass
     double tau = 1.0;
     int64_t reduction = 0;  // 0 none, 1 sum, 2 mean
 
@@ -335,7 +335,7 @@ struct TopLogitDistillBackward : torch::autograd::Node {
         if (!g[0].defined()) return {Tensor()};
         const Logits l(z.unpack());  // rows, wherever they lie now
         const Tensor list = packed(ids.unpack()), work = packed(ws.unpack()), up = g[0].contiguous();  // fp32, as the loss
-        const bool first = std::exchange(taken, false);
+        const bool first = std::exchange(waiting, false);
         Tensor out;
         if (first) {
             out = packed(dz.unpack());
@@ -383,7 +383,7 @@ Tensor top_logit_distill(const Tensor& z, const Tensor& teacher, const Tensor& i
         node->z = torch::autograd::SavedVariable(z, false);
         node->ids = torch::autograd::SavedVariable(ids, false);
         node->ws = torch::autograd::SavedVariable(ws, false);
-        node->taken = dz.defined();
+        node->waiting = dz.defined();
         if (dz.defined()) node->dz = torch::autograd::SavedVariable(dz, false);
         node->tau = tau;
         node->reduction = reduction;

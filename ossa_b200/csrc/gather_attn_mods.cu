@@ -15,7 +15,8 @@
 // one after another through the same loop.  So does one whose result is not finite: a key that only some of
 // the heads list has no weight for the others, and 0 times its value row must be 0 there.
 //
-// Bound: shared-memory traffic and issue (16 KB a chunk of 16 keys, 12 KB of it operands).  Measured: packed
+// Bound: shared-memory traffic and issue (16 KB a chunk of 16 keys, 12 KB of it operands): the pipes are busy for 61 % and
+// 52 % of the time, the rest is waits between a chunk's steps.  Measured: packed
 // prefill B=2, 12/2 heads, N=4096, K=64, slopes: 111 us, 39 us of it for the lists, documents and the union of
 // keys (144 of 384 on average, 1.2 GB of key and value rows from L2); N=8192, K=128, B=1: 230 us.
 #include "gather_attn_kernels.cuh"

@@ -4,9 +4,11 @@
 //
 // Measured (B=2, 12/2 heads, N=4096, K=64, half of a row's keys recent: 6.3 M entries): row pass 156 us, of
 // which 57 us for the rows' q, dO, output and lists and the union of keys (144 of 384 on average), key pass
-// 183 us (3.6 M turned entries).  A group of 16 entries of the key pass moves 24 KB through shared memory
-// (8 KB in, 16 KB out as operands): 5.4 GB, 155 us at 128 bytes a cycle and SM, which is what bounds it; the
-// per-head forms of gather_bwd.cu took 752 and 1147 us here.
+// 183 us (3.6 M turned entries); the per-head forms of gather_bwd.cu took 752 and 1147 us here.
+// A group of 16 entries of the key pass moves 24 KB through shared memory (8 KB in, 16 KB out as operands): 5.4 GB, 145 us
+// at 128 bytes a cycle and SM and 1965 MHz, the nearest bound.  Counted, the shared-memory pipe is busy for 51 % of the
+// key pass (67 % of the row pass), the tensor pipe for 26 (15), issue slots for 44 (43): with 12 warps an SM (registers)
+// a group's steps, each waiting for the one before, are not covered whole, and blocks of keys differ in their lists.
 #include <algorithm>
 #include <cstdint>
 

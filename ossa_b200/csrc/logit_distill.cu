@@ -15,11 +15,12 @@
 // walk the rows with a fixed stride, as many as run at once.  Rows too long for that are read twice (kNV = 0).
 // Exponents are taken as exp2((z - max) * log2(e) / tau), the difference first, so that entries at the
 // type's lowest value and rows of them stay finite.
-// Measured, loss and gradient: 4096 x 151936 bf16 (2.49 GB) 602 us, 4.1 TB/s; 4096 x 32000 fp32 211 us, 5.0 TB/s;
-// 16 x 151936 bf16 15 us.  Of the 602 us about 100 go without the two exponentials a value needs, but by their
-// issue, not their unit: a polynomial on the fp32 pipe for a quarter of them gave 601, for half of them 726.
-// The first pass's exponentials kept for the gradient in 2 of a thread's 10 vectors gave 589, in 4 (spills) 647;
-// neither is worth its code.  What is left beside memory is one exchange a row.
+// Measured, loss and gradient: 4096 x 151936 bf16 (2.49 GB) 600 us, 4.1 TB/s; 4096 x 32000 fp32 211 us, 5.0 TB/s;
+// 16 x 151936 bf16 15 us.  No unit bounds the 600: DRAM is busy for 44 % of its peak, the exponentials' unit for 53 % (two a
+// value are 267 us of it at 16 a cycle and SM), issue slots for 45 %.  A CTA's warps take a row's sum, its exchange
+// and its gradient in step, so each of these waits for the others.  Without the exponentials (a probe) 100 us go; a polynomial
+// on the fp32 pipe for a quarter of them gave no change, for half of them +21 %; the first pass's exponentials kept
+// for the gradient in 2 of a thread's 10 vectors -2 %, in 4 (spills) +7 %; neither is worth its code.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -653,7 +654,7 @@ __global__ void __launch_bounds__(kBlock, row_ctas(kNV)) distill_rows_kernel(con
 // most 10 vectors a thread; few rows want more CTAs a row, up to 8, while they leave SMs without work (V =
 // 151936 bf16, clusters of 1, 2, 4, 8: one row 31, 23, 17, 14 us, 64 rows 32, 24, 21, 21).  Rows of more than 16
 // vectors a thread in 8 CTAs (over 262,144 bf16 values) are read twice; where both can run, 4096 x 151936 takes
-// 602 us held and 630 read twice (clusters of 2), 4096 x 32000 fp32 211 and 249.
+// 600 us held and 630 read twice (clusters of 2), 4096 x 32000 fp32 211 and 249.
 void pick(int T, long long vecs, int sms, int* C, int* nv) {
     int c = 1;
     while (c < kMaxCluster && vecs > (long long)c * kThreads * 10) c *= 2;

@@ -12,7 +12,9 @@
 // Measured (12 + 2 heads of 128, bf16; a plain copy runs at 6.45 TB/s): forward B=8, N=4096, 252 MB: 48 us,
 // 5.2 TB/s; backward B=4, N=4096, 185 MB: 48 us, 3.9 TB/s, and 4 us for the join of the weight gradients.
 //
-// Bound: HBM, every row read once and written once.  Layout: D / 16 lanes hold a row, each
+// Bound: HBM, every row read once and written once.  The backward pass does not reach it (60 % of the copy rate): its 16
+// warps an SM load, compute and store a step of two head rows one after another, and nothing covers the loads (the
+// largest part of a warp's waiting).  Layout: D / 16 lanes hold a row, each
 // 8 values of the low and the 8 matching values of the high half (16-byte loads at bf16),
 // so the rotation needs no exchange and the row sum log2(D / 16) shuffles; the lanes of a
 // row keep the position's cos and sin in registers while they walk the heads of a token.

@@ -149,7 +149,7 @@ __device__ __forceinline__ void stage_listed(uint32_t dst, const __nv_bfloat16* 
 
 // 2^x and tanh for the tensor-core forms.  ex2.approx: two units in the last place.  tanh x = 1 - 2 / (1 + e^2x)
 // is good to 2^-22 in absolute terms, which a score of size cap turns into cap * 2^-22; below 1, where most
-// scores of a cap lie, x times a polynomial in x^2 (least maximal relative error there, 2^-23) takes its place.
+// scores of a cap lie, x times a polynomial in x^2 (least maximal relative error there, 2^-22.6) takes its place.
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
