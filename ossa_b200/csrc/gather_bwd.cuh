@@ -43,7 +43,7 @@ struct RowSums {
     __device__ __forceinline__ RowSums(float p, float pd, float f, float xf, float d0) {
         const float inv = p == 0.f ? 0.f : 1.f / p;
         delta = pd * inv;
-        slope = ((delta - d0) * f - xf) * inv;
+        slope = p == 0.f ? 0.f : ((delta - d0) * f - xf) * inv;  // a row that sees nothing may have any dO
     }
 };
 
