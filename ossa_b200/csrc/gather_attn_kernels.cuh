@@ -24,7 +24,7 @@
 //    lane m.  Online softmax in fp32 (exp2 domain), then the same coalesced row
 //    loads of V accumulate p_m * v_m into each lane's dims.
 //  * Masked/padded slots read row 0 (always in bounds) and are zeroed, so the
-//    unrolled load loops carry no branches.
+//    unrolled load loops carry no branches (plain bf16 rows of 128 read a key that the row sees instead).
 //  * kMods compiles the per-head forms with the score modifiers of score_mods.cuh (cap,
 //    distance bias, documents, prefix) and the row statistic the backward pass reads.
 #pragma once
@@ -194,13 +194,21 @@ __device__ __forceinline__ void gather_row_bf16_d128(uint4 qv, const uint4* __re
         const int kk = kc + myslot;
         const long long jl = kk < K ? (long long)irow[kk] : -1ll;
         const bool valid = jl >= 0 && jl < N && rm.sees(jl, i, causal);
-        const int jv = valid ? (int)jl : -1;
+        int jv = valid ? (int)jl : -1;
+        const unsigned some = __ballot_sync(kFull, valid);
+        if (some == 0u) continue;
+        // Masked places have p = 0 and read a key that the row sees: any other row might not be finite.  (Zeros for
+        // their value rows, as with modifiers, cost the plain form a third: B=2, 8 heads, N=4096, K=64: 149 us, 205.)
+        if (!kMods) {
+            const int seen = __shfl_sync(kFull, jv, __ffs(some) - 1);
+            jv = valid ? jv : seen;
+        }
         int js[16];
         float part[16];
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
             js[m] = __shfl_sync(kFull, jv, 16 * half + m);
-            const uint4 kr = __ldg(kb + (size_t)max(js[m], 0) * (D / 8));
+            const uint4 kr = __ldg(kb + (size_t)(kMods ? max(js[m], 0) : js[m]) * (D / 8));
             part[m] = dot8_bf16(qv, kr);
         }
         // lane l of half h now holds key slot 2 * (l & 15) + h
@@ -218,7 +226,7 @@ __device__ __forceinline__ void gather_row_bf16_d128(uint4 qv, const uint4* __re
 #pragma unroll
         for (int m = 0; m < 16; ++m) {
             const uint32_t pm = __shfl_sync(kFull, pbits, 16 * half + m);
-            uint4 vr = __ldg(vb + (size_t)max(js[m], 0) * (D / 8));
+            uint4 vr = __ldg(vb + (size_t)(kMods ? max(js[m], 0) : js[m]) * (D / 8));
             if (kMods && js[m] < 0) vr = make_uint4(0u, 0u, 0u, 0u);  // key 0 may be masked and not finite
             axpy8_bf16(pm, vr, acc);
             // the training form takes p as a bf16 value and its rest, as the tensor-core form does
@@ -277,7 +285,8 @@ gather_attn_bf16_d128_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfl
 //     (valid entries first, strictly ascending); every valid key goes into an
 //     open-addressing hash with its head bit.  The union list (at most kMaxU keys) holds
 //     each key once with its head bits.  A repeated key, a row out of form (hash form)
-//     or a larger union sends the query through gather_row_bf16_d128 per head.
+//     or a larger union sends the query through the per-head form; so does a sum
+//     that is not finite.
 //  3. the union in chunks of 16 keys.  Key and value rows are copied to shared memory
 //     with cp.async (16-byte pieces XOR-swizzled by row): the key rows of chunk c + 1
 //     are in flight while chunk c is scored, the value rows of chunk c while its scores
@@ -476,144 +485,154 @@ gather_attn_bf16_d128_mma_kernel(const __nv_bfloat16* __restrict__ q, const __nv
         }
     }
     __syncwarp();  // the union list is complete; the staging area is free
-    if (!canon || U > kMaxU) {
-#pragma unroll 1
-        for (int t = 0; t < G; ++t) {
-            const size_t row = row0 + (size_t)t * Nq;
-            const uint4 qv = __ldg(reinterpret_cast<const uint4*>(q + row * D) + (lane & 15));
-            gather_row_bf16_d128<IdxT, false>(qv, reinterpret_cast<const uint4*>(kb) + (lane & 15),
-                                       reinterpret_cast<const uint4*>(vb) + (lane & 15), idx + row * K, K, N, i,
-                                       causal, scale_log2, out + row * D, lane, ScoreMods{}, b, g * G + t, row);
+    // ---- 3.-5. the heads together.  False, with nothing stored, where a sum is not finite: a key's row that is not,
+    // listed by some of the heads only, leaves 0 times it in the sums of the others.
+    auto together = [&]() -> bool {
+        // in chunks of kMmaChunk keys
+        const uint32_t st_s = (uint32_t)__cvta_generic_to_shared(stage);  // key rows: two chunk buffers
+        const uint32_t vst_s = st_s + 2u * kChunkBytes;                    // value rows of one chunk
+        // Staging: lane copies the 16-byte piece pc = lane % 16 of rows lane / 16 + 2 r of a
+        // chunk; rows past the chunk's keys are zero-filled (source size 0).
+        auto stage_rows = [&](uint32_t dst_base, const __nv_bfloat16* base, int c0) {
+            const int nk = min(kMmaChunk, U - c0);
+            const int pc = lane & 15;
+#pragma unroll
+            for (int r = 0; r < kMmaChunk / 2; ++r) {
+                const int row = 2 * r + (lane >> 4);
+                const bool valid = row < nk;
+                const int key = valid ? ukey[c0 + row] : 0;
+                const uint32_t dst = dst_base + (uint32_t)(row * kRowBytes + ((pc ^ (row & 7)) << 4));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                             "l"(base + (size_t)key * D + pc * 8), "r"(valid ? 16 : 0)
+                             : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // ldmatrix row addresses (16 rows of a chunk, 16-byte pieces).  Key rows, the A
+        // operand of S^T (no transpose): lanes 0-7 / 8-15 / 16-23 / 24-31 give key rows
+        // 0..7 / 8..15 / 0..7 / 8..15 at piece 2 s / 2 s / 2 s + 1 / 2 s + 1 (k-step s).
+        // Value rows, the A operand of O^T (transposed): key rows 0..7 / 0..7 / 8..15 /
+        // 8..15 at piece 2 mt / 2 mt + 1 / 2 mt / 2 mt + 1 (dims 16 mt .. 16 mt + 15).
+        const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
+        const int vrow = (lane & 7) + (lane >> 4) * 8, vpc = (lane >> 3) & 1;
+        // O^T accumulators: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
+        float oacc[8][4];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
+        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};  // heads 2 c4, 2 c4 + 1
+        const int nch = (U + kMmaChunk - 1) / kMmaChunk;
+        if (nch > 0) stage_rows(st_s, kb, 0);
+        for (int c = 0; c < nch; ++c) {
+            const int c0 = c * kMmaChunk;
+            const int nk = min(kMmaChunk, U - c0);
+            const bool more = c + 1 < nch;  // warp-uniform
+            __syncwarp();  // chunk c - 1 is done with the value rows and with key buffer (c + 1) & 1
+            stage_rows(vst_s, vb, c0);
+            if (more) stage_rows(st_s + (uint32_t)(((c + 1) & 1) * kChunkBytes), kb, c0 + kMmaChunk);
+            // groups in flight: key rows of c, value rows of c, key rows of c + 1 (if any)
+            if (more) cp_async_wait_pending<2>();
+            else cp_async_wait_pending<1>();
+            __syncwarp();
+            // S^T = K Q^T of the chunk: keys gq, gq + 8 x heads 2 c4, 2 c4 + 1
+            const uint32_t kst = st_s + (uint32_t)((c & 1) * kChunkBytes);
+            float sacc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const int piece = 2 * s + kpc;
+                uint32_t a0, a1, a2, a3;
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                             : "r"(kst + (uint32_t)(krow * kRowBytes + ((piece ^ (krow & 7)) << 4))));
+                mma_bf16_16816_a4(sacc, a0, a1, a2, a3, qa[2 * s], qa[2 * s + 1]);
+            }
+            // online softmax per head over its selected keys c0 + gq, c0 + gq + 8; a head's
+            // scores sit in the eight lanes of equal c4
+            bool sel[2][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int ul = gq + 8 * h;
+                const unsigned hb = ul < nk ? umask[c0 + ul] : 0u;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) sel[h][e] = 2 * c4 + e < G && ((hb >> (2 * c4 + e)) & 1u);
+            }
+            float mx[2], alpha[2], pr[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float s0 = sel[0][e] ? sacc[e] * scale_log2 : -INFINITY;
+                const float s1 = sel[1][e] ? sacc[2 + e] * scale_log2 : -INFINITY;
+                float m = fmaxf(s0, s1);
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
+                mx[e] = fmaxf(m_run[e], m);
+                const float ref = mx[e] == -INFINITY ? 0.f : mx[e];  // nothing selected so far, or NaN alone
+                alpha[e] = exp2f(m_run[e] - ref);
+                pr[0][e] = exp2f(s0 - ref);
+                pr[1][e] = exp2f(s1 - ref);
+                float sum = pr[0][e] + pr[1][e];
+                sum += __shfl_xor_sync(kFull, sum, 4);
+                sum += __shfl_xor_sync(kFull, sum, 8);
+                sum += __shfl_xor_sync(kFull, sum, 16);
+                l_run[e] = l_run[e] * alpha[e] + sum;
+                m_run[e] = mx[e];
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                oacc[n][0] *= alpha[0];
+                oacc[n][1] *= alpha[1];
+                oacc[n][2] *= alpha[0];
+                oacc[n][3] *= alpha[1];
+            }
+            // P^T as the B operand: each 8 x 8 (keys x heads) half of the score tile,
+            // rounded to bf16, transposed across the warp
+            const uint32_t pb0 = movmatrix_trans(pack_bf16x2(pr[0][0], pr[0][1]));
+            const uint32_t pb1 = movmatrix_trans(pack_bf16x2(pr[1][0], pr[1][1]));
+            // O^T += V^T P^T of the chunk
+            if (more) cp_async_wait_pending<1>();
+            else cp_async_wait_pending<0>();
+            __syncwarp();
+#pragma unroll
+            for (int mt = 0; mt < 8; ++mt) {
+                const int pc = 2 * mt + vpc;
+                uint32_t a0, a1, a2, a3;
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
+                             : "r"(vst_s + (uint32_t)(vrow * kRowBytes + ((pc ^ (vrow & 7)) << 4))));
+                mma_bf16_16816_a4(oacc[mt], a0, a1, a2, a3, pb0, pb1);
+            }
         }
-        return;
-    }
-
-    // ---- 3.-5. the union in chunks of kMmaChunk keys
-    const uint32_t st_s = (uint32_t)__cvta_generic_to_shared(stage);  // key rows: two chunk buffers
-    const uint32_t vst_s = st_s + 2u * kChunkBytes;                    // value rows of one chunk
-    // Staging: lane copies the 16-byte piece pc = lane % 16 of rows lane / 16 + 2 r of a
-    // chunk; rows past the chunk's keys are zero-filled (source size 0).
-    auto stage_rows = [&](uint32_t dst_base, const __nv_bfloat16* base, int c0) {
-        const int nk = min(kMmaChunk, U - c0);
-        const int pc = lane & 15;
-#pragma unroll
-        for (int r = 0; r < kMmaChunk / 2; ++r) {
-            const int row = 2 * r + (lane >> 4);
-            const bool valid = row < nk;
-            const int key = valid ? ukey[c0 + row] : 0;
-            const uint32_t dst = dst_base + (uint32_t)(row * kRowBytes + ((pc ^ (row & 7)) << 4));
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                         "l"(base + (size_t)key * D + pc * 8), "r"(valid ? 16 : 0)
-                         : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    // ldmatrix row addresses (16 rows of a chunk, 16-byte pieces).  Key rows, the A
-    // operand of S^T (no transpose): lanes 0-7 / 8-15 / 16-23 / 24-31 give key rows
-    // 0..7 / 8..15 / 0..7 / 8..15 at piece 2 s / 2 s / 2 s + 1 / 2 s + 1 (k-step s).
-    // Value rows, the A operand of O^T (transposed): key rows 0..7 / 0..7 / 8..15 /
-    // 8..15 at piece 2 mt / 2 mt + 1 / 2 mt / 2 mt + 1 (dims 16 mt .. 16 mt + 15).
-    const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kpc = lane >> 4;
-    const int vrow = (lane & 7) + (lane >> 4) * 8, vpc = (lane >> 3) & 1;
-    // O^T accumulators: dims 16 mt + gq (+8) of heads 2 c4, 2 c4 + 1
-    float oacc[8][4];
-#pragma unroll
-    for (int n = 0; n < 8; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};  // heads 2 c4, 2 c4 + 1
-    const int nch = (U + kMmaChunk - 1) / kMmaChunk;
-    if (nch > 0) stage_rows(st_s, kb, 0);
-    for (int c = 0; c < nch; ++c) {
-        const int c0 = c * kMmaChunk;
-        const int nk = min(kMmaChunk, U - c0);
-        const bool more = c + 1 < nch;  // warp-uniform
-        __syncwarp();  // chunk c - 1 is done with the value rows and with key buffer (c + 1) & 1
-        stage_rows(vst_s, vb, c0);
-        if (more) stage_rows(st_s + (uint32_t)(((c + 1) & 1) * kChunkBytes), kb, c0 + kMmaChunk);
-        // groups in flight: key rows of c, value rows of c, key rows of c + 1 (if any)
-        if (more) cp_async_wait_pending<2>();
-        else cp_async_wait_pending<1>();
-        __syncwarp();
-        // S^T = K Q^T of the chunk: keys gq, gq + 8 x heads 2 c4, 2 c4 + 1
-        const uint32_t kst = st_s + (uint32_t)((c & 1) * kChunkBytes);
-        float sacc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const int piece = 2 * s + kpc;
-            uint32_t a0, a1, a2, a3;
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
-                         : "r"(kst + (uint32_t)(krow * kRowBytes + ((piece ^ (krow & 7)) << 4))));
-            mma_bf16_16816_a4(sacc, a0, a1, a2, a3, qa[2 * s], qa[2 * s + 1]);
-        }
-        // online softmax per head over its selected keys c0 + gq, c0 + gq + 8; a head's
-        // scores sit in the eight lanes of equal c4
-        bool sel[2][2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int ul = gq + 8 * h;
-            const unsigned hb = ul < nk ? umask[c0 + ul] : 0u;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) sel[h][e] = 2 * c4 + e < G && ((hb >> (2 * c4 + e)) & 1u);
-        }
-        float mx[2], alpha[2], pr[2][2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const float s0 = sel[0][e] ? sacc[e] * scale_log2 : -INFINITY;
-            const float s1 = sel[1][e] ? sacc[2 + e] * scale_log2 : -INFINITY;
-            float m = fmaxf(s0, s1);
-            m = fmaxf(m, __shfl_xor_sync(kFull, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(kFull, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(kFull, m, 16));
-            mx[e] = fmaxf(m_run[e], m);
-            const float ref = mx[e] == -INFINITY ? 0.f : mx[e];  // nothing selected so far, or NaN alone
-            alpha[e] = exp2f(m_run[e] - ref);
-            pr[0][e] = exp2f(s0 - ref);
-            pr[1][e] = exp2f(s1 - ref);
-            float sum = pr[0][e] + pr[1][e];
-            sum += __shfl_xor_sync(kFull, sum, 4);
-            sum += __shfl_xor_sync(kFull, sum, 8);
-            sum += __shfl_xor_sync(kFull, sum, 16);
-            l_run[e] = l_run[e] * alpha[e] + sum;
-            m_run[e] = mx[e];
-        }
+        // a key's row that is not finite, listed by some of the heads only, leaves 0 times it in the others' sums
+        float bad = 0.f;  // 0 while every sum is finite
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            oacc[n][0] *= alpha[0];
-            oacc[n][1] *= alpha[1];
-            oacc[n][2] *= alpha[0];
-            oacc[n][3] *= alpha[1];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) bad = fmaf(oacc[n][x], 0.f, bad);
         }
-        // P^T as the B operand: each 8 x 8 (keys x heads) half of the score tile,
-        // rounded to bf16, transposed across the warp
-        const uint32_t pb0 = movmatrix_trans(pack_bf16x2(pr[0][0], pr[0][1]));
-        const uint32_t pb1 = movmatrix_trans(pack_bf16x2(pr[1][0], pr[1][1]));
-        // O^T += V^T P^T of the chunk
-        if (more) cp_async_wait_pending<1>();
-        else cp_async_wait_pending<0>();
-        __syncwarp();
+        if (__any_sync(kFull, bad != 0.f)) return false;
+        // each head's row divided by its sum; the 8 x 8 (dims x heads) halves of every O^T
+        // tile transposed back, so lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
+        const float inv0 = l_run[0] > 0.f ? 1.f / l_run[0] : 0.f;
+        const float inv1 = l_run[1] > 0.f ? 1.f / l_run[1] : 0.f;
+        __nv_bfloat16* orow = out + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D + 2 * c4;
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) {
-            const int pc = 2 * mt + vpc;
-            uint32_t a0, a1, a2, a3;
-            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(a0), "=r"(a1), "=r"(a2), "=r"(a3)
-                         : "r"(vst_s + (uint32_t)(vrow * kRowBytes + ((pc ^ (vrow & 7)) << 4))));
-            mma_bf16_16816_a4(oacc[mt], a0, a1, a2, a3, pb0, pb1);
+            const uint32_t lo = movmatrix_trans(pack_bf16x2(oacc[mt][0] * inv0, oacc[mt][1] * inv1));
+            const uint32_t hi = movmatrix_trans(pack_bf16x2(oacc[mt][2] * inv0, oacc[mt][3] * inv1));
+            if (gq < G) {
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
+                *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
+            }
         }
-    }
-    // each head's row divided by its sum; the 8 x 8 (dims x heads) halves of every O^T
-    // tile transposed back, so lane (gq, c4) stores dims 2 c4, 2 c4 + 1 of head gq
-    const float inv0 = l_run[0] > 0.f ? 1.f / l_run[0] : 0.f;
-    const float inv1 = l_run[1] > 0.f ? 1.f / l_run[1] : 0.f;
-    __nv_bfloat16* orow = out + (row0 + (size_t)(gq < G ? gq : 0) * Nq) * D + 2 * c4;
-#pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-        const uint32_t lo = movmatrix_trans(pack_bf16x2(oacc[mt][0] * inv0, oacc[mt][1] * inv1));
-        const uint32_t hi = movmatrix_trans(pack_bf16x2(oacc[mt][2] * inv0, oacc[mt][3] * inv1));
-        if (gq < G) {
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt) = lo;
-            *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8) = hi;
-        }
+        return true;
+    };
+    if (canon && U <= kMaxU && together()) return;  // warp-uniform
+#pragma unroll 1
+    for (int t = 0; t < G; ++t) {
+        const size_t row = row0 + (size_t)t * Nq;
+        const uint4 qv = __ldg(reinterpret_cast<const uint4*>(q + row * D) + (lane & 15));
+        gather_row_bf16_d128<IdxT, false>(qv, reinterpret_cast<const uint4*>(kb) + (lane & 15),
+                                          reinterpret_cast<const uint4*>(vb) + (lane & 15), idx + row * K, K, N, i,
+                                          causal, scale_log2, out + row * D, lane, ScoreMods{}, b, g * G + t, row);
     }
 }
 
